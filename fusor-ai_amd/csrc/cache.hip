@@ -1,0 +1,394 @@
+// The paged 8-bit cache (fg_cache): its pages, the new tokens' keys and values quantized into them, and
+// read back. cache_layout.h says where a level lies; cache_attend.hip reads the pages.
+#include <algorithm>
+#include <new>
+
+#include "cache.h"
+
+namespace fg {
+namespace {
+
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));  // four floats at any float's address
+
+struct StoreParams {
+    BatchParams b;
+    uint8_t *records;
+    int pages, kv_heads, head_dim, padded;
+    const float *in[2];  // keys, values
+    float *out[2];
+    size_t stride[2];
+};
+
+// The scale of a head whose largest magnitude is amax, and four of its levels as stored (level + 128).
+__device__ __forceinline__ float head_levels(float amax, const v4f &x, unsigned &packed)
+{
+    int l0, l1, l2, l3;
+    float d;
+    if (amax >= 0x1p-52f && amax <= 0x1p66f) {
+        d = scale_and_levels(amax, x.x, x.y, x.z, x.w, l0, l1, l2, l3);
+    } else {
+        d = amax / 127.0f;
+        d = d == 0.0f ? 1.0f : d;
+        l0 = quantize_level(x.x, d);
+        l1 = quantize_level(x.y, d);
+        l2 = quantize_level(x.z, d);
+        l3 = quantize_level(x.w, d);
+    }
+    packed = unsigned(pack4(l0, l1, l2, l3)) ^ 0x80808080u;
+    return d;
+}
+
+// The largest magnitude of four values, NaN ignored.
+__device__ __forceinline__ float amax4(const v4f &x)
+{
+    return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+}
+
+// ... over 32 aligned lanes, or over all 64
+__device__ __forceinline__ float team_max(float v, bool wide)
+{
+    v = fmaxf(v, __int_as_float(xor1(__float_as_int(v))));
+    v = fmaxf(v, __int_as_float(xor2(__float_as_int(v))));
+    v = fmaxf(v, __int_as_float(mirror8(__float_as_int(v))));
+    v = fmaxf(v, xor8(v));
+    const float2 r = row_pair(v);
+    v = fmaxf(r.x, r.y);
+    if (wide) {
+        const float2 h = half_pair(v);
+        v = fmaxf(h.x, h.y);
+    }
+    return v;
+}
+
+__device__ __forceinline__ v4f levels_to_values(unsigned packed, float d)
+{
+    v4f x;
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = float(int((packed >> (8 * j)) & 255u) - 128) * d;
+    return x;
+}
+
+// Pages of zero levels and scales of 1.
+__global__ __launch_bounds__(256) void cache_clear_kernel(uint8_t *records, size_t dwords, unsigned levels, unsigned record)
+{
+    for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < dwords; i += size_t(gridDim.x) * 256)
+        reinterpret_cast<unsigned *>(records)[i] = i % record < levels ? 0x80808080u : 0x3F800000u;
+}
+
+// A wave per new row and head, for few new tokens a sequence. Four dimensions a lane; heads of up to 128
+// take half a wave for the key and half for the value. A value's levels go to single bytes 16 apart
+// (cache_layout.h): 8 bytes a cycle of stores for one token, which is why runs of tokens take the
+// kernels below.
+template <bool WRITE>
+__global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
+{
+    const unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int row = int(unit / unsigned(p.kv_heads)), head = int(unit % unsigned(p.kv_heads));
+    if (row >= p.b.rows) return;  // a whole wave
+    const int s = sequence_of_row(p.b, row);
+    if (s < 0) return;
+    const Span span = sequence_span(p.b, s);
+    const int at = row - span.begin;
+    if (at < 0 || at >= span.rows) return;
+    const int position = span.first + at;
+    const int page = position < 0 ? -1 : page_at(p.b.pages + size_t(s) * p.b.max_pages, position / kPage, p.b.max_pages, p.pages);
+    if (WRITE && page < 0) return;
+    const bool wide = p.padded > 128;
+    const int token = position & (kPage - 1), dim = (wide ? lane : lane & 31) * 4;
+    uint8_t *record = p.records + (size_t(page < 0 ? 0 : page) * p.kv_heads + head) * record_bytes(p.padded);
+    const bool live = dim < p.head_dim;
+    for (int i = 0; i < (wide ? 2 : 1); i++) {
+        const bool value = wide ? i != 0 : lane >= 32;
+        const size_t place = size_t(row) * p.stride[value] + size_t(head) * p.head_dim + dim;
+        float *scale = reinterpret_cast<float *>(record + (value ? value_scale_byte(p.padded, token) : key_scale_byte(p.padded, token)));
+        if (WRITE) {
+            v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (live) x = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + place);
+            unsigned packed;
+            const float d = head_levels(team_max(amax4(x), wide), x, packed);
+            if (live && !value) *reinterpret_cast<unsigned *>(record + key_byte(p.padded, token, dim)) = packed;
+            if (live && value) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) record[value_byte(p.padded, token, dim + j)] = uint8_t(packed >> (8 * j));
+            }
+            if (dim == 0) *scale = d;
+        } else if (live) {
+            v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (page >= 0) {
+                unsigned packed = 0;
+                if (value) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) packed |= unsigned(record[value_byte(p.padded, token, dim + j)]) << (8 * j);
+                } else {
+                    packed = *reinterpret_cast<const unsigned *>(record + key_byte(p.padded, token, dim));
+                }
+                x = levels_to_values(packed, *scale);
+            }
+            *reinterpret_cast<v4f_any *>((value ? p.out[1] : p.out[0]) + place) = x;
+        }
+    }
+}
+
+// A workgroup per page that new tokens lie in and head. A thread takes four tokens (an aligned run, so
+// one dword of each dimension's values) of four dimensions; the levels meet in LDS in the record's
+// order, and whole 16-byte pieces go to the page or come from it. Pieces that also hold other tokens'
+// values are written in part.
+template <bool WRITE>
+__global__ __launch_bounds__(256) void cache_pages_kernel(StoreParams p)
+{
+    extern __shared__ __align__(16) uint8_t levels[];
+    __shared__ float scales[2][kPage];
+    const int tid = threadIdx.x, head = int(blockIdx.y);
+    int index;
+    const int s = find_unit(p.b.sequences, int(blockIdx.x), &index, [&](int q) {
+        const PageRange r = pages_of_new(sequence_span(p.b, q));
+        return r.hi - r.lo;
+    });
+    if (s < 0) return;  // the whole workgroup
+    const Span span = sequence_span(p.b, s);
+    const int place = pages_of_new(span).lo + index;
+    const int page = page_at(p.b.pages + size_t(s) * p.b.max_pages, place, p.b.max_pages, p.pages);
+    if (WRITE && page < 0) return;
+    // the page's tokens [t0, t1) are new
+    const int t0 = max(span.first - place * kPage, 0), t1 = min(span.first + span.rows - place * kPage, kPage);
+    uint8_t *record = p.records + (size_t(page < 0 ? 0 : page) * p.kv_heads + head) * record_bytes(p.padded);
+    const bool wide = p.padded > 128;
+    const int lanes = wide ? 64 : 32, quads = 256 / lanes, dim = (tid & (lanes - 1)) * 4;
+    const bool live = dim < p.head_dim;
+    const size_t row0 = size_t(span.begin) + size_t(place * kPage - span.first);  // the row of the page's token 0 (may wrap below 0)
+    const int pieces = 2 * kPage * p.padded / 16;
+    if (WRITE) {
+        if (p.head_dim != p.padded) {  // the padding's levels
+            for (int i = tid; i < pieces; i += 256) reinterpret_cast<uint4 *>(levels)[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            __syncthreads();
+        }
+    } else {
+        for (int i = tid; i < pieces; i += 256)
+            reinterpret_cast<uint4 *>(levels)[i] =
+                page < 0 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u) : reinterpret_cast<const uint4 *>(record)[i];
+        if (tid < 2 * kPage)
+            (&scales[0][0])[tid] = page < 0 ? 1.0f : *reinterpret_cast<const float *>(record + key_scale_byte(p.padded, tid));
+        __syncthreads();
+    }
+    for (int unit = tid / lanes; unit < 2 * (kPage / 4); unit += quads) {  // whole teams: keys' quads, then values'
+        const int value = unit / (kPage / 4), t = unit % (kPage / 4) * 4;
+        if (t + 4 <= t0 || t >= t1) continue;
+        unsigned packed[4];
+        if (WRITE) {
+            v4f x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                if (live && t + i >= t0 && t + i < t1)
+                    x[i] = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + (row0 + t + i) * p.stride[value] +
+                                                              size_t(head) * p.head_dim + dim);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float d = head_levels(team_max(amax4(x[i]), wide), x[i], packed[i]);
+                if (dim == 0) scales[value][t + i] = d;
+            }
+        }
+        if (!value) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                unsigned *at = reinterpret_cast<unsigned *>(levels + key_byte(p.padded, t + i, dim));
+                if (WRITE && live) *at = packed[i];
+                if (!WRITE && live) packed[i] = *at;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {  // dimension dim + j of the four tokens
+                unsigned *at = reinterpret_cast<unsigned *>(levels + value_byte(p.padded, t, dim + j));
+                if (WRITE && live) {
+                    unsigned w = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w |= (packed[i] >> (8 * j) & 255u) << (8 * i);
+                    *at = w;
+                }
+                if (!WRITE) {
+                    const unsigned w = live ? *at : 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) packed[i] = (j ? packed[i] : 0) | (w >> (8 * i) & 255u) << (8 * j);
+                }
+            }
+        }
+        if (!WRITE && live) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (t + i >= t0 && t + i < t1)
+                    *reinterpret_cast<v4f_any *>((value ? p.out[1] : p.out[0]) + (row0 + t + i) * p.stride[value] +
+                                                 size_t(head) * p.head_dim + dim) = levels_to_values(packed[i], scales[value][t + i]);
+        }
+    }
+    if (!WRITE) return;
+    __syncthreads();
+    const int key_pieces = pieces / 2;
+    for (int i = tid; i < pieces; i += 256) {
+        const int lane = i & 63, block = (i < key_pieces ? i : i - key_pieces) >> 6;
+        const uint4 w = reinterpret_cast<const uint4 *>(levels)[i];
+        uint8_t *at = record + size_t(i) * 16;
+        if (i < key_pieces) {  // one token's
+            const int t = block / (p.padded >> 5) * 32 + (lane & 31);
+            if (t >= t0 && t < t1) *reinterpret_cast<uint4 *>(at) = w;
+            continue;
+        }
+        const int t = (block & 1) * 32 + (lane >> 5) * 4;  // tokens t + 8 j + i
+        if (t >= t0 && t + 28 <= t1) {
+            *reinterpret_cast<uint4 *>(at) = w;
+            continue;
+        }
+        const unsigned dword[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int q = t + 8 * j;
+            if (q >= t0 && q + 4 <= t1) {
+                reinterpret_cast<unsigned *>(at)[j] = dword[j];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (q + k >= t0 && q + k < t1) at[4 * j + k] = uint8_t(dword[j] >> (8 * k));
+            }
+        }
+    }
+    if (tid < 2 * kPage) {
+        const int t = tid & (kPage - 1);
+        if (t >= t0 && t < t1) *reinterpret_cast<float *>(record + key_scale_byte(p.padded, tid)) = (&scales[0][0])[tid];
+    }
+}
+
+template <bool WRITE>
+int launch_store(const StoreParams &p, hipStream_t s)
+{
+    if (p.b.rows == 0 || p.b.sequences == 0) return FG_OK;
+    if (p.b.rows <= 4 * p.b.sequences) {
+        const size_t units = size_t(p.b.rows) * p.kv_heads;
+        cache_rows_kernel<WRITE><<<unsigned((units + 3) / 4), 256, 0, s>>>(p);
+    } else {
+        // a run of n rows lies in at most (n + 62) / 64 + 1 pages
+        const size_t units = size_t(p.b.rows) / kPage + 2 * size_t(std::min(p.b.sequences, p.b.rows));
+        cache_pages_kernel<WRITE><<<dim3(unsigned(units), unsigned(p.kv_heads)), 256, size_t(2 * kPage * p.padded), s>>>(p);
+    }
+    FG_HIP(hipGetLastError());
+    return FG_OK;
+}
+
+}  // namespace
+
+int check_batch(const fg_cache *c, const fg_batch *b, const char *who)
+{
+    const std::string name(who);
+    if (!c || !b) return set_error(FG_ERR_ARG, name + ": a null cache or batch");
+    if (b->sequences > 65536 || b->rows > (size_t(1) << 24) || b->max_pages > (size_t(1) << 24))
+        return set_error(FG_ERR_SHAPE, name + ": at most 65536 sequences, 2^24 rows and 2^24 pages a sequence");
+    if (b->sequences && (!b->row_starts || !b->lengths || (b->max_pages && !b->pages)))
+        return set_error(FG_ERR_ARG, name + ": a null array of the batch");
+    int device = 0;
+    FG_HIP(hipGetDevice(&device));
+    if (device != c->device)
+        return set_error(FG_ERR_ARG, name + ": the cache is on device " + std::to_string(c->device) + ", the current one is " +
+                                         std::to_string(device));
+    return FG_OK;
+}
+
+namespace {
+
+int check_store(const fg_cache *c, const fg_batch *b, const void *key, size_t key_stride, const void *value, size_t value_stride,
+                bool writes_rows, const char *who)
+{
+    const int rc = check_batch(c, b, who);
+    if (rc) return rc;
+    if (b->rows && b->sequences && (!key || !value)) return set_error(FG_ERR_ARG, std::string(who) + ": null keys or values");
+    const size_t width = size_t(c->kv_heads) * c->head_dim;
+    // rows that are only read may overlap (one row for all of them, stride 0)
+    if (writes_rows && b->rows > 1 && (key_stride < width || value_stride < width))
+        return set_error(FG_ERR_SHAPE, std::string(who) + ": a row's heads run past the row stride");
+    return FG_OK;
+}
+
+StoreParams store_params(const fg_cache *c, const fg_batch *b, size_t key_stride, size_t value_stride)
+{
+    StoreParams p{};
+    p.b = batch_params(b);
+    p.records = c->records;
+    p.pages = c->pages;
+    p.kv_heads = c->kv_heads;
+    p.head_dim = c->head_dim;
+    p.padded = c->padded;
+    p.stride[0] = key_stride;
+    p.stride[1] = value_stride;
+    return p;
+}
+
+}  // namespace
+}  // namespace fg
+
+using namespace fg;
+
+extern "C" {
+
+int fg_cache_create(size_t pages, size_t kv_heads, size_t head_dim, void *stream, fg_cache **out)
+{
+    if (!out) return set_error(FG_ERR_ARG, "fg_cache_create: a null output handle");
+    *out = nullptr;
+    if (!kv_heads || !head_dim || head_dim % 4 || head_dim > 256)
+        return set_error(FG_ERR_SHAPE, "fg_cache_create: heads of whole quads, at most 256 values, and at least one head");
+    if (kv_heads > 4096 || pages > (size_t(1) << 24))
+        return set_error(FG_ERR_SHAPE, "fg_cache_create: at most 4096 heads and 2^24 pages");
+    const int padded = padded_head(int(head_dim));
+    const size_t bytes = pages * kv_heads * size_t(record_bytes(padded));
+    int device = 0;
+    FG_HIP(hipGetDevice(&device));
+    uint8_t *records = nullptr;
+    hipError_t e = hipMalloc(reinterpret_cast<void **>(&records), std::max<size_t>(bytes, 16));
+    if (e != hipSuccess) return check_hip(e, "fg_cache_create: hipMalloc");
+    if (bytes) {
+        const hipStream_t s = as_stream(stream);
+        cache_clear_kernel<<<4096, 256, 0, s>>>(records, bytes / 4, unsigned(2 * kPage * padded / 4), unsigned(record_bytes(padded) / 4));
+        e = hipGetLastError();
+        if (e == hipSuccess) e = hipStreamSynchronize(s);
+        if (e != hipSuccess) {
+            (void)hipFree(records);
+            return check_hip(e, "fg_cache_create");
+        }
+    }
+    fg_cache *c = new (std::nothrow) fg_cache{device, int(pages), int(kv_heads), int(head_dim), padded, records};
+    if (!c) {
+        (void)hipFree(records);
+        return set_error(FG_ERR_NOMEM, "fg_cache_create: host memory");
+    }
+    *out = c;
+    return FG_OK;
+}
+
+int fg_cache_free(fg_cache *c)
+{
+    if (!c) return FG_OK;
+    (void)hipFree(c->records);
+    delete c;
+    return FG_OK;
+}
+
+int fg_cache_write(fg_cache *c, const fg_batch *b, const float *key, size_t key_stride, const float *value, size_t value_stride,
+                   void *stream)
+{
+    const int rc = check_store(c, b, key, key_stride, value, value_stride, false, "fg_cache_write");
+    if (rc) return rc;
+    StoreParams p = store_params(c, b, key_stride, value_stride);
+    p.in[0] = key;
+    p.in[1] = value;
+    return launch_store<true>(p, as_stream(stream));
+}
+
+int fg_cache_read(const fg_cache *c, const fg_batch *b, float *key, size_t key_stride, float *value, size_t value_stride, void *stream)
+{
+    const int rc = check_store(c, b, key, key_stride, value, value_stride, true, "fg_cache_read");
+    if (rc) return rc;
+    StoreParams p = store_params(c, b, key_stride, value_stride);
+    p.out[0] = key;
+    p.out[1] = value;
+    return launch_store<false>(p, as_stream(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,823 @@
+// Attention of a step's new tokens over the paged 8-bit cache (fg_cache_attend).
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+
+#include "cache.h"
+
+namespace fg {
+namespace {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+
+struct AttendParams {
+    BatchParams b;
+    const uint8_t *records;
+    int pages, kv_heads, heads, group, head_dim;
+    const float *query;
+    size_t query_stride;
+    float *out;
+    size_t out_stride;
+    float scale2;  // the scale times log2 e
+    int window;
+    int grid;      // tasks a head there is room for
+    int target;    // tasks a head aims at; 0: no row tile is split
+    float *partial;
+};
+
+constexpr int kMaxSplit = 64;   // parts of one row tile
+constexpr int kMinPages = 4;    // pages of a part, a wave each
+
+// ---------------------------------------------------------------------------- the plan
+//
+// The rows of a tile are (new token, query head of the key head's group) pairs, token-major: tile t of a
+// sequence holds pairs t·TM .. of its rows·group. A tile's pages are split over the sequence's nsplit
+// tasks. Every workgroup finds its task from the batch's arrays by itself: nothing about the lengths is
+// known on the host.
+struct Task {
+    int seq, tile, split, nsplit;
+    int slot;  // of the tile's first part, in order over all tasks
+    Span span;
+};
+
+__device__ __forceinline__ int tiles_of(const AttendParams &p, const Span &s, int TM) { return (s.rows * p.group + TM - 1) / TM; }
+
+// Pages that a tile of the sequence sees at most.
+__device__ __forceinline__ int tile_pages(const AttendParams &p, const Span &s, int TM)
+{
+    if (s.rows <= 0) return 0;
+    const PageRange r = pages_seen(s, 0, s.rows - 1, p.window, p.b.max_pages);
+    const int all = r.hi - r.lo;
+    return p.window > 0 ? min(all, (p.window + TM / p.group + 1) / kPage + 2) : all;
+}
+
+// Pages a part takes: the whole work spread over the target.
+__device__ __forceinline__ int part_pages(const AttendParams &p, int TM)
+{
+    if (!p.target) return INT_MAX;
+    const int lane = threadIdx.x & 63;
+    unsigned long long work = 0;
+    for (int s = lane; s < p.b.sequences; s += 64) {
+        const Span span = sequence_span(p.b, s);
+        work += (unsigned long long)tiles_of(p, span, TM) * tile_pages(p, span, TM);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
+    const unsigned long long part = (work + p.target - 1) / p.target;
+    return part < kMinPages ? kMinPages : part > INT_MAX / 2 ? INT_MAX / 2 : int(part);
+}
+
+__device__ __forceinline__ int splits_of(int pages, int part)
+{
+    return pages <= part ? 1 : min((pages + part - 1) / part, kMaxSplit);
+}
+
+// The task of index x (TILES: the row tile of index x, its first part), or seq -1.
+template <bool TILES>
+__device__ __forceinline__ Task find_task(const AttendParams &p, int x, int TM)
+{
+    const int part = part_pages(p, TM);
+    Task t;
+    int within;
+    if (!TILES) {
+        t.seq = find_unit(p.b.sequences, x, &within, [&](int s) {
+            const Span span = sequence_span(p.b, s);
+            return tiles_of(p, span, TM) * splits_of(tile_pages(p, span, TM), part);
+        });
+        if (t.seq < 0) return t;
+        t.span = sequence_span(p.b, t.seq);
+        t.nsplit = splits_of(tile_pages(p, t.span, TM), part);
+        // the last tiles see the most keys: they come first
+        t.tile = tiles_of(p, t.span, TM) - 1 - within / t.nsplit;
+        t.split = within % t.nsplit;
+        t.slot = x - t.split;
+        return t;
+    }
+    const int lane = threadIdx.x & 63;
+    int before = 0, slots = 0;
+    t.seq = -1;
+    for (int s0 = 0; s0 < p.b.sequences; s0 += 64) {
+        int tiles = 0, tasks = 0;
+        if (s0 + lane < p.b.sequences) {
+            const Span span = sequence_span(p.b, s0 + lane);
+            tiles = tiles_of(p, span, TM);
+            tasks = tiles * splits_of(tile_pages(p, span, TM), part);
+        }
+        int total, all;
+        const int upto = before + wave_scan(tiles, &total), upto_tasks = slots + wave_scan(tasks, &all);
+        const unsigned long long here = __ballot(x < upto);
+        if (here) {
+            const int at = __builtin_ctzll(here);
+            within = x - __shfl(upto - tiles, at, 64);
+            t.seq = s0 + at;
+            t.span = sequence_span(p.b, t.seq);
+            t.nsplit = splits_of(tile_pages(p, t.span, TM), part);
+            t.tile = tiles_of(p, t.span, TM) - 1 - within;
+            t.split = 0;
+            t.slot = __shfl(upto_tasks - tasks, at, 64) + within * t.nsplit;
+            return t;
+        }
+        before += total;
+        slots += all;
+    }
+    return t;
+}
+
+// The pages [lo, hi) of a task.
+__device__ __forceinline__ PageRange task_pages(const AttendParams &p, const Task &t, int TM)
+{
+    const int row = t.tile * TM / p.group, last = min((t.tile * TM + TM - 1) / p.group, t.span.rows - 1);
+    PageRange r = pages_seen(t.span, row, last, p.window, p.b.max_pages);
+    const int n = (r.hi - r.lo + t.nsplit - 1) / t.nsplit;
+    r.lo = min(r.lo + t.split * n, r.hi);
+    r.hi = min(r.lo + n, r.hi);
+    return r;
+}
+
+// One pair of a tile: its operand row, query head and position.
+struct Pair {
+    int row, head, position;
+    bool live;
+};
+__device__ __forceinline__ Pair pair_of(const AttendParams &p, const Task &t, int kv, int m)
+{
+    const int pairs = t.span.rows * p.group;
+    Pair r;
+    r.live = m < pairs;
+    m = min(m, pairs - 1);  // the last again past the pairs
+    const int at = m / p.group;
+    r.row = t.span.begin + at;
+    r.head = kv * p.group + (m - at * p.group);
+    r.position = t.span.first + at;
+    return r;
+}
+
+// -------------------------------------------------------------------------- the numerics
+//
+// A level is exact in f16, so the products take f16 operands and f32 sums, and the f32 side of each is
+// split into two f16 pieces, x = hi + lo to 2^-22 of x (and to 2^-35 of the row's largest, where lo falls
+// under f16's normal range):
+//   queries: a row is scaled by a power of two to a largest magnitude in [2^9, 2^10);
+//   weights: 2^(t - r) times the value's scale, for t the score times log2 e and r a reference of the row,
+//            a whole number. r is set when a weight passes 2^15, so that the largest is in (2^9, 2^11], and
+//            the row's sums are scaled by the power of two between; the total of 2^(t - r) is kept in f32,
+//            and r cancels in the quotient.
+// r rises with the largest of a weight times its value's scale, not with the largest weight alone: a
+// value far larger than the others whose weight is next to nothing does not cost the others their bits.
+
+// Eight stored levels (level + 128, two dwords) as f16: 0x6400 + u is 1024 + u.
+__device__ __forceinline__ v8h widen8(unsigned a, unsigned b)
+{
+    union {
+        unsigned u[4];
+        v2h h[4];
+        v8h v;
+    } w;
+    w.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    w.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    w.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    w.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+    const v2h bias = {_Float16(-1152.0f), _Float16(-1152.0f)};
+#pragma unroll
+    for (int i = 0; i < 4; i++) w.h[i] = w.h[i] + bias;
+    return w.v;
+}
+
+__device__ __forceinline__ void split8(const float *x, v8h &hi, v8h &lo)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        hi[i] = _Float16(x[i]);
+        lo[i] = _Float16(__builtin_fmaf(float(hi[i]), -1.0f, x[i]));
+    }
+}
+
+// Eight query values from dimension d on (0 past the head's).
+__device__ __forceinline__ void load8(const float *row, int d, int head_dim, float *x)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+        v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (d + i < head_dim) v = *reinterpret_cast<const v4f_any *>(row + d + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i + j] = v[j];
+    }
+}
+
+// The power of two that brings a row's largest magnitude to [2^9, 2^10).
+__device__ __forceinline__ int query_shift(float amax)
+{
+    return amax > 0.0f ? min(10 - __builtin_amdgcn_frexp_expf(amax), 126) : 0;
+}
+
+constexpr float kWeightLimit = 32768.0f;
+
+// The running sums of a row: its reference r (-inf: no key yet, and then a total of 0) and the total of 2^(t - r) over the
+// keys that this lane holds.
+struct RowSums {
+    float r, total;
+};
+
+// N scores of one row in this lane, t = s · key scale · f, to weights times the values' scales, in
+// place; the row's other scores are in the lanes that COMBINE joins. edge: keys outside [low, high] are
+// masked (key(i) is score i's position). rescale(a) scales the row's sums of this lane by a.
+template <int N, class Key, class Combine, class Rescale>
+__device__ __forceinline__ void weigh(float (&s)[N], const float *ks, const float *vs, float f, bool edge, int low, int high,
+                                      RowSums &sums, Key key, Combine combine, Rescale rescale)
+{
+    float t[N];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        t[i] = s[i] * ks[i] * f;
+        const float e = __builtin_amdgcn_exp2f(t[i] - sums.r);
+        float x = e * vs[i];
+        if (edge) x = key(i) >= low && key(i) <= high ? x : 0.0f;
+        s[i] = x;
+        top = fmaxf(top, x);
+    }
+    if (__any(top > kWeightLimit)) {
+        top = combine(top);
+        float u = -INFINITY, m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const bool seen = !edge || (key(i) >= low && key(i) <= high);
+            u = seen ? fmaxf(u, t[i] + __builtin_amdgcn_logf(vs[i])) : u;
+            m = seen ? fmaxf(m, t[i]) : m;
+        }
+        u = combine(u);
+        m = combine(m);
+        if (top > kWeightLimit) {
+            // (a weight alone stays under 2^100, whatever the values' scales)
+            const float r = fmaxf(ceilf(u) - 10.0f, ceilf(m) - 100.0f);
+            const float a = __builtin_amdgcn_exp2f(sums.r - r);
+            sums.r = r;
+            sums.total = sums.total * a;
+            rescale(a);
+        }
+    }
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float e = __builtin_amdgcn_exp2f(t[i] - sums.r);
+        float x = e * vs[i];
+        if (edge) {
+            const bool seen = key(i) >= low && key(i) <= high;
+            e = seen ? e : 0.0f;
+            x = seen ? x : 0.0f;
+        }
+        s[i] = x;
+        total = total + e;
+    }
+    sums.total = sums.total + total;
+}
+
+// The factor of a part's sums in the joined ones, whose reference is the largest of the parts'.
+__device__ __forceinline__ float part_factor(float r, float joined) { return r == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(r - joined); }
+
+// ---------------------------------------------------------------- few rows: decode steps
+//
+// A workgroup of four waves takes MT x 16 pairs of one key head over its task's pages; each wave takes
+// whole pages (the task's first, fifth ...), straight from memory to registers: nothing is shared
+// between waves until their sums are joined at the end. The products are 16 x 16 x 32; lane l holds
+// pair l % 16, and with g = l / 16 and 4 t + r the record's own order of values:
+//   scores:  four products of 16 keys: row i of product t is key 32 (i / 8) + 8 t + i % 8, so lane l gets
+//            the scores of keys 32 (g / 2) + 8 t + 4 (g % 2) + r, r = 0 .. 3;
+//   values:  16 dimensions by 32 keys: the lane's 16 bytes of dimension l % 16 are those keys', in order.
+template <int DP, int MT>
+__global__ __launch_bounds__(256) void attend_few_kernel(AttendParams p)
+{
+    constexpr int TM = 16 * MT, J = (DP + 63) / 64, T = DP / 16, R = DP / 32;
+    __shared__ __align__(16) float joined[2][MT * (T * 4 + 2)][64];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, kv = int(blockIdx.x % unsigned(p.kv_heads));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Task task = find_task<false>(p, int(blockIdx.x / unsigned(p.kv_heads)), TM);
+    if (task.seq < 0) return;  // the whole workgroup
+    const PageRange range = task_pages(p, task, TM);
+
+    v8h qh[MT][J][2], ql[MT][J][2];
+    float f[MT];
+    Pair pair[MT];
+    RowSums sums[MT];
+    v4f o[MT][T];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        pair[mt] = pair_of(p, task, kv, task.tile * TM + mt * 16 + i);
+        const float *row = p.query + size_t(pair[mt].row) * p.query_stride + size_t(pair[mt].head) * p.head_dim;
+        float x[J][2][8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                load8(row, 64 * j + 16 * g + 8 * e, p.head_dim, x[j][e]);
+#pragma unroll
+                for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(x[j][e][k]));
+            }
+        float2 w = row_pair(amax);
+        w = half_pair(fmaxf(w.x, w.y));
+        const int shift = query_shift(fmaxf(w.x, w.y));
+        f[mt] = ldexpf(p.scale2, -shift);
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[j][e][k] = ldexpf(x[j][e][k], shift);
+                split8(x[j][e], qh[mt][j][e], ql[mt][j][e]);
+            }
+        sums[mt] = RowSums{-INFINITY, 0.0f};
+#pragma unroll
+        for (int d = 0; d < T; d++) o[mt][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const int first = task.span.first + task.tile * TM / p.group;  // positions of the tile's first and last rows
+    const int last = task.span.first + min((task.tile * TM + TM - 1) / p.group, task.span.rows - 1);
+    const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
+    for (int page = range.lo + wave; page < range.hi; page += 4) {
+        const int id = __builtin_amdgcn_readfirstlane(page_at(table, page, p.b.max_pages, p.pages));
+        if (id < 0) continue;
+        const uint8_t *record = p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP);
+        uint4 k[4][J], v[T];
+        v4f ks[4], vs[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int block = min(2 * j + (g >> 1), R - 1);  // (the last dimensions of an odd count again: the queries' are 0)
+                k[t][j] = *reinterpret_cast<const uint4 *>(record + ((i >> 3) * R + block) * 1024 + ((g & 1) * 32 + 8 * t + (i & 7)) * 16);
+            }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int token = 32 * (g >> 1) + 8 * t + 4 * (g & 1);
+            ks[t] = *reinterpret_cast<const v4f *>(record + key_scale_byte(DP, token));
+            vs[t] = *reinterpret_cast<const v4f *>(record + value_scale_byte(DP, token));
+        }
+#pragma unroll
+        for (int d = 0; d < T; d++)
+            v[d] = *reinterpret_cast<const uint4 *>(record + kPage * DP + ((d >> 1) * 2 + (g >> 1)) * 1024 + ((g & 1) * 32 + (d & 1) * 16 + i) * 16);
+        v4f s[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) s[mt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const v8h a = e ? widen8(k[t][j].z, k[t][j].w) : widen8(k[t][j].x, k[t][j].y);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[mt][j][e], s[mt][t], 0, 0, 0);
+                        s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[mt][j][e], s[mt][t], 0, 0, 0);
+                    }
+                }
+        const int base = page * kPage + 32 * (g >> 1) + 4 * (g & 1);
+        const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
+        v8h wh[MT][2], wl[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            float x[16], kk[16], vv[16];
+#pragma unroll
+            for (int n = 0; n < 16; n++) {
+                x[n] = s[mt][n / 4][n % 4];
+                kk[n] = ks[n / 4][n % 4];
+                vv[n] = vs[n / 4][n % 4];
+            }
+            const int high = pair[mt].position, low = p.window > 0 ? high - p.window + 1 : 0;
+            weigh<16>(x, kk, vv, f[mt], edge, low, high, sums[mt], [&](int n) { return base + 8 * (n / 4) + n % 4; },
+                      [](float a) {
+                          float2 w = row_pair(a);
+                          w = half_pair(fmaxf(w.x, w.y));
+                          return fmaxf(w.x, w.y);
+                      },
+                      [&](float a) {
+#pragma unroll
+                          for (int d = 0; d < T; d++)
+#pragma unroll
+                              for (int r = 0; r < 4; r++) o[mt][d][r] = o[mt][d][r] * a;
+                      });
+            split8(x, wh[mt][0], wl[mt][0]);
+            split8(x + 8, wh[mt][1], wl[mt][1]);
+        }
+#pragma unroll
+        for (int d = 0; d < T; d++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const v8h a = e ? widen8(v[d].z, v[d].w) : widen8(v[d].x, v[d].y);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    o[mt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl[mt][e], o[mt][d], 0, 0, 0);
+                    o[mt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wh[mt][e], o[mt][d], 0, 0, 0);
+                }
+            }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        float2 w = row_pair(sums[mt].total);
+        w = half_pair(w.x + w.y);
+        sums[mt].total = w.x + w.y;
+    }
+    // the waves' sums joined, lane by lane: waves 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+    for (int step = 2; step >= 1; step >>= 1) {
+        float(*to)[64] = joined[wave & 1];
+        if (wave >= step && wave < 2 * step) {
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                const int at = mt * (T * 4 + 2);
+                to[at][lane] = sums[mt].r;
+                to[at + 1][lane] = sums[mt].total;
+#pragma unroll
+                for (int d = 0; d < T; d++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) to[at + 2 + d * 4 + r][lane] = o[mt][d][r];
+            }
+        }
+        __syncthreads();
+        if (wave < step) {
+            float(*from)[64] = joined[(wave + step) & 1];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                const int at = mt * (T * 4 + 2);
+                const float other = from[at][lane], r = fmaxf(sums[mt].r, other);
+                const float a = part_factor(sums[mt].r, r), b = part_factor(other, r);
+                sums[mt].r = r;
+                sums[mt].total = sums[mt].total * a + from[at + 1][lane] * b;
+#pragma unroll
+                for (int d = 0; d < T; d++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[mt][d][c] = o[mt][d][c] * a + from[at + 2 + d * 4 + c][lane] * b;
+            }
+        }
+        __syncthreads();
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        if (task.nsplit > 1) {
+            float *part = p.partial + ((size_t(task.slot + task.split) * p.kv_heads + kv) * MT + mt) * (16 * DP + 128);
+            part[lane] = sums[mt].r;
+            part[64 + lane] = sums[mt].total;
+#pragma unroll
+            for (int d = 0; d < T; d++) *reinterpret_cast<v4f *>(part + 128 + d * 256 + lane * 4) = o[mt][d];
+            continue;
+        }
+        if (!pair[mt].live) continue;
+        float *row = p.out + size_t(pair[mt].row) * p.out_stride + size_t(pair[mt].head) * p.head_dim;
+        const float total = sums[mt].total;
+#pragma unroll
+        for (int d = 0; d < T; d++) {
+            v4f x;
+#pragma unroll
+            for (int c = 0; c < 4; c++) x[c] = total == 0.0f ? 0.0f : o[mt][d][c] / total;
+            if (16 * d + 4 * g < p.head_dim) *reinterpret_cast<v4f_any *>(row + 16 * d + 4 * g) = x;
+        }
+    }
+}
+
+// -------------------------------------------------------------------- many rows: prompts
+//
+// A workgroup of four waves takes 128 pairs of one key head, 32 a wave, and walks its task's pages
+// together: a page's levels are widened to f16 once, by all four waves, into one of two LDS buffers in
+// the products' operand order (16 bytes a lane, lane after lane: no bank conflicts), while the other is
+// read. The products are 32 x 32 x 16; lane l holds pair l % 32 and, with h = l / 32, the scores of
+// keys 8 j + 4 h + i in register 4 j + i: the order of the values' record.
+template <int DP>
+constexpr size_t many_lds() { return size_t(2) * (256 * DP + 2 * kPage * 4); }
+
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(AttendParams p)
+{
+    constexpr int TM = 128, K = DP / 16, T = DP / 32, L = DP / 32;  // steps, tiles of 32 dimensions, 16-byte loads a thread
+    extern __shared__ __align__(16) uint8_t lds[];
+    constexpr int kBuffer = 256 * DP + 2 * kPage * 4;
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5, kv = int(blockIdx.x % unsigned(p.kv_heads));
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Task task = find_task<false>(p, int(blockIdx.x / unsigned(p.kv_heads)), TM);
+    if (task.seq < 0) return;  // the whole workgroup
+    const PageRange range = task_pages(p, task, TM);
+    const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
+
+    uint4 staged[L];
+    float staged_scale = 0.0f;
+    auto load = [&](int page) {  // the page's record into registers (nothing where it has none)
+        const int id = page < range.hi ? page_at(table, page, p.b.max_pages, p.pages) : -1;
+        if (id < 0) return;
+        const uint8_t *record = p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP);
+#pragma unroll
+        for (int c = 0; c < L; c++) staged[c] = *reinterpret_cast<const uint4 *>(record + (c * 256 + tid) * 16);
+        if (tid < 2 * kPage) staged_scale = *reinterpret_cast<const float *>(record + key_scale_byte(DP, tid));
+    };
+    auto store = [&](uint8_t *to) {  // ... widened into a buffer: each kilobyte of 64 lanes as two
+#pragma unroll
+        for (int c = 0; c < L; c++) {
+            const int piece = c * 256 + tid;
+            uint8_t *at = to + (piece >> 6) * 2048 + (piece & 63) * 16;
+            *reinterpret_cast<v8h *>(at) = widen8(staged[c].x, staged[c].y);
+            *reinterpret_cast<v8h *>(at + 1024) = widen8(staged[c].z, staged[c].w);
+        }
+        if (tid < 2 * kPage) reinterpret_cast<float *>(to + 256 * DP)[tid] = staged_scale;
+    };
+#pragma unroll
+    for (int c = 0; c < L; c++) staged[c] = make_uint4(0, 0, 0, 0);
+    load(range.lo);
+
+    const Pair pair = pair_of(p, task, kv, task.tile * TM + wave * 32 + l31);
+    v8h qh[K], ql[K];
+    float f;
+    {
+        const float *row = p.query + size_t(pair.row) * p.query_stride + size_t(pair.head) * p.head_dim;
+        float x[K][8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            load8(row, 32 * (k >> 1) + 16 * h + 8 * (k & 1), p.head_dim, x[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[k][e]));
+        }
+        const float2 w = half_pair(amax);
+        const int shift = query_shift(fmaxf(w.x, w.y));
+        f = ldexpf(p.scale2, -shift);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[k][e] = ldexpf(x[k][e], shift);
+            split8(x[k], qh[k], ql[k]);
+        }
+    }
+    RowSums sums{-INFINITY, 0.0f};
+    v16f o[T];
+#pragma unroll
+    for (int d = 0; d < T; d++) o[d] = v16f{};
+    const int pairs = task.span.rows * p.group, m0 = task.tile * TM + wave * 32;
+    // the wave's pairs: the positions of its first and last
+    const int first = task.span.first + min(m0, pairs - 1) / p.group, last = task.span.first + min(m0 + 31, pairs - 1) / p.group;
+    const bool any = m0 < pairs;
+
+    store(lds);
+    load(range.lo + 1);
+    __syncthreads();
+    for (int page = range.lo; page < range.hi; page++) {
+        const int b = (page - range.lo) & 1;
+        if (page + 1 < range.hi) {
+            store(lds + (b ^ 1) * kBuffer);
+            load(page + 2);
+        }
+        const uint8_t *buffer = lds + b * kBuffer;
+        const float *key_scales = reinterpret_cast<const float *>(buffer + 256 * DP), *value_scales = key_scales + kPage;
+        const bool seen = any && page * kPage <= last && (p.window <= 0 || page * kPage + kPage - 1 > first - p.window) &&
+                          page_at(table, page, p.b.max_pages, p.pages) >= 0;
+        if (seen) {
+            const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
+            v16f s[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                s[kt] = v16f{};
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    const v8h a = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + lane * 16);
+                    s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], s[kt], 0, 0, 0);
+                    s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], s[kt], 0, 0, 0);
+                }
+            }
+            float x[32], ks[32], vs[32];
+#pragma unroll
+            for (int n = 0; n < 32; n += 4) {
+                const int token = 32 * (n / 16) + 8 * (n % 16 / 4) + 4 * h;
+                const v4f a = *reinterpret_cast<const v4f *>(key_scales + token), c = *reinterpret_cast<const v4f *>(value_scales + token);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    ks[n + r] = a[r];
+                    vs[n + r] = c[r];
+                    x[n + r] = s[n / 16][n % 16 + r];
+                }
+            }
+            const int high = pair.position, low = p.window > 0 ? high - p.window + 1 : 0;
+            weigh<32>(x, ks, vs, f, edge, low, high, sums,
+                      [&](int n) { return page * kPage + 32 * (n / 16) + 8 * (n % 16 / 4) + 4 * h + n % 4; },
+                      [](float a) {
+                          const float2 w = half_pair(a);
+                          return fmaxf(w.x, w.y);
+                      },
+                      [&](float a) {
+#pragma unroll
+                          for (int d = 0; d < T; d++)
+#pragma unroll
+                              for (int r = 0; r < 16; r++) o[d][r] = o[d][r] * a;
+                      });
+            const uint8_t *values = buffer + 128 * DP;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {  // 16 keys: kt = c / 2, e = c % 2
+                v8h wh, wl;
+                split8(x + 8 * c, wh, wl);
+#pragma unroll
+                for (int d = 0; d < T; d++) {
+                    const v8h a = *reinterpret_cast<const v8h *>(values + ((d * 2 + c / 2) * 2 + c % 2) * 1024 + lane * 16);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wl, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wh, o[d], 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const float2 w = half_pair(sums.total);
+    sums.total = w.x + w.y;
+    if (task.nsplit > 1) {
+        float *part = p.partial + ((size_t(task.slot + task.split) * p.kv_heads + kv) * 4 + wave) * (32 * DP + 128);
+        part[lane] = sums.r;
+        part[64 + lane] = sums.total;
+#pragma unroll
+        for (int d = 0; d < T; d++)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                *reinterpret_cast<v4f *>(part + 128 + (d * 4 + c) * 256 + lane * 4) = v4f{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
+        return;
+    }
+    if (!pair.live) return;
+    float *row = p.out + size_t(pair.row) * p.out_stride + size_t(pair.head) * p.head_dim;
+#pragma unroll
+    for (int d = 0; d < T; d++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            v4f x;
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[r] = sums.total == 0.0f ? 0.0f : o[d][4 * c + r] / sums.total;
+            const int dim = 32 * d + 8 * c + 4 * h;
+            if (dim < p.head_dim) *reinterpret_cast<v4f_any *>(row + dim) = x;
+        }
+}
+
+// The parts of split tiles joined: a workgroup per row tile and head, a wave's lanes as the kernels above
+// hold a tile of ROWS pairs; the waves take the tiles' pieces of dimensions in turn.
+template <int DP, int ROWS, int TILES>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p)
+{
+    constexpr int TM = ROWS * TILES, C = ROWS * DP / 256;  // pieces of four dimensions a lane
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kv = int(blockIdx.x % unsigned(p.kv_heads));
+    const Task task = find_task<true>(p, int(blockIdx.x / unsigned(p.kv_heads)), TM);
+    if (task.seq < 0 || task.nsplit == 1 || task.slot + task.nsplit > p.grid) return;  // (the last: starts that fall)
+    constexpr size_t kPart = ROWS * DP + 128;
+    const size_t step = size_t(p.kv_heads) * TILES * kPart;
+    for (int tile = 0; tile < TILES; tile++) {
+        const float *part = p.partial + ((size_t(task.slot) * p.kv_heads + kv) * TILES + tile) * kPart;
+        const Pair pair = pair_of(p, task, kv, task.tile * TM + tile * ROWS + (lane & (ROWS - 1)));
+        float r = -INFINITY;
+        for (int s = 0; s < task.nsplit; s++) r = fmaxf(r, part[s * step + lane]);
+        float total = 0.0f;
+        v4f o[(C + 3) / 4];
+#pragma unroll
+        for (int c = 0; c < (C + 3) / 4; c++) o[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < task.nsplit; s++) {
+            const float *from = part + s * step;
+            const float a = part_factor(from[lane], r);
+            total = total + from[64 + lane] * a;
+#pragma unroll
+            for (int c = 0; c < (C + 3) / 4; c++) {
+                if (4 * c + wave >= C) continue;
+                const v4f x = *reinterpret_cast<const v4f *>(from + 128 + (4 * c + wave) * 256 + lane * 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[c][e] = o[c][e] + x[e] * a;
+            }
+        }
+        if (!pair.live) continue;
+        float *row = p.out + size_t(pair.row) * p.out_stride + size_t(pair.head) * p.head_dim;
+#pragma unroll
+        for (int c = 0; c < (C + 3) / 4; c++) {
+            const int dim = (4 * c + wave) * (256 / ROWS) + 4 * (lane / ROWS);
+            v4f x;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = total == 0.0f ? 0.0f : o[c][e] / total;
+            if (4 * c + wave < C && dim < p.head_dim) *reinterpret_cast<v4f_any *>(row + dim) = x;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------ the host
+
+struct Launch {
+    int tile_rows, tiles;      // pairs of a tile: tile_rows a wave tile, tiles of them
+    size_t grid, row_tiles;    // bounds on the tasks of a head and on its row tiles
+    int target;
+    size_t partial_bytes;
+};
+
+// Workgroups that a step's tasks aim at, all heads together: two a CU.
+constexpr size_t kWorkgroups = 512;
+
+Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
+{
+    Launch l{};
+    const size_t group = heads / c->kv_heads, pairs = b->rows * group, sequences = std::min(b->sequences, b->rows);
+    const bool few = pairs <= 32 * sequences;
+    l.tile_rows = few ? 16 : 32;
+    l.tiles = few ? (pairs > 16 * sequences && c->padded <= 128 ? 2 : 1) : 4;
+    const size_t tm = size_t(l.tile_rows) * l.tiles;
+    l.row_tiles = pairs / tm + sequences;
+    l.grid = l.row_tiles;
+    // tiles enough to fill the chip are not split
+    const size_t target = std::max<size_t>(kWorkgroups / c->kv_heads, 1);
+    if (pairs / tm < target && b->max_pages > size_t(kMinPages)) {
+        l.target = int(target);
+        const size_t most = std::min<size_t>((b->max_pages + kMinPages - 1) / kMinPages, kMaxSplit);
+        l.grid = std::min(l.row_tiles * most, l.row_tiles + target);
+        l.partial_bytes = l.grid * c->kv_heads * l.tiles * (size_t(l.tile_rows) * c->padded + 128) * 4;
+    }
+    return l;
+}
+
+template <int DP>
+int launch_attend(const AttendParams &p, const Launch &l, hipStream_t s)
+{
+    const unsigned grid = unsigned(p.kv_heads * l.grid), tiles = unsigned(p.kv_heads * l.row_tiles);
+    if (l.tiles == 1) {
+        attend_few_kernel<DP, 1><<<grid, 256, 0, s>>>(p);
+        FG_HIP(hipGetLastError());
+        if (l.target) attend_join_kernel<DP, 16, 1><<<tiles, 256, 0, s>>>(p);
+    } else if (l.tiles == 2) {
+        if constexpr (DP <= 128) {
+            attend_few_kernel<DP, 2><<<grid, 256, 0, s>>>(p);
+            FG_HIP(hipGetLastError());
+            if (l.target) attend_join_kernel<DP, 16, 2><<<tiles, 256, 0, s>>>(p);
+        }
+    } else {
+        if (many_lds<DP>() > 64 * 1024) {  // more than the default limit: raised once a device
+            static std::atomic<unsigned long long> raised{0};
+            int device = 0;
+            FG_HIP(hipGetDevice(&device));
+            const unsigned long long bit = 1ull << (device & 63);
+            if (device > 63 || !(raised.load() & bit)) {
+                FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(attend_many_kernel<DP>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, int(many_lds<DP>())));
+                raised.fetch_or(bit);
+            }
+        }
+        attend_many_kernel<DP><<<grid, 256, many_lds<DP>(), s>>>(p);
+        FG_HIP(hipGetLastError());
+        if (l.target) attend_join_kernel<DP, 32, 4><<<tiles, 256, 0, s>>>(p);
+    }
+    FG_HIP(hipGetLastError());
+    return FG_OK;
+}
+
+}  // namespace
+}  // namespace fg
+
+using namespace fg;
+
+extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float *query, size_t query_stride, size_t heads,
+                               float scale, size_t window, float *out, size_t out_stride, void *stream)
+{
+    int rc = check_batch(c, b, "fg_cache_attend");
+    if (rc) return rc;
+    if (!heads || heads % c->kv_heads || heads > 65536)
+        return set_error(FG_ERR_SHAPE, "fg_cache_attend: the heads must be a positive multiple of the cache's, at most 65536");
+    if (!(std::fabs(scale) <= 3.4e38f)) return set_error(FG_ERR_ARG, "fg_cache_attend: the scale must be finite");
+    if (!b->rows || !b->sequences) return FG_OK;
+    if (!query || !out) return set_error(FG_ERR_ARG, "fg_cache_attend: a null query or output");
+    const size_t width = heads * c->head_dim;
+    if (b->rows > 1 && out_stride < width) return set_error(FG_ERR_SHAPE, "fg_cache_attend: a row's heads run past the row stride");
+    if (b->rows * (heads / c->kv_heads) > (size_t(1) << 30))
+        return set_error(FG_ERR_SHAPE, "fg_cache_attend: at most 2^30 rows times heads of a key head");
+    const hipStream_t s = as_stream(stream);
+    const Launch l = plan_launch(c, b, heads);
+    if (l.grid * c->kv_heads > 0x7fffffff) return set_error(FG_ERR_SHAPE, "fg_cache_attend: too many rows");
+    AttendParams p{};
+    p.b = batch_params(b);
+    p.records = c->records;
+    p.pages = c->pages;
+    p.kv_heads = c->kv_heads;
+    p.heads = int(heads);
+    p.group = int(heads) / c->kv_heads;
+    p.head_dim = c->head_dim;
+    p.query = query;
+    p.query_stride = query_stride;
+    p.out = out;
+    p.out_stride = out_stride;
+    p.scale2 = scale * 1.44269504088896340736f;
+    p.window = int(std::min<size_t>(window, INT_MAX));
+    p.grid = int(l.grid);
+    p.target = l.target;
+    void *ws = nullptr;
+    bool owned = false;
+    FG_HIP(stream_scratch(l.partial_bytes, s, &ws, &owned));
+    p.partial = static_cast<float *>(ws);
+    switch (c->padded) {
+    case 32: rc = launch_attend<32>(p, l, s); break;
+    case 64: rc = launch_attend<64>(p, l, s); break;
+    case 96: rc = launch_attend<96>(p, l, s); break;
+    case 128: rc = launch_attend<128>(p, l, s); break;
+    case 192: rc = launch_attend<192>(p, l, s); break;
+    default: rc = launch_attend<256>(p, l, s); break;
+    }
+    if (owned) {
+        const hipError_t e = hipFreeAsync(ws, s);
+        if (rc == FG_OK && e != hipSuccess) rc = check_hip(e, "hipFreeAsync");
+    }
+    return rc;
+}

@@ -2187,6 +2187,11 @@ hipError_t scratch_for(const ProductArgs &a, size_t bytes, hipStream_t s, void *
     return workspace_alloc(ws, bytes, s);
 }
 
+hipError_t stream_scratch(size_t bytes, hipStream_t s, void **ws, bool *owned)
+{
+    return scratch_for(ProductArgs{}, bytes, s, ws, owned);
+}
+
 int launch_t2(const ProductArgs &a, hipStream_t s)
 {
     const fg_table *t = a.t;

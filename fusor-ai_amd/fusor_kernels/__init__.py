@@ -3,7 +3,8 @@
 The names follow the reference crate's public API (kernels/src/lib.rs:22-31): DType, Tensor,
 Table, Matrix, Vector, QuantFormat, QuantizedRows, Quantized, Input, quantize_rows, matmul,
 Linear, project, project_input, project_residual, project_residual_input, conv.project_rows,
-QuantizedMatrix and the constants, and the blocks crate's int8 attention (attention::attend). Every computation runs in the
+QuantizedMatrix and the constants, and the blocks crate's int8 attention (attention::attend). Beside them serving.py has what a
+program of many sequences needs: PagedCache, Batch and sample. Every computation runs in the
 HIP library libfusor_gpu.so through its C ABI (include/fusor_gpu.h); there is no CPU fallback.
 """
 
@@ -16,6 +17,7 @@ from .linear import (COLUMN_ALIGN, NARROW_COLUMN_ALIGN, Ctx, Linear, SharedRows,
 from .matmul import (ROWS_PER_CALL, Input, Quantized, QuantizedMatrix, QuantizedRows, matmul, matmul_dots,
                      quantize_rows)
 from .qwen2 import Qwen2, Shape
+from .serving import PAGE, Batch, PagedCache, sample
 from .tensor import BLOCK, QUAD, TERNARY_GROUP, DType, Matrix, QuantFormat, Table, TableUpload, Tensor, Vector, byte_len
 
 __all__ = [
@@ -25,5 +27,6 @@ __all__ = [
     "QuantizedRows", "QuantizedMatrix", "Quantized", "Input", "quantize_rows", "matmul", "matmul_dots",
     "Linear", "Ctx", "SharedRows", "project", "project_input", "project_residual", "project_residual_input",
     "Patches", "project_rows", "Qwen2", "Shape", "Call", "Operand", "Exponentials", "attend",
+    "PAGE", "Batch", "PagedCache", "sample",
     "Error", "FormatError", "ShapeError", "GpuError", "lib",
 ]

@@ -48,6 +48,14 @@ class FgQwen2Probe(ctypes.Structure):
                 ("scales", _P), ("corrections", _P), ("out", _P)]
 
 
+class FgBatch(ctypes.Structure):
+    _fields_ = [("sequences", _S), ("rows", _S), ("max_pages", _S), ("row_starts", _P), ("lengths", _P), ("pages", _P)]
+
+
+class FgSampling(ctypes.Structure):
+    _fields_ = [("random", _P), ("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P)]
+
+
 # Every symbol include/fusor_gpu.h declares, with its signature.
 SIGNATURES = {
     "fg_last_error": (ctypes.c_char_p, []),
@@ -71,6 +79,12 @@ SIGNATURES = {
     "fg_qmatrix_set_rows": (_I, [_P, _S, _S, _P, _P]),
     "fg_qmatrix_set_block": (_I, [_P, _S, _S, _P, _P]),
     "fg_attend": (_I, [ctypes.POINTER(FgAttention), _P, _P]),
+    "fg_cache_create": (_I, [_S, _S, _S, _P, ctypes.POINTER(_P)]),
+    "fg_cache_free": (_I, [_P]),
+    "fg_cache_write": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
+    "fg_cache_read": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
+    "fg_cache_attend": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _S, _F, _S, _P, _S, _P]),
+    "fg_sample": (_I, [_P, _S, _S, _S, ctypes.POINTER(FgSampling), _P, _P, _P]),
     "fg_quantize_rows": (_I, [_P, _S, _I, _P, _P, _P, _P]),
     "fg_matmul": (_I, [_P, ctypes.POINTER(FgInput), _S, _S, _S, _P, _P, _S, _I, _P]),
     "fg_matmul_noalloc": (_I, [_P, ctypes.POINTER(FgInput), _S, _S, _S, _P, _P, _S, _I, _P]),

@@ -1,0 +1,192 @@
+"""Many sequences at once: a paged 8-bit cache of keys and values, the attention of a step's new
+tokens over it, and the draw of the next tokens.
+
+The reference reads and decodes one sequence over a cache of fixed capacity (transformer.rs:166-219)
+and predicts its most likely token (lm.rs:147-166); these have no counterpart there. Activations are
+float32 device tensors, the arrays that describe a step int32 ones.
+"""
+
+import contextlib
+import ctypes
+import math
+
+from . import _lib
+from ._lib import FgBatch, FgSampling, ShapeError, check, lib, ptr, stream_handle
+
+PAGE = 64  # tokens of a page: FG_CACHE_PAGE
+
+
+@contextlib.contextmanager
+def _on(device, stream):
+    """The tensors' device current, and with `stream` that stream too (outputs are then its own)."""
+    import torch
+    with torch.cuda.device(device):
+        if stream is None:
+            yield
+        else:
+            with torch.cuda.stream(stream):
+                yield
+
+
+def _place(device, stream):
+    import torch
+    if stream is None and torch.cuda.is_initialized() and device.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return _on(device, stream)
+
+
+def _check_ints(name, t, shape):
+    import torch
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+        raise ShapeError(f"{name}: a contiguous int32 device tensor")
+    if shape is not None and list(t.shape) != shape:
+        raise ShapeError(f"{name} of shape {list(t.shape)}, {shape} expected")
+
+
+def _check_heads(name, t, heads, head_dim, device, written):
+    """[rows, heads, head_dim] float32 whose rows are runs of heads * head_dim values."""
+    import torch
+    if t.dtype != torch.float32 or t.device != device:
+        raise ShapeError(f"{name}: a float32 tensor on {device}")
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
+        raise ShapeError(f"{name} of shape {list(t.shape)}, [rows, {heads}, {head_dim}] expected")
+    if t.shape[0] == 0:
+        return
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim):
+        raise ShapeError(f"{name}: a row's heads lie one after the other")
+    if written and t.shape[0] > 1 and t.stride(0) < heads * head_dim:
+        raise ShapeError(f"{name}: its rows overlap")
+
+
+class Batch:
+    """The new tokens of a step's sequences (fg_batch), as int32 device tensors that the kernels read:
+    a captured graph's replay reads what they hold then.
+
+    `row_starts` [sequences + 1]: sequence s has the rows row_starts[s] .. row_starts[s + 1] - 1 of the
+    operands as new tokens (rows that no sequence holds are left alone); `lengths` [sequences]: its
+    tokens, the new ones included; `pages` [sequences, max_pages]: the page of its tokens 64 p on at p.
+    """
+
+    def __init__(self, row_starts, lengths, pages):
+        if pages.dim() != 2:
+            raise ShapeError("pages: [sequences, max_pages]")
+        sequences = pages.shape[0]
+        _check_ints("row_starts", row_starts, [sequences + 1])
+        _check_ints("lengths", lengths, [sequences])
+        _check_ints("pages", pages, None)
+        if not row_starts.device == lengths.device == pages.device:
+            raise ShapeError("a batch's tensors are on one device")
+        self.row_starts, self.lengths, self.pages = row_starts, lengths, pages
+
+    @property
+    def sequences(self):
+        return self.lengths.shape[0]
+
+    def _ffi(self, rows):
+        p = self.pages
+        return FgBatch(p.shape[0], rows, p.shape[1], ptr(self.row_starts), ptr(self.lengths), ptr(p))
+
+
+class PagedCache:
+    """The keys and values of one layer's attention over many sequences (fg_cache): `pages` pages of
+    PAGE tokens for `kv_heads` heads of `head_dim` values (whole quads, at most 256), each token's
+    key and value of a head as int8 levels and one float32 scale."""
+
+    def __init__(self, pages, kv_heads, head_dim, device=None, stream=None):
+        import torch
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ShapeError("a cache is on a GPU")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.pages, self.kv_heads, self.head_dim, self.device = pages, kv_heads, head_dim, device
+        handle = ctypes.c_void_p()
+        with _place(device, stream):
+            check(lib().fg_cache_create(pages, kv_heads, head_dim, stream_handle(), ctypes.byref(handle)))
+        self.handle = handle
+
+    def __del__(self):
+        h = getattr(self, "handle", None)
+        if h is not None and _lib._lib is not None:
+            _lib._lib.fg_cache_free(h)
+            self.handle = None
+
+    def _rows(self, batch, keys, values, written):
+        if batch.pages.device != self.device:
+            raise ShapeError(f"the batch is on {batch.pages.device}, the cache on {self.device}")
+        _check_heads("keys", keys, self.kv_heads, self.head_dim, self.device, written)
+        _check_heads("values", values, self.kv_heads, self.head_dim, self.device, written)
+        if keys.shape[0] != values.shape[0]:
+            raise ShapeError(f"{keys.shape[0]} rows of keys and {values.shape[0]} of values")
+        return batch._ffi(keys.shape[0])
+
+    def write(self, batch, keys, values, stream=None):
+        """The new tokens' `keys` and `values` [rows, kv_heads, head_dim] quantized into their pages
+        (a page that is written to belongs to one sequence)."""
+        fg = self._rows(batch, keys, values, False)
+        with _place(self.device, stream):
+            check(lib().fg_cache_write(self.handle, ctypes.byref(fg), ptr(keys), keys.stride(0), ptr(values),
+                                       values.stride(0), stream_handle()))
+
+    def read(self, batch, keys, values, stream=None):
+        """The same tokens read back into `keys` and `values`: level * scale."""
+        fg = self._rows(batch, keys, values, True)
+        with _place(self.device, stream):
+            check(lib().fg_cache_read(self.handle, ctypes.byref(fg), ptr(keys), keys.stride(0), ptr(values),
+                                      values.stride(0), stream_handle()))
+
+    def attend(self, batch, queries, out=None, scale=None, window=0, stream=None):
+        """The attention of the new tokens' `queries` [rows, heads, head_dim] (their keys and values
+        written before): each token sees its sequence's tokens up to itself, with `window` the last
+        `window` of them. `scale` is 1 / sqrt(head_dim) unless given. A token without a key gives 0;
+        rows of `out` that no sequence holds are left as they are (0 in an `out` made here)."""
+        import torch
+        if batch.pages.device != self.device:
+            raise ShapeError(f"the batch is on {batch.pages.device}, the cache on {self.device}")
+        if queries.dim() != 3:
+            raise ShapeError("queries: [rows, heads, head_dim]")
+        heads = queries.shape[1]
+        _check_heads("queries", queries, heads, self.head_dim, self.device, False)
+        if window < 0:
+            raise ShapeError("a window of at least one token, or 0 for all")
+        with _place(self.device, stream):
+            if out is None:
+                out = torch.zeros(queries.shape, dtype=torch.float32, device=self.device)
+            _check_heads("out", out, heads, self.head_dim, self.device, True)
+            if out.shape[0] != queries.shape[0]:
+                raise ShapeError(f"{queries.shape[0]} rows of queries and {out.shape[0]} of out")
+            fg = batch._ffi(queries.shape[0])
+            check(lib().fg_cache_attend(self.handle, ctypes.byref(fg), ptr(queries), queries.stride(0), heads,
+                                        1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, ptr(out),
+                                        out.stride(0), stream_handle()))
+        return out
+
+
+def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, chances=None, stream=None):
+    """The next token of every row of `logits` [rows, vocab] and its chance (fg_sample), drawn by
+    `random` [rows] in [0, 1). The settings are device tensors [rows]: float32 `temperature` (0: the
+    most likely token), int32 `top_k` (0: no limit), float32 `top_p` (1: no limit) and `min_p` (0: no
+    limit), applied in that order. Returns (tokens int32 [rows], chances float32 [rows])."""
+    import torch
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+        raise ShapeError("logits: a float32 device tensor [rows, vocab]")
+    rows, vocab = logits.shape
+    if rows and vocab > 1 and logits.stride(1) != 1:
+        raise ShapeError("logits: a row's values lie one after the other")
+    given = {"random": (random, torch.float32), "temperature": (temperature, torch.float32), "top_k": (top_k, torch.int32),
+             "top_p": (top_p, torch.float32), "min_p": (min_p, torch.float32), "tokens": (tokens, torch.int32),
+             "chances": (chances, torch.float32)}
+    for name, (t, dtype) in given.items():
+        if t is None and name != "random":
+            continue
+        if t.dtype != dtype or t.device != logits.device or list(t.shape) != [rows] or not t.is_contiguous():
+            raise ShapeError(f"{name}: a contiguous {dtype} tensor [{rows}] on {logits.device}")
+    with _place(logits.device, stream):
+        if tokens is None:
+            tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        if chances is None:
+            chances = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        fg = FgSampling(ptr(random), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p))
+        check(lib().fg_sample(ptr(logits), rows, vocab, logits.stride(0), ctypes.byref(fg), ptr(tokens), ptr(chances),
+                              stream_handle()))
+    return tokens, chances

@@ -166,6 +166,81 @@ typedef struct fg_attention {
  * from and returns to a stream-ordered pool): `out` is ready once the stream's work is. */
 int fg_attend(const fg_attention *call, float *out, void *stream);
 
+/* --------------------------------------------------- many sequences: a cache in pages */
+
+/* The keys and values of one layer's attention over many sequences, in pages of FG_CACHE_PAGE tokens
+ * that a serving program hands out (no counterpart in the reference, whose caches hold one sequence
+ * of fixed capacity). A token's key and value of one head are `head_dim` int8 levels and one f32
+ * scale each: scale = a / 127 for the largest magnitude a (NaN ignored; 1 where a / 127 is 0), level
+ * rint(x / scale) clamped to +-127, NaN to 0 (the rule of quantize_rows with a head for its group).
+ * The handle owns its device memory: pages of zero levels and scales of 1 until written. It belongs
+ * to the device that was current when it was created, and every call on it needs that device
+ * current. Calls on one cache may run at once; their order on the device is the caller's, by streams. */
+typedef struct fg_cache fg_cache;
+#define FG_CACHE_PAGE 64
+
+/* `pages` pages for `kv_heads` heads of `head_dim` values (whole quads, at most 256). Waits for
+ * `stream`, on which the pages are cleared. */
+int fg_cache_create(size_t pages, size_t kv_heads, size_t head_dim, void *stream, fg_cache **out);
+int fg_cache_free(fg_cache *cache);
+
+/* The new tokens of a step's sequences, as device int32 arrays that the kernels read (a captured
+ * graph's replay reads what they hold then):
+ *   row_starts [sequences + 1], not falling: sequence s's new tokens are the rows row_starts[s] ..
+ *              row_starts[s + 1] - 1 of the call's operands, none where the two are equal. Rows that
+ *              no sequence holds (a padded batch's) are not read, and their outputs not written;
+ *   lengths    [sequences]: the sequence's tokens, the new ones included; row r of n new ones is at
+ *              position length - n + r. A row at a negative position has no token: nothing is
+ *              written for it, and its outputs are 0;
+ *   pages      [sequences][max_pages]: page id of the positions 64 p .. 64 p + 63 at p. An id outside
+ *              the cache's pages, like a position past max_pages, holds no tokens: writes to it are
+ *              dropped, reads give 0, attention passes over it.
+ * A page that fg_cache_write writes to belongs to one sequence; pages that are only read may be
+ * shared. */
+typedef struct {
+    size_t sequences; /* at most 65536 */
+    size_t rows;      /* of the operands, at most 2^24 */
+    size_t max_pages; /* at most 2^24 */
+    const int32_t *row_starts, *lengths, *pages;
+} fg_batch;
+
+/* The new tokens' keys and values quantized into the cache. Head h of row r is the head_dim device
+ * f32 values at r * stride + h * head_dim. */
+int fg_cache_write(fg_cache *cache, const fg_batch *batch, const float *key, size_t key_stride, const float *value,
+                   size_t value_stride, void *stream);
+/* The same tokens' keys and values read back as f32, level * scale. */
+int fg_cache_read(const fg_cache *cache, const fg_batch *batch, float *key, size_t key_stride, float *value,
+                  size_t value_stride, void *stream);
+/* The attention of the new tokens' queries (written before this call: a token sees itself): row r at
+ * position p sees its sequence's keys at positions max(0, p - window + 1) .. p, all up to p where
+ * `window` is 0. Head h of row r is the head_dim device f32 values at r * stride + h * head_dim of
+ * `query` and `out`; `heads` query heads share the cache's heads in consecutive runs. Scores are
+ * scale * q.k; a row that sees no key gives 0. The work is ordered on `stream`; scratch as for
+ * fg_matmul, under capture included. */
+int fg_cache_attend(const fg_cache *cache, const fg_batch *batch, const float *query, size_t query_stride, size_t heads,
+                    float scale, size_t window, float *out, size_t out_stride, void *stream);
+
+/* Next tokens drawn from logits (Prediction::predict, lm.rs:147-166, takes the largest). Row r of the
+ * device f32 `logits`, at r * stride, orders its tokens by logit, the largest first, equal ones by
+ * index; NaN counts as -inf. A token's weight is exp((logit - largest) / temperature); -inf weighs 0.
+ * Of the tokens are kept the first top_k; of these the fewest first ones whose weights reach top_p of
+ * these tokens' total; of these the ones that weigh at least min_p of the first. The first is always
+ * kept. The token drawn is the first kept one, by index, whose running total passes random times the
+ * kept total; its chance is its weight over that total. Sums are 64-bit integers: the order in which
+ * they are formed changes nothing. */
+typedef struct {
+    const float *random;      /* device [rows], in [0, 1) */
+    const float *temperature; /* device [rows] or NULL: 1. 0 and less, and NaN: the first token */
+    const int32_t *top_k;     /* device [rows] or NULL: no limit, as 0 and less */
+    const float *top_p;       /* device [rows] or NULL: no limit, as 1 and more, and NaN */
+    const float *min_p;       /* device [rows] or NULL: no limit, as 0 and less, and NaN */
+} fg_sampling;
+
+/* The tokens of `rows` rows of `vocab` logits (at most 2^22) into device `tokens` [rows]; `chances`
+ * [rows] may be NULL. A row with no logit above -inf gives token -1 and chance 0. */
+int fg_sample(const float *logits, size_t rows, size_t vocab, size_t stride, const fg_sampling *settings,
+              int32_t *tokens, float *chances, void *stream);
+
 /* ------------------------------------------------------------------------ activations */
 
 /* quantize_rows (matmul.rs:233-257): `count` device f32 values, whole groups of the weight
