@@ -31,16 +31,17 @@ __device__ __forceinline__ Span sequence_span(const BatchParams &b, int s)
     return span_of(b.row_starts[s], b.row_starts[s + 1], b.lengths[s], b.rows);
 }
 
-// The sum over the wave's lanes up to this one, and over all of them.
+// The sum over the wave's lanes up to this one, and over all of them: within rows of 16 lanes, then
+// each row's last lane to the rows behind it (DPP throughout).
 __device__ __forceinline__ int wave_scan(int v, int *total)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int up = __shfl_up(v, d, 64);
-        if (lane >= d) v += up;
-    }
-    *total = __shfl(v, 63, 64);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15: to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31: to rows 2 and 3
+    *total = __builtin_amdgcn_readlane(v, 63);
     return v;
 }
 
@@ -58,7 +59,7 @@ __device__ __forceinline__ int find_unit(int sequences, int index, int *within, 
         const unsigned long long here = __ballot(index < upto);
         if (here) {
             const int at = __builtin_ctzll(here);
-            *within = index - __shfl(upto - n, at, 64);
+            *within = index - __builtin_amdgcn_readlane(upto - n, at);
             return s0 + at;
         }
         before += total;

@@ -341,7 +341,7 @@ int fg_cache_create(size_t pages, size_t kv_heads, size_t head_dim, void *stream
     int device = 0;
     FG_HIP(hipGetDevice(&device));
     uint8_t *records = nullptr;
-    hipError_t e = hipMalloc(reinterpret_cast<void **>(&records), std::max<size_t>(bytes, 16));
+    hipError_t e = hipMalloc(reinterpret_cast<void **>(&records), std::max(bytes, size_t(record_bytes(padded))));  // (a record to read, at least)
     if (e != hipSuccess) return check_hip(e, "fg_cache_create: hipMalloc");
     if (bytes) {
         const hipStream_t s = as_stream(stream);

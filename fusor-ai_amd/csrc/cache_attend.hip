@@ -14,6 +14,8 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 
+struct Note;
+
 struct AttendParams {
     BatchParams b;
     const uint8_t *records;
@@ -27,6 +29,7 @@ struct AttendParams {
     int grid;      // tasks a head there is room for
     int target;    // tasks a head aims at; 0: no row tile is split
     float *partial;
+    Note *notes;   // [grid]
 };
 
 constexpr int kMaxSplit = 64;   // parts of one row tile
@@ -40,7 +43,7 @@ constexpr int kMinPages = 4;    // pages of a part, a wave each
 // known on the host.
 struct Task {
     int seq, tile, split, nsplit;
-    int slot;  // of the tile's first part, in order over all tasks
+    int slot;  // the task's index
     Span span;
 };
 
@@ -55,20 +58,20 @@ __device__ __forceinline__ int tile_pages(const AttendParams &p, const Span &s, 
     return p.window > 0 ? min(all, (p.window + TM / p.group + 1) / kPage + 2) : all;
 }
 
-// Pages a part takes: the whole work spread over the target.
+// Pages a part takes: the whole work spread over the target (a little more than its share: the sum is
+// in f32).
 __device__ __forceinline__ int part_pages(const AttendParams &p, int TM)
 {
     if (!p.target) return INT_MAX;
     const int lane = threadIdx.x & 63;
-    unsigned long long work = 0;
-    for (int s = lane; s < p.b.sequences; s += 64) {
-        const Span span = sequence_span(p.b, s);
-        work += (unsigned long long)tiles_of(p, span, TM) * tile_pages(p, span, TM);
+    float work = 0.0f;
+    for (int s0 = 0; s0 < p.b.sequences; s0 += 64) {
+        if (s0 + lane >= p.b.sequences) continue;
+        const Span span = sequence_span(p.b, s0 + lane);
+        work = work + float(tiles_of(p, span, TM)) * float(tile_pages(p, span, TM));
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
-    const unsigned long long part = (work + p.target - 1) / p.target;
-    return part < kMinPages ? kMinPages : part > INT_MAX / 2 ? INT_MAX / 2 : int(part);
+    const float part = wave_allsum(work) * 1.00001f / float(p.target) + 1.0f;
+    return __builtin_amdgcn_readfirstlane(part < float(kMinPages) ? kMinPages : part > 1e9f ? 1000000000 : int(part));
 }
 
 __device__ __forceinline__ int splits_of(int pages, int part)
@@ -76,55 +79,45 @@ __device__ __forceinline__ int splits_of(int pages, int part)
     return pages <= part ? 1 : min((pages + part - 1) / part, kMaxSplit);
 }
 
-// The task of index x (TILES: the row tile of index x, its first part), or seq -1.
-template <bool TILES>
+// The task of index x, or seq -1.
 __device__ __forceinline__ Task find_task(const AttendParams &p, int x, int TM)
 {
     const int part = part_pages(p, TM);
-    Task t;
+    Task t{};
     int within;
-    if (!TILES) {
-        t.seq = find_unit(p.b.sequences, x, &within, [&](int s) {
-            const Span span = sequence_span(p.b, s);
-            return tiles_of(p, span, TM) * splits_of(tile_pages(p, span, TM), part);
-        });
-        if (t.seq < 0) return t;
-        t.span = sequence_span(p.b, t.seq);
-        t.nsplit = splits_of(tile_pages(p, t.span, TM), part);
-        // the last tiles see the most keys: they come first
-        t.tile = tiles_of(p, t.span, TM) - 1 - within / t.nsplit;
-        t.split = within % t.nsplit;
-        t.slot = x - t.split;
-        return t;
-    }
-    const int lane = threadIdx.x & 63;
-    int before = 0, slots = 0;
-    t.seq = -1;
-    for (int s0 = 0; s0 < p.b.sequences; s0 += 64) {
-        int tiles = 0, tasks = 0;
-        if (s0 + lane < p.b.sequences) {
-            const Span span = sequence_span(p.b, s0 + lane);
-            tiles = tiles_of(p, span, TM);
-            tasks = tiles * splits_of(tile_pages(p, span, TM), part);
-        }
-        int total, all;
-        const int upto = before + wave_scan(tiles, &total), upto_tasks = slots + wave_scan(tasks, &all);
-        const unsigned long long here = __ballot(x < upto);
-        if (here) {
-            const int at = __builtin_ctzll(here);
-            within = x - __shfl(upto - tiles, at, 64);
-            t.seq = s0 + at;
-            t.span = sequence_span(p.b, t.seq);
-            t.nsplit = splits_of(tile_pages(p, t.span, TM), part);
-            t.tile = tiles_of(p, t.span, TM) - 1 - within;
-            t.split = 0;
-            t.slot = __shfl(upto_tasks - tasks, at, 64) + within * t.nsplit;
-            return t;
-        }
-        before += total;
-        slots += all;
-    }
+    t.seq = find_unit(p.b.sequences, x, &within, [&](int s) {
+        const Span span = sequence_span(p.b, s);
+        return tiles_of(p, span, TM) * splits_of(tile_pages(p, span, TM), part);
+    });
+    if (t.seq < 0) return t;
+    t.span = sequence_span(p.b, t.seq);
+    t.nsplit = splits_of(tile_pages(p, t.span, TM), part);
+    // the last tiles see the most keys: they come first
+    t.tile = tiles_of(p, t.span, TM) - 1 - within / t.nsplit;
+    t.split = within % t.nsplit;
+    t.slot = x;
     return t;
+}
+
+// A task in scalar registers (every wave finds it whole).
+__device__ __forceinline__ Task uniform(Task t)
+{
+    auto same = [](int &x) { x = __builtin_amdgcn_readfirstlane(x); };
+    same(t.seq), same(t.tile), same(t.split), same(t.nsplit), same(t.slot);
+    same(t.span.begin), same(t.span.rows), same(t.span.first), same(t.span.length);
+    return t;
+}
+
+// What the join takes of a task, by its slot: the parts that start here (0: none, or one alone) and the
+// tile's rows. Every workgroup of the grid leaves a note, those without a task too.
+struct Note {
+    int parts, tile, begin, rows, first;
+};
+__device__ __forceinline__ void leave_note(const AttendParams &p, const Task &t, int x, int kv)
+{
+    if (!p.target || kv != 0 || threadIdx.x != 0) return;
+    const bool starts = t.seq >= 0 && t.split == 0 && t.nsplit > 1;
+    p.notes[x] = Note{starts ? t.nsplit : 0, t.tile, t.span.begin, t.span.rows, t.span.first};
 }
 
 // The pages [lo, hi) of a task.
@@ -189,11 +182,23 @@ __device__ __forceinline__ v8h widen8(unsigned a, unsigned b)
 
 __device__ __forceinline__ void split8(const float *x, v8h &hi, v8h &lo)
 {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    union {
+        unsigned u[4];
+        v8h v;
+    } h, l;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        hi[i] = _Float16(x[i]);
-        lo[i] = _Float16(__builtin_fmaf(float(hi[i]), -1.0f, x[i]));
+    for (int i = 0; i < 4; i++) {
+        const v2h top = __builtin_convertvector((v2f{x[2 * i], x[2 * i + 1]}), v2h);
+        h.u[i] = __builtin_bit_cast(unsigned, top);
+        // x - hi, exactly, straight from the packed pair
+        v2f rest;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest.x) : "v"(h.u[i]), "v"(x[2 * i]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest.y) : "v"(h.u[i]), "v"(x[2 * i + 1]));
+        l.u[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, v2h));
     }
+    hi = h.v;
+    lo = l.v;
 }
 
 // Eight query values from dimension d on (0 past the head's).
@@ -222,32 +227,47 @@ struct RowSums {
     float r, total;
 };
 
-// N scores of one row in this lane, t = s · key scale · f, to weights times the values' scales, in
-// place; the row's other scores are in the lanes that COMBINE joins. edge: keys outside [low, high] are
+// N scores of one row in this lane, t = s * f, to weights times the values' scales, into x; the row's other scores are in the lanes that `combine` joins. edge: keys outside [low, high] are
 // masked (key(i) is score i's position). rescale(a) scales the row's sums of this lane by a.
 template <int N, class Key, class Combine, class Rescale>
-__device__ __forceinline__ void weigh(float (&s)[N], const float *ks, const float *vs, float f, bool edge, int low, int high,
-                                      RowSums &sums, Key key, Combine combine, Rescale rescale)
+__device__ __forceinline__ void weigh(const float (&s)[N], float (&x)[N], const float *vs, float f, bool edge, int low,
+                                      int high, RowSums &sums, Key key, Combine combine, Rescale rescale)
 {
-    float t[N];
-    float top = 0.0f;
+    float top = 0.0f, total = 0.0f;
+    auto weights = [&]() {
+        top = total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        t[i] = s[i] * ks[i] * f;
-        const float e = __builtin_amdgcn_exp2f(t[i] - sums.r);
-        float x = e * vs[i];
-        if (edge) x = key(i) >= low && key(i) <= high ? x : 0.0f;
-        s[i] = x;
-        top = fmaxf(top, x);
-    }
-    if (__any(top > kWeightLimit)) {
+        for (int i = 0; i < N; i++) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], f, -sums.r));
+            x[i] = e * vs[i];
+            total = total + e;
+            top = fmaxf(top, x[i]);
+        }
+    };
+    auto masked = [&]() {
+        top = total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const bool seen = key(i) >= low && key(i) <= high;
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], f, -sums.r));
+            x[i] = seen ? e * vs[i] : 0.0f;
+            total = total + (seen ? e : 0.0f);
+            top = fmaxf(top, x[i]);
+        }
+    };
+    if (edge) masked();
+    else weights();
+    if (__builtin_expect(__any(top > kWeightLimit), 0)) {
         top = combine(top);
         float u = -INFINITY, m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < N; i++) {
+            float v = vs[i];
+            asm volatile("" : "+v"(v));  // (keeps the logarithms in this branch)
+            const float t = s[i] * f;
             const bool seen = !edge || (key(i) >= low && key(i) <= high);
-            u = seen ? fmaxf(u, t[i] + __builtin_amdgcn_logf(vs[i])) : u;
-            m = seen ? fmaxf(m, t[i]) : m;
+            u = seen ? fmaxf(u, t + __builtin_amdgcn_logf(v)) : u;
+            m = seen ? fmaxf(m, t) : m;
         }
         u = combine(u);
         m = combine(m);
@@ -259,19 +279,8 @@ __device__ __forceinline__ void weigh(float (&s)[N], const float *ks, const floa
             sums.total = sums.total * a;
             rescale(a);
         }
-    }
-    float total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        float e = __builtin_amdgcn_exp2f(t[i] - sums.r);
-        float x = e * vs[i];
-        if (edge) {
-            const bool seen = key(i) >= low && key(i) <= high;
-            e = seen ? e : 0.0f;
-            x = seen ? x : 0.0f;
-        }
-        s[i] = x;
-        total = total + e;
+        if (edge) masked();
+        else weights();
     }
     sums.total = sums.total + total;
 }
@@ -289,13 +298,14 @@ __device__ __forceinline__ float part_factor(float r, float joined) { return r =
 //            the scores of keys 32 (g / 2) + 8 t + 4 (g % 2) + r, r = 0 .. 3;
 //   values:  16 dimensions by 32 keys: the lane's 16 bytes of dimension l % 16 are those keys', in order.
 template <int DP, int MT>
-__global__ __launch_bounds__(256) void attend_few_kernel(AttendParams p)
+__global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel(AttendParams p)
 {
     constexpr int TM = 16 * MT, J = (DP + 63) / 64, T = DP / 16, R = DP / 32;
     __shared__ __align__(16) float joined[2][MT * (T * 4 + 2)][64];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, kv = int(blockIdx.x % unsigned(p.kv_heads));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Task task = find_task<false>(p, int(blockIdx.x / unsigned(p.kv_heads)), TM);
+    const Task task = uniform(find_task(p, int(blockIdx.x / unsigned(p.kv_heads)), TM));
+    leave_note(p, task, int(blockIdx.x / unsigned(p.kv_heads)), kv);
     if (task.seq < 0) return;  // the whole workgroup
     const PageRange range = task_pages(p, task, TM);
 
@@ -337,12 +347,14 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendParams p)
     const int first = task.span.first + task.tile * TM / p.group;  // positions of the tile's first and last rows
     const int last = task.span.first + min((task.tile * TM + TM - 1) / p.group, task.span.rows - 1);
     const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
-    for (int page = range.lo + wave; page < range.hi; page += 4) {
-        const int id = __builtin_amdgcn_readfirstlane(page_at(table, page, p.b.max_pages, p.pages));
-        if (id < 0) continue;
-        const uint8_t *record = p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP);
-        uint4 k[4][J], v[T];
-        v4f ks[4], vs[4];
+    // A page's levels and scales stay in the same registers as the next one's: the keys' are asked for
+    // when this page's scores are formed, the values' when it is done, the id a page before.
+    uint4 k[4][J], v[T];
+    v4f ks[4], vs[4];
+    auto id_of = [&](int page) { return page < range.hi ? page_at(table, page, p.b.max_pages, p.pages) : -1; };
+    auto record_of = [&](int id) { return p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP); };
+    auto load_keys = [&](int id) {
+        const uint8_t *record = record_of(id);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -351,14 +363,32 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendParams p)
                 k[t][j] = *reinterpret_cast<const uint4 *>(record + ((i >> 3) * R + block) * 1024 + ((g & 1) * 32 + 8 * t + (i & 7)) * 16);
             }
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int token = 32 * (g >> 1) + 8 * t + 4 * (g & 1);
-            ks[t] = *reinterpret_cast<const v4f *>(record + key_scale_byte(DP, token));
-            vs[t] = *reinterpret_cast<const v4f *>(record + value_scale_byte(DP, token));
-        }
+        for (int t = 0; t < 4; t++)
+            ks[t] = *reinterpret_cast<const v4f *>(record + key_scale_byte(DP, 32 * (g >> 1) + 8 * t + 4 * (g & 1)));
+    };
+    auto load_values = [&](int id) {
+        const uint8_t *record = record_of(id);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            vs[t] = *reinterpret_cast<const v4f *>(record + value_scale_byte(DP, 32 * (g >> 1) + 8 * t + 4 * (g & 1)));
 #pragma unroll
         for (int d = 0; d < T; d++)
             v[d] = *reinterpret_cast<const uint4 *>(record + kPage * DP + ((d >> 1) * 2 + (g >> 1)) * 1024 + ((g & 1) * 32 + (d & 1) * 16 + i) * 16);
+    };
+    int id = id_of(range.lo + wave), next = id_of(range.lo + wave + 4), loaded = max(id, 0);
+    load_keys(loaded);
+    load_values(loaded);
+    for (int page = range.lo + wave; page < range.hi; page += 4) {
+        const int after = id_of(page + 8);
+        const bool held = id >= 0;
+        loaded = next >= 0 ? next : loaded;  // (what is loaded already, again, where there is no next one)
+        id = next;
+        next = after;
+        if (!held) {
+            load_keys(loaded);
+            load_values(loaded);
+            continue;
+        }
         v4f s[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
@@ -377,20 +407,26 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendParams p)
                         s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[mt][j][e], s[mt][t], 0, 0, 0);
                     }
                 }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[mt][t][r] = s[mt][t][r] * ks[t][r];
+        load_keys(loaded);
         const int base = page * kPage + 32 * (g >> 1) + 4 * (g & 1);
         const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
         v8h wh[MT][2], wl[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            float x[16], kk[16], vv[16];
+            float scores[16], x[16], vv[16];
 #pragma unroll
             for (int n = 0; n < 16; n++) {
-                x[n] = s[mt][n / 4][n % 4];
-                kk[n] = ks[n / 4][n % 4];
+                scores[n] = s[mt][n / 4][n % 4];
                 vv[n] = vs[n / 4][n % 4];
             }
             const int high = pair[mt].position, low = p.window > 0 ? high - p.window + 1 : 0;
-            weigh<16>(x, kk, vv, f[mt], edge, low, high, sums[mt], [&](int n) { return base + 8 * (n / 4) + n % 4; },
+            weigh<16>(scores, x, vv, f[mt], edge, low, high, sums[mt], [&](int n) { return base + 8 * (n / 4) + n % 4; },
                       [](float a) {
                           float2 w = row_pair(a);
                           w = half_pair(fmaxf(w.x, w.y));
@@ -416,6 +452,7 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendParams p)
                     o[mt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wh[mt][e], o[mt][d], 0, 0, 0);
                 }
             }
+        load_values(loaded);
     }
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
@@ -461,7 +498,7 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendParams p)
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
         if (task.nsplit > 1) {
-            float *part = p.partial + ((size_t(task.slot + task.split) * p.kv_heads + kv) * MT + mt) * (16 * DP + 128);
+            float *part = p.partial + ((size_t(task.slot) * p.kv_heads + kv) * MT + mt) * (16 * DP + 128);
             part[lane] = sums[mt].r;
             part[64 + lane] = sums[mt].total;
 #pragma unroll
@@ -499,15 +536,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     constexpr int kBuffer = 256 * DP + 2 * kPage * 4;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5, kv = int(blockIdx.x % unsigned(p.kv_heads));
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Task task = find_task<false>(p, int(blockIdx.x / unsigned(p.kv_heads)), TM);
+    const Task task = uniform(find_task(p, int(blockIdx.x / unsigned(p.kv_heads)), TM));
+    leave_note(p, task, int(blockIdx.x / unsigned(p.kv_heads)), kv);
     if (task.seq < 0) return;  // the whole workgroup
     const PageRange range = task_pages(p, task, TM);
     const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
 
     uint4 staged[L];
     float staged_scale = 0.0f;
-    auto load = [&](int page) {  // the page's record into registers (nothing where it has none)
-        const int id = page < range.hi ? page_at(table, page, p.b.max_pages, p.pages) : -1;
+    auto id_of = [&](int page) { return page < range.hi ? page_at(table, page, p.b.max_pages, p.pages) : -1; };
+    auto load = [&](int id) {  // a page's record into registers
         if (id < 0) return;
         const uint8_t *record = p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP);
 #pragma unroll
@@ -526,7 +564,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     };
 #pragma unroll
     for (int c = 0; c < L; c++) staged[c] = make_uint4(0, 0, 0, 0);
-    load(range.lo);
+    // the pages read (-1: nothing there), staged, and known
+    int here = id_of(range.lo), next = id_of(range.lo + 1), after = id_of(range.lo + 2);
+    load(here);
 
     const Pair pair = pair_of(p, task, kv, task.tile * TM + wave * 32 + l31);
     v8h qh[K], ql[K];
@@ -561,45 +601,47 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     const bool any = m0 < pairs;
 
     store(lds);
-    load(range.lo + 1);
+    load(next);
     __syncthreads();
     for (int page = range.lo; page < range.hi; page++) {
         const int b = (page - range.lo) & 1;
-        if (page + 1 < range.hi) {
-            store(lds + (b ^ 1) * kBuffer);
-            load(page + 2);
-        }
+        const bool held = here >= 0;
+        if (next >= 0) store(lds + (b ^ 1) * kBuffer);
+        load(after);
+        here = next;
+        next = after;
+        after = id_of(page + 3);
         const uint8_t *buffer = lds + b * kBuffer;
         const float *key_scales = reinterpret_cast<const float *>(buffer + 256 * DP), *value_scales = key_scales + kPage;
-        const bool seen = any && page * kPage <= last && (p.window <= 0 || page * kPage + kPage - 1 > first - p.window) &&
-                          page_at(table, page, p.b.max_pages, p.pages) >= 0;
+        const bool seen = held && any && page * kPage <= last && (p.window <= 0 || page * kPage + kPage - 1 > first - p.window);
         if (seen) {
             const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
             v16f s[2];
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-                s[kt] = v16f{};
+            for (int kt = 0; kt < 2; kt++) s[kt] = v16f{};
 #pragma unroll
-                for (int k = 0; k < K; k++) {
-                    const v8h a = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + lane * 16);
-                    s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], s[kt], 0, 0, 0);
-                    s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], s[kt], 0, 0, 0);
-                }
+            for (int k = 0; k < K; k++) {
+                v8h a[2];
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) a[kt] = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + lane * 16);
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kt], ql[k], s[kt], 0, 0, 0);
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kt], qh[k], s[kt], 0, 0, 0);
             }
-            float x[32], ks[32], vs[32];
+            float scores[32], x[32], vs[32];
 #pragma unroll
             for (int n = 0; n < 32; n += 4) {
                 const int token = 32 * (n / 16) + 8 * (n % 16 / 4) + 4 * h;
                 const v4f a = *reinterpret_cast<const v4f *>(key_scales + token), c = *reinterpret_cast<const v4f *>(value_scales + token);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    ks[n + r] = a[r];
                     vs[n + r] = c[r];
-                    x[n + r] = s[n / 16][n % 16 + r];
+                    scores[n + r] = s[n / 16][n % 16 + r] * a[r];
                 }
             }
             const int high = pair.position, low = p.window > 0 ? high - p.window + 1 : 0;
-            weigh<32>(x, ks, vs, f, edge, low, high, sums,
+            weigh<32>(scores, x, vs, f, edge, low, high, sums,
                       [&](int n) { return page * kPage + 32 * (n / 16) + 8 * (n % 16 / 4) + 4 * h + n % 4; },
                       [](float a) {
                           const float2 w = half_pair(a);
@@ -614,14 +656,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
             const uint8_t *values = buffer + 128 * DP;
 #pragma unroll
             for (int c = 0; c < 4; c++) {  // 16 keys: kt = c / 2, e = c % 2
-                v8h wh, wl;
+                v8h wh, wl, a[T];
                 split8(x + 8 * c, wh, wl);
 #pragma unroll
                 for (int d = 0; d < T; d++) {
-                    const v8h a = *reinterpret_cast<const v8h *>(values + ((d * 2 + c / 2) * 2 + c % 2) * 1024 + lane * 16);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wl, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wh, o[d], 0, 0, 0);
+                    a[d] = *reinterpret_cast<const v8h *>(values + ((d * 2 + c / 2) * 2 + c % 2) * 1024 + lane * 16);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[d], wl, o[d], 0, 0, 0);
                 }
+#pragma unroll
+                for (int d = 0; d < T; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[d], wh, o[d], 0, 0, 0);
             }
         }
         __syncthreads();
@@ -629,7 +672,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     const float2 w = half_pair(sums.total);
     sums.total = w.x + w.y;
     if (task.nsplit > 1) {
-        float *part = p.partial + ((size_t(task.slot + task.split) * p.kv_heads + kv) * 4 + wave) * (32 * DP + 128);
+        float *part = p.partial + ((size_t(task.slot) * p.kv_heads + kv) * 4 + wave) * (32 * DP + 128);
         part[lane] = sums.r;
         part[64 + lane] = sums.total;
 #pragma unroll
@@ -653,58 +696,69 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
         }
 }
 
-// The parts of split tiles joined: a workgroup per row tile and head, a wave's lanes as the kernels above
-// hold a tile of ROWS pairs; the waves take the tiles' pieces of dimensions in turn.
+// The parts of split tiles joined: per slot where a tile's parts start and head, a wave for each tile of
+// ROWS pairs and piece of dimensions (four a lane, the lanes as the kernels above hold them).
 template <int DP, int ROWS, int TILES>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p)
 {
-    constexpr int TM = ROWS * TILES, C = ROWS * DP / 256;  // pieces of four dimensions a lane
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kv = int(blockIdx.x % unsigned(p.kv_heads));
-    const Task task = find_task<true>(p, int(blockIdx.x / unsigned(p.kv_heads)), TM);
-    if (task.seq < 0 || task.nsplit == 1 || task.slot + task.nsplit > p.grid) return;  // (the last: starts that fall)
+    constexpr int TM = ROWS * TILES, C = ROWS * DP / 256;  // pieces
+    const int lane = threadIdx.x & 63, kv = int(blockIdx.x % unsigned(p.kv_heads)), x = int(blockIdx.x / unsigned(p.kv_heads));
+    const int unit = __builtin_amdgcn_readfirstlane(int(blockIdx.y) * 4 + int(threadIdx.x >> 6));
+    const Note note = p.notes[x];
+    const int parts = __builtin_amdgcn_readfirstlane(note.parts);
+    if (parts == 0 || x + parts > p.grid || unit >= TILES * C) return;  // (the second: starts that fall)
+    const int tile = unit / C, c = unit % C;
     constexpr size_t kPart = ROWS * DP + 128;
     const size_t step = size_t(p.kv_heads) * TILES * kPart;
-    for (int tile = 0; tile < TILES; tile++) {
-        const float *part = p.partial + ((size_t(task.slot) * p.kv_heads + kv) * TILES + tile) * kPart;
-        const Pair pair = pair_of(p, task, kv, task.tile * TM + tile * ROWS + (lane & (ROWS - 1)));
-        float r = -INFINITY;
-        for (int s = 0; s < task.nsplit; s++) r = fmaxf(r, part[s * step + lane]);
-        float total = 0.0f;
-        v4f o[(C + 3) / 4];
+    const float *part = p.partial + ((size_t(x) * p.kv_heads + kv) * TILES + tile) * kPart;
+    Task t{};
+    t.span = Span{note.begin, note.rows, note.first, note.first + note.rows};
+    const Pair pair = pair_of(p, t, kv, note.tile * TM + tile * ROWS + (lane & (ROWS - 1)));
+    // eight parts at a time, joined like the waves' sums
+    constexpr int kAhead = 8;
+    float r = -INFINITY, total = 0.0f;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < parts; s0 += kAhead) {
+        float rs[kAhead], totals[kAhead];
+        v4f os[kAhead];
 #pragma unroll
-        for (int c = 0; c < (C + 3) / 4; c++) o[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < task.nsplit; s++) {
-            const float *from = part + s * step;
-            const float a = part_factor(from[lane], r);
-            total = total + from[64 + lane] * a;
-#pragma unroll
-            for (int c = 0; c < (C + 3) / 4; c++) {
-                if (4 * c + wave >= C) continue;
-                const v4f x = *reinterpret_cast<const v4f *>(from + 128 + (4 * c + wave) * 256 + lane * 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[c][e] = o[c][e] + x[e] * a;
-            }
+        for (int i = 0; i < kAhead; i++) {
+            const float *from = part + min(s0 + i, parts - 1) * step;
+            rs[i] = from[lane];
+            totals[i] = from[64 + lane];
+            os[i] = *reinterpret_cast<const v4f *>(from + 128 + c * 256 + lane * 4);
         }
-        if (!pair.live) continue;
-        float *row = p.out + size_t(pair.row) * p.out_stride + size_t(pair.head) * p.head_dim;
+        float top = r;
 #pragma unroll
-        for (int c = 0; c < (C + 3) / 4; c++) {
-            const int dim = (4 * c + wave) * (256 / ROWS) + 4 * (lane / ROWS);
-            v4f x;
+        for (int i = 0; i < kAhead; i++) top = s0 + i < parts ? fmaxf(top, rs[i]) : top;
+        const float a = part_factor(r, top);
+        r = top;
+        total = total * a;
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = total == 0.0f ? 0.0f : o[c][e] / total;
-            if (4 * c + wave < C && dim < p.head_dim) *reinterpret_cast<v4f_any *>(row + dim) = x;
+        for (int e = 0; e < 4; e++) o[e] = o[e] * a;
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            if (s0 + i >= parts) continue;
+            const float b = part_factor(rs[i], top);
+            total = total + totals[i] * b;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = o[e] + os[i][e] * b;
         }
     }
+    const int dim = c * (256 / ROWS) + 4 * (lane / ROWS);
+    if (!pair.live || dim >= p.head_dim) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = total == 0.0f ? 0.0f : o[e] / total;
+    *reinterpret_cast<v4f_any *>(p.out + size_t(pair.row) * p.out_stride + size_t(pair.head) * p.head_dim + dim) = o;
 }
 
 // ------------------------------------------------------------------------------ the host
 
 struct Launch {
     int tile_rows, tiles;      // pairs of a tile: tile_rows a wave tile, tiles of them
-    size_t grid, row_tiles;    // bounds on the tasks of a head and on its row tiles
+    size_t grid;               // a bound on the tasks of a head
     int target;
-    size_t partial_bytes;
+    size_t note_bytes, partial_bytes;
 };
 
 // Workgroups that a step's tasks aim at, all heads together: two a CU.
@@ -718,14 +772,14 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
     l.tile_rows = few ? 16 : 32;
     l.tiles = few ? (pairs > 16 * sequences && c->padded <= 128 ? 2 : 1) : 4;
     const size_t tm = size_t(l.tile_rows) * l.tiles;
-    l.row_tiles = pairs / tm + sequences;
-    l.grid = l.row_tiles;
-    // tiles enough to fill the chip are not split
-    const size_t target = std::max<size_t>(kWorkgroups / c->kv_heads, 1);
-    if (pairs / tm < target && b->max_pages > size_t(kMinPages)) {
-        l.target = int(target);
+    const size_t row_tiles = pairs / tm + sequences, slots = std::max<size_t>(kWorkgroups / c->kv_heads, 2);
+    l.grid = row_tiles;
+    // fewer tiles than the chip takes at once: their pages are split so that all tasks run at once
+    if (pairs / tm < slots / 2 && b->max_pages > size_t(kMinPages)) {
+        l.target = int(slots - std::min(row_tiles, slots / 2));
         const size_t most = std::min<size_t>((b->max_pages + kMinPages - 1) / kMinPages, kMaxSplit);
-        l.grid = std::min(l.row_tiles * most, l.row_tiles + target);
+        l.grid = std::min(row_tiles * most, row_tiles + l.target);
+        l.note_bytes = (l.grid * sizeof(Note) + 255) / 256 * 256;
         l.partial_bytes = l.grid * c->kv_heads * l.tiles * (size_t(l.tile_rows) * c->padded + 128) * 4;
     }
     return l;
@@ -734,16 +788,17 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
 template <int DP>
 int launch_attend(const AttendParams &p, const Launch &l, hipStream_t s)
 {
-    const unsigned grid = unsigned(p.kv_heads * l.grid), tiles = unsigned(p.kv_heads * l.row_tiles);
+    const unsigned grid = unsigned(p.kv_heads * l.grid);
+    const dim3 pieces(grid, unsigned((l.tiles * l.tile_rows * DP / 256 + 3) / 4));
     if (l.tiles == 1) {
         attend_few_kernel<DP, 1><<<grid, 256, 0, s>>>(p);
         FG_HIP(hipGetLastError());
-        if (l.target) attend_join_kernel<DP, 16, 1><<<tiles, 256, 0, s>>>(p);
+        if (l.target) attend_join_kernel<DP, 16, 1><<<pieces, 256, 0, s>>>(p);
     } else if (l.tiles == 2) {
         if constexpr (DP <= 128) {
             attend_few_kernel<DP, 2><<<grid, 256, 0, s>>>(p);
             FG_HIP(hipGetLastError());
-            if (l.target) attend_join_kernel<DP, 16, 2><<<tiles, 256, 0, s>>>(p);
+            if (l.target) attend_join_kernel<DP, 16, 2><<<pieces, 256, 0, s>>>(p);
         }
     } else {
         if (many_lds<DP>() > 64 * 1024) {  // more than the default limit: raised once a device
@@ -759,7 +814,7 @@ int launch_attend(const AttendParams &p, const Launch &l, hipStream_t s)
         }
         attend_many_kernel<DP><<<grid, 256, many_lds<DP>(), s>>>(p);
         FG_HIP(hipGetLastError());
-        if (l.target) attend_join_kernel<DP, 32, 4><<<tiles, 256, 0, s>>>(p);
+        if (l.target) attend_join_kernel<DP, 32, 4><<<pieces, 256, 0, s>>>(p);
     }
     FG_HIP(hipGetLastError());
     return FG_OK;
@@ -805,8 +860,9 @@ extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float
     p.target = l.target;
     void *ws = nullptr;
     bool owned = false;
-    FG_HIP(stream_scratch(l.partial_bytes, s, &ws, &owned));
-    p.partial = static_cast<float *>(ws);
+    FG_HIP(stream_scratch(l.note_bytes + l.partial_bytes, s, &ws, &owned));
+    p.notes = static_cast<Note *>(ws);
+    p.partial = reinterpret_cast<float *>(static_cast<char *>(ws) + l.note_bytes);
     switch (c->padded) {
     case 32: rc = launch_attend<32>(p, l, s); break;
     case 64: rc = launch_attend<64>(p, l, s); break;
