@@ -5,18 +5,15 @@
 // it: the weights' logarithms z = (logit - largest) / temperature are counted and summed in kBins bins of
 // 1/32, the bin of a cut follows from the running sums, and only that bin's tokens are looked at one by one.
 //   1 top      the largest logit of each chunk of the row, and its first index;
-//   2 bins     the tokens and the weight of every bin;
-//   3 collect  from the bins: which are kept whole, and which hold a cut. The kept weight of each segment
-//              (a wave's run of the row), and a list of the tokens whose bins hold a cut (or of all
-//              tokens up to the cut, where they are few);
-//   4 draw     the cut among the list; the segment, or the listed token, on which the random number falls.
+//   2 bins     the tokens and the weight of every bin, chunk by chunk;
+//   3 cut      from the bins, which are kept whole and which hold a cut, and the logits between them;
+//   4 collect  a list of the tokens whose bins hold a cut (or of all tokens up to it, where they are few);
+//   5 draw     the cut among the list; the chunk, or the listed token, on which the random number falls.
 // Weights are 64-bit: exp in f64 (one ulp), rounded to a whole number of units of 2^-45 of the first token's
 // (less for more than 2^18 tokens), so that every sum is exact and their order changes nothing. Tokens
 // under half a unit (z < -31.9) weigh 0; the last bin holds only such.
-// Bound: the row is read three times, the first from memory and the others mostly from the caches (rows are
-// taken in batches that fit the Infinity Cache), and twice about 25 f64 operations for a weight.
 #include <algorithm>
-#include <atomic>
+#include <type_traits>
 
 #include "cache.h"
 
@@ -26,23 +23,38 @@ namespace {
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned long long u64;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 1024;      // of the kernels that walk a row, and of the draw
+constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 1024;
 constexpr float kPerUnit = 32.0f;   // bins a unit of z
-constexpr int kList = 3584;         // tokens a row's list holds
-constexpr int kMaxChunks = 64;      // workgroups of a row; four segments each
+constexpr int kList = 3072;         // tokens a row's list holds
+constexpr int kFew = 1024;          // up to so many tokens before the cut are all listed
+constexpr int kMaxChunks = 16;      // workgroups of a row
+constexpr int kCutThreads = 256;
+
+// What the bins say of a row. Tokens of bins under `low` are kept whole; those of [low, high] and of
+// `last` are listed; the others are not kept. last: the bin of top-k's cut (kBins: none).
+struct Cut {
+    int low, high, last;
+    unsigned before_last;     // tokens of the bins under `last`
+    u64 mass_last, mass_low;  // weight of the bins under `last`, under `low`
+    // the smallest logits of the bins up to low - 1, high, last - 1 and last (NaN: of none)
+    float whole, listed, before, tie;
+    int lists, by_p;          // whether any bin is listed, and whether top-p's cut is in one
+};
 
 struct SampleParams {
     const float *logits;
     size_t stride;
-    int vocab, chunks, segment;  // segment: tokens of a wave
+    int vocab, chunks, chunk;    // chunk: tokens of a workgroup, whole runs of 256
     const float *random, *temperature, *top_p, *min_p;
     const int32_t *top_k;
     double unit;                 // units of the first token's weight, a power of two
     u64 *top;                    // [rows][chunks]: (ordered logit, ~index)
-    u64 *mass;                   // [rows][kBins]
-    unsigned *count;             // [rows][kBins]
-    u64 *segments;               // [rows][chunks * 4]
+    u64 *mass;                   // [rows][chunks][kBins]
+    unsigned *count;             // [rows][chunks][kBins], where top_k asks
+    u64 *whole;                  // [rows][chunks]: weight of a chunk's tokens kept whole
+    Cut *cuts;                   // [rows]
     unsigned *listed;            // [rows]: tokens of the list (past kList: not all are in it)
     u64 *list;                   // [rows][kList]: (logit bits, index)
     int32_t *tokens;
@@ -74,7 +86,7 @@ __device__ __forceinline__ Row row_of(const SampleParams &p, int row)
     r.has_k = r.top_k > 0 && r.top_k < p.vocab;
     r.has_p = tp < 1.0f;
     r.top_p = tp;
-    r.min_p = mp;
+    r.min_p = mp > 0.0f ? mp : 0.0f;
     r.greedy = !(t > 0.0f) || r.top_k == 1 || tp <= 0.0f || mp > 1.0f;
     r.inverse = 1.0 / double(t);
     return r;
@@ -119,85 +131,108 @@ __device__ __forceinline__ int bin_of(double z)
     return b < float(kBins - 1) ? int(b) : kBins - 1;
 }
 
-__device__ __forceinline__ u64 wave_sum(u64 v)
+// 64-bit sums over the wave's lanes up to this one (DPP: rows of 16, then their last lanes).
+__device__ __forceinline__ u64 wave_upto(u64 v)
 {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    auto step = [&](auto control, auto rows) {
+        const unsigned lo = __builtin_amdgcn_update_dpp(0, int(unsigned(v)), decltype(control)::value, decltype(rows)::value, 0xF, false);
+        const unsigned hi = __builtin_amdgcn_update_dpp(0, int(unsigned(v >> 32)), decltype(control)::value, decltype(rows)::value, 0xF, false);
+        v += u64(hi) << 32 | lo;
+    };
+    using All = std::integral_constant<int, 0xF>;
+    step(std::integral_constant<int, 0x111>{}, All{});
+    step(std::integral_constant<int, 0x112>{}, All{});
+    step(std::integral_constant<int, 0x114>{}, All{});
+    step(std::integral_constant<int, 0x118>{}, All{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
     return v;
 }
+__device__ __forceinline__ u64 lane_of(u64 v, int lane)
+{
+    return u64(unsigned(__builtin_amdgcn_readlane(int(unsigned(v >> 32)), lane))) << 32 |
+           unsigned(__builtin_amdgcn_readlane(int(unsigned(v)), lane));
+}
 
-// The workgroup's sum of a value before this thread's, and of all. `part` is LDS of four; every thread calls.
+// The workgroup's sum of a value before this thread's, and of all. `part` is LDS of a value a wave; every
+// thread calls.
+template <int WAVES>
 __device__ __forceinline__ u64 block_before(u64 v, u64 *part, u64 *total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u64 x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 up = __shfl_up(x, d, 64);
-        if (lane >= d) x += up;
-    }
+    const u64 x = wave_upto(v);
     __syncthreads();
     if (lane == 63) part[wave] = x;
     __syncthreads();
-    u64 before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) {
-        if (w < wave) before += part[w];
-        all += part[w];
-    }
-    *total = all;
-    return before + x - v;
+    const u64 sums = wave_upto(lane < WAVES ? part[lane] : 0);
+    *total = lane_of(sums, WAVES - 1);
+    return x - v + (wave ? lane_of(sums, __builtin_amdgcn_readfirstlane(wave) - 1) : 0);
 }
 
-// The row's largest logit from its chunks', (ordered logit, ~index); every wave of the workgroup by itself.
+// The row's largest logit from its chunks', (ordered logit, ~index); every wave by itself.
 __device__ __forceinline__ u64 row_top(const SampleParams &p, int row)
 {
     const int lane = threadIdx.x & 63;
-    u64 t = lane < p.chunks ? p.top[size_t(row) * p.chunks + lane] : 0;
+    u64 t = p.top[size_t(row) * p.chunks + min(lane & 15, p.chunks - 1)];
 #pragma unroll
-    for (int d = 32; d; d >>= 1) {
+    for (int d = 8; d; d >>= 1) {
         const u64 o = __shfl_xor(t, d, 64);
         t = o > t ? o : t;
     }
     return t;
 }
 
-// Calls f(logit, index) for this wave's segment, in runs of 256 tokens, four a lane.
+// Calls f(logit, index) for the tokens [begin, end) of a row, four a thread of `threads`; the loads of
+// several runs are asked for together.
 template <class F>
-__device__ __forceinline__ void for_segment(const SampleParams &p, int row, int segment, F f)
+__device__ __forceinline__ void for_tokens(const float *x, int begin, int end, int thread, int threads, F f)
 {
-    const float *x = p.logits + size_t(row) * p.stride;
-    const int lane = threadIdx.x & 63;
-    const int begin = segment * p.segment, end = min(begin + p.segment, p.vocab);  // (segments past the row: empty)
-    int i = begin + lane * 4;
     constexpr int kAhead = 4;
-    for (; i + (kAhead - 1) * 256 + 4 <= end; i += kAhead * 256) {
+    int i = begin + thread * 4;
+    for (; i + (kAhead - 1) * threads * 4 + 4 <= end; i += kAhead * threads * 4) {
         v4f v[kAhead];
 #pragma unroll
-        for (int a = 0; a < kAhead; a++) v[a] = *reinterpret_cast<const v4f_any *>(x + i + a * 256);
+        for (int a = 0; a < kAhead; a++) v[a] = *reinterpret_cast<const v4f_any *>(x + i + a * threads * 4);
 #pragma unroll
         for (int a = 0; a < kAhead; a++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) f(plain_logit(v[a][j]), i + a * 256 + j);
+            for (int j = 0; j < 4; j++) f(plain_logit(v[a][j]), i + a * threads * 4 + j);
     }
-    for (; i < end; i += 256)
-        for (int j = 0; j < 4 && i + j < end; j++) f(plain_logit(x[i + j]), i + j);
+    for (; i < end; i += threads * 4) {
+        if (i + 4 <= end) {
+            const v4f v = *reinterpret_cast<const v4f_any *>(x + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) f(plain_logit(v[j]), i + j);
+        } else {
+            for (int j = 0; i + j < end; j++) f(plain_logit(x[i + j]), i + j);
+        }
+    }
+}
+
+// The workgroup's row and chunk, and the chunk's tokens.
+struct Place {
+    int row, chunk, begin, end;
+    const float *x;
+};
+__device__ __forceinline__ Place place_of(const SampleParams &p)
+{
+    Place a;
+    a.row = int(blockIdx.x / unsigned(p.chunks));
+    a.chunk = int(blockIdx.x % unsigned(p.chunks));
+    a.begin = min(a.chunk * p.chunk, p.vocab);
+    a.end = min(a.begin + p.chunk, p.vocab);
+    a.x = p.logits + size_t(a.row) * p.stride;
+    return a;
 }
 
 __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleParams p)
 {
-    __shared__ u64 tops[kThreads / 64];
-    const int row = int(blockIdx.x / unsigned(p.chunks)), chunk = int(blockIdx.x % unsigned(p.chunks));
-    const int wave = threadIdx.x >> 6;
-    // the row's bins start at nothing
-    for (int i = chunk * kThreads + int(threadIdx.x); i < kBins; i += p.chunks * kThreads) {
-        p.mass[size_t(row) * kBins + i] = 0;
-        p.count[size_t(row) * kBins + i] = 0;
-    }
-    if (chunk == 0 && threadIdx.x == 0) p.listed[row] = 0;
+    __shared__ u64 tops[kWaves];
+    const Place a = place_of(p);
+    if (a.chunk == 0 && threadIdx.x == 0) p.listed[a.row] = 0;
     float best = -INFINITY;
     int at = p.vocab;
-    for_segment(p, row, chunk * 4 + wave, [&](float x, int i) {
+    for_tokens(a.x, a.begin, a.end, threadIdx.x, kThreads, [&](float x, int i) {
         if (x > best) {
             best = x;
             at = i;
@@ -209,11 +244,11 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleParams p)
         const u64 o = __shfl_xor(t, d, 64);
         t = o > t ? o : t;
     }
-    if ((threadIdx.x & 63) == 0) tops[wave] = t;
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = t;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 64; w++) t = tops[w] > t ? tops[w] : t;
-        p.top[size_t(row) * p.chunks + chunk] = t;
+        for (int w = 1; w < kWaves; w++) t = tops[w] > t ? tops[w] : t;
+        p.top[size_t(a.row) * p.chunks + a.chunk] = t;
     }
 }
 
@@ -221,71 +256,92 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams p)
 {
     __shared__ u64 mass[kBins];
     __shared__ unsigned count[kBins];
-    const int row = int(blockIdx.x / unsigned(p.chunks)), chunk = int(blockIdx.x % unsigned(p.chunks));
-    const Row r = row_of(p, row);
-    const float top = unordered(unsigned(row_top(p, row) >> 32));
-    if (r.greedy || top == -INFINITY || !(r.has_k || r.has_p)) return;  // the whole workgroup
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        mass[i] = 0;
-        count[i] = 0;
-    }
+    const Place a = place_of(p);
+    const Row r = row_of(p, a.row);
+    const float top = unordered(unsigned(row_top(p, a.row) >> 32));
+    if (r.greedy || top == -INFINITY) return;  // the whole workgroup
+    const int tid = threadIdx.x;
+    static_assert(kBins == kThreads, "a bin a thread");
+    mass[tid] = 0;
+    count[tid] = 0;
     __syncthreads();
-    for_segment(p, row, chunk * 4 + (threadIdx.x >> 6), [&](float x, int) {
+    for_tokens(a.x, a.begin, a.end, tid, kThreads, [&](float x, int) {
         const double z = z_of(x, top, r.inverse);
         const int b = bin_of(z);
         if (b == kBins - 1) return;  // weighs 0
-        atomicAdd(&count[b], 1u);
-        if (r.has_p) atomicAdd(&mass[b], units_of(weight_of(z), p.unit));
+        if (r.has_k) atomicAdd(&count[b], 1u);
+        atomicAdd(&mass[b], units_of(weight_of(z), p.unit));
     });
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        if (count[i] == 0) continue;
-        atomicAdd(&p.count[size_t(row) * kBins + i], count[i]);
-        if (r.has_p) atomicAdd(&p.mass[size_t(row) * kBins + i], mass[i]);
-    }
+    const size_t at = (size_t(a.row) * p.chunks + a.chunk) * kBins + tid;
+    p.mass[at] = mass[tid];
+    if (r.has_k) p.count[at] = count[tid];
 }
 
-// What the bins say. Tokens of bins under `low` are kept but for min-p; those of [low, high] and of `last`
-// are listed; the others are not kept. last: the bin of top-k's cut (kBins: none, and then all tokens that
-// weigh anything are in the first `kBins - 1` bins).
-struct Cut {
-    int low, high, last;
-    unsigned before_last;      // tokens of the bins under `last`
-    u64 mass_last, mass_low;   // weight of the bins under `last`, under `low`
-};
 struct CutShared {
-    u64 part[4];
+    u64 part[kCutThreads / 64];
     int last, low, high;
     unsigned before_last, upto;
     u64 mass_last, mass_after, mass_low;
+    u64 whole[kMaxChunks];
+    float edge[4];
 };
 
-__device__ Cut cut_of(const SampleParams &p, int row, const Row &r, CutShared &sh)
+// The smallest logit whose bin is at most b, by halving the order of floats 64 ways at a time.
+__device__ __forceinline__ float smallest_of_bin(int b, float top, double inverse)
 {
-    Cut c{kBins, kBins, kBins, 0, 0, 0};
-    if (!(r.has_k || r.has_p)) {
-        c.high = -1;
-        return c;
+    if (b >= kBins - 1) return -INFINITY;
+    if (b < 0) return __builtin_nanf("");  // nothing is >= NaN
+    const int lane = threadIdx.x & 63;
+    unsigned lo = 0, n = ordered(top);  // the answer is in (lo, lo + n]; ordered(top) has bin 0
+    while (n > 1) {
+        const unsigned step = (n + 63) / 64, at = lo + (lane + 1) * step;
+        const bool inside = u64(lane + 1) * step <= n;
+        const float x = plain_logit(unordered(inside ? at : lo + n));
+        const bool yes = bin_of(z_of(x, top, inverse)) <= b && x > -INFINITY;
+        const int k = __builtin_ctzll(__ballot(yes || !inside) | 1ull << 63);
+        const unsigned from = lo + unsigned(k) * step, to = lo + n;
+        lo = from;
+        n = min(step, to - from);
     }
-    const int tid = threadIdx.x;
-    constexpr int kEach = kBins / kThreads;
-    u64 n[kEach], m[kEach], here_n = 0, here_m = 0, all_n, all_m;
+    return unordered(lo + n);
+}
+
+// One workgroup a row: its bins summed over the chunks, four a thread.
+__global__ __launch_bounds__(kCutThreads) void sample_cut_kernel(SampleParams p)
+{
+    __shared__ CutShared sh;
+    const int row = int(blockIdx.x), tid = threadIdx.x;
+    const Row r = row_of(p, row);
+    const float top = unordered(unsigned(row_top(p, row) >> 32));
+    if (r.greedy || top == -INFINITY) return;
+    constexpr int kEach = kBins / kCutThreads;
+    u64 n[kEach] = {}, m[kEach] = {}, here_n = 0, here_m = 0, all_n = 0, all_m, before_n = 0;
+    const u64 *mass = p.mass + size_t(row) * p.chunks * kBins + tid * kEach;
+    for (int c = 0; c < p.chunks; c++) {
+        if (r.has_k) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p.count + (size_t(row) * p.chunks + c) * kBins + tid * kEach);
+            n[0] += v.x, n[1] += v.y, n[2] += v.z, n[3] += v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; i++) m[i] += mass[size_t(c) * kBins + i];
+    }
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
-        n[i] = p.count[size_t(row) * kBins + tid * kEach + i];
-        m[i] = p.mass[size_t(row) * kBins + tid * kEach + i];
         here_n += n[i];
         here_m += m[i];
     }
-    const u64 before_n = block_before(here_n, sh.part, &all_n), before_m = block_before(here_m, sh.part, &all_m);
+    const u64 before_m = block_before<kCutThreads / 64>(here_m, sh.part, &all_m);
+    if (r.has_k) before_n = block_before<kCutThreads / 64>(here_n, sh.part, &all_n);
     __syncthreads();
     if (tid == 0) {
         sh.last = kBins;
         sh.low = sh.high = kBins - 1;
         sh.mass_last = sh.mass_after = all_m;
-        sh.before_last = sh.upto = unsigned(all_n);
-        sh.mass_low = 0;
+        sh.before_last = 0;
+        sh.mass_low = all_m;
     }
+    if (tid < kMaxChunks) sh.whole[tid] = 0;
     __syncthreads();
     if (r.has_k && u64(r.top_k) < all_n) {  // (else every token that weighs anything is among the first top_k)
         u64 a = before_n, b = before_m;
@@ -294,7 +350,6 @@ __device__ Cut cut_of(const SampleParams &p, int row, const Row &r, CutShared &s
             if (a < u64(r.top_k) && a + n[i] >= u64(r.top_k)) {
                 sh.last = tid * kEach + i;
                 sh.before_last = unsigned(a);
-                sh.upto = unsigned(a + n[i]);
                 sh.mass_last = b;
                 sh.mass_after = b + m[i];
             }
@@ -303,9 +358,7 @@ __device__ Cut cut_of(const SampleParams &p, int row, const Row &r, CutShared &s
         }
     }
     __syncthreads();
-    c.last = sh.last;
-    c.before_last = sh.before_last;
-    c.mass_last = sh.mass_last;
+    Cut c{kBins, -1, sh.last, sh.before_last, sh.mass_last, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0, r.has_p};
     if (r.has_p) {
         // the cut's bin, for a total between the weight under `last` and that up to it
         const double least = double(r.top_p) * double(sh.mass_last) * (1.0 - 0x1p-50);
@@ -313,76 +366,117 @@ __device__ Cut cut_of(const SampleParams &p, int row, const Row &r, CutShared &s
         u64 b = before_m;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            if (n[i]) {
-                if (double(b) < least && double(b + m[i]) >= least) sh.low = tid * kEach + i;
-                if (double(b) < most && double(b + m[i]) >= most) sh.high = tid * kEach + i;
-                if (b == 0 && least <= 0.0) sh.low = 0;
+            if (m[i]) {
+                if ((b == 0 || double(b) < least) && double(b + m[i]) >= least) sh.low = tid * kEach + i;
+                if ((b == 0 || double(b) < most) && double(b + m[i]) >= most) sh.high = tid * kEach + i;
             }
             b += m[i];
         }
         __syncthreads();
-        c.low = sh.low;
-        c.high = max(sh.high, sh.low);
-        if (c.last < kBins) {
-            c.high = min(c.high, c.last);
-            c.low = min(c.low, c.high);
-        }
-    } else {
+        c.high = min(max(sh.high, sh.low), c.last);
+        c.low = min(sh.low, c.high);
+    } else if (c.last < kBins) {
         c.low = c.high = c.last;
-        if (c.last == kBins) c.high = -1;  // top_k of more tokens than weigh anything
     }
-    // few tokens up to the last listed bin: all of them are listed
-    const int end = c.last < kBins ? c.last : c.high;
-    if (end >= 0 && end < kBins) {
+    if (r.min_p > 0.0f) {
+        // min-p's cut is in the bins of ln(min_p), to more than the rounding of weights
+        const double z = log(double(r.min_p));
+        const int first = bin_of(z + 1e-9 < 0.0 ? z + 1e-9 : 0.0), last = bin_of(z - 1e-9);
+        if (last < c.low) {  // before any other cut: the others change nothing
+            c.low = first;
+            c.high = last;
+            c.last = kBins;
+            c.by_p = 0;
+        } else if (first <= c.high) {
+            c.low = min(c.low, first);
+        }
+    }
+    const bool lists = c.high >= 0;
+    if (lists) {
+        c.high = min(c.high, kBins - 2);  // (the last bin's tokens weigh 0)
+        c.low = min(c.low, c.high);
+    }
+    __syncthreads();
+    u64 b = before_m;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        if (tid * kEach + i == c.low) sh.mass_low = b;
+        b += m[i];
+    }
+    __syncthreads();
+    c.mass_low = sh.mass_low;
+    c.lists = lists;
+    // few tokens up to the last listed bin (counted only under top-k, which is what leaves few): all are listed
+    if (lists && r.has_k && c.last < kBins) {
+        if (tid == 0) sh.upto = 0;
+        __syncthreads();
         u64 a = before_n;
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
             a += n[i];
-            if (tid * kEach + i == end) sh.upto = unsigned(a);
+            if (tid * kEach + i == c.last) sh.upto = unsigned(a);
         }
         __syncthreads();
-        if (sh.upto <= unsigned(kList)) {
+        if (sh.upto <= unsigned(kFew)) {
             c.low = 0;
-            c.high = end;
+            c.high = c.last;
+            c.mass_low = 0;
         }
-        u64 b = before_m;
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            if (tid * kEach + i == c.low) sh.mass_low = b;
-            b += m[i];
-        }
-        __syncthreads();
-        c.mass_low = sh.mass_low;
     }
-    return c;
+    // the chunks' weight under `low`
+    if (c.low > 0) {
+        for (int k = 0; k < p.chunks; k++) {
+            u64 w = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; i++) w += tid * kEach + i < c.low ? mass[size_t(k) * kBins + i] : 0;
+            w = wave_upto(w);
+            if ((tid & 63) == 63) atomicAdd(&sh.whole[k], w);
+        }
+    }
+    const int wave = tid >> 6;
+    const int edge = wave == 0 ? c.low - 1 : wave == 1 ? c.high : wave == 2 ? c.last - 1 : c.last;
+    if (lists) {
+        const float x = smallest_of_bin(edge, top, r.inverse);
+        if ((tid & 63) == 0) sh.edge[wave] = x;
+    }
+    __syncthreads();
+    if (tid < p.chunks) p.whole[size_t(row) * p.chunks + tid] = sh.whole[tid];
+    if (tid == 0) {
+        c.whole = sh.edge[0];
+        c.listed = sh.edge[1];
+        c.before = sh.edge[2];
+        c.tie = c.last < kBins ? sh.edge[3] : __builtin_nanf("");
+        p.cuts[row] = c;
+    }
 }
 
 __device__ __forceinline__ bool is_listed(const Cut &c, int bin) { return (bin >= c.low && bin <= c.high) || bin == c.last; }
 
 __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleParams p)
 {
-    __shared__ CutShared sh;
-    const int row = int(blockIdx.x / unsigned(p.chunks)), chunk = int(blockIdx.x % unsigned(p.chunks));
-    const Row r = row_of(p, row);
-    const float top = unordered(unsigned(row_top(p, row) >> 32));
+    __shared__ u64 found[kList];
+    __shared__ unsigned count, base;
+    const Place a = place_of(p);
+    const Row r = row_of(p, a.row);
+    const float top = unordered(unsigned(row_top(p, a.row) >> 32));
     if (r.greedy || top == -INFINITY) return;  // the whole workgroup
-    const Cut c = cut_of(p, row, r, sh);
-    u64 sum = 0;
-    const int segment = chunk * 4 + (threadIdx.x >> 6);
-    for_segment(p, row, segment, [&](float x, int i) {
-        const double z = z_of(x, top, r.inverse);
-        const int b = bin_of(z);
-        if (b == kBins - 1) return;
-        if (b < c.low) {
-            const double e = weight_of(z);
-            if (!(e < double(r.min_p))) sum += units_of(e, p.unit);
-        } else if (is_listed(c, b)) {
-            const unsigned at = atomicAdd(&p.listed[row], 1u);
-            if (at < unsigned(kList)) p.list[size_t(row) * kList + at] = u64(__float_as_uint(x)) << 32 | unsigned(i);
-        }
+    const Cut c = p.cuts[a.row];
+    if (!c.lists) return;
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    const float whole = c.whole, listed = c.listed, before = c.before, tie = c.tie;
+    for_tokens(a.x, a.begin, a.end, threadIdx.x, kThreads, [&](float x, int i) {
+        if (!((x >= listed && !(x >= whole)) || (x >= tie && !(x >= before)))) return;
+        const unsigned at = atomicAdd(&count, 1u);
+        if (at < unsigned(kList)) found[at] = u64(__float_as_uint(x)) << 32 | unsigned(i);
     });
-    sum = wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) p.segments[size_t(row) * p.chunks * 4 + segment] = sum;
+    __syncthreads();
+    const unsigned n = count;
+    if (n == 0) return;
+    if (threadIdx.x == 0) base = atomicAdd(&p.listed[a.row], n);
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < n && i < unsigned(kList); i += kThreads)
+        if (base + i < unsigned(kList)) p.list[size_t(a.row) * kList + base + i] = found[i];
 }
 
 // One workgroup a row. The listed tokens are in LDS, or, if they are too many, found in the row again by
@@ -392,18 +486,17 @@ struct DrawShared {
     u64 weight[kList];
     u64 mass[256];
     unsigned count[256];
-    u64 part[4];
+    u64 part[kWaves];
     u64 chosen;         // the digit's results
     u64 mass_before;
     unsigned count_before, digit, inside;
-    CutShared cut;
 };
+static_assert(sizeof(DrawShared) <= 64 * 1024, "within the default limit of LDS");
 
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
 {
-    extern __shared__ __align__(16) unsigned char memory[];
-    DrawShared &sh = *reinterpret_cast<DrawShared *>(memory);
-    const int row = int(blockIdx.x), tid = threadIdx.x;
+    __shared__ DrawShared sh;
+    const int row = int(blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Row r = row_of(p, row);
     const u64 t = row_top(p, row);
     const float top = unordered(unsigned(t >> 32));
@@ -418,21 +511,20 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         sh.chosen = sh.mass_before = 0;
         sh.count_before = sh.digit = sh.inside = 0;
     }
-    const Cut c = cut_of(p, row, r, sh.cut);
-    __syncthreads();
-    const unsigned listed = c.high < 0 && c.last == kBins ? 0 : p.listed[row];
+    const Cut c = p.cuts[row];
+    const float *x = p.logits + size_t(row) * p.stride;
+    const unsigned listed = c.lists ? p.listed[row] : 0;
     const bool kept_here = listed <= unsigned(kList);
     const double least = double(r.min_p);
     // f(key, weight, bin) for the listed tokens
     auto for_listed = [&](auto f) {
         if (kept_here) {
             for (unsigned i = tid; i < listed; i += kThreads) {
-                const float x = unordered(~unsigned(sh.key[i] >> 32));
-                f(sh.key[i], sh.weight[i], bin_of(z_of(x, top, r.inverse)));
+                const float v = unordered(~unsigned(sh.key[i] >> 32));
+                f(sh.key[i], sh.weight[i], bin_of(z_of(v, top, r.inverse)));
             }
             return;
         }
-        const float *x = p.logits + size_t(row) * p.stride;
         for (int i = tid; i < p.vocab; i += kThreads) {
             const float v = plain_logit(x[i]);
             const double z = z_of(v, top, r.inverse);
@@ -444,21 +536,23 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     if (kept_here) {
         for (unsigned i = tid; i < listed; i += kThreads) {
             const u64 e = p.list[size_t(row) * kList + i];
-            const float x = __uint_as_float(unsigned(e >> 32));
-            sh.key[i] = u64(~ordered(x)) << 32 | unsigned(e);
-            sh.weight[i] = units_of(weight_of(z_of(x, top, r.inverse)), p.unit);
+            const float v = __uint_as_float(unsigned(e >> 32));
+            sh.key[i] = u64(~ordered(v)) << 32 | unsigned(e);
+            sh.weight[i] = units_of(weight_of(z_of(v, top, r.inverse)), p.unit);
         }
-        __syncthreads();
     }
+    __syncthreads();
     // The key at which, in ascending order of key(token) among the tokens that `take` takes, the first
-    // `count` tokens end (BY_COUNT), or the token on which the running weight first exceeds `mass`;
+    // `count` tokens end (by_count), or the token on which the running weight first exceeds `mass`;
     // *mass_upto: the weight up to and with it. Eight bits of the key, of `bits`, at a time.
     auto select = [&](int bits, bool by_count, unsigned count, u64 mass, auto key, auto take, u64 *mass_upto) {
         u64 prefix = 0, mass_before = 0;
         unsigned count_before = 0;
         for (int shift = bits - 8; shift >= 0; shift -= 8) {
-            sh.mass[tid] = 0;
-            sh.count[tid] = 0;
+            if (tid < 256) {
+                sh.mass[tid] = 0;
+                sh.count[tid] = 0;
+            }
             __syncthreads();
             for_listed([&](u64 k, u64 w, int b) {
                 if (!take(k, w, b)) return;
@@ -468,17 +562,29 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
                 atomicAdd(&sh.mass[(q >> shift) & 255], w);
             });
             __syncthreads();
-            const u64 m = sh.mass[tid];
-            const unsigned n = sh.count[tid];
-            u64 all;
-            const u64 before = mass_before + block_before(m, sh.part, &all);
-            const unsigned before_n = count_before + unsigned(block_before(n, sh.part, &all));
-            if (by_count ? before_n < count && before_n + n >= count : before <= mass && before + m > mass) {
-                sh.digit = tid;
-                sh.inside = n;
-                sh.mass_before = before;
-                sh.count_before = before_n;
-                sh.chosen = m;
+            if (wave == 0) {  // four digits a lane
+                u64 m[4], sum = 0;
+                unsigned n[4], tokens = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    sum += m[i] = sh.mass[lane * 4 + i];
+                    tokens += n[i] = sh.count[lane * 4 + i];
+                }
+                int all;
+                u64 before = mass_before + wave_upto(sum) - sum;
+                unsigned before_n = count_before + unsigned(wave_scan(int(tokens), &all)) - tokens;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (by_count ? before_n < count && before_n + n[i] >= count : before <= mass && before + m[i] > mass) {
+                        sh.digit = lane * 4 + i;
+                        sh.inside = n[i];
+                        sh.mass_before = before;
+                        sh.count_before = before_n;
+                        sh.chosen = m[i];
+                    }
+                    before += m[i];
+                    before_n += n[i];
+                }
             }
             __syncthreads();
             prefix |= u64(sh.digit) << shift;
@@ -508,7 +614,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         cut = select(64, true, unsigned(r.top_k) - c.before_last, 0, order, [&](u64, u64, int b) { return b == c.last; }, &upto);
         total = c.mass_last + upto;
     }
-    if (r.has_p) {
+    if (c.by_p) {
         // the first token whose running weight reaches top_p of the total: exceeds the whole number before
         const double goal = double(r.top_p) * double(total);
         u64 over = u64(ceil(goal));
@@ -519,31 +625,29 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         const u64 k = select(64, false, 0, over, order, [&](u64 q, u64, int b) { return b >= c.low && b <= c.high && q <= cut; }, &upto);
         cut = k < cut ? k : cut;
     }
-    // the kept weight: the segments', and the listed tokens up to the cut
+    // the kept weight: the chunks', and the listed tokens up to the cut
     auto kept = [&](u64 k, double e) { return k <= cut && !(e < least); };
     auto keeps = [&](u64 k, u64, int) {
-        return kept(k, weight_of(z_of(unordered(~unsigned(k >> 32)), top, r.inverse)));
+        return k <= cut && (least == 0.0 || kept(k, weight_of(z_of(unordered(~unsigned(k >> 32)), top, r.inverse))));
     };
-    const int segments = p.chunks * 4;
     const bool whole = c.low > 0;  // some bins are kept whole
-    sh.mass[tid] = whole && tid < segments ? p.segments[size_t(row) * segments + tid] : 0;
+    if (tid < 256) sh.mass[tid] = whole && tid < p.chunks ? p.whole[size_t(row) * p.chunks + tid] : 0;
     __syncthreads();
     for_listed([&](u64 k, u64 w, int b) {
-        if (keeps(k, w, b)) atomicAdd(&sh.mass[whole ? unsigned(k) / unsigned(p.segment) : 0], w);
+        if (keeps(k, w, b)) atomicAdd(&sh.mass[whole ? unsigned(k) / unsigned(p.chunk) : 0], w);
     });
     __syncthreads();
     u64 all;
-    const u64 m = sh.mass[tid], before = block_before(m, sh.part, &all);
+    const u64 m = tid < 256 ? sh.mass[tid] : 0, before = block_before<kWaves>(m, sh.part, &all);
     float u = p.random[row];
     u = u > 0.0f ? u : 0.0f;  // (NaN too)
-    u64 goal = u64(double(u) * double(all));
+    u64 goal = u64(double(u < 1.0f ? u : 1.0f) * double(all));
     goal = goal < all ? goal : all - 1;
     if (!whole) {
         u64 upto;
         const u64 k = select(24, false, 0, goal, [](u64 q) { return q & 0xFFFFFFFFull; }, keeps, &upto);
-        // the token's weight
         for_listed([&](u64 q, u64 w, int) {
-            if ((q & 0xFFFFFFFFull) == k) sh.mass_before = w;
+            if ((q & 0xFFFFFFFFull) == k) sh.mass_before = w;  // the token's weight
         });
         __syncthreads();
         if (tid == 0) {
@@ -557,26 +661,36 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         sh.mass_before = before;
     }
     __syncthreads();
-    // the segment again: a run of tokens a thread
-    const int begin = int(sh.digit) * p.segment, end = min(begin + p.segment, p.vocab);
+    // the chunk again: which wave's part of it, then which token of that
+    const int begin = int(sh.digit) * p.chunk, end = min(begin + p.chunk, p.vocab);
     goal -= sh.mass_before;
-    const int run = (p.segment + kThreads - 1) / kThreads, first = begin + tid * run, last = min(first + run, end);
-    const float *x = p.logits + size_t(row) * p.stride;
-    auto units = [&](int i) {
-        const float v = plain_logit(x[i]);
+    auto units = [&](float v, int i) {
         const double z = z_of(v, top, r.inverse);
         const int b = bin_of(z);
         if (b == kBins - 1 || !(b < c.low || is_listed(c, b))) return u64(0);
         const double e = weight_of(z);
-        if (e < least || (b >= c.low && !kept(u64(~ordered(v)) << 32 | unsigned(i), e))) return u64(0);
+        if (b >= c.low && !kept(u64(~ordered(v)) << 32 | unsigned(i), e)) return u64(0);
         return units_of(e, p.unit);
     };
-    u64 mine = 0, sum;
-    for (int i = first; i < last; i++) mine += units(i);
-    u64 running = block_before(mine, sh.part, &sum);
+    const int share = (p.chunk + kThreads * 4 - 1) / (kThreads * 4) * 256;  // tokens of a wave's part
+    u64 sum = 0, ignored;
+    for_tokens(x, begin + wave * share, min(begin + (wave + 1) * share, end), lane, 64, [&](float v, int i) { sum += units(v, i); });
+    sum = lane_of(wave_upto(sum), 63);
+    const u64 first = block_before<kWaves>(lane == 0 ? sum : 0, sh.part, &ignored);
+    if (lane == 0 && first <= goal && first + sum > goal) {
+        sh.digit = wave;
+        sh.mass_before = first;
+    }
+    __syncthreads();
+    goal -= sh.mass_before;
+    const int part = begin + int(sh.digit) * share, part_end = min(part + share, end);
+    const int run = (share + kThreads - 1) / kThreads, i0 = part + tid * run, i1 = min(i0 + run, part_end);
+    u64 mine = 0;
+    for (int i = i0; i < i1; i++) mine += units(plain_logit(x[i]), i);
+    u64 running = block_before<kWaves>(mine, sh.part, &ignored);
     if (running <= goal && running + mine > goal) {
-        for (int i = first; i < last; i++) {
-            const u64 w = units(i);
+        for (int i = i0; i < i1; i++) {
+            const u64 w = units(plain_logit(x[i]), i);
             running += w;
             if (running > goal) {
                 p.tokens[row] = i;
@@ -609,31 +723,25 @@ extern "C" int fg_sample(const float *logits, size_t rows, size_t vocab, size_t 
     while ((size_t(1) << bits) < vocab) bits++;
     p.unit = double(size_t(1) << std::min(45, 63 - bits));
     // rows of a batch: what the Infinity Cache (256 MB) holds beside the rest
-    const size_t batch = std::max<size_t>(1, std::min(rows, (size_t(192) << 20) / (vocab * 4)));
+    const size_t batch = std::max<size_t>(1, std::min({rows, (size_t(192) << 20) / (vocab * 4), size_t(2048)}));
     // workgroups enough to fill the chip, of at least 4096 logits
-    p.chunks = int(std::min<size_t>({kMaxChunks, (2048 + batch - 1) / batch, (vocab + 4095) / 4096}));
-    p.segment = int((vocab + size_t(p.chunks) * 4 - 1) / (size_t(p.chunks) * 4) + 255) / 256 * 256;
-    const size_t sizes[6] = {batch * p.chunks * 8, batch * kBins * 8, batch * kBins * 4, batch * p.chunks * 32, batch * 4, batch * kList * 8};
-    size_t at[7] = {0};
-    for (int i = 0; i < 6; i++) at[i + 1] = at[i] + (sizes[i] + 255) / 256 * 256;
-    static std::atomic<u64> raised{0};  // the devices where the draw's LDS limit is raised
-    int device = 0;
-    FG_HIP(hipGetDevice(&device));
-    if (sizeof(DrawShared) > 64 * 1024 && (device > 63 || !(raised.load() >> device & 1))) {
-        FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(sample_draw_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                   int(sizeof(DrawShared))));
-        raised.fetch_or(u64(1) << (device & 63));
-    }
+    p.chunks = int(std::min<size_t>({kMaxChunks, (1024 + batch - 1) / batch, (vocab + 4095) / 4096}));
+    p.chunk = int((vocab + size_t(p.chunks) - 1) / size_t(p.chunks) + 255) / 256 * 256;
+    const size_t work = batch * p.chunks;
+    const size_t sizes[7] = {work * 8, work * kBins * 8, work * kBins * 4, work * 8, batch * sizeof(Cut), batch * 4, batch * kList * 8};
+    size_t at[8] = {0};
+    for (int i = 0; i < 7; i++) at[i + 1] = at[i] + (sizes[i] + 255) / 256 * 256;
     void *ws = nullptr;
     bool owned = false;
-    FG_HIP(stream_scratch(at[6], s, &ws, &owned));
+    FG_HIP(stream_scratch(at[7], s, &ws, &owned));
     char *base = static_cast<char *>(ws);
     p.top = reinterpret_cast<u64 *>(base + at[0]);
     p.mass = reinterpret_cast<u64 *>(base + at[1]);
     p.count = reinterpret_cast<unsigned *>(base + at[2]);
-    p.segments = reinterpret_cast<u64 *>(base + at[3]);
-    p.listed = reinterpret_cast<unsigned *>(base + at[4]);
-    p.list = reinterpret_cast<u64 *>(base + at[5]);
+    p.whole = reinterpret_cast<u64 *>(base + at[3]);
+    p.cuts = reinterpret_cast<Cut *>(base + at[4]);
+    p.listed = reinterpret_cast<unsigned *>(base + at[5]);
+    p.list = reinterpret_cast<u64 *>(base + at[6]);
     int rc = FG_OK;
     for (size_t r = 0; r < rows && rc == FG_OK; r += batch) {
         const unsigned n = unsigned(std::min(batch, rows - r)), grid = n * unsigned(p.chunks);
@@ -646,9 +754,10 @@ extern "C" int fg_sample(const float *logits, size_t rows, size_t vocab, size_t 
         p.tokens = tokens + r;
         p.chances = chances ? chances + r : nullptr;
         sample_top_kernel<<<grid, kThreads, 0, s>>>(p);
-        if (p.top_k || p.top_p) sample_bins_kernel<<<grid, kThreads, 0, s>>>(p);
-        sample_collect_kernel<<<grid, kThreads, 0, s>>>(p);
-        sample_draw_kernel<<<n, kThreads, sizeof(DrawShared), s>>>(p);
+        sample_bins_kernel<<<grid, kThreads, 0, s>>>(p);
+        sample_cut_kernel<<<n, kCutThreads, 0, s>>>(p);
+        if (p.top_k || p.top_p || p.min_p) sample_collect_kernel<<<grid, kThreads, 0, s>>>(p);
+        sample_draw_kernel<<<n, kThreads, 0, s>>>(p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) rc = check_hip(e, "fg_sample");
     }
