@@ -27,10 +27,10 @@ constexpr int kThreads = 1024;      // of the kernels that walk a row, and of th
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 1024;
 constexpr float kPerUnit = 32.0f;   // bins a unit of z
-constexpr int kList = 3072;         // tokens a row's list holds
+constexpr int kList = 2560;         // tokens a row's list holds
+constexpr int kRank = 128;          // up to so many listed tokens are compared with each other
 constexpr int kFew = 1024;          // up to so many tokens before the cut are all listed
 constexpr int kMaxChunks = 16;      // workgroups of a row
-constexpr int kCutThreads = 256;
 
 // What the bins say of a row. Tokens of bins under `low` are kept whole; those of [low, high] and of
 // `last` are listed; the others are not kept. last: the bin of top-k's cut (kBins: none).
@@ -72,7 +72,7 @@ __device__ __forceinline__ float unordered(unsigned o) { return __uint_as_float(
 
 // What a row asks for.
 struct Row {
-    double inverse;  // 1 / temperature
+    double scale;    // bins a logit: 32 / temperature
     float top_p, min_p;
     int top_k;
     bool greedy, has_k, has_p;
@@ -88,14 +88,22 @@ __device__ __forceinline__ Row row_of(const SampleParams &p, int row)
     r.top_p = tp;
     r.min_p = mp > 0.0f ? mp : 0.0f;
     r.greedy = !(t > 0.0f) || r.top_k == 1 || tp <= 0.0f || mp > 1.0f;
-    r.inverse = 1.0 / double(t);
+    r.scale = fmax(double(kPerUnit) / double(t), 1e-290);  // (an infinite temperature: every finite logit weighs 1)
     return r;
 }
 
-// exp(z) for z in [-40, 0]: z = n ln 2 + r, the Taylor series of exp to r^12 (|r| <= 0.347: the next term is
-// under 2^-52 of it), times 2^n.
-__device__ __forceinline__ double weight_of(double z)
+// -z in bins of a logit: 32 (largest - logit) / temperature, at least 0. All kernels go by `bins_of` and
+// `weight_of`, so a token's bin and weight are the same in each. (A largest logit of +inf is taken as
+// 1e300: the infinite ones are above it, and all others weigh nothing.)
+__device__ __forceinline__ double bins_of(float x, double top, double scale) { return fmax((top - double(x)) * scale, 0.0); }
+__device__ __forceinline__ int bin_of(double t) { return min(int(t), kBins - 1); }
+__device__ __forceinline__ double top_of(float x) { return x == INFINITY ? 1e300 : double(x); }
+
+// exp(-(b + 1/2) / 32), a bin's middle: -(b + 1/2) / 32 = n ln 2 + r, the Taylor series of exp to r^12
+// (|r| <= 0.347: the next term is under 2^-52 of it), times 2^n.
+__device__ __forceinline__ double middle_of(int b)
 {
+    const double z = (double(b) + 0.5) * (-1.0 / kPerUnit);
     const double n = __builtin_rint(z * 1.4426950408889634);
     double r = __builtin_fma(n, -0.6931471805599453, z);
     r = __builtin_fma(n, -2.3190468138462996e-17, r);
@@ -114,30 +122,36 @@ __device__ __forceinline__ double weight_of(double z)
     e = __builtin_fma(e, r, 1.0);
     return __builtin_ldexp(e, int(n));
 }
-// Whole units of a weight: below 2^52 a sum with 2^52 rounds to them.
-__device__ __forceinline__ u64 units_of(double e, double unit)
+// A weight exp(-t / 32), in the units of its bin's `middle`: that times exp(d / 32) for d = 1/2 less t's
+// fraction, the Taylor series to d^6 (|d / 32| <= 2^-6: the next term is under 2^-54).
+__device__ __forceinline__ double weight_of(double t, double middle)
 {
-    return u64(__double_as_longlong(__builtin_fma(e, unit, 4503599627370496.0))) & 0xFFFFFFFFFFFFFull;
+    const double d = 0.5 - __builtin_amdgcn_fract(t);
+    double e = 1.0 / 720.0 / 1073741824.0;
+    e = __builtin_fma(e, d, 1.0 / 120.0 / 33554432.0);
+    e = __builtin_fma(e, d, 1.0 / 24.0 / 1048576.0);
+    e = __builtin_fma(e, d, 1.0 / 6.0 / 32768.0);
+    e = __builtin_fma(e, d, 0.5 / 1024.0);
+    e = __builtin_fma(e, d, 1.0 / 32.0);
+    e = __builtin_fma(e, d, 1.0);
+    return e * middle;
+}
+// Whole units: below 2^52 a sum with 2^52 rounds to them. (The first token's are exact: 2^45 and some
+// 2^-7 of a unit.)
+__device__ __forceinline__ u64 units_of(double weight)
+{
+    return u64(__double_as_longlong(weight + 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
 }
 
-// z of a logit, and its bin. The first token's z is 0 (its difference is, infinite or not).
-__device__ __forceinline__ double z_of(float x, float top, double inverse)
-{
-    return x == top ? 0.0 : (double(x) - double(top)) * inverse;
-}
-__device__ __forceinline__ int bin_of(double z)
-{
-    const float b = float(z) * -kPerUnit;  // (monotone in z: a rounding and a multiplication)
-    return b < float(kBins - 1) ? int(b) : kBins - 1;
-}
-
-// 64-bit sums over the wave's lanes up to this one (DPP: rows of 16, then their last lanes).
-__device__ __forceinline__ u64 wave_upto(u64 v)
+// A value combined over the wave's lanes up to this one (DPP: rows of 16, then their last lanes); 0 changes
+// nothing.
+template <class F>
+__device__ __forceinline__ u64 wave_combine(u64 v, F combine)
 {
     auto step = [&](auto control, auto rows) {
         const unsigned lo = __builtin_amdgcn_update_dpp(0, int(unsigned(v)), decltype(control)::value, decltype(rows)::value, 0xF, false);
         const unsigned hi = __builtin_amdgcn_update_dpp(0, int(unsigned(v >> 32)), decltype(control)::value, decltype(rows)::value, 0xF, false);
-        v += u64(hi) << 32 | lo;
+        v = combine(v, u64(hi) << 32 | lo);
     };
     using All = std::integral_constant<int, 0xF>;
     step(std::integral_constant<int, 0x111>{}, All{});
@@ -147,6 +161,14 @@ __device__ __forceinline__ u64 wave_upto(u64 v)
     step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
     step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
     return v;
+}
+__device__ __forceinline__ u64 wave_upto(u64 v)
+{
+    return wave_combine(v, [](u64 a, u64 b) { return a + b; });
+}
+__device__ __forceinline__ u64 wave_or(u64 v)
+{
+    return wave_combine(v, [](u64 a, u64 b) { return a | b; });
 }
 __device__ __forceinline__ u64 lane_of(u64 v, int lane)
 {
@@ -256,22 +278,29 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams p)
 {
     __shared__ u64 mass[kBins];
     __shared__ unsigned count[kBins];
+    __shared__ double middles[kBins];
     const Place a = place_of(p);
     const Row r = row_of(p, a.row);
-    const float top = unordered(unsigned(row_top(p, a.row) >> 32));
-    if (r.greedy || top == -INFINITY) return;  // the whole workgroup
+    const float first = unordered(unsigned(row_top(p, a.row) >> 32));
+    if (r.greedy || first == -INFINITY) return;  // the whole workgroup
     const int tid = threadIdx.x;
+    const double top = top_of(first);
     static_assert(kBins == kThreads, "a bin a thread");
     mass[tid] = 0;
     count[tid] = 0;
+    middles[tid] = middle_of(tid) * p.unit;
     __syncthreads();
-    for_tokens(a.x, a.begin, a.end, tid, kThreads, [&](float x, int) {
-        const double z = z_of(x, top, r.inverse);
-        const int b = bin_of(z);
-        if (b == kBins - 1) return;  // weighs 0
-        if (r.has_k) atomicAdd(&count[b], 1u);
-        atomicAdd(&mass[b], units_of(weight_of(z), p.unit));
-    });
+    auto add = [&](float x) {
+        x = x != x ? -INFINITY : x;
+        const double t = bins_of(x, top, r.scale);
+        const int b = bin_of(t);
+        const u64 w = units_of(weight_of(t, middles[b]));
+        if (b < kBins - 1) {  // (the last bin's weigh 0)
+            if (r.has_k) atomicAdd(&count[b], 1u);
+            atomicAdd(&mass[b], w);
+        }
+    };
+    for_tokens(a.x, a.begin, a.end, tid, kThreads, [&](float x, int) { add(x); });
     __syncthreads();
     const size_t at = (size_t(a.row) * p.chunks + a.chunk) * kBins + tid;
     p.mass[at] = mass[tid];
@@ -279,7 +308,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams p)
 }
 
 struct CutShared {
-    u64 part[kCutThreads / 64];
+    u64 part[kWaves];
     int last, low, high;
     unsigned before_last, upto;
     u64 mass_last, mass_after, mass_low;
@@ -288,17 +317,18 @@ struct CutShared {
 };
 
 // The smallest logit whose bin is at most b, by halving the order of floats 64 ways at a time.
-__device__ __forceinline__ float smallest_of_bin(int b, float top, double inverse)
+__device__ __forceinline__ float smallest_of_bin(int b, float first, double scale)
 {
     if (b >= kBins - 1) return -INFINITY;
     if (b < 0) return __builtin_nanf("");  // nothing is >= NaN
     const int lane = threadIdx.x & 63;
-    unsigned lo = 0, n = ordered(top);  // the answer is in (lo, lo + n]; ordered(top) has bin 0
+    const double top = top_of(first);
+    unsigned lo = 0, n = ordered(first);  // the answer is in (lo, lo + n]; the first token has bin 0
     while (n > 1) {
         const unsigned step = (n + 63) / 64, at = lo + (lane + 1) * step;
         const bool inside = u64(lane + 1) * step <= n;
         const float x = plain_logit(unordered(inside ? at : lo + n));
-        const bool yes = bin_of(z_of(x, top, inverse)) <= b && x > -INFINITY;
+        const bool yes = bin_of(bins_of(x, top, scale)) <= b && x > -INFINITY;
         const int k = __builtin_ctzll(__ballot(yes || !inside) | 1ull << 63);
         const unsigned from = lo + unsigned(k) * step, to = lo + n;
         lo = from;
@@ -307,55 +337,44 @@ __device__ __forceinline__ float smallest_of_bin(int b, float top, double invers
     return unordered(lo + n);
 }
 
-// One workgroup a row: its bins summed over the chunks, four a thread.
-__global__ __launch_bounds__(kCutThreads) void sample_cut_kernel(SampleParams p)
+// One workgroup a row, a bin a thread.
+__global__ __launch_bounds__(kThreads, 8) void sample_cut_kernel(SampleParams p)
 {
     __shared__ CutShared sh;
     const int row = int(blockIdx.x), tid = threadIdx.x;
     const Row r = row_of(p, row);
+    // the chunks' weights stay in registers for the sums under `low`
+    u64 masses[kMaxChunks], m = 0, n = 0, all_n = 0, all_m, before_n = 0;
+    const u64 *mass = p.mass + size_t(row) * p.chunks * kBins + tid;
+    const unsigned *count = p.count + size_t(row) * p.chunks * kBins + tid;
+#pragma unroll
+    for (int c = 0; c < kMaxChunks; c++) masses[c] = c < p.chunks ? mass[c * kBins] : 0;
+    if (r.has_k) {
+#pragma unroll
+        for (int c = 0; c < kMaxChunks; c++) n += c < p.chunks ? count[c * kBins] : 0;
+    }
     const float top = unordered(unsigned(row_top(p, row) >> 32));
-    if (r.greedy || top == -INFINITY) return;
-    constexpr int kEach = kBins / kCutThreads;
-    u64 n[kEach] = {}, m[kEach] = {}, here_n = 0, here_m = 0, all_n = 0, all_m, before_n = 0;
-    const u64 *mass = p.mass + size_t(row) * p.chunks * kBins + tid * kEach;
-    for (int c = 0; c < p.chunks; c++) {
-        if (r.has_k) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(p.count + (size_t(row) * p.chunks + c) * kBins + tid * kEach);
-            n[0] += v.x, n[1] += v.y, n[2] += v.z, n[3] += v.w;
-        }
+    if (r.greedy || top == -INFINITY) return;  // (its bins are not written: what was read is not used)
 #pragma unroll
-        for (int i = 0; i < kEach; i++) m[i] += mass[size_t(c) * kBins + i];
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        here_n += n[i];
-        here_m += m[i];
-    }
-    const u64 before_m = block_before<kCutThreads / 64>(here_m, sh.part, &all_m);
-    if (r.has_k) before_n = block_before<kCutThreads / 64>(here_n, sh.part, &all_n);
-    __syncthreads();
+    for (int c = 0; c < kMaxChunks; c++) m += masses[c];
+    const u64 before_m = block_before<kWaves>(m, sh.part, &all_m);
+    if (r.has_k) before_n = block_before<kWaves>(n, sh.part, &all_n);
     if (tid == 0) {
         sh.last = kBins;
         sh.low = sh.high = kBins - 1;
         sh.mass_last = sh.mass_after = all_m;
-        sh.before_last = 0;
+        sh.before_last = sh.upto = 0;
         sh.mass_low = all_m;
     }
     if (tid < kMaxChunks) sh.whole[tid] = 0;
     __syncthreads();
-    if (r.has_k && u64(r.top_k) < all_n) {  // (else every token that weighs anything is among the first top_k)
-        u64 a = before_n, b = before_m;
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            if (a < u64(r.top_k) && a + n[i] >= u64(r.top_k)) {
-                sh.last = tid * kEach + i;
-                sh.before_last = unsigned(a);
-                sh.mass_last = b;
-                sh.mass_after = b + m[i];
-            }
-            a += n[i];
-            b += m[i];
-        }
+    // (top_k of all that weigh anything, or more: no cut)
+    if (r.has_k && u64(r.top_k) < all_n && before_n < u64(r.top_k) && before_n + n >= u64(r.top_k)) {
+        sh.last = tid;
+        sh.before_last = unsigned(before_n);
+        sh.upto = unsigned(before_n + n);
+        sh.mass_last = before_m;
+        sh.mass_after = before_m + m;
     }
     __syncthreads();
     Cut c{kBins, -1, sh.last, sh.before_last, sh.mass_last, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0, r.has_p};
@@ -363,14 +382,9 @@ __global__ __launch_bounds__(kCutThreads) void sample_cut_kernel(SampleParams p)
         // the cut's bin, for a total between the weight under `last` and that up to it
         const double least = double(r.top_p) * double(sh.mass_last) * (1.0 - 0x1p-50);
         const double most = double(r.top_p) * double(sh.mass_after) * (1.0 + 0x1p-50);
-        u64 b = before_m;
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            if (m[i]) {
-                if ((b == 0 || double(b) < least) && double(b + m[i]) >= least) sh.low = tid * kEach + i;
-                if ((b == 0 || double(b) < most) && double(b + m[i]) >= most) sh.high = tid * kEach + i;
-            }
-            b += m[i];
+        if (m) {
+            if ((before_m == 0 || double(before_m) < least) && double(before_m + m) >= least) sh.low = tid;
+            if ((before_m == 0 || double(before_m) < most) && double(before_m + m) >= most) sh.high = tid;
         }
         __syncthreads();
         c.high = min(max(sh.high, sh.low), c.last);
@@ -380,8 +394,8 @@ __global__ __launch_bounds__(kCutThreads) void sample_cut_kernel(SampleParams p)
     }
     if (r.min_p > 0.0f) {
         // min-p's cut is in the bins of ln(min_p), to more than the rounding of weights
-        const double z = log(double(r.min_p));
-        const int first = bin_of(z + 1e-9 < 0.0 ? z + 1e-9 : 0.0), last = bin_of(z - 1e-9);
+        const double t = log(double(r.min_p)) * -double(kPerUnit);
+        const int first = bin_of(t > 1e-9 ? t - 1e-9 : 0.0), last = bin_of(t + 1e-9);
         if (last < c.low) {  // before any other cut: the others change nothing
             c.low = first;
             c.high = last;
@@ -396,52 +410,31 @@ __global__ __launch_bounds__(kCutThreads) void sample_cut_kernel(SampleParams p)
         c.high = min(c.high, kBins - 2);  // (the last bin's tokens weigh 0)
         c.low = min(c.low, c.high);
     }
-    __syncthreads();
-    u64 b = before_m;
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        if (tid * kEach + i == c.low) sh.mass_low = b;
-        b += m[i];
+    // few tokens up to top-k's bin: all of them are listed
+    if (lists && c.last < kBins && sh.upto <= unsigned(kFew)) {
+        c.low = 0;
+        c.high = c.last;
     }
-    __syncthreads();
-    c.mass_low = sh.mass_low;
-    c.lists = lists;
-    // few tokens up to the last listed bin (counted only under top-k, which is what leaves few): all are listed
-    if (lists && r.has_k && c.last < kBins) {
-        if (tid == 0) sh.upto = 0;
-        __syncthreads();
-        u64 a = before_n;
-#pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            a += n[i];
-            if (tid * kEach + i == c.last) sh.upto = unsigned(a);
-        }
-        __syncthreads();
-        if (sh.upto <= unsigned(kFew)) {
-            c.low = 0;
-            c.high = c.last;
-            c.mass_low = 0;
-        }
-    }
+    if (tid == c.low) sh.mass_low = before_m;
     // the chunks' weight under `low`
     if (c.low > 0) {
-        for (int k = 0; k < p.chunks; k++) {
-            u64 w = 0;
 #pragma unroll
-            for (int i = 0; i < kEach; i++) w += tid * kEach + i < c.low ? mass[size_t(k) * kBins + i] : 0;
-            w = wave_upto(w);
-            if ((tid & 63) == 63) atomicAdd(&sh.whole[k], w);
+        for (int k = 0; k < kMaxChunks; k++) {
+            const u64 w = wave_upto(tid < c.low ? masses[k] : 0);
+            if ((tid & 63) == 63 && w) atomicAdd(&sh.whole[k], w);
         }
     }
     const int wave = tid >> 6;
     const int edge = wave == 0 ? c.low - 1 : wave == 1 ? c.high : wave == 2 ? c.last - 1 : c.last;
-    if (lists) {
-        const float x = smallest_of_bin(edge, top, r.inverse);
+    if (lists && wave < 4) {
+        const float x = smallest_of_bin(edge, top, r.scale);
         if ((tid & 63) == 0) sh.edge[wave] = x;
     }
     __syncthreads();
     if (tid < p.chunks) p.whole[size_t(row) * p.chunks + tid] = sh.whole[tid];
     if (tid == 0) {
+        c.mass_low = sh.mass_low;
+        c.lists = lists;
         c.whole = sh.edge[0];
         c.listed = sh.edge[1];
         c.before = sh.edge[2];
@@ -484,12 +477,17 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleParams p
 struct DrawShared {
     u64 key[kList];     // (~ordered logit, index): the order, ascending
     u64 weight[kList];
+    unsigned short bin[kList];
     u64 mass[256];
     unsigned count[256];
     u64 part[kWaves];
+    ulonglong2 ranked[kRank];  // few tokens' keys and weights
+    u64 before[kRank];         // the weight and the number of tokens before each
+    unsigned tokens[kRank];
     u64 chosen;         // the digit's results
     u64 mass_before;
     unsigned count_before, digit, inside;
+    double middles[kBins];
 };
 static_assert(sizeof(DrawShared) <= 64 * 1024, "within the default limit of LDS");
 
@@ -498,39 +496,42 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     __shared__ DrawShared sh;
     const int row = int(blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Row r = row_of(p, row);
-    const u64 t = row_top(p, row);
-    const float top = unordered(unsigned(t >> 32));
-    if (r.greedy || top == -INFINITY) {
+    const u64 first_token = row_top(p, row);
+    const float first_logit = unordered(unsigned(first_token >> 32));
+    if (r.greedy || first_logit == -INFINITY) {
         if (tid == 0) {
-            p.tokens[row] = top == -INFINITY ? -1 : int(~unsigned(t));
-            if (p.chances) p.chances[row] = top == -INFINITY ? 0.0f : 1.0f;
+            p.tokens[row] = first_logit == -INFINITY ? -1 : int(~unsigned(first_token));
+            if (p.chances) p.chances[row] = first_logit == -INFINITY ? 0.0f : 1.0f;
         }
         return;
     }
+    const double top = top_of(first_logit);
     if (tid == 0) {
         sh.chosen = sh.mass_before = 0;
         sh.count_before = sh.digit = sh.inside = 0;
     }
+    sh.middles[tid] = middle_of(tid) * p.unit;
+    __syncthreads();
+    auto weight = [&](double t, int b) { return weight_of(t, sh.middles[b]); };
     const Cut c = p.cuts[row];
     const float *x = p.logits + size_t(row) * p.stride;
     const unsigned listed = c.lists ? p.listed[row] : 0;
     const bool kept_here = listed <= unsigned(kList);
-    const double least = double(r.min_p);
+    const double least = double(r.min_p) * (1.0 - 0x1p-50) * p.unit;  // (less than the rounding of weights)
     // f(key, weight, bin) for the listed tokens
     auto for_listed = [&](auto f) {
         if (kept_here) {
             for (unsigned i = tid; i < listed; i += kThreads) {
-                const float v = unordered(~unsigned(sh.key[i] >> 32));
-                f(sh.key[i], sh.weight[i], bin_of(z_of(v, top, r.inverse)));
+                f(sh.key[i], sh.weight[i], int(sh.bin[i]));
             }
             return;
         }
         for (int i = tid; i < p.vocab; i += kThreads) {
             const float v = plain_logit(x[i]);
-            const double z = z_of(v, top, r.inverse);
-            const int b = bin_of(z);
+            const double t = bins_of(v, top, r.scale);
+            const int b = bin_of(t);
             if (b == kBins - 1 || !is_listed(c, b)) continue;
-            f(u64(~ordered(v)) << 32 | unsigned(i), units_of(weight_of(z), p.unit), b);
+            f(u64(~ordered(v)) << 32 | unsigned(i), units_of(weight(t, b)), b);
         }
     };
     if (kept_here) {
@@ -538,17 +539,80 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
             const u64 e = p.list[size_t(row) * kList + i];
             const float v = __uint_as_float(unsigned(e >> 32));
             sh.key[i] = u64(~ordered(v)) << 32 | unsigned(e);
-            sh.weight[i] = units_of(weight_of(z_of(v, top, r.inverse)), p.unit);
+            const double t = bins_of(v, top, r.scale);
+            sh.weight[i] = units_of(weight(t, bin_of(t)));
+            sh.bin[i] = (unsigned short)(bin_of(t));
         }
     }
     __syncthreads();
     // The key at which, in ascending order of key(token) among the tokens that `take` takes, the first
     // `count` tokens end (by_count), or the token on which the running weight first exceeds `mass`;
-    // *mass_upto: the weight up to and with it. Eight bits of the key, of `bits`, at a time.
-    auto select = [&](int bits, bool by_count, unsigned count, u64 mass, auto key, auto take, u64 *mass_upto) {
-        u64 prefix = 0, mass_before = 0;
+    // *mass_upto: the weight up to and with it. Few tokens: each against all others, by as many threads a
+    // token as there are. Many: eight bits of the key, of `bits`, at a time.
+    auto select = [&](bool by_count, unsigned count, u64 mass, auto key, auto take, u64 *mass_upto) {
+        if (kept_here && listed <= unsigned(kRank)) {
+            int width = 64;  // threads of a round: one a token
+            while (width < int(listed)) width *= 2;
+            const int i = tid & (width - 1), rounds = kThreads / width;
+            if (tid < kRank) {
+                sh.before[tid] = 0;
+                sh.tokens[tid] = 0;
+            }
+            __syncthreads();
+            if (tid < kRank) {
+                const bool taken = tid < int(listed) && take(sh.key[tid], sh.weight[tid], sh.bin[tid]);
+                sh.ranked[tid] = taken ? ulonglong2{key(sh.key[tid]), sh.weight[tid]} : ulonglong2{~0ull, 0};
+            }
+            __syncthreads();
+            const u64 q = sh.ranked[i].x;
+            const bool mine = q != ~0ull;
+            if (mine) {
+                u64 m = 0;
+                unsigned n = 0;
+#pragma unroll 4
+                for (int j = tid / width; j < width; j += rounds) {
+                    const ulonglong2 other = sh.ranked[j];
+                    const bool sooner = other.x < q;
+                    m += sooner ? other.y : 0;
+                    n += sooner;
+                }
+                atomicAdd(&sh.before[i], m);
+                atomicAdd(&sh.tokens[i], n);
+            }
+            __syncthreads();
+            if (tid < width && mine) {
+                const u64 m = sh.before[i], w = sh.ranked[i].y;
+                if (by_count ? sh.tokens[i] + 1 == count : m <= mass && m + w > mass) {
+                    sh.chosen = q;
+                    sh.mass_before = m + w;
+                }
+            }
+            __syncthreads();
+            const u64 found = sh.chosen;
+            *mass_upto = sh.mass_before;
+            __syncthreads();
+            return found;
+        }
+        if (tid == 0) sh.before[0] = 0;
+        for_listed([&](u64 k, u64 w, int b) {
+            if (take(k, w, b)) sh.chosen = key(k);  // any one
+        });
+        __syncthreads();
+        const u64 some = sh.chosen;
+        u64 differ = 0;
+        for_listed([&](u64 k, u64 w, int b) {
+            if (take(k, w, b)) differ |= key(k) ^ some;
+        });
+        differ = wave_or(differ);
+        if (lane == 63) atomicOr(&sh.before[0], differ);
+        __syncthreads();
+        differ = sh.before[0];
+        const int start = differ ? max(56 - __builtin_clzll(differ), 0) : 0;
+        u64 prefix = start + 8 < 64 ? some >> (start + 8) << (start + 8) : 0, mass_before = 0;
         unsigned count_before = 0;
-        for (int shift = bits - 8; shift >= 0; shift -= 8) {
+        for (int shift = start, above = start + 8;;) {  // the key's bits from `shift` up to `above`
+            const u64 known = above < 64 ? prefix >> above : 0;
+            const unsigned digits = (1u << (above - shift)) - 1;
             if (tid < 256) {
                 sh.mass[tid] = 0;
                 sh.count[tid] = 0;
@@ -557,9 +621,10 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
             for_listed([&](u64 k, u64 w, int b) {
                 if (!take(k, w, b)) return;
                 const u64 q = key(k);
-                if (shift < bits - 8 && q >> (shift + 8) != prefix >> (shift + 8)) return;
-                atomicAdd(&sh.count[(q >> shift) & 255], 1u);
-                atomicAdd(&sh.mass[(q >> shift) & 255], w);
+                if (above < 64 && q >> above != known) return;
+                const unsigned digit = unsigned(q >> shift) & digits;
+                atomicAdd(&sh.count[digit], 1u);
+                atomicAdd(&sh.mass[digit], w);
             });
             __syncthreads();
             if (wave == 0) {  // four digits a lane
@@ -604,14 +669,16 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
                 __syncthreads();
                 return q;
             }
+            if (shift == 0) return prefix;
+            above = shift;
+            shift = max(shift - 8, 0);
         }
-        return prefix;
     };
     auto order = [](u64 k) { return k; };
     u64 cut = ~0ull, total = c.mass_last;
     if (c.last < kBins) {
         u64 upto;
-        cut = select(64, true, unsigned(r.top_k) - c.before_last, 0, order, [&](u64, u64, int b) { return b == c.last; }, &upto);
+        cut = select(true, unsigned(r.top_k) - c.before_last, 0, order, [&](u64, u64, int b) { return b == c.last; }, &upto);
         total = c.mass_last + upto;
     }
     if (c.by_p) {
@@ -622,13 +689,13 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         over = over >= total ? total - 1 : over;
         over = over > c.mass_low ? over - c.mass_low : 0;
         u64 upto;
-        const u64 k = select(64, false, 0, over, order, [&](u64 q, u64, int b) { return b >= c.low && b <= c.high && q <= cut; }, &upto);
+        const u64 k = select(false, 0, over, order, [&](u64 q, u64, int b) { return b >= c.low && b <= c.high && q <= cut; }, &upto);
         cut = k < cut ? k : cut;
     }
     // the kept weight: the chunks', and the listed tokens up to the cut
     auto kept = [&](u64 k, double e) { return k <= cut && !(e < least); };
-    auto keeps = [&](u64 k, u64, int) {
-        return k <= cut && (least == 0.0 || kept(k, weight_of(z_of(unordered(~unsigned(k >> 32)), top, r.inverse))));
+    auto keeps = [&](u64 k, u64, int b) {
+        return k <= cut && (least == 0.0 || kept(k, weight(bins_of(unordered(~unsigned(k >> 32)), top, r.scale), b)));
     };
     const bool whole = c.low > 0;  // some bins are kept whole
     if (tid < 256) sh.mass[tid] = whole && tid < p.chunks ? p.whole[size_t(row) * p.chunks + tid] : 0;
@@ -645,7 +712,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     goal = goal < all ? goal : all - 1;
     if (!whole) {
         u64 upto;
-        const u64 k = select(24, false, 0, goal, [](u64 q) { return q & 0xFFFFFFFFull; }, keeps, &upto);
+        const u64 k = select(false, 0, goal, [](u64 q) { return q & 0xFFFFFFFFull; }, keeps, &upto);
         for_listed([&](u64 q, u64 w, int) {
             if ((q & 0xFFFFFFFFull) == k) sh.mass_before = w;  // the token's weight
         });
@@ -665,12 +732,12 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     const int begin = int(sh.digit) * p.chunk, end = min(begin + p.chunk, p.vocab);
     goal -= sh.mass_before;
     auto units = [&](float v, int i) {
-        const double z = z_of(v, top, r.inverse);
-        const int b = bin_of(z);
+        const double t = bins_of(v, top, r.scale);
+        const int b = bin_of(t);
         if (b == kBins - 1 || !(b < c.low || is_listed(c, b))) return u64(0);
-        const double e = weight_of(z);
+        const double e = weight(t, b);
         if (b >= c.low && !kept(u64(~ordered(v)) << 32 | unsigned(i), e)) return u64(0);
-        return units_of(e, p.unit);
+        return units_of(e);
     };
     const int share = (p.chunk + kThreads * 4 - 1) / (kThreads * 4) * 256;  // tokens of a wave's part
     u64 sum = 0, ignored;
@@ -723,9 +790,19 @@ extern "C" int fg_sample(const float *logits, size_t rows, size_t vocab, size_t 
     while ((size_t(1) << bits) < vocab) bits++;
     p.unit = double(size_t(1) << std::min(45, 63 - bits));
     // rows of a batch: what the Infinity Cache (256 MB) holds beside the rest
-    const size_t batch = std::max<size_t>(1, std::min({rows, (size_t(192) << 20) / (vocab * 4), size_t(2048)}));
-    // workgroups enough to fill the chip, of at least 4096 logits
-    p.chunks = int(std::min<size_t>({kMaxChunks, (1024 + batch - 1) / batch, (vocab + 4095) / 4096}));
+    const size_t most = std::max<size_t>(1, std::min({rows, (size_t(192) << 20) / (vocab * 4), size_t(2048)}));
+    const size_t batches = (rows + most - 1) / most, batch = (rows + batches - 1) / batches;
+    // Chunks of a row: the chip takes 512 workgroups at once, each of which costs about 2 us and 0.6 ns a
+    // logit (the bins of 64 rows of 151936: 8 chunks, one round, 13 us; 16 chunks, two rounds, 16 us), and
+    // the draw walks one chunk of every row, 0.4 ns a logit (331 rows: 3 chunks 44 us, 6 chunks 32).
+    double best = 0.0;
+    for (size_t c = 1; c <= size_t(kMaxChunks) && (c == 1 || (vocab + c - 1) / c >= 4096); c++) {
+        const double cost = double((batch * c + 511) / 512) * (2000.0 + 0.6 * double(vocab) / double(c)) + 0.4 * double(vocab) / double(c);
+        if (c == 1 || cost < best) {
+            best = cost;
+            p.chunks = int(c);
+        }
+    }
     p.chunk = int((vocab + size_t(p.chunks) - 1) / size_t(p.chunks) + 255) / 256 * 256;
     const size_t work = batch * p.chunks;
     const size_t sizes[7] = {work * 8, work * kBins * 8, work * kBins * 4, work * 8, batch * sizeof(Cut), batch * 4, batch * kList * 8};
@@ -755,7 +832,7 @@ extern "C" int fg_sample(const float *logits, size_t rows, size_t vocab, size_t 
         p.chances = chances ? chances + r : nullptr;
         sample_top_kernel<<<grid, kThreads, 0, s>>>(p);
         sample_bins_kernel<<<grid, kThreads, 0, s>>>(p);
-        sample_cut_kernel<<<n, kCutThreads, 0, s>>>(p);
+        sample_cut_kernel<<<n, kThreads, 0, s>>>(p);
         if (p.top_k || p.top_p || p.min_p) sample_collect_kernel<<<grid, kThreads, 0, s>>>(p);
         sample_draw_kernel<<<n, kThreads, 0, s>>>(p);
         const hipError_t e = hipGetLastError();
