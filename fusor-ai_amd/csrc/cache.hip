@@ -130,16 +130,18 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
     }
 }
 
-// A workgroup per page that new tokens lie in and head. A thread takes four tokens (an aligned run, so
-// one dword of each dimension's values) of four dimensions; the levels meet in LDS in the record's
-// order, and whole 16-byte pieces go to the page or come from it. Pieces that also hold other tokens'
-// values are written in part.
+// A workgroup per page that new tokens lie in, head, and keys or values. A thread takes four tokens (an
+// aligned run, so one dword of each dimension's values) of four dimensions, heads of up to 128 all of a page
+// at once; the levels meet in LDS in the record's order, and whole 16-byte pieces go to the page or come from it.
+// Pieces that also hold other tokens' values are written in part.
+constexpr int kPageThreads = 512;
+
 template <bool WRITE>
-__global__ __launch_bounds__(256) void cache_pages_kernel(StoreParams p)
+__global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p)
 {
     extern __shared__ __align__(16) uint8_t levels[];
-    __shared__ float scales[2][kPage];
-    const int tid = threadIdx.x, head = int(blockIdx.y);
+    __shared__ float scales[kPage];
+    const int tid = threadIdx.x, head = int(blockIdx.y), value = int(blockIdx.z);
     int index;
     const int s = find_unit(p.b.sequences, int(blockIdx.x), &index, [&](int q) {
         const PageRange r = pages_of_new(sequence_span(p.b, q));
@@ -152,63 +154,65 @@ __global__ __launch_bounds__(256) void cache_pages_kernel(StoreParams p)
     if (WRITE && page < 0) return;
     // the page's tokens [t0, t1) are new
     const int t0 = max(span.first - place * kPage, 0), t1 = min(span.first + span.rows - place * kPage, kPage);
+    // this half of the record, and the byte in it of a token's dimension
     uint8_t *record = p.records + (size_t(page < 0 ? 0 : page) * p.kv_heads + head) * record_bytes(p.padded);
+    uint8_t *half = record + (value ? kPage * p.padded : 0);
+    float *record_scales = reinterpret_cast<float *>(record + (value ? value_scale_byte(p.padded, 0) : key_scale_byte(p.padded, 0)));
     const bool wide = p.padded > 128;
-    const int lanes = wide ? 64 : 32, quads = 256 / lanes, dim = (tid & (lanes - 1)) * 4;
+    const int lanes = wide ? 64 : 32, quads = kPageThreads / lanes, dim = (tid & (lanes - 1)) * 4;
     const bool live = dim < p.head_dim;
     const size_t row0 = size_t(span.begin) + size_t(place * kPage - span.first);  // the row of the page's token 0 (may wrap below 0)
-    const int pieces = 2 * kPage * p.padded / 16;
+    const int pieces = kPage * p.padded / 16;
+    const uint4 none = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
     if (WRITE) {
         if (p.head_dim != p.padded) {  // the padding's levels
-            for (int i = tid; i < pieces; i += 256) reinterpret_cast<uint4 *>(levels)[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            for (int i = tid; i < pieces; i += kPageThreads) reinterpret_cast<uint4 *>(levels)[i] = none;
             __syncthreads();
         }
     } else {
-        for (int i = tid; i < pieces; i += 256)
-            reinterpret_cast<uint4 *>(levels)[i] =
-                page < 0 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u) : reinterpret_cast<const uint4 *>(record)[i];
-        if (tid < 2 * kPage)
-            (&scales[0][0])[tid] = page < 0 ? 1.0f : *reinterpret_cast<const float *>(record + key_scale_byte(p.padded, tid));
+        for (int i = tid; i < pieces; i += kPageThreads)
+            reinterpret_cast<uint4 *>(levels)[i] = page < 0 ? none : reinterpret_cast<const uint4 *>(half)[i];
+        if (tid < kPage) scales[tid] = page < 0 ? 1.0f : record_scales[tid];
         __syncthreads();
     }
-    for (int unit = tid / lanes; unit < 2 * (kPage / 4); unit += quads) {  // whole teams: keys' quads, then values'
-        const int value = unit / (kPage / 4), t = unit % (kPage / 4) * 4;
+    const size_t stride = p.stride[value];
+    for (int unit = tid / lanes; unit < kPage / 4; unit += quads) {  // whole teams
+        const int t = unit * 4;
         if (t + 4 <= t0 || t >= t1) continue;
+        const size_t at = (row0 + t) * stride + size_t(head) * p.head_dim + dim;
         unsigned packed[4];
         if (WRITE) {
             v4f x[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 x[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-                if (live && t + i >= t0 && t + i < t1)
-                    x[i] = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + (row0 + t + i) * p.stride[value] +
-                                                              size_t(head) * p.head_dim + dim);
+                if (live && t + i >= t0 && t + i < t1) x[i] = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + at + i * stride);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float d = head_levels(team_max(amax4(x[i]), wide), x[i], packed[i]);
-                if (dim == 0) scales[value][t + i] = d;
+                if (dim == 0) scales[t + i] = d;
             }
         }
         if (!value) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                unsigned *at = reinterpret_cast<unsigned *>(levels + key_byte(p.padded, t + i, dim));
-                if (WRITE && live) *at = packed[i];
-                if (!WRITE && live) packed[i] = *at;
+                unsigned *word = reinterpret_cast<unsigned *>(levels + key_byte(p.padded, t + i, dim));
+                if (WRITE && live) *word = packed[i];
+                if (!WRITE && live) packed[i] = *word;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++) {  // dimension dim + j of the four tokens
-                unsigned *at = reinterpret_cast<unsigned *>(levels + value_byte(p.padded, t, dim + j));
+                unsigned *word = reinterpret_cast<unsigned *>(levels + value_byte(p.padded, t, dim + j) - kPage * p.padded);
                 if (WRITE && live) {
                     unsigned w = 0;
 #pragma unroll
                     for (int i = 0; i < 4; i++) w |= (packed[i] >> (8 * j) & 255u) << (8 * i);
-                    *at = w;
+                    *word = w;
                 }
                 if (!WRITE) {
-                    const unsigned w = live ? *at : 0;
+                    const unsigned w = live ? *word : 0;
 #pragma unroll
                     for (int i = 0; i < 4; i++) packed[i] = (j ? packed[i] : 0) | (w >> (8 * i) & 255u) << (8 * j);
                 }
@@ -218,18 +222,16 @@ __global__ __launch_bounds__(256) void cache_pages_kernel(StoreParams p)
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (t + i >= t0 && t + i < t1)
-                    *reinterpret_cast<v4f_any *>((value ? p.out[1] : p.out[0]) + (row0 + t + i) * p.stride[value] +
-                                                 size_t(head) * p.head_dim + dim) = levels_to_values(packed[i], scales[value][t + i]);
+                    *reinterpret_cast<v4f_any *>((value ? p.out[1] : p.out[0]) + at + i * stride) = levels_to_values(packed[i], scales[t + i]);
         }
     }
     if (!WRITE) return;
     __syncthreads();
-    const int key_pieces = pieces / 2;
-    for (int i = tid; i < pieces; i += 256) {
-        const int lane = i & 63, block = (i < key_pieces ? i : i - key_pieces) >> 6;
+    for (int i = tid; i < pieces; i += kPageThreads) {
+        const int lane = i & 63, block = i >> 6;
         const uint4 w = reinterpret_cast<const uint4 *>(levels)[i];
-        uint8_t *at = record + size_t(i) * 16;
-        if (i < key_pieces) {  // one token's
+        uint8_t *at = half + size_t(i) * 16;
+        if (!value) {  // one token's
             const int t = block / (p.padded >> 5) * 32 + (lane & 31);
             if (t >= t0 && t < t1) *reinterpret_cast<uint4 *>(at) = w;
             continue;
@@ -252,10 +254,7 @@ __global__ __launch_bounds__(256) void cache_pages_kernel(StoreParams p)
             }
         }
     }
-    if (tid < 2 * kPage) {
-        const int t = tid & (kPage - 1);
-        if (t >= t0 && t < t1) *reinterpret_cast<float *>(record + key_scale_byte(p.padded, tid)) = (&scales[0][0])[tid];
-    }
+    if (tid < kPage && tid >= t0 && tid < t1) record_scales[tid] = scales[tid];
 }
 
 template <bool WRITE>
@@ -268,7 +267,7 @@ int launch_store(const StoreParams &p, hipStream_t s)
     } else {
         // a run of n rows lies in at most (n + 62) / 64 + 1 pages
         const size_t units = size_t(p.b.rows) / kPage + 2 * size_t(std::min(p.b.sequences, p.b.rows));
-        cache_pages_kernel<WRITE><<<dim3(unsigned(units), unsigned(p.kv_heads)), 256, size_t(2 * kPage * p.padded), s>>>(p);
+        cache_pages_kernel<WRITE><<<dim3(unsigned(units), unsigned(p.kv_heads), 2), kPageThreads, size_t(kPage * p.padded), s>>>(p);
     }
     FG_HIP(hipGetLastError());
     return FG_OK;
