@@ -41,6 +41,10 @@ struct Cut {
     // the smallest logits of the bins up to low - 1, high, last - 1 and last (NaN: of none)
     float whole, listed, before, tie;
     int lists, by_p;          // whether any bin is listed, and whether top-p's cut is in one
+    int done;                 // whether the row's token is there already
+    int top_k;
+    float top_p;
+    double top, scale, least;  // the largest logit, bins a logit, and the weight that min-p asks for
 };
 
 struct SampleParams {
@@ -353,8 +357,17 @@ __global__ __launch_bounds__(kThreads, 8) void sample_cut_kernel(SampleParams p)
 #pragma unroll
         for (int c = 0; c < kMaxChunks; c++) n += c < p.chunks ? count[c * kBins] : 0;
     }
-    const float top = unordered(unsigned(row_top(p, row) >> 32));
-    if (r.greedy || top == -INFINITY) return;  // (its bins are not written: what was read is not used)
+    const u64 first = row_top(p, row);
+    const float top = unordered(unsigned(first >> 32));
+    if (r.greedy || top == -INFINITY) {  // (its bins are not written: what was read is not used)
+        if (tid == 0) {
+            p.tokens[row] = top == -INFINITY ? -1 : int(~unsigned(first));
+            if (p.chances) p.chances[row] = top == -INFINITY ? 0.0f : 1.0f;
+            p.cuts[row].done = 1;
+            p.cuts[row].lists = 0;
+        }
+        return;
+    }
 #pragma unroll
     for (int c = 0; c < kMaxChunks; c++) m += masses[c];
     const u64 before_m = block_before<kWaves>(m, sh.part, &all_m);
@@ -377,7 +390,8 @@ __global__ __launch_bounds__(kThreads, 8) void sample_cut_kernel(SampleParams p)
         sh.mass_after = before_m + m;
     }
     __syncthreads();
-    Cut c{kBins, -1, sh.last, sh.before_last, sh.mass_last, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0, r.has_p};
+    Cut c{kBins, -1, sh.last, sh.before_last, sh.mass_last, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0, r.has_p, 0, r.top_k, r.top_p,
+          top_of(top), r.scale, double(r.min_p) * (1.0 - 0x1p-50) * p.unit};  // (a little less: the rounding of weights)
     if (r.has_p) {
         // the cut's bin, for a total between the weight under `last` and that up to it
         const double least = double(r.top_p) * double(sh.mass_last) * (1.0 - 0x1p-50);
@@ -450,14 +464,11 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleParams p
     __shared__ u64 found[kList];
     __shared__ unsigned count, base;
     const Place a = place_of(p);
-    const Row r = row_of(p, a.row);
-    const float top = unordered(unsigned(row_top(p, a.row) >> 32));
-    if (r.greedy || top == -INFINITY) return;  // the whole workgroup
-    const Cut c = p.cuts[a.row];
-    if (!c.lists) return;
+    const Cut &c = p.cuts[a.row];
+    if (!c.lists) return;  // the whole workgroup
     if (threadIdx.x == 0) count = 0;
-    __syncthreads();
     const float whole = c.whole, listed = c.listed, before = c.before, tie = c.tie;
+    __syncthreads();
     for_tokens(a.x, a.begin, a.end, threadIdx.x, kThreads, [&](float x, int i) {
         if (!((x >= listed && !(x >= whole)) || (x >= tie && !(x >= before)))) return;
         const unsigned at = atomicAdd(&count, 1u);
@@ -495,29 +506,17 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
 {
     __shared__ DrawShared sh;
     const int row = int(blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Row r = row_of(p, row);
-    const u64 first_token = row_top(p, row);
-    const float first_logit = unordered(unsigned(first_token >> 32));
-    if (r.greedy || first_logit == -INFINITY) {
-        if (tid == 0) {
-            p.tokens[row] = first_logit == -INFINITY ? -1 : int(~unsigned(first_token));
-            if (p.chances) p.chances[row] = first_logit == -INFINITY ? 0.0f : 1.0f;
-        }
-        return;
-    }
-    const double top = top_of(first_logit);
+    const Cut c = p.cuts[row];
+    if (c.done) return;
+    const double top = c.top, scale = c.scale, least = c.least;
     if (tid == 0) {
         sh.chosen = sh.mass_before = 0;
         sh.count_before = sh.digit = sh.inside = 0;
     }
-    sh.middles[tid] = middle_of(tid) * p.unit;
-    __syncthreads();
-    auto weight = [&](double t, int b) { return weight_of(t, sh.middles[b]); };
-    const Cut c = p.cuts[row];
     const float *x = p.logits + size_t(row) * p.stride;
     const unsigned listed = c.lists ? p.listed[row] : 0;
     const bool kept_here = listed <= unsigned(kList);
-    const double least = double(r.min_p) * (1.0 - 0x1p-50) * p.unit;  // (less than the rounding of weights)
+    auto weight = [&](double t, int b) { return weight_of(t, middle_of(b) * p.unit); };
     // f(key, weight, bin) for the listed tokens
     auto for_listed = [&](auto f) {
         if (kept_here) {
@@ -528,7 +527,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         }
         for (int i = tid; i < p.vocab; i += kThreads) {
             const float v = plain_logit(x[i]);
-            const double t = bins_of(v, top, r.scale);
+            const double t = bins_of(v, top, scale);
             const int b = bin_of(t);
             if (b == kBins - 1 || !is_listed(c, b)) continue;
             f(u64(~ordered(v)) << 32 | unsigned(i), units_of(weight(t, b)), b);
@@ -539,7 +538,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
             const u64 e = p.list[size_t(row) * kList + i];
             const float v = __uint_as_float(unsigned(e >> 32));
             sh.key[i] = u64(~ordered(v)) << 32 | unsigned(e);
-            const double t = bins_of(v, top, r.scale);
+            const double t = bins_of(v, top, scale);
             sh.weight[i] = units_of(weight(t, bin_of(t)));
             sh.bin[i] = (unsigned short)(bin_of(t));
         }
@@ -678,12 +677,12 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     u64 cut = ~0ull, total = c.mass_last;
     if (c.last < kBins) {
         u64 upto;
-        cut = select(true, unsigned(r.top_k) - c.before_last, 0, order, [&](u64, u64, int b) { return b == c.last; }, &upto);
+        cut = select(true, unsigned(c.top_k) - c.before_last, 0, order, [&](u64, u64, int b) { return b == c.last; }, &upto);
         total = c.mass_last + upto;
     }
     if (c.by_p) {
         // the first token whose running weight reaches top_p of the total: exceeds the whole number before
-        const double goal = double(r.top_p) * double(total);
+        const double goal = double(c.top_p) * double(total);
         u64 over = u64(ceil(goal));
         over = over > 0 ? over - 1 : 0;
         over = over >= total ? total - 1 : over;
@@ -695,7 +694,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     // the kept weight: the chunks', and the listed tokens up to the cut
     auto kept = [&](u64 k, double e) { return k <= cut && !(e < least); };
     auto keeps = [&](u64 k, u64, int b) {
-        return k <= cut && (least == 0.0 || kept(k, weight(bins_of(unordered(~unsigned(k >> 32)), top, r.scale), b)));
+        return k <= cut && (least == 0.0 || kept(k, weight(bins_of(unordered(~unsigned(k >> 32)), top, scale), b)));
     };
     const bool whole = c.low > 0;  // some bins are kept whole
     if (tid < 256) sh.mass[tid] = whole && tid < p.chunks ? p.whole[size_t(row) * p.chunks + tid] : 0;
@@ -728,14 +727,16 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         sh.mass_before = before;
     }
     __syncthreads();
+    sh.middles[tid] = middle_of(tid) * p.unit;
     // the chunk again: which wave's part of it, then which token of that
+    __syncthreads();
     const int begin = int(sh.digit) * p.chunk, end = min(begin + p.chunk, p.vocab);
     goal -= sh.mass_before;
     auto units = [&](float v, int i) {
-        const double t = bins_of(v, top, r.scale);
+        const double t = bins_of(v, top, scale);
         const int b = bin_of(t);
         if (b == kBins - 1 || !(b < c.low || is_listed(c, b))) return u64(0);
-        const double e = weight(t, b);
+        const double e = weight_of(t, sh.middles[b]);
         if (b >= c.low && !kept(u64(~ordered(v)) << 32 | unsigned(i), e)) return u64(0);
         return units_of(e);
     };
