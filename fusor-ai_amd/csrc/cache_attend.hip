@@ -775,7 +775,8 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
     const size_t row_tiles = pairs / tm + sequences, slots = std::max<size_t>(kWorkgroups / c->kv_heads, 2);
     l.grid = row_tiles;
     // fewer tiles than the chip takes at once: their pages are split so that all tasks run at once
-    if (pairs / tm < slots / 2 && b->max_pages > size_t(kMinPages)) {
+    // (not tables of few pages: joining costs about the time of four pages, and as much again on the host)
+    if (pairs / tm < slots / 2 && b->max_pages > size_t(4 * kMinPages)) {
         l.target = int(slots - std::min(row_tiles, slots / 2));
         const size_t most = std::min<size_t>((b->max_pages + kMinPages - 1) / kMinPages, kMaxSplit);
         l.grid = std::min(row_tiles * most, row_tiles + l.target);
@@ -825,8 +826,16 @@ int launch_attend(const AttendParams &p, const Launch &l, hipStream_t s)
 
 using namespace fg;
 
+extern "C" size_t fg_cache_attend_scratch(const fg_cache *c, const fg_batch *b, size_t heads)
+{
+    if (!c || !b || !heads || heads % c->kv_heads) return 0;
+    const Launch l = plan_launch(c, b, heads);
+    return l.note_bytes + l.partial_bytes;
+}
+
 extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float *query, size_t query_stride, size_t heads,
-                               float scale, size_t window, float *out, size_t out_stride, void *stream)
+                               float scale, size_t window, float *out, size_t out_stride, void *scratch, size_t scratch_bytes,
+                               void *stream)
 {
     int rc = check_batch(c, b, "fg_cache_attend");
     if (rc) return rc;
@@ -860,7 +869,8 @@ extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float
     p.target = l.target;
     void *ws = nullptr;
     bool owned = false;
-    FG_HIP(stream_scratch(l.note_bytes + l.partial_bytes, s, &ws, &owned));
+    rc = stream_scratch(scratch, scratch_bytes, l.note_bytes + l.partial_bytes, "fg_cache_attend", s, &ws, &owned);
+    if (rc) return rc;
     p.notes = static_cast<Note *>(ws);
     p.partial = reinterpret_cast<float *>(static_cast<char *>(ws) + l.note_bytes);
     switch (c->padded) {

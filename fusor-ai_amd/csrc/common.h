@@ -466,9 +466,10 @@ struct ProductArgs {
 size_t product_scratch_bytes(const ProductArgs &a);
 // A stream-ordered allocation from this device's workspace pool (kept across calls).
 hipError_t workspace_alloc(void **ptr, size_t bytes, hipStream_t s);
-// Scratch of one call queued on `s`: the capture's graph owns it while `s` is capturing, else it comes
-// from the workspace pool and *owned says that the caller frees it on `s` once its work is queued.
-hipError_t stream_scratch(size_t bytes, hipStream_t s, void **ws, bool *owned);
+// Scratch of one call queued on `s`: what the program gives it, if that is enough; else the capture's graph
+// owns it while `s` is capturing; else it comes from the workspace pool and *owned says that the caller
+// frees it on `s` once its work is queued.
+int stream_scratch(void *given, size_t given_bytes, size_t bytes, const char *who, hipStream_t s, void **ws, bool *owned);
 int launch_matvec(const ProductArgs &a, hipStream_t s);
 int launch_gemm(const ProductArgs &a, hipStream_t s);
 // `items` products of pre-quantized rows of one shape in one launch (the staged kernel): item z's

@@ -2187,9 +2187,18 @@ hipError_t scratch_for(const ProductArgs &a, size_t bytes, hipStream_t s, void *
     return workspace_alloc(ws, bytes, s);
 }
 
-hipError_t stream_scratch(size_t bytes, hipStream_t s, void **ws, bool *owned)
+int stream_scratch(void *given, size_t given_bytes, size_t bytes, const char *who, hipStream_t s, void **ws, bool *owned)
 {
-    return scratch_for(ProductArgs{}, bytes, s, ws, owned);
+    *owned = false;
+    if (given && bytes) {
+        if (given_bytes < bytes || (reinterpret_cast<uintptr_t>(given) & 15))
+            return set_error(FG_ERR_SHAPE, std::string(who) + ": " + std::to_string(given_bytes) + " bytes of scratch, " +
+                                               std::to_string(bytes) + " needed, 16-byte aligned");
+        *ws = given;
+        return FG_OK;
+    }
+    FG_HIP(scratch_for(ProductArgs{}, bytes, s, ws, owned));
+    return FG_OK;
 }
 
 int launch_t2(const ProductArgs &a, hipStream_t s)

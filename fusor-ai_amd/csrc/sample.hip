@@ -774,8 +774,49 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
 
 using namespace fg;
 
+namespace {
+
+// How a call's rows are taken: the rows of a batch, the chunks of a row, and the scratch.
+struct Shape {
+    size_t batch;
+    int chunks, chunk;
+    size_t at[8];  // where the scratch's parts start, and its end
+};
+
+Shape shape_of(size_t rows, size_t vocab)
+{
+    Shape s{};
+    // rows of a batch: what the Infinity Cache (256 MB) holds beside the rest
+    const size_t most = std::max<size_t>(1, std::min({rows, (size_t(192) << 20) / (vocab * 4), size_t(2048)}));
+    const size_t batches = (rows + most - 1) / most;
+    s.batch = (rows + batches - 1) / batches;
+    // Chunks of a row: the chip takes 512 workgroups at once, each of which costs about 2 us and 0.6 ns a
+    // logit (the bins of 64 rows of 151936: 8 chunks, one round, 13 us; 16 chunks, two rounds, 16 us), and
+    // the draw walks one chunk of every row, 0.4 ns a logit (331 rows: 3 chunks 44 us, 6 chunks 32).
+    double best = 0.0;
+    for (size_t c = 1; c <= size_t(kMaxChunks) && (c == 1 || (vocab + c - 1) / c >= 4096); c++) {
+        const double cost = double((s.batch * c + 511) / 512) * (2000.0 + 0.6 * double(vocab) / double(c)) + 0.4 * double(vocab) / double(c);
+        if (c == 1 || cost < best) {
+            best = cost;
+            s.chunks = int(c);
+        }
+    }
+    s.chunk = int((vocab + size_t(s.chunks) - 1) / size_t(s.chunks) + 255) / 256 * 256;
+    const size_t work = s.batch * s.chunks;
+    const size_t sizes[7] = {work * 8, work * kBins * 8, work * kBins * 4, work * 8, s.batch * sizeof(Cut), s.batch * 4, s.batch * kList * 8};
+    for (int i = 0; i < 7; i++) s.at[i + 1] = s.at[i] + (sizes[i] + 255) / 256 * 256;
+    return s;
+}
+
+}  // namespace
+
+extern "C" size_t fg_sample_scratch(size_t rows, size_t vocab)
+{
+    return rows && vocab && rows <= (size_t(1) << 20) && vocab <= (size_t(1) << 22) ? shape_of(rows, vocab).at[7] : 0;
+}
+
 extern "C" int fg_sample(const float *logits, size_t rows, size_t vocab, size_t stride, const fg_sampling *settings, int32_t *tokens,
-                         float *chances, void *stream)
+                         float *chances, void *scratch, size_t scratch_bytes, void *stream)
 {
     if (rows > (size_t(1) << 20) || vocab > (size_t(1) << 22))
         return set_error(FG_ERR_SHAPE, "fg_sample: at most 2^20 rows and 2^22 logits a row");
@@ -790,37 +831,22 @@ extern "C" int fg_sample(const float *logits, size_t rows, size_t vocab, size_t 
     int bits = 0;
     while ((size_t(1) << bits) < vocab) bits++;
     p.unit = double(size_t(1) << std::min(45, 63 - bits));
-    // rows of a batch: what the Infinity Cache (256 MB) holds beside the rest
-    const size_t most = std::max<size_t>(1, std::min({rows, (size_t(192) << 20) / (vocab * 4), size_t(2048)}));
-    const size_t batches = (rows + most - 1) / most, batch = (rows + batches - 1) / batches;
-    // Chunks of a row: the chip takes 512 workgroups at once, each of which costs about 2 us and 0.6 ns a
-    // logit (the bins of 64 rows of 151936: 8 chunks, one round, 13 us; 16 chunks, two rounds, 16 us), and
-    // the draw walks one chunk of every row, 0.4 ns a logit (331 rows: 3 chunks 44 us, 6 chunks 32).
-    double best = 0.0;
-    for (size_t c = 1; c <= size_t(kMaxChunks) && (c == 1 || (vocab + c - 1) / c >= 4096); c++) {
-        const double cost = double((batch * c + 511) / 512) * (2000.0 + 0.6 * double(vocab) / double(c)) + 0.4 * double(vocab) / double(c);
-        if (c == 1 || cost < best) {
-            best = cost;
-            p.chunks = int(c);
-        }
-    }
-    p.chunk = int((vocab + size_t(p.chunks) - 1) / size_t(p.chunks) + 255) / 256 * 256;
-    const size_t work = batch * p.chunks;
-    const size_t sizes[7] = {work * 8, work * kBins * 8, work * kBins * 4, work * 8, batch * sizeof(Cut), batch * 4, batch * kList * 8};
-    size_t at[8] = {0};
-    for (int i = 0; i < 7; i++) at[i + 1] = at[i] + (sizes[i] + 255) / 256 * 256;
+    const Shape shape = shape_of(rows, vocab);
+    const size_t batch = shape.batch;
+    p.chunks = shape.chunks;
+    p.chunk = shape.chunk;
     void *ws = nullptr;
     bool owned = false;
-    FG_HIP(stream_scratch(at[7], s, &ws, &owned));
+    int rc = stream_scratch(scratch, scratch_bytes, shape.at[7], "fg_sample", s, &ws, &owned);
+    if (rc) return rc;
     char *base = static_cast<char *>(ws);
-    p.top = reinterpret_cast<u64 *>(base + at[0]);
-    p.mass = reinterpret_cast<u64 *>(base + at[1]);
-    p.count = reinterpret_cast<unsigned *>(base + at[2]);
-    p.whole = reinterpret_cast<u64 *>(base + at[3]);
-    p.cuts = reinterpret_cast<Cut *>(base + at[4]);
-    p.listed = reinterpret_cast<unsigned *>(base + at[5]);
-    p.list = reinterpret_cast<u64 *>(base + at[6]);
-    int rc = FG_OK;
+    p.top = reinterpret_cast<u64 *>(base + shape.at[0]);
+    p.mass = reinterpret_cast<u64 *>(base + shape.at[1]);
+    p.count = reinterpret_cast<unsigned *>(base + shape.at[2]);
+    p.whole = reinterpret_cast<u64 *>(base + shape.at[3]);
+    p.cuts = reinterpret_cast<Cut *>(base + shape.at[4]);
+    p.listed = reinterpret_cast<unsigned *>(base + shape.at[5]);
+    p.list = reinterpret_cast<u64 *>(base + shape.at[6]);
     for (size_t r = 0; r < rows && rc == FG_OK; r += batch) {
         const unsigned n = unsigned(std::min(batch, rows - r)), grid = n * unsigned(p.chunks);
         p.logits = logits + r * stride;

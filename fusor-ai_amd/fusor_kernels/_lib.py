@@ -83,8 +83,10 @@ SIGNATURES = {
     "fg_cache_free": (_I, [_P]),
     "fg_cache_write": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
     "fg_cache_read": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
-    "fg_cache_attend": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _S, _F, _S, _P, _S, _P]),
-    "fg_sample": (_I, [_P, _S, _S, _S, ctypes.POINTER(FgSampling), _P, _P, _P]),
+    "fg_cache_attend": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _S, _F, _S, _P, _S, _P, _S, _P]),
+    "fg_cache_attend_scratch": (_S, [_P, ctypes.POINTER(FgBatch), _S]),
+    "fg_sample": (_I, [_P, _S, _S, _S, ctypes.POINTER(FgSampling), _P, _P, _P, _S, _P]),
+    "fg_sample_scratch": (_S, [_S, _S]),
     "fg_quantize_rows": (_I, [_P, _S, _I, _P, _P, _P, _P]),
     "fg_matmul": (_I, [_P, ctypes.POINTER(FgInput), _S, _S, _S, _P, _P, _S, _I, _P]),
     "fg_matmul_noalloc": (_I, [_P, ctypes.POINTER(FgInput), _S, _S, _S, _P, _P, _S, _I, _P]),

@@ -16,9 +16,21 @@ from ._lib import FgBatch, FgSampling, ShapeError, check, lib, ptr, stream_handl
 PAGE = 64  # tokens of a page: FG_CACHE_PAGE
 
 
+class _Here:
+    """A context that changes nothing (contextlib.nullcontext costs a call twice as much)."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *error):
+        pass
+
+
+_here = _Here()
+
+
 @contextlib.contextmanager
 def _on(device, stream):
-    """The tensors' device current, and with `stream` that stream too (outputs are then its own)."""
     import torch
     with torch.cuda.device(device):
         if stream is None:
@@ -29,10 +41,19 @@ def _on(device, stream):
 
 
 def _place(device, stream):
+    """The tensors' device current, and with `stream` that stream too (what a call allocates is then its
+    own)."""
     import torch
-    if stream is None and torch.cuda.is_initialized() and device.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
+    if stream is None and device.index == torch._C._cuda_getDevice():
+        return _here
     return _on(device, stream)
+
+
+def _scratch(size, device):
+    """Device memory of a call from torch's allocator, which hands it out again in the stream's order
+    (a graph that is captured keeps what it uses), for about a fifth of what the library's pool costs."""
+    import torch
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def _check_ints(name, t, shape):
@@ -46,15 +67,17 @@ def _check_ints(name, t, shape):
 def _check_heads(name, t, heads, head_dim, device, written):
     """[rows, heads, head_dim] float32 whose rows are runs of heads * head_dim values."""
     import torch
-    if t.dtype != torch.float32 or t.device != device:
+    if t.dtype is not torch.float32 or t.device != device:
         raise ShapeError(f"{name}: a float32 tensor on {device}")
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-        raise ShapeError(f"{name} of shape {list(t.shape)}, [rows, {heads}, {head_dim}] expected")
-    if t.shape[0] == 0:
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ShapeError(f"{name} of shape {list(shape)}, [rows, {heads}, {head_dim}] expected")
+    row, head, value = t.stride()
+    if shape[0] == 0:
         return
-    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim):
+    if value != 1 or (heads > 1 and head != head_dim):
         raise ShapeError(f"{name}: a row's heads lie one after the other")
-    if written and t.shape[0] > 1 and t.stride(0) < heads * head_dim:
+    if written and shape[0] > 1 and row < heads * head_dim:
         raise ShapeError(f"{name}: its rows overlap")
 
 
@@ -155,10 +178,12 @@ class PagedCache:
             _check_heads("out", out, heads, self.head_dim, self.device, True)
             if out.shape[0] != queries.shape[0]:
                 raise ShapeError(f"{queries.shape[0]} rows of queries and {out.shape[0]} of out")
-            fg = batch._ffi(queries.shape[0])
-            check(lib().fg_cache_attend(self.handle, ctypes.byref(fg), ptr(queries), queries.stride(0), heads,
-                                        1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, ptr(out),
-                                        out.stride(0), stream_handle()))
+            fg, library = ctypes.byref(batch._ffi(queries.shape[0])), lib()
+            size = library.fg_cache_attend_scratch(self.handle, fg, heads)
+            scratch = _scratch(size, self.device)
+            check(library.fg_cache_attend(self.handle, fg, ptr(queries), queries.stride(0), heads,
+                                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, ptr(out),
+                                          out.stride(0), ptr(scratch), size, stream_handle()))
         return out
 
 
@@ -173,20 +198,21 @@ def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None,
     rows, vocab = logits.shape
     if rows and vocab > 1 and logits.stride(1) != 1:
         raise ShapeError("logits: a row's values lie one after the other")
-    given = {"random": (random, torch.float32), "temperature": (temperature, torch.float32), "top_k": (top_k, torch.int32),
-             "top_p": (top_p, torch.float32), "min_p": (min_p, torch.float32), "tokens": (tokens, torch.int32),
-             "chances": (chances, torch.float32)}
-    for name, (t, dtype) in given.items():
-        if t is None and name != "random":
-            continue
-        if t.dtype != dtype or t.device != logits.device or list(t.shape) != [rows] or not t.is_contiguous():
-            raise ShapeError(f"{name}: a contiguous {dtype} tensor [{rows}] on {logits.device}")
+    device, shape, f32, i32 = logits.device, (rows,), torch.float32, torch.int32
+    if random is None:
+        raise ShapeError("random: one number a row")
+    for name, t, dtype in (("random", random, f32), ("temperature", temperature, f32), ("top_k", top_k, i32), ("top_p", top_p, f32),
+                           ("min_p", min_p, f32), ("tokens", tokens, i32), ("chances", chances, f32)):
+        if t is not None and (t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous()):
+            raise ShapeError(f"{name}: a contiguous {dtype} tensor [{rows}] on {device}")
     with _place(logits.device, stream):
         if tokens is None:
             tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
         if chances is None:
             chances = torch.empty(rows, dtype=torch.float32, device=logits.device)
         fg = FgSampling(ptr(random), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p))
+        size = lib().fg_sample_scratch(rows, vocab)
+        scratch = _scratch(size, logits.device)
         check(lib().fg_sample(ptr(logits), rows, vocab, logits.stride(0), ctypes.byref(fg), ptr(tokens), ptr(chances),
-                              stream_handle()))
+                              ptr(scratch), size, stream_handle()))
     return tokens, chances

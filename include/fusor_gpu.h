@@ -215,10 +215,14 @@ int fg_cache_read(const fg_cache *cache, const fg_batch *batch, float *key, size
  * position p sees its sequence's keys at positions max(0, p - window + 1) .. p, all up to p where
  * `window` is 0. Head h of row r is the head_dim device f32 values at r * stride + h * head_dim of
  * `query` and `out`; `heads` query heads share the cache's heads in consecutive runs. Scores are
- * scale * q.k; a row that sees no key gives 0. The work is ordered on `stream`; scratch as for
- * fg_matmul, under capture included. */
+ * scale * q.k; a row that sees no key gives 0. The work is ordered on `stream`.
+ * `scratch`: device memory of at least fg_cache_attend_scratch's bytes, 16-byte aligned, that nothing else
+ * uses until the call's work is done (two graphs that replay at once need one each); NULL: taken from the
+ * library's pool as for fg_matmul, under capture too, which costs the call about 8 us of host time. */
+size_t fg_cache_attend_scratch(const fg_cache *cache, const fg_batch *batch, size_t heads);
 int fg_cache_attend(const fg_cache *cache, const fg_batch *batch, const float *query, size_t query_stride, size_t heads,
-                    float scale, size_t window, float *out, size_t out_stride, void *stream);
+                    float scale, size_t window, float *out, size_t out_stride, void *scratch, size_t scratch_bytes,
+                    void *stream);
 
 /* Next tokens drawn from logits (Prediction::predict, lm.rs:147-166, takes the largest). Row r of the
  * device f32 `logits`, at r * stride, orders its tokens by logit, the largest first, equal ones by
@@ -237,9 +241,11 @@ typedef struct {
 } fg_sampling;
 
 /* The tokens of `rows` rows of `vocab` logits (at most 2^22) into device `tokens` [rows]; `chances`
- * [rows] may be NULL. A row with no logit above -inf gives token -1 and chance 0. */
+ * [rows] may be NULL. A row with no logit above -inf gives token -1 and chance 0. `scratch` as for
+ * fg_cache_attend, of at least fg_sample_scratch's bytes, or NULL. */
+size_t fg_sample_scratch(size_t rows, size_t vocab);
 int fg_sample(const float *logits, size_t rows, size_t vocab, size_t stride, const fg_sampling *settings,
-              int32_t *tokens, float *chances, void *stream);
+              int32_t *tokens, float *chances, void *scratch, size_t scratch_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ activations */
 

@@ -116,16 +116,20 @@ def test_refusals_before_any_device_work():
     batch = _lib.FgBatch(1, 1, 1, None, None, None)
     for rc, message in (call("fg_cache_write", None, ctypes.byref(batch), None, 0, None, 0, None),
                         call("fg_cache_read", None, ctypes.byref(batch), None, 0, None, 0, None),
-                        call("fg_cache_attend", None, ctypes.byref(batch), None, 0, 2, 1.0, 0, None, 0, None)):
+                        call("fg_cache_attend", None, ctypes.byref(batch), None, 0, 2, 1.0, 0, None, 0, None, 0, None)):
         assert rc == _lib.FG_ERR_ARG and "null cache" in message
     settings = _lib.FgSampling(None, None, None, None, None)
     some = ctypes.c_void_p(256)  # refused before it is looked at
-    assert call("fg_sample", some, 1, 8, 8, None, some, None, None)[0] == _lib.FG_ERR_ARG
-    assert call("fg_sample", some, 1, 8, 8, ctypes.byref(settings), some, None, None)[0] == _lib.FG_ERR_ARG
-    assert call("fg_sample", some, 1, 0, 8, ctypes.byref(settings), some, None, None)[0] == _lib.FG_ERR_SHAPE
-    assert call("fg_sample", some, 1, (1 << 22) + 1, 8, ctypes.byref(settings), some, None, None)[0] == _lib.FG_ERR_SHAPE
-    assert call("fg_sample", some, (1 << 20) + 1, 8, 8, ctypes.byref(settings), some, None, None)[0] == _lib.FG_ERR_SHAPE
-    assert call("fg_sample", None, 0, 8, 8, ctypes.byref(settings), None, None, None)[0] == _lib.FG_OK  # no rows
+    assert call("fg_sample", some, 1, 8, 8, None, some, None, None, 0, None)[0] == _lib.FG_ERR_ARG
+    assert call("fg_sample", some, 1, 8, 8, ctypes.byref(settings), some, None, None, 0, None)[0] == _lib.FG_ERR_ARG
+    assert call("fg_sample", some, 1, 0, 8, ctypes.byref(settings), some, None, None, 0, None)[0] == _lib.FG_ERR_SHAPE
+    assert call("fg_sample", some, 1, (1 << 22) + 1, 8, ctypes.byref(settings), some, None, None, 0, None)[0] == _lib.FG_ERR_SHAPE
+    assert call("fg_sample", some, (1 << 20) + 1, 8, 8, ctypes.byref(settings), some, None, None, 0, None)[0] == _lib.FG_ERR_SHAPE
+    assert call("fg_sample", None, 0, 8, 8, ctypes.byref(settings), None, None, None, 0, None)[0] == _lib.FG_OK  # no rows
+    # scratch sizes: of calls that would be refused, none
+    sizes = _lib.lib().fg_sample_scratch
+    assert sizes(0, 8) == sizes(8, 0) == sizes(1, (1 << 22) + 1) == 0 and 0 < sizes(1, 8) <= sizes(7, 8) <= sizes(7, 151936)
+    assert _lib.lib().fg_cache_attend_scratch(None, ctypes.byref(batch), 2) == 0
 
 
 def test_the_plain_forms_agree_with_torch():
