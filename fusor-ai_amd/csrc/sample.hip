@@ -9,6 +9,8 @@
 //   3 cut      from the bins, which are kept whole and which hold a cut, and the logits between them;
 //   4 collect  a list of the tokens whose bins hold a cut (or of all tokens up to it, where they are few);
 //   5 draw     the cut among the list; the chunk, or the listed token, on which the random number falls.
+// Few rows take a launch for each, their chunks over the chip; many rows all five in one workgroup a row
+// (sample_route.h).
 // Weights are 64-bit: exp in f64 (one ulp), rounded to a whole number of units of 2^-45 of the first token's
 // (less for more than 2^18 tokens), so that every sum is exact and their order changes nothing. Tokens
 // under half a unit (z < -31.9) weigh 0; the last bin holds only such.
@@ -16,6 +18,7 @@
 #include <type_traits>
 
 #include "cache.h"
+#include "sample_route.h"
 
 namespace fg {
 namespace {
@@ -30,7 +33,7 @@ constexpr float kPerUnit = 32.0f;   // bins a unit of z
 constexpr int kList = 2560;         // tokens a row's list holds
 constexpr int kRank = 128;          // up to so many listed tokens are compared with each other
 constexpr int kFew = 1024;          // up to so many tokens before the cut are all listed
-constexpr int kMaxChunks = 16;      // workgroups of a row
+constexpr int kMaxChunks = kSampleChunks;
 
 // What the bins say of a row. Tokens of bins under `low` are kept whole; those of [low, high] and of
 // `last` are listed; the others are not kept. last: the bin of top-k's cut (kBins: none).
@@ -66,7 +69,7 @@ struct SampleParams {
 };
 
 // A logit's place in the order of floats as an unsigned integer; NaN is -inf, and -0 is 0.
-__device__ __forceinline__ float plain_logit(float x) { return x != x ? -INFINITY : x + 0.0f; }
+__device__ __forceinline__ float plain_logit(float x) { return fmaxf(x, -INFINITY) + 0.0f; }
 __device__ __forceinline__ unsigned ordered(float x)
 {
     const unsigned b = __float_as_uint(x);
@@ -251,16 +254,15 @@ __device__ __forceinline__ Place place_of(const SampleParams &p)
     return a;
 }
 
-__global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleParams p)
+// The largest logit of the tokens [begin, end) and its first index, (ordered logit, ~index), to every thread of
+// the workgroup. `part` is LDS of a value a wave.
+__device__ __forceinline__ u64 top_of_tokens(const float *x, int begin, int end, int none, u64 *part)
 {
-    __shared__ u64 tops[kWaves];
-    const Place a = place_of(p);
-    if (a.chunk == 0 && threadIdx.x == 0) p.listed[a.row] = 0;
     float best = -INFINITY;
-    int at = p.vocab;
-    for_tokens(a.x, a.begin, a.end, threadIdx.x, kThreads, [&](float x, int i) {
-        if (x > best) {
-            best = x;
+    int at = none;
+    for_tokens(x, begin, end, threadIdx.x, kThreads, [&](float v, int i) {
+        if (v > best) {
+            best = v;
             at = i;
         }
     });
@@ -270,12 +272,47 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleParams p)
         const u64 o = __shfl_xor(t, d, 64);
         t = o > t ? o : t;
     }
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = t;
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = t;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kWaves; w++) t = tops[w] > t ? tops[w] : t;
-        p.top[size_t(a.row) * p.chunks + a.chunk] = t;
+    t = part[threadIdx.x & (kWaves - 1)];
+#pragma unroll
+    for (int d = kWaves / 2; d; d >>= 1) {
+        const u64 o = __shfl_xor(t, d, 64);
+        t = o > t ? o : t;
     }
+    return t;
+}
+
+// The tokens [begin, end) added to the bins' weights, and with top-k to their counts (LDS).
+__device__ __forceinline__ void add_to_bins(const float *x, int begin, int end, double top, double scale, bool counts, u64 *mass,
+                                            unsigned *count, const double *middles)
+{
+    for_tokens(x, begin, end, threadIdx.x, kThreads, [&](float v, int) {
+        const double t = bins_of(v, top, scale);
+        const int b = bin_of(t);
+        const u64 w = units_of(weight_of(t, middles[b]));
+        if (b < kBins - 1) {  // (the last bin's weigh 0)
+            if (counts) atomicAdd(&count[b], 1u);
+            atomicAdd(&mass[b], w);
+        }
+    });
+}
+
+// The token of a row that keeps its first alone, or has no logit above -inf.
+__device__ __forceinline__ void write_first(const SampleParams &p, int row, u64 first)
+{
+    const bool none = unordered(unsigned(first >> 32)) == -INFINITY;
+    p.tokens[row] = none ? -1 : int(~unsigned(first));
+    if (p.chances) p.chances[row] = none ? 0.0f : 1.0f;
+}
+
+__global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleParams p)
+{
+    __shared__ u64 part[kWaves];
+    const Place a = place_of(p);
+    if (a.chunk == 0 && threadIdx.x == 0) p.listed[a.row] = 0;
+    const u64 t = top_of_tokens(a.x, a.begin, a.end, p.vocab, part);
+    if (threadIdx.x == 0) p.top[size_t(a.row) * p.chunks + a.chunk] = t;
 }
 
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams p)
@@ -288,23 +325,12 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams p)
     const float first = unordered(unsigned(row_top(p, a.row) >> 32));
     if (r.greedy || first == -INFINITY) return;  // the whole workgroup
     const int tid = threadIdx.x;
-    const double top = top_of(first);
     static_assert(kBins == kThreads, "a bin a thread");
     mass[tid] = 0;
     count[tid] = 0;
     middles[tid] = middle_of(tid) * p.unit;
     __syncthreads();
-    auto add = [&](float x) {
-        x = x != x ? -INFINITY : x;
-        const double t = bins_of(x, top, r.scale);
-        const int b = bin_of(t);
-        const u64 w = units_of(weight_of(t, middles[b]));
-        if (b < kBins - 1) {  // (the last bin's weigh 0)
-            if (r.has_k) atomicAdd(&count[b], 1u);
-            atomicAdd(&mass[b], w);
-        }
-    };
-    for_tokens(a.x, a.begin, a.end, tid, kThreads, [&](float x, int) { add(x); });
+    add_to_bins(a.x, a.begin, a.end, top_of(first), r.scale, r.has_k, mass, count, middles);
     __syncthreads();
     const size_t at = (size_t(a.row) * p.chunks + a.chunk) * kBins + tid;
     p.mass[at] = mass[tid];
@@ -341,35 +367,14 @@ __device__ __forceinline__ float smallest_of_bin(int b, float first, double scal
     return unordered(lo + n);
 }
 
-// One workgroup a row, a bin a thread.
-__global__ __launch_bounds__(kThreads, 8) void sample_cut_kernel(SampleParams p)
+// The cuts of a row, from the weight m and the tokens n of this thread's bin; chunk_mass(k): the bin's
+// weight in chunk k. Every thread of the workgroup calls and gets the result; sh.whole has the chunks' weight
+// of whole bins.
+template <class F>
+__device__ __forceinline__ Cut cut_of(const SampleParams &p, const Row &r, float top, u64 m, u64 n, CutShared &sh, F chunk_mass)
 {
-    __shared__ CutShared sh;
-    const int row = int(blockIdx.x), tid = threadIdx.x;
-    const Row r = row_of(p, row);
-    // the chunks' weights stay in registers for the sums under `low`
-    u64 masses[kMaxChunks], m = 0, n = 0, all_n = 0, all_m, before_n = 0;
-    const u64 *mass = p.mass + size_t(row) * p.chunks * kBins + tid;
-    const unsigned *count = p.count + size_t(row) * p.chunks * kBins + tid;
-#pragma unroll
-    for (int c = 0; c < kMaxChunks; c++) masses[c] = c < p.chunks ? mass[c * kBins] : 0;
-    if (r.has_k) {
-#pragma unroll
-        for (int c = 0; c < kMaxChunks; c++) n += c < p.chunks ? count[c * kBins] : 0;
-    }
-    const u64 first = row_top(p, row);
-    const float top = unordered(unsigned(first >> 32));
-    if (r.greedy || top == -INFINITY) {  // (its bins are not written: what was read is not used)
-        if (tid == 0) {
-            p.tokens[row] = top == -INFINITY ? -1 : int(~unsigned(first));
-            if (p.chances) p.chances[row] = top == -INFINITY ? 0.0f : 1.0f;
-            p.cuts[row].done = 1;
-            p.cuts[row].lists = 0;
-        }
-        return;
-    }
-#pragma unroll
-    for (int c = 0; c < kMaxChunks; c++) m += masses[c];
+    const int tid = threadIdx.x;
+    u64 all_n = 0, all_m, before_n = 0;
     const u64 before_m = block_before<kWaves>(m, sh.part, &all_m);
     if (r.has_k) before_n = block_before<kWaves>(n, sh.part, &all_n);
     if (tid == 0) {
@@ -432,9 +437,8 @@ __global__ __launch_bounds__(kThreads, 8) void sample_cut_kernel(SampleParams p)
     if (tid == c.low) sh.mass_low = before_m;
     // the chunks' weight under `low`
     if (c.low > 0) {
-#pragma unroll
-        for (int k = 0; k < kMaxChunks; k++) {
-            const u64 w = wave_upto(tid < c.low ? masses[k] : 0);
+        for (int k = 0; k < p.chunks; k++) {
+            const u64 w = wave_upto(tid < c.low ? chunk_mass(k) : 0);
             if ((tid & 63) == 63 && w) atomicAdd(&sh.whole[k], w);
         }
     }
@@ -445,19 +449,58 @@ __global__ __launch_bounds__(kThreads, 8) void sample_cut_kernel(SampleParams p)
         if ((tid & 63) == 0) sh.edge[wave] = x;
     }
     __syncthreads();
-    if (tid < p.chunks) p.whole[size_t(row) * p.chunks + tid] = sh.whole[tid];
-    if (tid == 0) {
-        c.mass_low = sh.mass_low;
-        c.lists = lists;
-        c.whole = sh.edge[0];
-        c.listed = sh.edge[1];
-        c.before = sh.edge[2];
-        c.tie = c.last < kBins ? sh.edge[3] : __builtin_nanf("");
-        p.cuts[row] = c;
+    c.mass_low = sh.mass_low;
+    c.lists = lists;
+    c.whole = sh.edge[0];
+    c.listed = sh.edge[1];
+    c.before = sh.edge[2];
+    c.tie = c.last < kBins ? sh.edge[3] : __builtin_nanf("");
+    return c;
+}
+
+// One workgroup a row, a bin a thread.
+__global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleParams p)
+{
+    __shared__ CutShared sh;
+    const int row = int(blockIdx.x), tid = threadIdx.x;
+    const Row r = row_of(p, row);
+    u64 m = 0, n = 0;
+    const u64 *mass = p.mass + size_t(row) * p.chunks * kBins + tid;
+    const unsigned *count = p.count + size_t(row) * p.chunks * kBins + tid;
+#pragma unroll
+    for (int c = 0; c < kMaxChunks; c++) m += c < p.chunks ? mass[c * kBins] : 0;
+    if (r.has_k) {
+#pragma unroll
+        for (int c = 0; c < kMaxChunks; c++) n += c < p.chunks ? count[c * kBins] : 0;
     }
+    const u64 first = row_top(p, row);
+    const float top = unordered(unsigned(first >> 32));
+    if (r.greedy || top == -INFINITY) {  // (its bins are not written: what was read is not used)
+        if (tid == 0) {
+            write_first(p, row, first);
+            p.cuts[row].done = 1;
+            p.cuts[row].lists = 0;
+        }
+        return;
+    }
+    const Cut c = cut_of(p, r, top, m, n, sh, [&](int k) { return mass[k * kBins]; });
+    if (tid < p.chunks) p.whole[size_t(row) * p.chunks + tid] = sh.whole[tid];
+    if (tid == 0) p.cuts[row] = c;
 }
 
 __device__ __forceinline__ bool is_listed(const Cut &c, int bin) { return (bin >= c.low && bin <= c.high) || bin == c.last; }
+
+// The listed ones of the tokens [begin, end) into `found` (LDS, kList of them), (logit bits, index); *count is
+// how many there are.
+__device__ __forceinline__ void list_tokens(const float *x, int begin, int end, const Cut &c, u64 *found, unsigned *count)
+{
+    const float whole = c.whole, listed = c.listed, before = c.before, tie = c.tie;
+    for_tokens(x, begin, end, threadIdx.x, kThreads, [&](float v, int i) {
+        if (!((v >= listed && !(v >= whole)) || (v >= tie && !(v >= before)))) return;
+        const unsigned at = atomicAdd(count, 1u);
+        if (at < unsigned(kList)) found[at] = u64(__float_as_uint(v)) << 32 | unsigned(i);
+    });
+}
 
 __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleParams p)
 {
@@ -467,13 +510,8 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleParams p
     const Cut &c = p.cuts[a.row];
     if (!c.lists) return;  // the whole workgroup
     if (threadIdx.x == 0) count = 0;
-    const float whole = c.whole, listed = c.listed, before = c.before, tie = c.tie;
     __syncthreads();
-    for_tokens(a.x, a.begin, a.end, threadIdx.x, kThreads, [&](float x, int i) {
-        if (!((x >= listed && !(x >= whole)) || (x >= tie && !(x >= before)))) return;
-        const unsigned at = atomicAdd(&count, 1u);
-        if (at < unsigned(kList)) found[at] = u64(__float_as_uint(x)) << 32 | unsigned(i);
-    });
+    list_tokens(a.x, a.begin, a.end, c, found, &count);
     __syncthreads();
     const unsigned n = count;
     if (n == 0) return;
@@ -483,8 +521,6 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleParams p
         if (base + i < unsigned(kList)) p.list[size_t(a.row) * kList + base + i] = found[i];
 }
 
-// One workgroup a row. The listed tokens are in LDS, or, if they are too many, found in the row again by
-// every pass over them.
 struct DrawShared {
     u64 key[kList];     // (~ordered logit, index): the order, ascending
     u64 weight[kList];
@@ -500,21 +536,20 @@ struct DrawShared {
     unsigned count_before, digit, inside;
     double middles[kBins];
 };
-static_assert(sizeof(DrawShared) <= 64 * 1024, "within the default limit of LDS");
 
-__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
+// A row's token from its cuts, by one workgroup. The list's `listed` tokens are (logit bits, index) in sh.key, or,
+// if they are too many, found in the row again by every pass over them. whole_of(k): the weight of chunk k's
+// whole bins.
+template <class F>
+__device__ __forceinline__ void draw_token(const SampleParams &p, int row, const Cut &c, unsigned listed, DrawShared &sh, F whole_of)
 {
-    __shared__ DrawShared sh;
-    const int row = int(blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Cut c = p.cuts[row];
-    if (c.done) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const double top = c.top, scale = c.scale, least = c.least;
     if (tid == 0) {
         sh.chosen = sh.mass_before = 0;
         sh.count_before = sh.digit = sh.inside = 0;
     }
     const float *x = p.logits + size_t(row) * p.stride;
-    const unsigned listed = c.lists ? p.listed[row] : 0;
     const bool kept_here = listed <= unsigned(kList);
     auto weight = [&](double t, int b) { return weight_of(t, middle_of(b) * p.unit); };
     // f(key, weight, bin) for the listed tokens
@@ -535,7 +570,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     };
     if (kept_here) {
         for (unsigned i = tid; i < listed; i += kThreads) {
-            const u64 e = p.list[size_t(row) * kList + i];
+            const u64 e = sh.key[i];
             const float v = __uint_as_float(unsigned(e >> 32));
             sh.key[i] = u64(~ordered(v)) << 32 | unsigned(e);
             const double t = bins_of(v, top, scale);
@@ -697,7 +732,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
         return k <= cut && (least == 0.0 || kept(k, weight(bins_of(unordered(~unsigned(k >> 32)), top, scale), b)));
     };
     const bool whole = c.low > 0;  // some bins are kept whole
-    if (tid < 256) sh.mass[tid] = whole && tid < p.chunks ? p.whole[size_t(row) * p.chunks + tid] : 0;
+    if (tid < 256) sh.mass[tid] = whole && tid < p.chunks ? whole_of(tid) : 0;
     __syncthreads();
     for_listed([&](u64 k, u64 w, int b) {
         if (keeps(k, w, b)) atomicAdd(&sh.mass[whole ? unsigned(k) / unsigned(p.chunk) : 0], w);
@@ -769,6 +804,67 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
     }
 }
 
+// One workgroup a row.
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleParams p)
+{
+    __shared__ DrawShared sh;
+    const int row = int(blockIdx.x);
+    const Cut c = p.cuts[row];
+    if (c.done) return;
+    const unsigned listed = c.lists ? p.listed[row] : 0;
+    for (unsigned i = threadIdx.x; i < min(listed, unsigned(kList)); i += kThreads) sh.key[i] = p.list[size_t(row) * kList + i];
+    draw_token(p, row, c, listed, sh, [&](int k) { return p.whole[size_t(row) * p.chunks + k]; });
+}
+
+// All of it for a row in one workgroup, for many rows: each row's passes over its logits and its arithmetic
+// run beside the other rows', and nothing but the chunks' bins goes through memory.
+struct RowShared {
+    union {
+        DrawShared draw;
+        struct {
+            u64 mass[kBins];
+            unsigned count[kBins];
+        } bins;
+    };
+    CutShared cut;
+    unsigned listed;
+};
+static_assert(sizeof(RowShared) <= 64 * 1024, "within the default limit of LDS");
+
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleParams p)
+{
+    __shared__ RowShared sh;
+    const int row = int(blockIdx.x), tid = threadIdx.x;
+    const Row r = row_of(p, row);
+    const float *x = p.logits + size_t(row) * p.stride;
+    const u64 first = top_of_tokens(x, 0, p.vocab, p.vocab, sh.cut.part);
+    const float top = unordered(unsigned(first >> 32));
+    if (r.greedy || top == -INFINITY) {
+        if (tid == 0) write_first(p, row, first);
+        return;
+    }
+    // (the middles lie behind the bins in the union)
+    double *middles = sh.draw.middles;
+    sh.bins.mass[tid] = 0;
+    sh.bins.count[tid] = 0;
+    middles[tid] = middle_of(tid) * p.unit;
+    u64 *upto = p.mass + size_t(row) * p.chunks * kBins + tid;  // this bin's weight up to each chunk's end
+    u64 m = 0;
+    for (int c = 0; c < p.chunks; c++) {
+        __syncthreads();
+        add_to_bins(x, c * p.chunk, min((c + 1) * p.chunk, p.vocab), top_of(top), r.scale, r.has_k, sh.bins.mass, sh.bins.count, middles);
+        __syncthreads();
+        upto[c * kBins] = m = sh.bins.mass[tid];
+    }
+    const Cut c = cut_of(p, r, top, m, r.has_k ? sh.bins.count[tid] : 0, sh.cut,
+                         [&](int k) { return upto[k * kBins] - (k ? upto[(k - 1) * kBins] : 0); });
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();  // (the bins are read: the list takes their place)
+    if (c.lists) list_tokens(x, 0, p.vocab, c, sh.draw.key, &sh.listed);
+    __syncthreads();
+    draw_token(p, row, c, sh.listed, sh.draw, [&](int k) { return sh.cut.whole[k]; });
+}
+
 }  // namespace
 }  // namespace fg
 
@@ -778,6 +874,7 @@ namespace {
 
 // How a call's rows are taken: the rows of a batch, the chunks of a row, and the scratch.
 struct Shape {
+    bool by_rows;
     size_t batch;
     int chunks, chunk;
     size_t at[8];  // where the scratch's parts start, and its end
@@ -786,25 +883,17 @@ struct Shape {
 Shape shape_of(size_t rows, size_t vocab)
 {
     Shape s{};
-    // rows of a batch: what the Infinity Cache (256 MB) holds beside the rest
-    const size_t most = std::max<size_t>(1, std::min({rows, (size_t(192) << 20) / (vocab * 4), size_t(2048)}));
+    s.by_rows = sample_by_rows(rows, vocab);
+    // rows of a batch: bounded scratch; by chunks, what the Infinity Cache (256 MB) holds beside the rest
+    size_t most = std::min<size_t>(rows, 2048);
+    if (!s.by_rows) most = std::max<size_t>(1, std::min(most, (size_t(192) << 20) / (vocab * 4)));
     const size_t batches = (rows + most - 1) / most;
     s.batch = (rows + batches - 1) / batches;
-    // Chunks of a row: the chip takes 512 workgroups at once, each of which costs about 2 us and 0.6 ns a
-    // logit (the bins of 64 rows of 151936: 8 chunks, one round, 13 us; 16 chunks, two rounds, 16 us), and
-    // the draw walks one chunk of every row, 0.4 ns a logit (331 rows: 3 chunks 44 us, 6 chunks 32).
-    double best = 0.0;
-    for (size_t c = 1; c <= size_t(kMaxChunks) && (c == 1 || (vocab + c - 1) / c >= 4096); c++) {
-        const double cost = double((s.batch * c + 511) / 512) * (2000.0 + 0.6 * double(vocab) / double(c)) + 0.4 * double(vocab) / double(c);
-        if (c == 1 || cost < best) {
-            best = cost;
-            s.chunks = int(c);
-        }
-    }
+    s.chunks = sample_chunks(s.batch, vocab, s.by_rows);
     s.chunk = int((vocab + size_t(s.chunks) - 1) / size_t(s.chunks) + 255) / 256 * 256;
     const size_t work = s.batch * s.chunks;
-    const size_t sizes[7] = {work * 8, work * kBins * 8, work * kBins * 4, work * 8, s.batch * sizeof(Cut), s.batch * 4, s.batch * kList * 8};
-    for (int i = 0; i < 7; i++) s.at[i + 1] = s.at[i] + (sizes[i] + 255) / 256 * 256;
+    size_t sizes[7] = {work * 8, work * kBins * 8, work * kBins * 4, work * 8, s.batch * sizeof(Cut), s.batch * 4, s.batch * kList * 8};
+    for (int i = 0; i < 7; i++) s.at[i + 1] = s.at[i] + (s.by_rows && i != 1 ? 0 : (sizes[i] + 255) / 256 * 256);
     return s;
 }
 
@@ -857,11 +946,15 @@ extern "C" int fg_sample(const float *logits, size_t rows, size_t vocab, size_t 
         p.min_p = settings->min_p ? settings->min_p + r : nullptr;
         p.tokens = tokens + r;
         p.chances = chances ? chances + r : nullptr;
-        sample_top_kernel<<<grid, kThreads, 0, s>>>(p);
-        sample_bins_kernel<<<grid, kThreads, 0, s>>>(p);
-        sample_cut_kernel<<<n, kThreads, 0, s>>>(p);
-        if (p.top_k || p.top_p || p.min_p) sample_collect_kernel<<<grid, kThreads, 0, s>>>(p);
-        sample_draw_kernel<<<n, kThreads, 0, s>>>(p);
+        if (shape.by_rows) {
+            sample_row_kernel<<<n, kThreads, 0, s>>>(p);
+        } else {
+            sample_top_kernel<<<grid, kThreads, 0, s>>>(p);
+            sample_bins_kernel<<<grid, kThreads, 0, s>>>(p);
+            sample_cut_kernel<<<n, kThreads, 0, s>>>(p);
+            if (p.top_k || p.top_p || p.min_p) sample_collect_kernel<<<grid, kThreads, 0, s>>>(p);
+            sample_draw_kernel<<<n, kThreads, 0, s>>>(p);
+        }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) rc = check_hip(e, "fg_sample");
     }
