@@ -3,6 +3,7 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
+#include <utility>
 
 #include "cache.h"
 
@@ -221,54 +222,73 @@ __device__ __forceinline__ int query_shift(float amax)
 
 constexpr float kWeightLimit = 32768.0f;
 
+// Lane n of each row of 16 lanes, to every lane of its row (DPP row_newbcast, which the multiplication that
+// takes it reads by itself). A lane's scores are those of 16 keys that its row of lanes shares, so one register
+// of 16 scales a row of lanes serves them all: read by every lane the scales took as much of LDS as half
+// the levels did.
+template <int N>
+__device__ __forceinline__ float of_row_lane(float x)
+{
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + N, 0xF, 0xF, true));
+}
+template <class F, size_t... N>
+__device__ __forceinline__ void for_row_lanes(float x, F f, std::index_sequence<N...>)
+{
+    (f(int(N), of_row_lane<int(N)>(x)), ...);
+}
+// f(n, the row's scale n) for the 16 of them
+template <class F>
+__device__ __forceinline__ void for_scales(float x, F f)
+{
+    for_row_lanes(x, f, std::make_index_sequence<16>{});
+}
+
 // The running sums of a row: its reference r (-inf: no key yet, and then a total of 0) and the total of 2^(t - r) over the
 // keys that this lane holds.
 struct RowSums {
     float r, total;
 };
 
-// N scores of one row in this lane, t = s * f, to weights times the values' scales, into x; the row's other scores are in the lanes that `combine` joins. edge: keys outside [low, high] are
+// 16 scores of one row in this lane, t = s * f, to weights times the values' scales, into x; the row's other scores are in the lanes that `combine` joins. edge: keys outside [low, high] are
 // masked (key(i) is score i's position). rescale(a) scales the row's sums of this lane by a.
-template <int N, class Key, class Combine, class Rescale>
-__device__ __forceinline__ void weigh(const float (&s)[N], float (&x)[N], const float *vs, float f, bool edge, int low,
+template <class Key, class Combine, class Rescale>
+__device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], float vs, float f, bool edge, int low,
                                       int high, RowSums &sums, Key key, Combine combine, Rescale rescale)
 {
     float top = 0.0f, total = 0.0f;
     auto weights = [&]() {
         top = total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
+        for_scales(vs, [&](int i, float v) {
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], f, -sums.r));
-            x[i] = e * vs[i];
+            x[i] = v * e;
             total = total + e;
             top = fmaxf(top, x[i]);
-        }
+        });
     };
     auto masked = [&]() {
         top = total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
+        for_scales(vs, [&](int i, float v) {
             const bool seen = key(i) >= low && key(i) <= high;
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], f, -sums.r));
-            x[i] = seen ? e * vs[i] : 0.0f;
+            x[i] = seen ? v * e : 0.0f;
             total = total + (seen ? e : 0.0f);
             top = fmaxf(top, x[i]);
-        }
+        });
     };
     if (edge) masked();
     else weights();
     if (__builtin_expect(__any(top > kWeightLimit), 0)) {
         top = combine(top);
         float u = -INFINITY, m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            float v = vs[i];
-            asm volatile("" : "+v"(v));  // (keeps the logarithms in this branch)
+        float logs = vs;
+        asm volatile("" : "+v"(logs));  // (keeps the logarithm in this branch)
+        logs = __builtin_amdgcn_logf(logs);
+        for_scales(logs, [&](int i, float v) {
             const float t = s[i] * f;
             const bool seen = !edge || (key(i) >= low && key(i) <= high);
-            u = seen ? fmaxf(u, t + __builtin_amdgcn_logf(v)) : u;
+            u = seen ? fmaxf(u, t + v) : u;
             m = seen ? fmaxf(m, t) : m;
-        }
+        });
         u = combine(u);
         m = combine(m);
         if (top > kWeightLimit) {
@@ -348,10 +368,13 @@ __global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel
     const int last = task.span.first + min((task.tile * TM + TM - 1) / p.group, task.span.rows - 1);
     const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
     // A page's levels and scales stay in the same registers as the next one's: the keys' are asked for
-    // when this page's scores are formed, the values' when it is done, the id a page before.
+    // when this page's scores are formed, the values' when it is done, the id a page
+    // before, and it is looked at a page later: loads come back in order.
     uint4 k[4][J], v[T];
-    v4f ks[4], vs[4];
-    auto id_of = [&](int page) { return page < range.hi ? page_at(table, page, p.b.max_pages, p.pages) : -1; };
+    float ks, vs;  // of key and value i of the lane's row of 16
+    const int token = 32 * (g >> 1) + 8 * (i >> 2) + 4 * (g & 1) + (i & 3);
+    auto entry_of = [&](int page) { return page < range.hi ? table[page] : -1; };
+    auto id_of = [&](int entry) { return __builtin_amdgcn_readfirstlane(valid_page(entry, p.pages)); };
     auto record_of = [&](int id) { return p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP); };
     auto load_keys = [&](int id) {
         const uint8_t *record = record_of(id);
@@ -362,28 +385,23 @@ __global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel
                 const int block = min(2 * j + (g >> 1), R - 1);  // (the last dimensions of an odd count again: the queries' are 0)
                 k[t][j] = *reinterpret_cast<const uint4 *>(record + ((i >> 3) * R + block) * 1024 + ((g & 1) * 32 + 8 * t + (i & 7)) * 16);
             }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-            ks[t] = *reinterpret_cast<const v4f *>(record + key_scale_byte(DP, 32 * (g >> 1) + 8 * t + 4 * (g & 1)));
+        ks = *reinterpret_cast<const float *>(record + key_scale_byte(DP, token));
     };
     auto load_values = [&](int id) {
         const uint8_t *record = record_of(id);
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-            vs[t] = *reinterpret_cast<const v4f *>(record + value_scale_byte(DP, 32 * (g >> 1) + 8 * t + 4 * (g & 1)));
+        vs = *reinterpret_cast<const float *>(record + value_scale_byte(DP, token));
 #pragma unroll
         for (int d = 0; d < T; d++)
             v[d] = *reinterpret_cast<const uint4 *>(record + kPage * DP + ((d >> 1) * 2 + (g >> 1)) * 1024 + ((g & 1) * 32 + (d & 1) * 16 + i) * 16);
     };
-    int id = id_of(range.lo + wave), next = id_of(range.lo + wave + 4), loaded = max(id, 0);
+    int id = id_of(entry_of(range.lo + wave)), next = entry_of(range.lo + wave + 4), loaded = max(id, 0);
     load_keys(loaded);
     load_values(loaded);
     for (int page = range.lo + wave; page < range.hi; page += 4) {
-        const int after = id_of(page + 8);
         const bool held = id >= 0;
-        loaded = next >= 0 ? next : loaded;  // (what is loaded already, again, where there is no next one)
-        id = next;
-        next = after;
+        id = id_of(next);
+        loaded = id >= 0 ? id : loaded;  // (what is loaded already, again, where there is no next one)
+        next = entry_of(page + 8);
         if (!held) {
             load_keys(loaded);
             load_values(loaded);
@@ -407,26 +425,18 @@ __global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel
                         s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[mt][j][e], s[mt][t], 0, 0, 0);
                     }
                 }
+        float scores[MT][16];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) s[mt][t][r] = s[mt][t][r] * ks[t][r];
+        for (int mt = 0; mt < MT; mt++) for_scales(ks, [&](int n, float k) { scores[mt][n] = k * s[mt][n / 4][n % 4]; });
         load_keys(loaded);
         const int base = page * kPage + 32 * (g >> 1) + 4 * (g & 1);
         const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
         v8h wh[MT][2], wl[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            float scores[16], x[16], vv[16];
-#pragma unroll
-            for (int n = 0; n < 16; n++) {
-                scores[n] = s[mt][n / 4][n % 4];
-                vv[n] = vs[n / 4][n % 4];
-            }
+            float x[16];
             const int high = pair[mt].position, low = p.window > 0 ? high - p.window + 1 : 0;
-            weigh<16>(scores, x, vv, f[mt], edge, low, high, sums[mt], [&](int n) { return base + 8 * (n / 4) + n % 4; },
+            weigh(scores[mt], x, vs, f[mt], edge, low, high, sums[mt], [&](int n) { return base + 8 * (n / 4) + n % 4; },
                       [](float a) {
                           float2 w = row_pair(a);
                           w = half_pair(fmaxf(w.x, w.y));
@@ -544,7 +554,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
 
     uint4 staged[L];
     float staged_scale = 0.0f;
-    auto id_of = [&](int page) { return page < range.hi ? page_at(table, page, p.b.max_pages, p.pages) : -1; };
+    // (a table's entry is looked at an iteration after it was asked for: loads come back in order, and a
+    // look would wait for the records asked for before it)
+    auto entry_of = [&](int page) { return page < range.hi ? table[page] : -1; };
+    auto id_of = [&](int entry) { return __builtin_amdgcn_readfirstlane(valid_page(entry, p.pages)); };
     auto load = [&](int id) {  // a page's record into registers
         if (id < 0) return;
         const uint8_t *record = p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP);
@@ -564,8 +577,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     };
 #pragma unroll
     for (int c = 0; c < L; c++) staged[c] = make_uint4(0, 0, 0, 0);
-    // the pages read (-1: nothing there), staged, and known
-    int here = id_of(range.lo), next = id_of(range.lo + 1), after = id_of(range.lo + 2);
+    // the pages read (-1: nothing there), staged, and the entry of the one after
+    int here = id_of(entry_of(range.lo)), next = id_of(entry_of(range.lo + 1)), after = entry_of(range.lo + 2);
     load(here);
 
     const Pair pair = pair_of(p, task, kv, task.tile * TM + wave * 32 + l31);
@@ -607,64 +620,89 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
         const int b = (page - range.lo) & 1;
         const bool held = here >= 0;
         if (next >= 0) store(lds + (b ^ 1) * kBuffer);
-        load(after);
         here = next;
-        next = after;
-        after = id_of(page + 3);
+        next = id_of(after);
+        load(next);
+        after = entry_of(page + 3);
         const uint8_t *buffer = lds + b * kBuffer;
         const float *key_scales = reinterpret_cast<const float *>(buffer + 256 * DP), *value_scales = key_scales + kPage;
         const bool seen = held && any && page * kPage <= last && (p.window <= 0 || page * kPage + kPage - 1 > first - p.window);
         if (seen) {
             const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
-            v16f s[2];
+            const uint8_t *values = buffer + 128 * DP;
+            // The operands of a step are read while the step before multiplies: left to itself the compiler reads
+            // each step's into the registers of the one before, and waits.
+            v16f s[2] = {};
+            v8h a[2][2];
+            float ks[2], vs[2];
+            auto read_keys = [&](int k) {
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++) s[kt] = v16f{};
+                for (int kt = 0; kt < 2; kt++) a[k & 1][kt] = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + lane * 16);
+            };
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                const int token = 32 * kt + 8 * ((lane >> 2) & 3) + 4 * h + (lane & 3);
+                ks[kt] = key_scales[token];
+                vs[kt] = value_scales[token];
+            }
+            read_keys(0);
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                v8h a[2];
+                if (k + 1 < K) read_keys(k + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++) a[kt] = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + lane * 16);
+                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k & 1][kt], ql[k], s[kt], 0, 0, 0);
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kt], ql[k], s[kt], 0, 0, 0);
-#pragma unroll
-                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[kt], qh[k], s[kt], 0, 0, 0);
-            }
-            float scores[32], x[32], vs[32];
-#pragma unroll
-            for (int n = 0; n < 32; n += 4) {
-                const int token = 32 * (n / 16) + 8 * (n % 16 / 4) + 4 * h;
-                const v4f a = *reinterpret_cast<const v4f *>(key_scales + token), c = *reinterpret_cast<const v4f *>(value_scales + token);
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    vs[n + r] = c[r];
-                    scores[n + r] = s[n / 16][n % 16 + r] * a[r];
-                }
+                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k & 1][kt], qh[k], s[kt], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
             const int high = pair.position, low = p.window > 0 ? high - p.window + 1 : 0;
-            weigh<32>(scores, x, vs, f, edge, low, high, sums,
-                      [&](int n) { return page * kPage + 32 * (n / 16) + 8 * (n % 16 / 4) + 4 * h + n % 4; },
-                      [](float a) {
-                          const float2 w = half_pair(a);
-                          return fmaxf(w.x, w.y);
-                      },
-                      [&](float a) {
+            v8h wh[4], wl[4], b[2][T];
+            auto read_values = [&](int c) {
 #pragma unroll
-                          for (int d = 0; d < T; d++)
+                for (int d = 0; d < T; d++) b[c & 1][d] = *reinterpret_cast<const v8h *>(values + ((d * 2 + c / 2) * 2 + c % 2) * 1024 + lane * 16);
+            };
 #pragma unroll
-                              for (int r = 0; r < 16; r++) o[d][r] = o[d][r] * a;
-                      });
-            const uint8_t *values = buffer + 128 * DP;
+            for (int kt = 0; kt < 2; kt++) {  // 32 keys at a time: half the registers
+                float scores[16], x[16];
+                for_scales(ks[kt], [&](int i, float k) { scores[i] = k * s[kt][i]; });
+                if (kt) read_values(0);
+                __builtin_amdgcn_sched_barrier(0);
+                weigh(scores, x, vs[kt], f, edge, low, high, sums,
+                          [&](int i) { return page * kPage + 32 * kt + 2 * (i & ~3) + 4 * h + i % 4; },
+                          [](float v) {
+                              const float2 w = half_pair(v);
+                              return fmaxf(w.x, w.y);
+                          },
+                          [&](float factor) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {  // 16 keys: kt = c / 2, e = c % 2
-                v8h wh, wl, a[T];
-                split8(x + 8 * c, wh, wl);
+                              for (int d = 0; d < T; d++)
 #pragma unroll
-                for (int d = 0; d < T; d++) {
-                    a[d] = *reinterpret_cast<const v8h *>(values + ((d * 2 + c / 2) * 2 + c % 2) * 1024 + lane * 16);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[d], wl, o[d], 0, 0, 0);
-                }
+                                  for (int r = 0; r < 16; r++) o[d][r] = o[d][r] * factor;
+                              // the first 32 keys' weights are not in the sums yet; the factor, a power of two, in two
+                              // steps, for f16's range
+                              if (kt) {
+                                  const float step = fmaxf(factor, 0x1p-14f);
+                                  const _Float16 once = _Float16(step), rest = _Float16(factor / step);
 #pragma unroll
-                for (int d = 0; d < T; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[d], wh, o[d], 0, 0, 0);
+                                  for (int c = 0; c < 2; c++) {
+                                      wh[c] = wh[c] * once * rest;
+                                      wl[c] = wl[c] * once * rest;
+                                  }
+                              }
+                          });
+                split8(x, wh[2 * kt], wl[2 * kt]);
+                split8(x + 8, wh[2 * kt + 1], wl[2 * kt + 1]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {  // 16 keys
+                if (c < 3) read_values(c + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = 0; d < T; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[c & 1][d], wl[c], o[d], 0, 0, 0);
+#pragma unroll
+                for (int d = 0; d < T; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[c & 1][d], wh[c], o[d], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         __syncthreads();

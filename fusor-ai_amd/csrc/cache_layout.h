@@ -57,11 +57,10 @@ FG_BOTH Span span_of(int start, int stop, int length, int total)
 }
 
 // The page of a sequence's table that holds its tokens 64 index on, or -1.
+FG_BOTH int valid_page(int id, int pages) { return id >= 0 && id < pages ? id : -1; }
 FG_BOTH int page_at(const int32_t *table, int index, int max_pages, int pages)
 {
-    if (index < 0 || index >= max_pages) return -1;
-    const int id = table[index];
-    return id >= 0 && id < pages ? id : -1;
+    return index >= 0 && index < max_pages ? valid_page(table[index], pages) : -1;
 }
 
 // Pages [lo, hi) of a sequence that the rows row .. last see (hi at most max_pages).
