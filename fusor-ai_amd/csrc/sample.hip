@@ -367,11 +367,11 @@ __device__ __forceinline__ float smallest_of_bin(int b, float first, double scal
     return unordered(lo + n);
 }
 
-// The cuts of a row, from the weight m and the tokens n of this thread's bin; chunk_mass(k): the bin's
-// weight in chunk k. Every thread of the workgroup calls and gets the result; sh.whole has the chunks' weight
-// of whole bins.
-template <class F>
-__device__ __forceinline__ Cut cut_of(const SampleParams &p, const Row &r, float top, u64 m, u64 n, CutShared &sh, F chunk_mass)
+// The cuts of a row, from the weight m and the tokens n of this thread's bin. `mass` is its bins' weights in
+// memory, [chunks][kBins], written before the workgroup's last barrier: of each chunk or (running) of each and those
+// before it. Every thread of the workgroup calls and gets the result; sh.whole has the chunks' weight of whole bins.
+__device__ __forceinline__ Cut cut_of(const SampleParams &p, const Row &r, float top, u64 m, u64 n, CutShared &sh, const u64 *mass,
+                                      bool running)
 {
     const int tid = threadIdx.x;
     u64 all_n = 0, all_m, before_n = 0;
@@ -435,20 +435,31 @@ __device__ __forceinline__ Cut cut_of(const SampleParams &p, const Row &r, float
         c.high = c.last;
     }
     if (tid == c.low) sh.mass_low = before_m;
-    // the chunks' weight under `low`
-    if (c.low > 0) {
-        for (int k = 0; k < p.chunks; k++) {
-            const u64 w = wave_upto(tid < c.low ? chunk_mass(k) : 0);
-            if ((tid & 63) == 63 && w) atomicAdd(&sh.whole[k], w);
+    const int wave = tid >> 6, lane = tid & 63;
+    // the chunks' weight under `low`, a wave each
+    static_assert(kMaxChunks == kWaves, "a wave a chunk");
+    if (c.low > 0 && wave < p.chunks) {
+        const ulonglong2 *of = reinterpret_cast<const ulonglong2 *>(mass + size_t(wave) * kBins);
+        u64 w = 0;
+#pragma unroll
+        for (int i = 0; i < kBins; i += 128) {
+            const ulonglong2 two = of[i / 2 + lane];
+            w += (i + 2 * lane < c.low ? two.x : 0) + (i + 2 * lane + 1 < c.low ? two.y : 0);
         }
+        w = wave_upto(w);
+        if (lane == 63) sh.whole[wave] = w;
     }
-    const int wave = tid >> 6;
     const int edge = wave == 0 ? c.low - 1 : wave == 1 ? c.high : wave == 2 ? c.last - 1 : c.last;
     if (lists && wave < 4) {
         const float x = smallest_of_bin(edge, top, r.scale);
-        if ((tid & 63) == 0) sh.edge[wave] = x;
+        if (lane == 0) sh.edge[wave] = x;
     }
     __syncthreads();
+    if (running) {
+        const u64 before = tid > 0 && tid < p.chunks ? sh.whole[tid - 1] : 0;
+        __syncthreads();
+        if (tid < p.chunks) sh.whole[tid] -= before;
+    }
     c.mass_low = sh.mass_low;
     c.lists = lists;
     c.whole = sh.edge[0];
@@ -483,7 +494,7 @@ __global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleParams p)
         }
         return;
     }
-    const Cut c = cut_of(p, r, top, m, n, sh, [&](int k) { return mass[k * kBins]; });
+    const Cut c = cut_of(p, r, top, m, n, sh, p.mass + size_t(row) * p.chunks * kBins, false);
     if (tid < p.chunks) p.whole[size_t(row) * p.chunks + tid] = sh.whole[tid];
     if (tid == 0) p.cuts[row] = c;
 }
@@ -856,8 +867,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleParams p)
         __syncthreads();
         upto[c * kBins] = m = sh.bins.mass[tid];
     }
-    const Cut c = cut_of(p, r, top, m, r.has_k ? sh.bins.count[tid] : 0, sh.cut,
-                         [&](int k) { return upto[k * kBins] - (k ? upto[(k - 1) * kBins] : 0); });
+    __syncthreads();
+    const Cut c = cut_of(p, r, top, m, r.has_k ? sh.bins.count[tid] : 0, sh.cut, p.mass + size_t(row) * p.chunks * kBins, true);
     if (tid == 0) sh.listed = 0;
     __syncthreads();  // (the bins are read: the list takes their place)
     if (c.lists) list_tokens(x, 0, p.vocab, c, sh.draw.key, &sh.listed);
