@@ -336,21 +336,20 @@ int fg_cache_create(size_t pages, size_t kv_heads, size_t head_dim, void *stream
     if (kv_heads > 4096 || pages > (size_t(1) << 24))
         return set_error(FG_ERR_SHAPE, "fg_cache_create: at most 4096 heads and 2^24 pages");
     const int padded = padded_head(int(head_dim));
-    const size_t bytes = pages * kv_heads * size_t(record_bytes(padded));
+    // (at least one page: attention's loads for a page that is not there read page 0)
+    const size_t bytes = std::max<size_t>(pages, 1) * kv_heads * size_t(record_bytes(padded));
     int device = 0;
     FG_HIP(hipGetDevice(&device));
     uint8_t *records = nullptr;
-    hipError_t e = hipMalloc(reinterpret_cast<void **>(&records), std::max(bytes, size_t(record_bytes(padded))));  // (a record to read, at least)
+    hipError_t e = hipMalloc(reinterpret_cast<void **>(&records), bytes);
     if (e != hipSuccess) return check_hip(e, "fg_cache_create: hipMalloc");
-    if (bytes) {
-        const hipStream_t s = as_stream(stream);
-        cache_clear_kernel<<<4096, 256, 0, s>>>(records, bytes / 4, unsigned(2 * kPage * padded / 4), unsigned(record_bytes(padded) / 4));
-        e = hipGetLastError();
-        if (e == hipSuccess) e = hipStreamSynchronize(s);
-        if (e != hipSuccess) {
-            (void)hipFree(records);
-            return check_hip(e, "fg_cache_create");
-        }
+    const hipStream_t s = as_stream(stream);
+    cache_clear_kernel<<<4096, 256, 0, s>>>(records, bytes / 4, unsigned(2 * kPage * padded / 4), unsigned(record_bytes(padded) / 4));
+    e = hipGetLastError();
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    if (e != hipSuccess) {
+        (void)hipFree(records);
+        return check_hip(e, "fg_cache_create");
     }
     fg_cache *c = new (std::nothrow) fg_cache{device, int(pages), int(kv_heads), int(head_dim), padded, records};
     if (!c) {

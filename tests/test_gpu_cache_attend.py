@@ -126,6 +126,19 @@ def test_rows_that_see_nothing(fk, gpu, rows, lengths):
     assert not bool(got[:sum(rows)].any())
 
 
+@pytest.mark.parametrize("rows", [1, 3, 150])
+def test_a_cache_of_no_pages(fk, gpu, rows):
+    """Nothing to see; the loads of a page that is not there stay inside the cache's memory, of every head."""
+    import torch
+    cache = fk.PagedCache(0, 8, 256, device=gpu)
+    step = serving.Step([rows], [rows], padding=1)
+    step.table[:] = -1
+    query = torch.randn(step.total(), 16, 256, generator=torch.Generator().manual_seed(0)).to(gpu)
+    out = torch.full_like(query, 5.0)
+    cache.attend(step.batch(fk, gpu), query, out=out)
+    assert not bool(out[:rows].any()) and bool((out[rows:] == 5.0).all())
+
+
 def test_rows_past_their_sequence_length(fk, gpu):
     """More new rows than tokens: the first rows have no position."""
     import torch
