@@ -56,7 +56,7 @@ __device__ __forceinline__ int tile_pages(const AttendParams &p, const Span &s, 
     if (s.rows <= 0) return 0;
     const PageRange r = pages_seen(s, 0, s.rows - 1, p.window, p.b.max_pages);
     const int all = r.hi - r.lo;
-    return p.window > 0 ? min(all, (p.window + TM / p.group + 1) / kPage + 2) : all;
+    return p.window > 0 ? min(all, p.window / kPage + TM / p.group / kPage + 3) : all;
 }
 
 // Pages a part takes: the whole work spread over the target (a little more than its share: the sum is
@@ -430,12 +430,12 @@ __global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel
         for (int mt = 0; mt < MT; mt++) for_scales(ks, [&](int n, float k) { scores[mt][n] = k * s[mt][n / 4][n % 4]; });
         load_keys(loaded);
         const int base = page * kPage + 32 * (g >> 1) + 4 * (g & 1);
-        const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
+        const bool edge = page * kPage + kPage - 1 > first || page * kPage < first_seen(last, p.window);
         v8h wh[MT][2], wl[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
             float x[16];
-            const int high = pair[mt].position, low = p.window > 0 ? high - p.window + 1 : 0;
+            const int high = pair[mt].position, low = first_seen(high, p.window);
             weigh(scores[mt], x, vs, f[mt], edge, low, high, sums[mt], [&](int n) { return base + 8 * (n / 4) + n % 4; },
                       [](float a) {
                           float2 w = row_pair(a);
@@ -626,9 +626,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
         after = entry_of(page + 3);
         const uint8_t *buffer = lds + b * kBuffer;
         const float *key_scales = reinterpret_cast<const float *>(buffer + 256 * DP), *value_scales = key_scales + kPage;
-        const bool seen = held && any && page * kPage <= last && (p.window <= 0 || page * kPage + kPage - 1 > first - p.window);
+        const bool seen = held && any && page * kPage <= last && page * kPage + kPage - 1 >= first_seen(first, p.window);
         if (seen) {
-            const bool edge = page * kPage + kPage - 1 > first || (p.window > 0 && page * kPage <= last - p.window);
+            const bool edge = page * kPage + kPage - 1 > first || page * kPage < first_seen(last, p.window);
             const uint8_t *values = buffer + 128 * DP;
             // The operands of a step are read while the step before multiplies: left to itself the compiler reads
             // each step's into the registers of the one before, and waits.
@@ -656,7 +656,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
                 for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k & 1][kt], qh[k], s[kt], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const int high = pair.position, low = p.window > 0 ? high - p.window + 1 : 0;
+            const int high = pair.position, low = first_seen(high, p.window);
             v8h wh[4], wl[4], b[2][T];
             auto read_values = [&](int c) {
 #pragma unroll

@@ -63,6 +63,10 @@ FG_BOTH int page_at(const int32_t *table, int index, int max_pages, int pages)
     return index >= 0 && index < max_pages ? valid_page(table[index], pages) : -1;
 }
 
+// The first position that a row at `position` sees. (No difference is formed that a window longer than any
+// sequence, or a position before 0, could take out of range.)
+FG_BOTH int first_seen(int position, int window) { return window > 0 && position >= window ? position - window + 1 : 0; }
+
 // Pages [lo, hi) of a sequence that the rows row .. last see (hi at most max_pages).
 struct PageRange {
     int lo, hi;
@@ -71,9 +75,7 @@ FG_BOTH PageRange pages_seen(const Span &s, int row, int last, int window, int m
 {
     PageRange r;
     const int end = s.first + last + 1;  // one past the last row's position
-    const int far = s.first + row;       // the first row's position
-    const int low = window > 0 && far >= window ? far - window + 1 : 0;
-    r.lo = low / kPage;
+    r.lo = first_seen(s.first + row, window) / kPage;
     r.hi = end <= 0 ? 0 : (end - 1) / kPage + 1;
     if (r.hi > max_pages) r.hi = max_pages;
     if (r.lo > r.hi) r.lo = r.hi;

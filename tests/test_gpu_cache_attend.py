@@ -101,6 +101,17 @@ def test_windows(fk, gpu, rows, lengths, window):
     case.check(case.run(window=window), window=window)
 
 
+@pytest.mark.parametrize("rows,length", [(3, 2), (6, 70), (130, 70), (40, 3000)])
+@pytest.mark.parametrize("window", [2 ** 31 - 64, 2 ** 31 - 1, 2 ** 31, 2 ** 63])
+def test_windows_longer_than_any_sequence(fk, gpu, rows, length, window):
+    """... see what no window sees, rows before position 0 among them."""
+    import torch
+    case = Case(fk, gpu, [length], [length], 4, 2, 64)
+    case.step.rows, case.step.starts = [rows], np.array([0, rows], np.int32)
+    case.query = torch.randn(rows, 4, 64, generator=torch.Generator().manual_seed(1))
+    assert torch.equal(case.run(window=window), case.run())
+
+
 @pytest.mark.parametrize("rows,lengths,heads,kv_heads,dim", [
     ([1], [5000], 14, 2, 64), ([1, 1, 1], [9000, 1, 3001], 4, 1, 128), ([3], [4097], 8, 4, 128), ([40, 1], [2500, 1400], 4, 2, 64)])
 def test_long_caches_split_over_workgroups(fk, gpu, rows, lengths, heads, kv_heads, dim):
