@@ -12,6 +12,9 @@ struct fg_cache {
 
 namespace fg {
 
+// Workgroups of 256 that a launch takes (2^32 threads are too many).
+constexpr size_t kMaxGrid = 0xffffff;
+
 // What the kernels take of a batch.
 struct BatchParams {
     const int32_t *row_starts, *lengths, *pages;

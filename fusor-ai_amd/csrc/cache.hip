@@ -80,12 +80,10 @@ __global__ __launch_bounds__(256) void cache_clear_kernel(uint8_t *records, size
 // (cache_layout.h): 8 bytes a cycle of stores for one token, which is why runs of tokens take the
 // kernels below.
 template <bool WRITE>
-__global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
+__device__ __forceinline__ void store_row(const StoreParams &p, unsigned unit)
 {
-    const unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int row = int(unit / unsigned(p.kv_heads)), head = int(unit % unsigned(p.kv_heads));
-    if (row >= p.b.rows) return;  // a whole wave
     const int s = sequence_of_row(p.b, row);
     if (s < 0) return;
     const Span span = sequence_span(p.b, s);
@@ -128,6 +126,13 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
             *reinterpret_cast<v4f_any *>((value ? p.out[1] : p.out[0]) + place) = x;
         }
     }
+}
+
+template <bool WRITE>
+__global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
+{
+    const unsigned units = unsigned(p.b.rows) * unsigned(p.kv_heads);  // (at most 2^18 rows here, of 2^12 heads)
+    for (unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += gridDim.x * 4) store_row<WRITE>(p, unit);
 }
 
 // A workgroup per page that new tokens lie in, head, and keys or values. A thread takes four tokens (an
@@ -261,13 +266,13 @@ template <bool WRITE>
 int launch_store(const StoreParams &p, hipStream_t s)
 {
     if (p.b.rows == 0 || p.b.sequences == 0) return FG_OK;
+    const size_t units = size_t(p.b.rows) * p.kv_heads;
     if (p.b.rows <= 4 * p.b.sequences) {
-        const size_t units = size_t(p.b.rows) * p.kv_heads;
-        cache_rows_kernel<WRITE><<<unsigned((units + 3) / 4), 256, 0, s>>>(p);
+        cache_rows_kernel<WRITE><<<unsigned(std::min((units + 3) / 4, kMaxGrid)), 256, 0, s>>>(p);
     } else {
         // a run of n rows lies in at most (n + 62) / 64 + 1 pages
-        const size_t units = size_t(p.b.rows) / kPage + 2 * size_t(std::min(p.b.sequences, p.b.rows));
-        cache_pages_kernel<WRITE><<<dim3(unsigned(units), unsigned(p.kv_heads), 2), kPageThreads, size_t(kPage * p.padded), s>>>(p);
+        const size_t runs = size_t(p.b.rows) / kPage + 2 * size_t(std::min(p.b.sequences, p.b.rows));
+        cache_pages_kernel<WRITE><<<dim3(unsigned(runs), unsigned(p.kv_heads), 2), kPageThreads, size_t(kPage * p.padded), s>>>(p);
     }
     FG_HIP(hipGetLastError());
     return FG_OK;

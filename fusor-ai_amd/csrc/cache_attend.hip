@@ -879,7 +879,8 @@ extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float
     if (rc) return rc;
     if (!heads || heads % c->kv_heads || heads > 65536)
         return set_error(FG_ERR_SHAPE, "fg_cache_attend: the heads must be a positive multiple of the cache's, at most 65536");
-    if (!(std::fabs(scale) <= 3.4e38f)) return set_error(FG_ERR_ARG, "fg_cache_attend: the scale must be finite");
+    if (!(std::fabs(scale) <= 2e38f))  // (times log2 e it is in f32's range)
+        return set_error(FG_ERR_ARG, "fg_cache_attend: the scale must be a number of at most 2e38");
     if (!b->rows || !b->sequences) return FG_OK;
     if (!query || !out) return set_error(FG_ERR_ARG, "fg_cache_attend: a null query or output");
     const size_t width = heads * c->head_dim;
@@ -888,7 +889,7 @@ extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float
         return set_error(FG_ERR_SHAPE, "fg_cache_attend: at most 2^30 rows times heads of a key head");
     const hipStream_t s = as_stream(stream);
     const Launch l = plan_launch(c, b, heads);
-    if (l.grid * c->kv_heads > 0x7fffffff) return set_error(FG_ERR_SHAPE, "fg_cache_attend: too many rows");
+    if (l.grid * c->kv_heads > kMaxGrid) return set_error(FG_ERR_SHAPE, "fg_cache_attend: more sequences times heads than a launch takes");
     AttendParams p{};
     p.b = batch_params(b);
     p.records = c->records;

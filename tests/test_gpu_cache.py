@@ -162,6 +162,27 @@ def test_many_sequences(fk, gpu):
         assert same(got_k[:n], serving.quantized(x[:n])) and same(got_v[:n], serving.quantized(-x[:n]))
 
 
+def test_more_heads_than_a_launch_of_rows_takes(fk, gpu):
+    """One token each of 16400 sequences, of 4096 heads: past 2^32 threads of a wave a head. Attention, which
+    takes a workgroup a sequence and head, refuses them."""
+    import torch
+    heads, n = 4096, 16400
+    cache = fk.PagedCache(1, heads, 4, device=gpu)
+    pages = torch.full((n, 1), -1, dtype=torch.int32, device=gpu)
+    pages[n - 2] = 0
+    batch = fk.Batch(torch.arange(n + 1, dtype=torch.int32, device=gpu), torch.full((n,), 9, dtype=torch.int32, device=gpu), pages)
+    keys = torch.randn(n, heads, 4, device=gpu)
+    cache.write(batch, keys, -keys)
+    want = serving.quantized(keys[n - 2].cpu())
+    values, back = torch.full_like(keys, 3.0), torch.full_like(keys, 3.0)
+    cache.read(batch, back, values)
+    assert same(back[n - 2], want) and same(values[n - 2], -want + 0.0)
+    back[n - 2] = values[n - 2] = 0
+    assert not bool(back.any()) and not bool(values.any())
+    with pytest.raises(fk.ShapeError, match="than a launch takes"):
+        cache.attend(batch, keys)
+
+
 def test_refusals(fk, gpu):
     import torch
     step = serving.Step([2], [2])

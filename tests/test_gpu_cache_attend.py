@@ -302,7 +302,7 @@ def test_refusals(fk, gpu):
             case.cache.attend(batch, good, out=bad)
     with pytest.raises(fk.ShapeError):
         case.cache.attend(batch, good, window=-1)
-    for scale in (float("nan"), float("inf")):
+    for scale in (float("nan"), float("inf"), 3e38, -3e38):
         with pytest.raises(ValueError):
             case.cache.attend(batch, good, scale=scale)
     assert case.cache.attend(batch, good[:0]).shape == (0, 4, 64)
