@@ -310,60 +310,56 @@ __device__ __forceinline__ float part_factor(float r, float joined) { return r =
 
 // ---------------------------------------------------------------- few rows: decode steps
 //
-// A workgroup of four waves takes MT x 16 pairs of one key head over its task's pages; each wave takes
+// A workgroup of four waves takes 16 pairs of one key head over its task's pages; each wave takes
 // whole pages (the task's first, fifth ...), straight from memory to registers: nothing is shared
 // between waves until their sums are joined at the end. The products are 16 x 16 x 32; lane l holds
 // pair l % 16, and with g = l / 16 and 4 t + r the record's own order of values:
 //   scores:  four products of 16 keys: row i of product t is key 32 (i / 8) + 8 t + i % 8, so lane l gets
 //            the scores of keys 32 (g / 2) + 8 t + 4 (g % 2) + r, r = 0 .. 3;
 //   values:  16 dimensions by 32 keys: the lane's 16 bytes of dimension l % 16 are those keys', in order.
-template <int DP, int MT>
-__global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel(AttendParams p)
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(AttendParams p)
 {
-    constexpr int TM = 16 * MT, J = (DP + 63) / 64, T = DP / 16, R = DP / 32;
-    __shared__ __align__(16) float joined[2][MT * (T * 4 + 2)][64];
+    constexpr int TM = 16, J = (DP + 63) / 64, T = DP / 16, R = DP / 32;
+    __shared__ __align__(16) float joined[2][T * 4 + 2][64];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, kv = int(blockIdx.x % unsigned(p.kv_heads));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Task task = uniform(find_task(p, int(blockIdx.x / unsigned(p.kv_heads)), TM));
     leave_note(p, task, int(blockIdx.x / unsigned(p.kv_heads)), kv);
     if (task.seq < 0) return;  // the whole workgroup
     const PageRange range = task_pages(p, task, TM);
-
-    v8h qh[MT][J][2], ql[MT][J][2];
-    float f[MT];
-    Pair pair[MT];
-    RowSums sums[MT];
-    v4f o[MT][T];
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        pair[mt] = pair_of(p, task, kv, task.tile * TM + mt * 16 + i);
-        const float *row = p.query + size_t(pair[mt].row) * p.query_stride + size_t(pair[mt].head) * p.head_dim;
-        float x[J][2][8];
+    const Pair pair = pair_of(p, task, kv, task.tile * TM + i);
+    v8h qh[J][2], ql[J][2];
+    float f;
+    {
+        const float *row = p.query + size_t(pair.row) * p.query_stride + size_t(pair.head) * p.head_dim;
+        float q[J][2][8];
         float amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                load8(row, 64 * j + 16 * g + 8 * e, p.head_dim, x[j][e]);
+                load8(row, 64 * j + 16 * g + 8 * e, p.head_dim, q[j][e]);
 #pragma unroll
-                for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(x[j][e][k]));
+                for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(q[j][e][k]));
             }
         float2 w = row_pair(amax);
         w = half_pair(fmaxf(w.x, w.y));
         const int shift = query_shift(fmaxf(w.x, w.y));
-        f[mt] = ldexpf(p.scale2, -shift);
+        f = ldexpf(p.scale2, -shift);
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[j][e][k] = ldexpf(x[j][e][k], shift);
-                split8(x[j][e], qh[mt][j][e], ql[mt][j][e]);
+                for (int k = 0; k < 8; k++) q[j][e][k] = ldexpf(q[j][e][k], shift);
+                split8(q[j][e], qh[j][e], ql[j][e]);
             }
-        sums[mt] = RowSums{-INFINITY, 0.0f};
-#pragma unroll
-        for (int d = 0; d < T; d++) o[mt][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    RowSums sums{-INFINITY, 0.0f};
+    v4f o[T];
+#pragma unroll
+    for (int d = 0; d < T; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const int first = task.span.first + task.tile * TM / p.group;  // positions of the tile's first and last rows
     const int last = task.span.first + min((task.tile * TM + TM - 1) / p.group, task.span.rows - 1);
     const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
@@ -407,11 +403,9 @@ __global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel
             load_values(loaded);
             continue;
         }
-        v4f s[MT][4];
+        v4f s[4];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int t = 0; t < 4; t++) s[mt][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < 4; t++) s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
@@ -419,112 +413,87 @@ __global__ __launch_bounds__(256, DP * MT <= 128 ? 2 : 1) void attend_few_kernel
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
                     const v8h a = e ? widen8(k[t][j].z, k[t][j].w) : widen8(k[t][j].x, k[t][j].y);
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[mt][j][e], s[mt][t], 0, 0, 0);
-                        s[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[mt][j][e], s[mt][t], 0, 0, 0);
-                    }
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[j][e], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[j][e], s[t], 0, 0, 0);
                 }
-        float scores[MT][16];
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) for_scales(ks, [&](int n, float k) { scores[mt][n] = k * s[mt][n / 4][n % 4]; });
+        float scores[16], weights[16];
+        for_scales(ks, [&](int n, float k) { scores[n] = k * s[n / 4][n % 4]; });
         load_keys(loaded);
         const int base = page * kPage + 32 * (g >> 1) + 4 * (g & 1);
         const bool edge = page * kPage + kPage - 1 > first || page * kPage < first_seen(last, p.window);
-        v8h wh[MT][2], wl[MT][2];
+        const int high = pair.position, low = first_seen(high, p.window);
+        weigh(scores, weights, vs, f, edge, low, high, sums, [&](int n) { return base + 8 * (n / 4) + n % 4; },
+              [](float a) {
+                  float2 w = row_pair(a);
+                  w = half_pair(fmaxf(w.x, w.y));
+                  return fmaxf(w.x, w.y);
+              },
+              [&](float a) {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            float x[16];
-            const int high = pair[mt].position, low = first_seen(high, p.window);
-            weigh(scores[mt], x, vs, f[mt], edge, low, high, sums[mt], [&](int n) { return base + 8 * (n / 4) + n % 4; },
-                      [](float a) {
-                          float2 w = row_pair(a);
-                          w = half_pair(fmaxf(w.x, w.y));
-                          return fmaxf(w.x, w.y);
-                      },
-                      [&](float a) {
+                  for (int d = 0; d < T; d++)
 #pragma unroll
-                          for (int d = 0; d < T; d++)
-#pragma unroll
-                              for (int r = 0; r < 4; r++) o[mt][d][r] = o[mt][d][r] * a;
-                      });
-            split8(x, wh[mt][0], wl[mt][0]);
-            split8(x + 8, wh[mt][1], wl[mt][1]);
-        }
+                      for (int r = 0; r < 4; r++) o[d][r] = o[d][r] * a;
+              });
+        v8h wh[2], wl[2];
+        split8(weights, wh[0], wl[0]);
+        split8(weights + 8, wh[1], wl[1]);
 #pragma unroll
         for (int d = 0; d < T; d++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const v8h a = e ? widen8(v[d].z, v[d].w) : widen8(v[d].x, v[d].y);
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    o[mt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl[mt][e], o[mt][d], 0, 0, 0);
-                    o[mt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wh[mt][e], o[mt][d], 0, 0, 0);
-                }
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wl[e], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wh[e], o[d], 0, 0, 0);
             }
         load_values(loaded);
     }
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        float2 w = row_pair(sums[mt].total);
+    {
+        float2 w = row_pair(sums.total);
         w = half_pair(w.x + w.y);
-        sums[mt].total = w.x + w.y;
+        sums.total = w.x + w.y;
     }
     // the waves' sums joined, lane by lane: waves 2 and 3 into 0 and 1, then 1 into 0
 #pragma unroll
     for (int step = 2; step >= 1; step >>= 1) {
         float(*to)[64] = joined[wave & 1];
         if (wave >= step && wave < 2 * step) {
+            to[0][lane] = sums.r;
+            to[1][lane] = sums.total;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                const int at = mt * (T * 4 + 2);
-                to[at][lane] = sums[mt].r;
-                to[at + 1][lane] = sums[mt].total;
+            for (int d = 0; d < T; d++)
 #pragma unroll
-                for (int d = 0; d < T; d++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) to[at + 2 + d * 4 + r][lane] = o[mt][d][r];
-            }
+                for (int r = 0; r < 4; r++) to[2 + d * 4 + r][lane] = o[d][r];
         }
         __syncthreads();
         if (wave < step) {
             float(*from)[64] = joined[(wave + step) & 1];
+            const float other = from[0][lane], r = fmaxf(sums.r, other);
+            const float a = part_factor(sums.r, r), b = part_factor(other, r);
+            sums.r = r;
+            sums.total = sums.total * a + from[1][lane] * b;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                const int at = mt * (T * 4 + 2);
-                const float other = from[at][lane], r = fmaxf(sums[mt].r, other);
-                const float a = part_factor(sums[mt].r, r), b = part_factor(other, r);
-                sums[mt].r = r;
-                sums[mt].total = sums[mt].total * a + from[at + 1][lane] * b;
+            for (int d = 0; d < T; d++)
 #pragma unroll
-                for (int d = 0; d < T; d++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) o[mt][d][c] = o[mt][d][c] * a + from[at + 2 + d * 4 + c][lane] * b;
-            }
+                for (int c = 0; c < 4; c++) o[d][c] = o[d][c] * a + from[2 + d * 4 + c][lane] * b;
         }
         __syncthreads();
     }
-    if (wave != 0) return;
+    if (wave != 0 || !pair.live) return;
+    if (task.nsplit > 1) {
+        float *part = p.partial + (size_t(task.slot) * p.kv_heads + kv) * (16 * DP + 128);
+        part[lane] = sums.r;
+        part[64 + lane] = sums.total;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        if (task.nsplit > 1) {
-            float *part = p.partial + ((size_t(task.slot) * p.kv_heads + kv) * MT + mt) * (16 * DP + 128);
-            part[lane] = sums[mt].r;
-            part[64 + lane] = sums[mt].total;
+        for (int d = 0; d < T; d++) *reinterpret_cast<v4f *>(part + 128 + d * 256 + lane * 4) = o[d];
+        return;
+    }
+    float *row = p.out + size_t(pair.row) * p.out_stride + size_t(pair.head) * p.head_dim;
 #pragma unroll
-            for (int d = 0; d < T; d++) *reinterpret_cast<v4f *>(part + 128 + d * 256 + lane * 4) = o[mt][d];
-            continue;
-        }
-        if (!pair[mt].live) continue;
-        float *row = p.out + size_t(pair[mt].row) * p.out_stride + size_t(pair[mt].head) * p.head_dim;
-        const float total = sums[mt].total;
+    for (int d = 0; d < T; d++) {
+        v4f x;
 #pragma unroll
-        for (int d = 0; d < T; d++) {
-            v4f x;
-#pragma unroll
-            for (int c = 0; c < 4; c++) x[c] = total == 0.0f ? 0.0f : o[mt][d][c] / total;
-            if (16 * d + 4 * g < p.head_dim) *reinterpret_cast<v4f_any *>(row + 16 * d + 4 * g) = x;
-        }
+        for (int c = 0; c < 4; c++) x[c] = sums.total == 0.0f ? 0.0f : o[d][c] / sums.total;
+        if (16 * d + 4 * g < p.head_dim) *reinterpret_cast<v4f_any *>(row + 16 * d + 4 * g) = x;
     }
 }
 
@@ -709,6 +678,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     }
     const float2 w = half_pair(sums.total);
     sums.total = w.x + w.y;
+    if (!pair.live) return;
     if (task.nsplit > 1) {
         float *part = p.partial + ((size_t(task.slot) * p.kv_heads + kv) * 4 + wave) * (32 * DP + 128);
         part[lane] = sums.r;
@@ -720,7 +690,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
                 *reinterpret_cast<v4f *>(part + 128 + (d * 4 + c) * 256 + lane * 4) = v4f{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
         return;
     }
-    if (!pair.live) return;
     float *row = p.out + size_t(pair.row) * p.out_stride + size_t(pair.head) * p.head_dim;
 #pragma unroll
     for (int d = 0; d < T; d++)
@@ -752,6 +721,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p)
     Task t{};
     t.span = Span{note.begin, note.rows, note.first, note.first + note.rows};
     const Pair pair = pair_of(p, t, kv, note.tile * TM + tile * ROWS + (lane & (ROWS - 1)));
+    if (!pair.live) return;  // (its sums are not written)
     // eight parts at a time, joined like the waves' sums
     constexpr int kAhead = 8;
     float r = -INFINITY, total = 0.0f;
@@ -784,7 +754,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p)
         }
     }
     const int dim = c * (256 / ROWS) + 4 * (lane / ROWS);
-    if (!pair.live || dim >= p.head_dim) return;
+    if (dim >= p.head_dim) return;
 #pragma unroll
     for (int e = 0; e < 4; e++) o[e] = total == 0.0f ? 0.0f : o[e] / total;
     *reinterpret_cast<v4f_any *>(p.out + size_t(pair.row) * p.out_stride + size_t(pair.head) * p.head_dim + dim) = o;
@@ -793,33 +763,44 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p)
 // ------------------------------------------------------------------------------ the host
 
 struct Launch {
-    int tile_rows, tiles;      // pairs of a tile: tile_rows a wave tile, tiles of them
-    size_t grid;               // a bound on the tasks of a head
+    bool few;
+    size_t grid;  // a bound on the tasks of a head
     int target;
     size_t note_bytes, partial_bytes;
 };
 
-// Workgroups that a step's tasks aim at, all heads together: two a CU.
-constexpr size_t kWorkgroups = 512;
+constexpr size_t kUnits = 256;  // CUs
 
+// Which kernel a step takes, and whether its tiles are split, from what the host knows of it: microseconds of
+// decode steps and chunks over caches of random or equal lengths, 16 query heads of 128 over 4 key heads (a), 14 of
+// 64 over 2 (b), 8 of 128 over 1 (c).
+//
+// attend_few_kernel up to 96 pairs a sequence, few's time and many's: 64 sequences of up to 3200 tokens, 48 pairs
+// (a) 66 and 91, 84 pairs (b) 32 and 43, 96 pairs (a) 92 and 100, (c) 43 and 38; 128 pairs (a) 112 and 114, (c) 50
+// and 40.
+//
+// Tiles are split when there are at most as many as CUs, all heads together: 64 sequences of up to 8000 tokens
+// (a) 71 whole and 56 split, (b) 42 and 21; all of 8000, which a CU each serves evenly, (a) 98 and 108; 128 sequences
+// (a), two a CU, 132 and 135. Not over tables of up to 16 pages: joining costs about 4 us, as much as ten pages, and
+// as much again on the host (500 tokens: 10.3 whole, 11.2 split). Two workgroups a CU read at once what memory
+// gives, so the parts aimed at are two a CU, less half of one a tile, whose last part is half a part on average:
+// fewer leave some CUs two parts and others one (eight documents of 30000 to 70000 tokens: 288 parts 105, 350 98,
+// 512 88), more start and end too often (1024: 104). 64 sequences as above (a): 384 parts 61 and of equal lengths
+// 130, 512 56 and 108, 640 64 and 130.
 Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
 {
     Launch l{};
     const size_t group = heads / c->kv_heads, pairs = b->rows * group, sequences = std::min(b->sequences, b->rows);
-    const bool few = pairs <= 32 * sequences;
-    l.tile_rows = few ? 16 : 32;
-    l.tiles = few ? (pairs > 16 * sequences && c->padded <= 128 ? 2 : 1) : 4;
-    const size_t tm = size_t(l.tile_rows) * l.tiles;
-    const size_t row_tiles = pairs / tm + sequences, slots = std::max<size_t>(kWorkgroups / c->kv_heads, 2);
-    l.grid = row_tiles;
-    // fewer tiles than the chip takes at once: their pages are split so that all tasks run at once
-    // (not tables of few pages: joining costs about the time of four pages, and as much again on the host)
-    if (pairs / tm < slots / 2 && b->max_pages > size_t(4 * kMinPages)) {
-        l.target = int(slots - std::min(row_tiles, slots / 2));
+    l.few = pairs <= 96 * sequences;
+    const size_t tm = l.few ? 16 : 128, units = std::max<size_t>(kUnits / c->kv_heads, 1);
+    const size_t tiles = std::max(pairs / tm, sequences);  // about
+    l.grid = pairs / tm + sequences;
+    if (tiles <= units && b->max_pages > 16) {
+        l.target = int(2 * units - tiles / 2);
         const size_t most = std::min<size_t>((b->max_pages + kMinPages - 1) / kMinPages, kMaxSplit);
-        l.grid = std::min(row_tiles * most, row_tiles + l.target);
+        l.grid = std::min(l.grid * most, l.grid + l.target);
         l.note_bytes = (l.grid * sizeof(Note) + 255) / 256 * 256;
-        l.partial_bytes = l.grid * c->kv_heads * l.tiles * (size_t(l.tile_rows) * c->padded + 128) * 4;
+        l.partial_bytes = l.grid * c->kv_heads * (tm * c->padded + (l.few ? 1 : 4) * 128) * 4;
     }
     return l;
 }
@@ -828,17 +809,10 @@ template <int DP>
 int launch_attend(const AttendParams &p, const Launch &l, hipStream_t s)
 {
     const unsigned grid = unsigned(p.kv_heads * l.grid);
-    const dim3 pieces(grid, unsigned((l.tiles * l.tile_rows * DP / 256 + 3) / 4));
-    if (l.tiles == 1) {
-        attend_few_kernel<DP, 1><<<grid, 256, 0, s>>>(p);
+    if (l.few) {
+        attend_few_kernel<DP><<<grid, 256, 0, s>>>(p);
         FG_HIP(hipGetLastError());
-        if (l.target) attend_join_kernel<DP, 16, 1><<<pieces, 256, 0, s>>>(p);
-    } else if (l.tiles == 2) {
-        if constexpr (DP <= 128) {
-            attend_few_kernel<DP, 2><<<grid, 256, 0, s>>>(p);
-            FG_HIP(hipGetLastError());
-            if (l.target) attend_join_kernel<DP, 16, 2><<<pieces, 256, 0, s>>>(p);
-        }
+        if (l.target) attend_join_kernel<DP, 16, 1><<<dim3(grid, (16 * DP / 256 + 3) / 4), 256, 0, s>>>(p);
     } else {
         if (many_lds<DP>() > 64 * 1024) {  // more than the default limit: raised once a device
             static std::atomic<unsigned long long> raised{0};
@@ -853,7 +827,7 @@ int launch_attend(const AttendParams &p, const Launch &l, hipStream_t s)
         }
         attend_many_kernel<DP><<<grid, 256, many_lds<DP>(), s>>>(p);
         FG_HIP(hipGetLastError());
-        if (l.target) attend_join_kernel<DP, 32, 4><<<pieces, 256, 0, s>>>(p);
+        if (l.target) attend_join_kernel<DP, 32, 4><<<dim3(grid, 128 * DP / 256 / 4), 256, 0, s>>>(p);
     }
     FG_HIP(hipGetLastError());
     return FG_OK;
