@@ -76,9 +76,11 @@ __global__ __launch_bounds__(256) void cache_clear_kernel(uint8_t *records, size
 }
 
 // A wave per new row and head, for few new tokens a sequence. Four dimensions a lane; heads of up to 128
-// take half a wave for the key and half for the value. A value's levels go to single bytes 16 apart
-// (cache_layout.h): 8 bytes a cycle of stores for one token, which is why runs of tokens take the
-// kernels below.
+// take half a wave for the key and half for the value. A value's levels go to single bytes, 16 apart, of a kilobyte
+// that 64 tokens share (cache_layout.h): 64 stores of a byte a token, which is what bounds long runs of tokens,
+// and why they take the kernels below. A step's single tokens are bounded by the launch and its three loads one
+// after the other (the row's sequence, its page, its values): 8 tokens of 2 heads of 64 written in 3.4 us, read back
+// in 3.2; 512 of 8 heads of 128 in 7.8 and 5.0.
 template <bool WRITE>
 __device__ __forceinline__ void store_row(const StoreParams &p, unsigned unit)
 {
@@ -131,14 +133,17 @@ __device__ __forceinline__ void store_row(const StoreParams &p, unsigned unit)
 template <bool WRITE>
 __global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
 {
-    const unsigned units = unsigned(p.b.rows) * unsigned(p.kv_heads);  // (at most 2^18 rows here, of 2^12 heads)
+    const unsigned units = unsigned(p.b.rows) * unsigned(p.kv_heads);
     for (unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += gridDim.x * 4) store_row<WRITE>(p, unit);
 }
 
 // A workgroup per page that new tokens lie in, head, and keys or values. A thread takes four tokens (an
 // aligned run, so one dword of each dimension's values) of four dimensions, heads of up to 128 all of a page
 // at once; the levels meet in LDS in the record's order, and whole 16-byte pieces go to the page or come from it.
-// Pieces that also hold other tokens' values are written in part.
+// Pieces that also hold other tokens' values are written in part. Bounded by memory for long runs, and by one load's
+// wait after another for short ones: 3618 tokens of 4 heads of 128 (14.8 MB of f32, 3.8 MB of levels and scales) written
+// in 8.9 us, 2.1 TB/s, and read back in 7.8. Keys and values are each a workgroup's, for twice the loads in flight (both in
+// one: 16.8 and 9.8).
 constexpr int kPageThreads = 512;
 
 template <bool WRITE>
@@ -267,7 +272,12 @@ int launch_store(const StoreParams &p, hipStream_t s)
 {
     if (p.b.rows == 0 || p.b.sequences == 0) return FG_OK;
     const size_t units = size_t(p.b.rows) * p.kv_heads;
-    if (p.b.rows <= 4 * p.b.sequences) {
+    if (units > 0xf0000000) return set_error(FG_ERR_SHAPE, "the paged cache: more rows times heads than a launch takes");
+    // A wave a row and head, or a workgroup a page: the first up to 16 new tokens a sequence or 2048 rows times heads.
+    // Microseconds of a write, rows' and pages': 8 heads of 128, 64 sequences of 1 new token 3.8 and 9.5, 16 11.4 and
+    // 11.3, 32 17.6 and 13.2, 128 51 and 23; one of 128 3.8 and 4.8; 8 of 32 4.9 and 5.9, of 128 10.5 and 6.5;
+    // 512 (each workgroup of a page looks through all of them) of 1 7.8 and 80, 16 52 and 100, 64 190 and 148.
+    if (p.b.rows <= 16 * p.b.sequences || units <= 2048) {
         cache_rows_kernel<WRITE><<<unsigned(std::min((units + 3) / 4, kMaxGrid)), 256, 0, s>>>(p);
     } else {
         // a run of n rows lies in at most (n + 62) / 64 + 1 pages

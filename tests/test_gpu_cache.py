@@ -34,9 +34,10 @@ def stored(fk, cache, step, heads, dim, device, fill=float("nan")):
     return keys, values
 
 
-# rows of the sequences, their lengths; one token a sequence takes the row kernels, runs the page kernels
+# rows of the sequences, their lengths; more than 2048 rows, and than 16 a sequence, take the page kernels, others the row kernels
 STEPS = [([1], [1]), ([1, 1, 1], [64, 65, 130]), ([1, 0, 1, 0], [7, 0, 200, 3]), ([64], [64]), ([65, 3], [65, 130]),
-         ([200, 0, 1, 130], [201, 5, 77, 130]), ([63], [127]), ([5, 6], [61, 64 + 3])]
+         ([200, 0, 1, 130], [201, 5, 77, 130]), ([63], [127]), ([5, 6], [61, 64 + 3]),
+         ([2050, 66, 0, 3], [2060, 200, 5, 3]), ([64 * 33], [64 * 33]), ([700, 1, 1400], [701, 64, 1463])]
 HEADS = [(1, 4), (2, 64), (3, 36), (2, 128), (1, 132), (4, 72), (1, 256), (2, 192)]
 
 
@@ -79,18 +80,20 @@ def test_special_values(fk, gpu):
     x[6, 0, :2] = torch.tensor([float("inf"), 1.0])
     x[7, 0, :6] = torch.tensor([127.0, 0.5, 1.5, -2.5, 63.5, -126.5])
     x[8, 0] = torch.linspace(-1e-20, 1e-20, dim)
-    for rows, lengths in (([9], [9]), ([1] * 9, [1] * 9)):
+    for rows, lengths in (([9], [9]), ([1] * 9, [1] * 9), ([9 * 240], [9 * 240])):
+        if rows[0] > 9:
+            x = x.repeat(240, 1, 1)  # the page kernels
         step = serving.Step(rows, lengths)
         cache = fk.PagedCache(step.pages, 1, dim, device=gpu)
         cache.write(step.batch(fk, gpu), x.to(gpu), x.to(gpu))
         for got in stored(fk, cache, step, 1, dim, gpu):
             want = serving.quantized(x).float()
             nan = torch.isnan(want)
-            assert torch.equal(torch.isnan(got.cpu()), nan) and bool(nan[6].all()) and not bool(nan[5].any())
+            assert torch.equal(torch.isnan(got.cpu()), nan) and bool(nan[6::9].all()) and not bool(nan[5::9].any())
             assert torch.equal(got.cpu()[~nan], want[~nan])
 
 
-@pytest.mark.parametrize("rows,lengths", [([70], [70]), ([1, 1], [3, 70])])
+@pytest.mark.parametrize("rows,lengths", [([70], [70]), ([1, 1], [3, 70]), ([1100], [1111])])
 def test_strides_and_unaligned_rows(fk, gpu, rows, lengths):
     """Keys and values as slices of one projection's rows, at an address of any float; one row for all."""
     import torch
@@ -113,7 +116,7 @@ def test_strides_and_unaligned_rows(fk, gpu, rows, lengths):
     assert same(got_k, serving.quantized(one.cpu())) and same(got_v, got_k)
 
 
-@pytest.mark.parametrize("rows,lengths", [([3, 2, 2], [2, 130, 5]), ([100, 70], [40, 200])])
+@pytest.mark.parametrize("rows,lengths", [([3, 2, 2], [2, 130, 5]), ([100, 70], [40, 200]), ([1200, 70], [1090, 200])])
 def test_rows_without_a_place(fk, gpu, rows, lengths):
     """Rows before position 0, pages outside the cache and past the table: not written, read as 0."""
     import torch
@@ -135,10 +138,11 @@ def test_rows_without_a_place(fk, gpu, rows, lengths):
     assert same(got_k + 0.0, want + 0.0) and same(got_v + 0.0, 0.0 - want)
 
 
-def test_offsets_past_32_bits(fk, gpu):
+@pytest.mark.parametrize("rows,lengths", [([70, 1], [70, 200]), ([300, 1], [300, 200])])
+def test_offsets_past_32_bits(fk, gpu, rows, lengths):
     import torch
     heads, dim = 8, 256
-    step = serving.Step([70, 1], [70, 200], spare=0)
+    step = serving.Step(rows, lengths, spare=0)
     step.pages = 17000  # 17000 pages of 8 x 33 KB: 4.5 GB
     step.table[step.table >= 0] += step.pages - 1 - step.table.max()
     x = rows_of(step, heads, dim, 1)
@@ -151,9 +155,9 @@ def test_offsets_past_32_bits(fk, gpu):
 def test_many_sequences(fk, gpu):
     """More sequences than a wave has lanes, many without rows."""
     rng = np.random.default_rng(3)
-    for high in (2, 40):
-        rows = [int(r) if rng.random() < 0.6 else 0 for r in rng.integers(0, high, 4300)]
-        step = serving.Step(rows, [r + int(p) for r, p in zip(rows, rng.integers(0, 9, 4300))], padding=1)
+    for high, count in ((2, 4300), (40, 4300), (100, 300)):
+        rows = [int(r) if rng.random() < 0.6 else 0 for r in rng.integers(0, high, count)]
+        step = serving.Step(rows, [r + int(p) for r, p in zip(rows, rng.integers(0, 9, count))], padding=1)
         x = rows_of(step, 1, 32, 1)
         cache = fk.PagedCache(step.pages, 1, 32, device=gpu)
         cache.write(step.batch(fk, gpu), x.to(gpu), -x.to(gpu))
