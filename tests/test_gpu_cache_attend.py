@@ -13,8 +13,6 @@ the row's largest |weight * value| is added. (A row whose one heavy key has leve
 it: there W is next to nothing.)
 """
 
-import math
-
 import numpy as np
 import pytest
 
@@ -95,7 +93,7 @@ def test_against_64_bits(fk, gpu, rows, lengths, heads, kv_heads, dim):
 
 
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 100, 5000])
-@pytest.mark.parametrize("rows,lengths", [([1, 1], [300, 40]), ([150], [400]), ([4, 3], [70, 200])])
+@pytest.mark.parametrize("rows,lengths", [([1, 1], [300, 40]), ([150], [400]), ([4, 3], [70, 200]), ([130, 1], [1500, 2100])])
 def test_windows(fk, gpu, rows, lengths, window):
     case = Case(fk, gpu, rows, lengths, 4, 2, 64, seed=window)
     case.check(case.run(window=window), window=window)
@@ -113,7 +111,8 @@ def test_windows_longer_than_any_sequence(fk, gpu, rows, length, window):
 
 
 @pytest.mark.parametrize("rows,lengths,heads,kv_heads,dim", [
-    ([1], [5000], 14, 2, 64), ([1, 1, 1], [9000, 1, 3001], 4, 1, 128), ([3], [4097], 8, 4, 128), ([40, 1], [2500, 1400], 4, 2, 64)])
+    ([1], [5000], 14, 2, 64), ([1, 1, 1], [9000, 1, 3001], 4, 1, 128), ([3], [4097], 8, 4, 128), ([40, 1], [2500, 1400], 4, 2, 64),
+    ([400, 1], [2500, 1400], 4, 2, 64), ([150], [2600], 8, 2, 128), ([300], [2000], 3, 3, 72), ([120], [3000], 2, 1, 192)])
 def test_long_caches_split_over_workgroups(fk, gpu, rows, lengths, heads, kv_heads, dim):
     case = Case(fk, gpu, rows, lengths, heads, kv_heads, dim)
     got = case.run()
@@ -237,8 +236,8 @@ def test_nan_and_infinity_stay_in_their_rows(fk, gpu, rows):
 
 def test_strides_and_unaligned_rows(fk, gpu):
     import torch
-    for rows in ([1, 1], [90, 3]):
-        case = Case(fk, gpu, rows, [95, 100], 4, 2, 36)
+    for rows in ([1, 1], [90, 3], [200, 3]):
+        case = Case(fk, gpu, rows, [max(rows[0], 95), 100], 4, 2, 36)
         n, width = case.step.total(), 4 * 36
         flat = torch.full((n * 301 + 1,), 9.0, device=gpu)
         query = flat.as_strided((n, 4, 36), (301, 36, 1), 1)
