@@ -1,4 +1,5 @@
-// Attention of a step's new tokens over the paged 8-bit cache (fg_cache_attend).
+// Attention of a step's new tokens over the paged 8-bit cache (fg_cache_attend): out = sum_j w_j v_j / sum_j w_j,
+// w_j = exp(scale q.k_j - m), in one pass over the pages with a running reference in m's place.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -249,8 +250,9 @@ struct RowSums {
     float r, total;
 };
 
-// 16 scores of one row in this lane, t = s * f, to weights times the values' scales, into x; the row's other scores are in the lanes that `combine` joins. edge: keys outside [low, high] are
-// masked (key(i) is score i's position). rescale(a) scales the row's sums of this lane by a.
+// 16 scores of one row in this lane, t = s * f, to weights times the values' scales, into x; the row's other
+// scores are in the lanes that `combine` joins. edge: keys outside [low, high] are masked (key(i) is score i's
+// position). rescale(a) scales the row's sums of this lane by a.
 template <class Key, class Combine, class Rescale>
 __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], float vs, float f, bool edge, int low,
                                       int high, RowSums &sums, Key key, Combine combine, Rescale rescale)
@@ -317,6 +319,13 @@ __device__ __forceinline__ float part_factor(float r, float joined) { return r =
 //   scores:  four products of 16 keys: row i of product t is key 32 (i / 8) + 8 t + i % 8, so lane l gets
 //            the scores of keys 32 (g / 2) + 8 t + 4 (g % 2) + r, r = 0 .. 3;
 //   values:  16 dimensions by 32 keys: the lane's 16 bytes of dimension l % 16 are those keys', in order.
+// A decode step's pairs are the heads of a key head's group, 4 to 16 in most models: 16 rows leave the
+// matrix cores idle lanes that cost nothing, for memory is what bounds long caches: 8 sequences of 34000 to 70000 tokens,
+// 4 key heads of 128 (442 MB), 87 us, 5.1 TB/s, the rate of a large copy. 64 sequences of 6 to 8001 tokens (87 MB) take
+// 27 us, 3.2 TB/s, for parts of 16 pages or so that each start with a chain of waits (the plan, the
+// table, the first page); one of 511 tokens, 2 key heads of 64, is that chain alone, 7.6 us.
+// (Two tiles of rows a workgroup, which halves the reading of 17 to 32 pairs, left one workgroup a CU: 64 sequences
+// of up to 3200 tokens, 28 pairs, 25.5 against 24.1 us, 32 pairs over one key head 36.9 against 24.2.)
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(AttendParams p)
 {
@@ -504,6 +513,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(Atte
 // the products' operand order (16 bytes a lane, lane after lane: no bank conflicts), while the other is
 // read. The products are 32 x 32 x 16; lane l holds pair l % 32 and, with h = l / 32, the scores of
 // keys 8 j + 4 h + i in register 4 j + i: the order of the values' record.
+// Bounded by the matrix cores, with the vector units close behind: of a page and head of 128 a wave has
+// 64 products of 32 cycles and about 1600 cycles of vector work (per score a multiplication by the key's scale, an
+// exponential, the value's scale, the total, the maximum and two f16 pieces), and two waves a SIMD overlap them in part.
+// 8192 tokens of 16 heads of 128 over 4: 511 us, 1076 TFLOP/s in f16 products (two an operand, for the
+// pieces), the matrix cores busy 61 % of the time; a large f16 product of the library's reaches 1175. Chunks of 2700
+// tokens, 16 heads of 72 over a window of 1000: 75 us, 336 TFLOP/s: its 350 tiles of 19 pages leave 160 of 256 CUs with
+// one and 96 with two. 32 pairs a wave: with 64, or with four waves a SIMD, the sums do not fit the registers.
 template <int DP>
 constexpr size_t many_lds() { return size_t(2) * (256 * DP + 2 * kPage * 4); }
 
@@ -704,7 +720,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
 }
 
 // The parts of split tiles joined: per slot where a tile's parts start and head, a wave for each tile of
-// ROWS pairs and piece of dimensions (four a lane, the lanes as the kernels above hold them).
+// ROWS pairs and piece of dimensions (four a lane, the lanes as the kernels above hold them). Launch and
+// the chain of note, parts, division bound it: 4.2 us for 64 sequences of up to 8000 tokens, 8 for 500 parts of 8
+// long ones, 7 for chunks of 1300 rows, 14 heads of 64.
 template <int DP, int ROWS, int TILES>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p)
 {

@@ -14,6 +14,13 @@
 // Weights are 64-bit: exp in f64 (one ulp), rounded to a whole number of units of 2^-45 of the first token's
 // (less for more than 2^18 tokens), so that every sum is exact and their order changes nothing. Tokens
 // under half a unit (z < -31.9) weigh 0; the last bin holds only such.
+//
+// What it costs: a logit is read three times, by top, bins and collect (the draw reads one chunk more), mostly from
+// the Infinity Cache after the first, and takes about 35 vector instructions in f64 and one 64-bit LDS addition in
+// the bins. 64 rows of 151936 (39 MB): top 10 us, 3.7 TB/s; bins 17, the arithmetic; cut 9.5; collect 9.5, 4.1 TB/s;
+// draw 11. One row: 3.6, 5.9, 8.5, 3.9, 8.6: each launch is a chain of dependent steps on 1 to 16 CUs (the cut and
+// the draw some ten barriers). In one workgroup a row, 512 rows 202 us: two rounds of 256 of a third each of top and
+// collect from memory (311 MB, more than the Infinity Cache holds) and of the bins' arithmetic; 200 rows of 32003 36 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,9 +37,9 @@ constexpr int kThreads = 1024;      // of the kernels that walk a row, and of th
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 1024;
 constexpr float kPerUnit = 32.0f;   // bins a unit of z
-constexpr int kList = 2560;         // tokens a row's list holds
-constexpr int kRank = 128;          // up to so many listed tokens are compared with each other
-constexpr int kFew = 1024;          // up to so many tokens before the cut are all listed
+constexpr int kList = 2560;         // tokens a row's list holds: what 64 KB of LDS hold beside the rest
+constexpr int kRank = 128;          // up to so many listed tokens are compared with each other, all in one step
+constexpr int kFew = 1024;          // up to so many tokens before the cut are all listed: no chunk is walked then
 constexpr int kMaxChunks = kSampleChunks;
 
 // What the bins say of a row. Tokens of bins under `low` are kept whole; those of [low, high] and of

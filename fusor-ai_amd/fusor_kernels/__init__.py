@@ -3,9 +3,10 @@
 The names follow the reference crate's public API (kernels/src/lib.rs:22-31): DType, Tensor,
 Table, Matrix, Vector, QuantFormat, QuantizedRows, Quantized, Input, quantize_rows, matmul,
 Linear, project, project_input, project_residual, project_residual_input, conv.project_rows,
-QuantizedMatrix and the constants, and the blocks crate's int8 attention (attention::attend). Beside them serving.py has what a
-program of many sequences needs: PagedCache, Batch and sample. Every computation runs in the
-HIP library libfusor_gpu.so through its C ABI (include/fusor_gpu.h); there is no CPU fallback.
+QuantizedMatrix and the constants, and the blocks crate's int8 attention (attention::attend).
+Beside them serving.py has what a program of many sequences needs: PagedCache, Batch and sample.
+Every computation runs in the HIP library libfusor_gpu.so through its C ABI
+(include/fusor_gpu.h); there is no CPU fallback.
 """
 
 from ._lib import Error, FormatError, GpuError, ShapeError, lib
