@@ -11,9 +11,21 @@ import ctypes
 import math
 
 from . import _lib
-from ._lib import FgBatch, FgSampling, ShapeError, check, lib, ptr, stream_handle
+from ._lib import FgBatch, FgSampling, ShapeError, check, lib, stream_handle
 
 PAGE = 64  # tokens of a page: FG_CACHE_PAGE
+
+# A step makes these calls once a layer, and what they compute often takes less time than the call: of a
+# write's 7 us on the host the launch is 4. So torch is a name of the module from the first use on, addresses
+# go as whole numbers, and tensors of the plain layout are checked by their shape and contiguity alone.
+torch = None
+
+
+def _load():
+    global torch
+    if torch is None:
+        import torch as module
+        torch = module
 
 
 class _Here:
@@ -31,7 +43,6 @@ _here = _Here()
 
 @contextlib.contextmanager
 def _on(device, stream):
-    import torch
     with torch.cuda.device(device):
         if stream is None:
             yield
@@ -43,21 +54,27 @@ def _on(device, stream):
 def _place(device, stream):
     """The tensors' device current, and with `stream` that stream too (what a call allocates is then its
     own)."""
-    import torch
     if stream is None and device.index == torch._C._cuda_getDevice():
         return _here
     return _on(device, stream)
 
 
+def _stream(device):
+    """The current stream of `device`, which is current."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 def _scratch(size, device):
     """Device memory of a call from torch's allocator, which hands it out again in the stream's order
     (a graph that is captured keeps what it uses), for about a fifth of what the library's pool costs."""
-    import torch
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def _check_ints(name, t, shape):
-    import torch
     if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
         raise ShapeError(f"{name}: a contiguous int32 device tensor")
     if shape is not None and list(t.shape) != shape:
@@ -66,12 +83,13 @@ def _check_ints(name, t, shape):
 
 def _check_heads(name, t, heads, head_dim, device, written):
     """[rows, heads, head_dim] float32 whose rows are runs of heads * head_dim values."""
-    import torch
     if t.dtype is not torch.float32 or t.device != device:
         raise ShapeError(f"{name}: a float32 tensor on {device}")
     shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
         raise ShapeError(f"{name} of shape {list(shape)}, [rows, {heads}, {head_dim}] expected")
+    if t.is_contiguous():
+        return
     row, head, value = t.stride()
     if shape[0] == 0:
         return
@@ -91,6 +109,7 @@ class Batch:
     """
 
     def __init__(self, row_starts, lengths, pages):
+        _load()
         if pages.dim() != 2:
             raise ShapeError("pages: [sequences, max_pages]")
         sequences = pages.shape[0]
@@ -107,7 +126,8 @@ class Batch:
 
     def _ffi(self, rows):
         p = self.pages
-        return FgBatch(p.shape[0], rows, p.shape[1], ptr(self.row_starts), ptr(self.lengths), ptr(p))
+        sequences, max_pages = p.shape
+        return FgBatch(sequences, rows, max_pages, self.row_starts.data_ptr(), self.lengths.data_ptr(), p.data_ptr())
 
 
 class PagedCache:
@@ -116,7 +136,7 @@ class PagedCache:
     key and value of a head as int8 levels and one float32 scale."""
 
     def __init__(self, pages, kv_heads, head_dim, device=None, stream=None):
-        import torch
+        _load()
         device = torch.device("cuda" if device is None else device)
         if device.type != "cuda":
             raise ShapeError("a cache is on a GPU")
@@ -130,7 +150,7 @@ class PagedCache:
 
     def __del__(self):
         h = getattr(self, "handle", None)
-        if h is not None and _lib._lib is not None:
+        if h is not None and _lib is not None and _lib._lib is not None:  # (None as the interpreter ends)
             _lib._lib.fg_cache_free(h)
             self.handle = None
 
@@ -148,22 +168,21 @@ class PagedCache:
         (a page that is written to belongs to one sequence)."""
         fg = self._rows(batch, keys, values, False)
         with _place(self.device, stream):
-            check(lib().fg_cache_write(self.handle, ctypes.byref(fg), ptr(keys), keys.stride(0), ptr(values),
-                                       values.stride(0), stream_handle()))
+            check(lib().fg_cache_write(self.handle, ctypes.byref(fg), keys.data_ptr(), keys.stride(0), values.data_ptr(),
+                                       values.stride(0), _stream(self.device)))
 
     def read(self, batch, keys, values, stream=None):
         """The same tokens read back into `keys` and `values`: level * scale."""
         fg = self._rows(batch, keys, values, True)
         with _place(self.device, stream):
-            check(lib().fg_cache_read(self.handle, ctypes.byref(fg), ptr(keys), keys.stride(0), ptr(values),
-                                      values.stride(0), stream_handle()))
+            check(lib().fg_cache_read(self.handle, ctypes.byref(fg), keys.data_ptr(), keys.stride(0), values.data_ptr(),
+                                      values.stride(0), _stream(self.device)))
 
     def attend(self, batch, queries, out=None, scale=None, window=0, stream=None):
         """The attention of the new tokens' `queries` [rows, heads, head_dim] (their keys and values
         written before): each token sees its sequence's tokens up to itself, with `window` the last
         `window` of them. `scale` is 1 / sqrt(head_dim) unless given. A token without a key gives 0;
         rows of `out` that no sequence holds are left as they are (0 in an `out` made here)."""
-        import torch
         if batch.pages.device != self.device:
             raise ShapeError(f"the batch is on {batch.pages.device}, the cache on {self.device}")
         if queries.dim() != 3:
@@ -181,9 +200,9 @@ class PagedCache:
             fg, library = ctypes.byref(batch._ffi(queries.shape[0])), lib()
             size = library.fg_cache_attend_scratch(self.handle, fg, heads)
             scratch = _scratch(size, self.device)
-            check(library.fg_cache_attend(self.handle, fg, ptr(queries), queries.stride(0), heads,
-                                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, ptr(out),
-                                          out.stride(0), ptr(scratch), size, stream_handle()))
+            check(library.fg_cache_attend(self.handle, fg, queries.data_ptr(), queries.stride(0), heads,
+                                          1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, out.data_ptr(),
+                                          out.stride(0), _at(scratch), size, _stream(self.device)))
         return out
 
 
@@ -192,7 +211,7 @@ def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None,
     `random` [rows] in [0, 1). The settings are device tensors [rows]: float32 `temperature` (0: the
     most likely token), int32 `top_k` (0: no limit), float32 `top_p` (1: no limit) and `min_p` (0: no
     limit), applied in that order. Returns (tokens int32 [rows], chances float32 [rows])."""
-    import torch
+    _load()
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
         raise ShapeError("logits: a float32 device tensor [rows, vocab]")
     rows, vocab = logits.shape
@@ -205,14 +224,14 @@ def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None,
                            ("min_p", min_p, f32), ("tokens", tokens, i32), ("chances", chances, f32)):
         if t is not None and (t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous()):
             raise ShapeError(f"{name}: a contiguous {dtype} tensor [{rows}] on {device}")
-    with _place(logits.device, stream):
+    with _place(device, stream):
         if tokens is None:
-            tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+            tokens = torch.empty(rows, dtype=i32, device=device)
         if chances is None:
-            chances = torch.empty(rows, dtype=torch.float32, device=logits.device)
-        fg = FgSampling(ptr(random), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p))
-        size = lib().fg_sample_scratch(rows, vocab)
-        scratch = _scratch(size, logits.device)
-        check(lib().fg_sample(ptr(logits), rows, vocab, logits.stride(0), ctypes.byref(fg), ptr(tokens), ptr(chances),
-                              ptr(scratch), size, stream_handle()))
+            chances = torch.empty(rows, dtype=f32, device=device)
+        fg, library = FgSampling(random.data_ptr(), _at(temperature), _at(top_k), _at(top_p), _at(min_p)), lib()
+        size = library.fg_sample_scratch(rows, vocab)
+        scratch = _scratch(size, device)
+        check(library.fg_sample(logits.data_ptr(), rows, vocab, logits.stride(0), ctypes.byref(fg), tokens.data_ptr(),
+                                chances.data_ptr(), _at(scratch), size, _stream(device)))
     return tokens, chances
