@@ -353,19 +353,27 @@ struct CutShared {
     float edge[4];
 };
 
-// The smallest logit whose bin is at most b, by halving the order of floats 64 ways at a time.
+// The smallest logit whose bin is at most b: among the 64 floats around the bin's far end, or (rounding, next to 0,
+// may have put it elsewhere) by dividing the order of floats 64 ways at a time.
 __device__ __forceinline__ float smallest_of_bin(int b, float first, double scale)
 {
     if (b >= kBins - 1) return -INFINITY;
     if (b < 0) return __builtin_nanf("");  // nothing is >= NaN
     const int lane = threadIdx.x & 63;
     const double top = top_of(first);
+    auto within = [&](float x) { return bin_of(bins_of(x, top, scale)) <= b && x > -INFINITY; };
     unsigned lo = 0, n = ordered(first);  // the answer is in (lo, lo + n]; the first token has bin 0
+    const unsigned near = ordered(plain_logit(float(top - double(b + 1) / scale)));
+    if (near > 32 && near < n) {
+        const unsigned at = min(near - 32 + unsigned(lane), n);
+        const u64 yes = __ballot(within(plain_logit(unordered(at))));
+        if (yes && !(yes & 1)) return unordered(near - 32 + unsigned(__builtin_ctzll(yes)));
+    }
     while (n > 1) {
         const unsigned step = (n + 63) / 64, at = lo + (lane + 1) * step;
         const bool inside = u64(lane + 1) * step <= n;
         const float x = plain_logit(unordered(inside ? at : lo + n));
-        const bool yes = bin_of(bins_of(x, top, scale)) <= b && x > -INFINITY;
+        const bool yes = within(x);
         const int k = __builtin_ctzll(__ballot(yes || !inside) | 1ull << 63);
         const unsigned from = lo + unsigned(k) * step, to = lo + n;
         lo = from;
@@ -436,10 +444,15 @@ __device__ __forceinline__ Cut cut_of(const SampleParams &p, const Row &r, float
         c.high = min(c.high, kBins - 2);  // (the last bin's tokens weigh 0)
         c.low = min(c.low, c.high);
     }
-    // few tokens up to top-k's bin: all of them are listed
+    // few tokens up to top-k's bin, or (counted with top-k) up to the last cut's: all of them are listed
     if (lists && c.last < kBins && sh.upto <= unsigned(kFew)) {
         c.low = 0;
         c.high = c.last;
+    }
+    if (lists && c.last == kBins && r.has_k) {
+        if (tid == c.high) sh.upto = unsigned(before_n + n);
+        __syncthreads();
+        if (sh.upto <= unsigned(kFew)) c.low = 0;
     }
     if (tid == c.low) sh.mass_low = before_m;
     const int wave = tid >> 6, lane = tid & 63;
@@ -481,15 +494,23 @@ __global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleParams p)
 {
     __shared__ CutShared sh;
     const int row = int(blockIdx.x), tid = threadIdx.x;
-    const Row r = row_of(p, row);
-    u64 m = 0, n = 0;
+    // everything is asked for at once (past the last chunk that one's again), and looked at then
     const u64 *mass = p.mass + size_t(row) * p.chunks * kBins + tid;
     const unsigned *count = p.count + size_t(row) * p.chunks * kBins + tid;
+    u64 masses[kMaxChunks];
+    unsigned counts[kMaxChunks] = {};
 #pragma unroll
-    for (int c = 0; c < kMaxChunks; c++) m += c < p.chunks ? mass[c * kBins] : 0;
-    if (r.has_k) {
+    for (int c = 0; c < kMaxChunks; c++) masses[c] = mass[min(c, p.chunks - 1) * kBins];
+    if (p.top_k) {
 #pragma unroll
-        for (int c = 0; c < kMaxChunks; c++) n += c < p.chunks ? count[c * kBins] : 0;
+        for (int c = 0; c < kMaxChunks; c++) counts[c] = count[min(c, p.chunks - 1) * kBins];
+    }
+    const Row r = row_of(p, row);
+    u64 m = 0, n = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxChunks; c++) {
+        m += c < p.chunks ? masses[c] : 0;
+        n += c < p.chunks ? counts[c] : 0;
     }
     const u64 first = row_top(p, row);
     const float top = unordered(unsigned(first >> 32));
@@ -539,6 +560,24 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleParams p
         if (base + i < unsigned(kList)) p.list[size_t(a.row) * kList + base + i] = found[i];
 }
 
+// The running weight that top-p's first token passes, of a total: the first whose sum reaches top_p of it exceeds the
+// whole number before.
+__device__ __forceinline__ u64 weight_over(const Cut &c, u64 total)
+{
+    u64 over = u64(ceil(double(c.top_p) * double(total)));
+    over = over > 0 ? over - 1 : 0;
+    return over >= total ? total - 1 : over;
+}
+
+// The running total that the drawn token passes, of the kept one.
+__device__ __forceinline__ u64 goal_of(const SampleParams &p, int row, u64 all)
+{
+    float u = p.random[row];
+    u = u > 0.0f ? u : 0.0f;  // (NaN too)
+    const u64 goal = u64(double(u < 1.0f ? u : 1.0f) * double(all));
+    return goal < all ? goal : all - 1;
+}
+
 struct DrawShared {
     u64 key[kList];     // (~ordered logit, index): the order, ascending
     u64 weight[kList];
@@ -555,12 +594,126 @@ struct DrawShared {
     double middles[kBins];
 };
 
+// A row's token from its cuts, where no bin is kept whole and the list is of at most kRank tokens, (logit bits, index)
+// in sh.key: put in order by counting for each those before it, a wave then finds the cuts in the running
+// sums, and each kept one's running total by index is the sum of the kept ones of lower index.
+__device__ __forceinline__ void draw_few(const SampleParams &p, int row, const Cut &c, int listed, DrawShared &sh)
+{
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int width = listed <= 64 ? 64 : 128, rounds = kThreads / width, i = tid & (width - 1), part = tid / width;
+    u64 key = ~0ull, w = 0;
+    unsigned note = 0;  // the bin, and whether the weight is under min-p's
+    if (tid < listed) {
+        const u64 e = sh.key[tid];
+        const float v = __uint_as_float(unsigned(e >> 32));
+        const double t = bins_of(v, c.top, c.scale);
+        const int b = bin_of(t);
+        const double weight = weight_of(t, middle_of(b) * p.unit);
+        key = u64(~ordered(v)) << 32 | unsigned(e);
+        w = units_of(weight);
+        note = unsigned(b) | (weight < c.least ? 0x10000u : 0u);
+    }
+    if (tid < width) {
+        sh.ranked[tid] = ulonglong2{key, 0};
+        sh.tokens[tid] = 0;
+        sh.before[tid] = 0;
+    }
+    __syncthreads();
+    {
+        const u64 q = sh.ranked[i].x;
+        unsigned n = 0;
+#pragma unroll 4
+        for (int j = part; j < listed; j += rounds) n += sh.ranked[j].x < q;
+        if (i < listed) atomicAdd(&sh.tokens[i], n);
+    }
+    __syncthreads();
+    if (tid < listed) {
+        const unsigned at = sh.tokens[tid];
+        sh.ranked[at] = ulonglong2{key, w};
+        sh.count[at] = note;
+    }
+    __syncthreads();
+    if (tid < 64) {  // two tokens a lane, in order
+        const int at = 2 * lane;
+        ulonglong2 a[2];
+        int bin[2];
+        bool light[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const bool there = at + k < listed;
+            a[k] = there ? sh.ranked[at + k] : ulonglong2{~0ull, 0};
+            bin[k] = there ? int(sh.count[at + k] & 0xFFFF) : kBins;
+            light[k] = !there || (sh.count[at + k] & 0x10000u) != 0;
+        }
+        // the place and the running weight of the token of which hit(k) holds, in the sums of the tokens that take(k)
+        // takes; hit is given the running weight before it
+        auto find = [&](auto take, auto hit, u64 *upto) {
+            const u64 w0 = take(0) ? a[0].y : 0, w1 = take(1) ? a[1].y : 0;
+            const u64 sum = wave_upto(w0 + w1), before = sum - w0 - w1;
+            const bool hit0 = take(0) && hit(0, before, w0), hit1 = take(1) && hit(1, before + w0, w1);
+            const u64 lanes = __ballot(hit0 || hit1);
+            const int from = lanes ? __builtin_ctzll(lanes) : 63;
+            *upto = lane_of(hit0 ? before + w0 : sum, from);
+            return __builtin_amdgcn_readlane(hit0 ? at : at + 1, from);
+        };
+        int cut = kRank;
+        u64 total = c.mass_last;
+        if (c.last < kBins) {
+            const int n0 = bin[0] == c.last, n1 = bin[1] == c.last, need = c.top_k - int(c.before_last);
+            int ignored;
+            const int count = wave_scan(n0 + n1, &ignored);
+            u64 upto;
+            cut = find([&](int k) { return bin[k] == c.last; }, [&](int k, u64, u64) { return (k ? count : count - n1) == need; }, &upto);
+            total = c.mass_last + upto;
+        }
+        if (c.by_p) {
+            const u64 over = weight_over(c, total);
+            u64 upto;
+            const int k = find([&](int k) { return bin[k] <= c.high && at + k <= cut; },
+                               [&](int, u64 before, u64 w) { return before <= over && before + w > over; }, &upto);
+            cut = min(cut, k);
+        }
+        const bool keep0 = at <= cut && !light[0], keep1 = at + 1 <= cut && !light[1];
+        const u64 w0 = keep0 ? a[0].y : 0, w1 = keep1 ? a[1].y : 0;
+        const u64 all = lane_of(wave_upto(w0 + w1), 63);
+        if (at < listed) sh.ranked[at] = ulonglong2{a[0].x & 0xFFFFFFFFull, w0};
+        if (at + 1 < listed) sh.ranked[at + 1] = ulonglong2{a[1].x & 0xFFFFFFFFull, w1};
+        if (lane == 0) sh.mass_before = all;
+    }
+    __syncthreads();
+    const u64 all = sh.mass_before, goal = goal_of(p, row, all);
+    if (i < listed) {
+        const u64 q = sh.ranked[i].x;
+        u64 m = 0;
+#pragma unroll 4
+        for (int j = part; j < listed; j += rounds) {
+            const ulonglong2 other = sh.ranked[j];
+            m += other.x < q ? other.y : 0;
+        }
+        atomicAdd(&sh.before[i], m);
+    }
+    __syncthreads();
+    if (tid < listed) {
+        const ulonglong2 mine = sh.ranked[tid];
+        const u64 before = sh.before[tid];
+        if (before <= goal && before + mine.y > goal) {
+            p.tokens[row] = int(mine.x);
+            if (p.chances) p.chances[row] = float(double(mine.y) / double(all));
+        }
+    }
+}
+
 // A row's token from its cuts, by one workgroup. The list's `listed` tokens are (logit bits, index) in sh.key, or,
 // if they are too many, found in the row again by every pass over them. whole_of(k): the weight of chunk k's
 // whole bins.
 template <class F>
 __device__ __forceinline__ void draw_token(const SampleParams &p, int row, const Cut &c, unsigned listed, DrawShared &sh, F whole_of)
 {
+    if (c.low == 0 && listed <= unsigned(kRank)) {
+        __syncthreads();  // (the list is there)
+        draw_few(p, row, c, int(listed), sh);
+        return;
+    }
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const double top = c.top, scale = c.scale, least = c.least;
     if (tid == 0) {
@@ -734,11 +887,7 @@ __device__ __forceinline__ void draw_token(const SampleParams &p, int row, const
         total = c.mass_last + upto;
     }
     if (c.by_p) {
-        // the first token whose running weight reaches top_p of the total: exceeds the whole number before
-        const double goal = double(c.top_p) * double(total);
-        u64 over = u64(ceil(goal));
-        over = over > 0 ? over - 1 : 0;
-        over = over >= total ? total - 1 : over;
+        u64 over = weight_over(c, total);
         over = over > c.mass_low ? over - c.mass_low : 0;
         u64 upto;
         const u64 k = select(false, 0, over, order, [&](u64 q, u64, int b) { return b >= c.low && b <= c.high && q <= cut; }, &upto);
@@ -758,10 +907,7 @@ __device__ __forceinline__ void draw_token(const SampleParams &p, int row, const
     __syncthreads();
     u64 all;
     const u64 m = tid < 256 ? sh.mass[tid] : 0, before = block_before<kWaves>(m, sh.part, &all);
-    float u = p.random[row];
-    u = u > 0.0f ? u : 0.0f;  // (NaN too)
-    u64 goal = u64(double(u < 1.0f ? u : 1.0f) * double(all));
-    goal = goal < all ? goal : all - 1;
+    u64 goal = goal_of(p, row, all);
     if (!whole) {
         u64 upto;
         const u64 k = select(false, 0, goal, [](u64 q) { return q & 0xFFFFFFFFull; }, keeps, &upto);
