@@ -17,10 +17,10 @@
 //
 // What it costs: a logit is read three times, by top, bins and collect (the draw reads one chunk more), mostly from
 // the Infinity Cache after the first, and takes about 35 vector instructions in f64 and one 64-bit LDS addition in
-// the bins. 64 rows of 151936 (39 MB): top 10 us, 3.7 TB/s; bins 17, the arithmetic; cut 9.5; collect 9.5, 4.1 TB/s;
-// draw 11. One row: 3.6, 5.9, 8.5, 3.9, 8.6: each launch is a chain of dependent steps on 1 to 16 CUs (the cut and
-// the draw some ten barriers). In one workgroup a row, 512 rows 202 us: two rounds of 256 of a third each of top and
-// collect from memory (311 MB, more than the Infinity Cache holds) and of the bins' arithmetic; 200 rows of 32003 36 us.
+// the bins. 64 rows of 151936 (39 MB): top 11 us, 3.5 TB/s; bins 17, the arithmetic; cut 8.3; collect 9, 4.3 TB/s;
+// draw 10. One row: 3.7, 6.0, 7.2, 4.0, 4.2: each launch is a chain of dependent steps on 1 to 16 CUs. In one
+// workgroup a row, 512 rows 200 us: two rounds of 256, of cycles about 48 thousand top, 100 bins, 50 collect and 30 the
+// rest, so a third each is memory's first reading, arithmetic, and the others; 200 rows of 32003 35 us (8, 22, 10, 22).
 #include <algorithm>
 #include <type_traits>
 
@@ -41,6 +41,7 @@ constexpr int kList = 2560;         // tokens a row's list holds: what 64 KB of 
 constexpr int kRank = 128;          // up to so many listed tokens are compared with each other, all in one step
 constexpr int kFew = 1024;          // up to so many tokens before the cut are all listed: no chunk is walked then
 constexpr int kMaxChunks = kSampleChunks;
+static_assert(kSampleRun == kThreads * 4, "a run is four tokens a thread");
 
 // What the bins say of a row. Tokens of bins under `low` are kept whole; those of [low, high] and of
 // `last` are listed; the others are not kept. last: the bin of top-k's cut (kBins: none).
@@ -218,8 +219,8 @@ __device__ __forceinline__ u64 row_top(const SampleParams &p, int row)
     return t;
 }
 
-// Calls f(logit, index) for the tokens [begin, end) of a row, four a thread of `threads`; the loads of
-// several runs are asked for together.
+// Calls f(logit, index) for the tokens [begin, end) of a row, four a thread of `threads`, the logits as they are
+// there; the loads of several runs are asked for together.
 template <class F>
 __device__ __forceinline__ void for_tokens(const float *x, int begin, int end, int thread, int threads, F f)
 {
@@ -232,15 +233,15 @@ __device__ __forceinline__ void for_tokens(const float *x, int begin, int end, i
 #pragma unroll
         for (int a = 0; a < kAhead; a++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) f(plain_logit(v[a][j]), i + a * threads * 4 + j);
+            for (int j = 0; j < 4; j++) f(v[a][j], i + a * threads * 4 + j);
     }
     for (; i < end; i += threads * 4) {
         if (i + 4 <= end) {
             const v4f v = *reinterpret_cast<const v4f_any *>(x + i);
 #pragma unroll
-            for (int j = 0; j < 4; j++) f(plain_logit(v[j]), i + j);
+            for (int j = 0; j < 4; j++) f(v[j], i + j);
         } else {
-            for (int j = 0; i + j < end; j++) f(plain_logit(x[i + j]), i + j);
+            for (int j = 0; i + j < end; j++) f(x[i + j], i + j);
         }
     }
 }
@@ -268,12 +269,12 @@ __device__ __forceinline__ u64 top_of_tokens(const float *x, int begin, int end,
     float best = -INFINITY;
     int at = none;
     for_tokens(x, begin, end, threadIdx.x, kThreads, [&](float v, int i) {
-        if (v > best) {
+        if (v > best) {  // (not NaN; a zero of either sign is the first one's equal)
             best = v;
             at = i;
         }
     });
-    u64 t = u64(ordered(best)) << 32 | unsigned(~at);
+    u64 t = u64(ordered(plain_logit(best))) << 32 | unsigned(~at);
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
         const u64 o = __shfl_xor(t, d, 64);
@@ -290,19 +291,17 @@ __device__ __forceinline__ u64 top_of_tokens(const float *x, int begin, int end,
     return t;
 }
 
-// The tokens [begin, end) added to the bins' weights, and with top-k to their counts (LDS).
-__device__ __forceinline__ void add_to_bins(const float *x, int begin, int end, double top, double scale, bool counts, u64 *mass,
-                                            unsigned *count, const double *middles)
+// A token added to the bins' weights, and with top-k to their counts (LDS).
+__device__ __forceinline__ void add_to_bins(float v, double top, double scale, bool counts, u64 *mass, unsigned *count,
+                                            const double *middles)
 {
-    for_tokens(x, begin, end, threadIdx.x, kThreads, [&](float v, int) {
-        const double t = bins_of(v, top, scale);
-        const int b = bin_of(t);
-        const u64 w = units_of(weight_of(t, middles[b]));
-        if (b < kBins - 1) {  // (the last bin's weigh 0)
-            if (counts) atomicAdd(&count[b], 1u);
-            atomicAdd(&mass[b], w);
-        }
-    });
+    const double t = bins_of(fmaxf(v, -INFINITY), top, scale);
+    const int b = bin_of(t);
+    const u64 w = units_of(weight_of(t, middles[b]));
+    if (b < kBins - 1) {  // (the last bin's weigh 0)
+        if (counts) atomicAdd(&count[b], 1u);
+        atomicAdd(&mass[b], w);
+    }
 }
 
 // The token of a row that keeps its first alone, or has no logit above -inf.
@@ -337,7 +336,8 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams p)
     count[tid] = 0;
     middles[tid] = middle_of(tid) * p.unit;
     __syncthreads();
-    add_to_bins(a.x, a.begin, a.end, top_of(first), r.scale, r.has_k, mass, count, middles);
+    const double top = top_of(first);
+    for_tokens(a.x, a.begin, a.end, tid, kThreads, [&](float v, int) { add_to_bins(v, top, r.scale, r.has_k, mass, count, middles); });
     __syncthreads();
     const size_t at = (size_t(a.row) * p.chunks + a.chunk) * kBins + tid;
     p.mass[at] = mass[tid];
@@ -528,16 +528,19 @@ __global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleParams p)
 }
 
 __device__ __forceinline__ bool is_listed(const Cut &c, int bin) { return (bin >= c.low && bin <= c.high) || bin == c.last; }
+// No token under it is listed, or of a bin that is kept whole: most of a row is passed over by one comparison.
+__device__ __forceinline__ float floor_of(const Cut &c) { return c.lists ? fminf(c.listed, c.tie) : -INFINITY; }
 
 // The listed ones of the tokens [begin, end) into `found` (LDS, kList of them), (logit bits, index); *count is
 // how many there are.
 __device__ __forceinline__ void list_tokens(const float *x, int begin, int end, const Cut &c, u64 *found, unsigned *count)
 {
-    const float whole = c.whole, listed = c.listed, before = c.before, tie = c.tie;
+    const float whole = c.whole, listed = c.listed, before = c.before, tie = c.tie, floor = floor_of(c);
     for_tokens(x, begin, end, threadIdx.x, kThreads, [&](float v, int i) {
+        if (!(v >= floor)) return;  // (NaN too)
         if (!((v >= listed && !(v >= whole)) || (v >= tie && !(v >= before)))) return;
         const unsigned at = atomicAdd(count, 1u);
-        if (at < unsigned(kList)) found[at] = u64(__float_as_uint(v)) << 32 | unsigned(i);
+        if (at < unsigned(kList)) found[at] = u64(__float_as_uint(plain_logit(v))) << 32 | unsigned(i);
     });
 }
 
@@ -931,7 +934,10 @@ __device__ __forceinline__ void draw_token(const SampleParams &p, int row, const
     __syncthreads();
     const int begin = int(sh.digit) * p.chunk, end = min(begin + p.chunk, p.vocab);
     goal -= sh.mass_before;
-    auto units = [&](float v, int i) {
+    const float floor = floor_of(c);
+    auto units = [&](float x, int i) {
+        if (!(x >= floor)) return u64(0);
+        const float v = plain_logit(x);
         const double t = bins_of(v, top, scale);
         const int b = bin_of(t);
         if (b == kBins - 1 || !(b < c.low || is_listed(c, b))) return u64(0);
@@ -953,11 +959,11 @@ __device__ __forceinline__ void draw_token(const SampleParams &p, int row, const
     const int part = begin + int(sh.digit) * share, part_end = min(part + share, end);
     const int run = (share + kThreads - 1) / kThreads, i0 = part + tid * run, i1 = min(i0 + run, part_end);
     u64 mine = 0;
-    for (int i = i0; i < i1; i++) mine += units(plain_logit(x[i]), i);
+    for (int i = i0; i < i1; i++) mine += units(x[i], i);
     u64 running = block_before<kWaves>(mine, sh.part, &ignored);
     if (running <= goal && running + mine > goal) {
         for (int i = i0; i < i1; i++) {
-            const u64 w = units(plain_logit(x[i]), i);
+            const u64 w = units(x[i], i);
             running += w;
             if (running > goal) {
                 p.tokens[row] = i;
@@ -1014,13 +1020,35 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleParams p)
     middles[tid] = middle_of(tid) * p.unit;
     u64 *upto = p.mass + size_t(row) * p.chunks * kBins + tid;  // this bin's weight up to each chunk's end
     u64 m = 0;
-    for (int c = 0; c < p.chunks; c++) {
-        __syncthreads();
-        add_to_bins(x, c * p.chunk, min((c + 1) * p.chunk, p.vocab), top_of(top), r.scale, r.has_k, sh.bins.mass, sh.bins.count, middles);
-        __syncthreads();
-        upto[c * kBins] = m = sh.bins.mass[tid];
-    }
+    const double largest = top_of(top);
     __syncthreads();
+    constexpr int kAhead = 4, kRun = kSampleRun;  // runs of a chunk, asked for together whatever chunks they are of
+    for (int c = 0, begin = 0; c < p.chunks;) {
+        v4f v[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            const int i = begin + a * kRun + tid * 4;
+            if (i + 4 <= p.vocab) {
+                v[a] = *reinterpret_cast<const v4f_any *>(x + i);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[a][j] = i + j < p.vocab ? x[i + j] : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            if (c == p.chunks) break;
+#pragma unroll
+            for (int j = 0; j < 4; j++) add_to_bins(v[a][j], largest, r.scale, r.has_k, sh.bins.mass, sh.bins.count, middles);
+            begin += kRun;
+            if (begin == (c + 1) * p.chunk || begin >= p.vocab) {  // the chunk's end
+                __syncthreads();
+                upto[c * kBins] = m = sh.bins.mass[tid];
+                __syncthreads();
+                c++;
+            }
+        }
+    }
     const Cut c = cut_of(p, r, top, m, r.has_k ? sh.bins.count[tid] : 0, sh.cut, p.mass + size_t(row) * p.chunks * kBins, true);
     if (tid == 0) sh.listed = 0;
     __syncthreads();  // (the bins are read: the list takes their place)
@@ -1054,7 +1082,7 @@ Shape shape_of(size_t rows, size_t vocab)
     const size_t batches = (rows + most - 1) / most;
     s.batch = (rows + batches - 1) / batches;
     s.chunks = sample_chunks(s.batch, vocab, s.by_rows);
-    s.chunk = int((vocab + size_t(s.chunks) - 1) / size_t(s.chunks) + 255) / 256 * 256;
+    s.chunk = sample_chunk(vocab, s.by_rows, &s.chunks);
     const size_t work = s.batch * s.chunks;
     size_t sizes[7] = {work * 8, work * kBins * 8, work * kBins * 4, work * 8, s.batch * sizeof(Cut), s.batch * 4, s.batch * kList * 8};
     for (int i = 0; i < 7; i++) s.at[i + 1] = s.at[i] + (s.by_rows && i != 1 ? 0 : (sizes[i] + 255) / 256 * 256);

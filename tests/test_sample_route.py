@@ -22,11 +22,13 @@ def route(tmp_path_factory):
     source, lib = where / "route.cpp", where / "route.so"
     source.write_text('#include "sample_route.h"\n'
                       'extern "C" int by_rows(size_t rows, size_t vocab) { return fg::sample_by_rows(rows, vocab); }\n'
-                      'extern "C" int chunks(size_t rows, size_t vocab, int by) { return fg::sample_chunks(rows, vocab, by != 0); }\n')
+                      'extern "C" int chunks(size_t rows, size_t vocab, int by) { return fg::sample_chunks(rows, vocab, by != 0); }\n'
+                      'extern "C" int chunk(size_t vocab, int by, int *chunks) { return fg::sample_chunk(vocab, by != 0, chunks); }\n')
     subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", CSRC, str(source), "-o", str(lib)], check=True)
     lib = ctypes.CDLL(str(lib))
     lib.by_rows.argtypes = [ctypes.c_size_t] * 2
     lib.chunks.argtypes = [ctypes.c_size_t] * 2 + [ctypes.c_int]
+    lib.chunk.argtypes = [ctypes.c_size_t, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
     return lib
 
 
@@ -42,5 +44,7 @@ def test_chunks(route, rows, vocab):
     for by in (0, 1):
         chunks = route.chunks(rows, vocab, by)
         assert 1 <= chunks <= 16
-        chunk = ((vocab + chunks - 1) // chunks + 255) // 256 * 256
-        assert chunk * chunks >= vocab and chunk * (chunks - 1) < vocab + 256 * chunks
+        left = ctypes.c_int(chunks)
+        chunk = route.chunk(vocab, by, ctypes.byref(left))
+        assert chunk % (4096 if by else 256) == 0 and 1 <= left.value <= chunks
+        assert chunk * left.value >= vocab > chunk * (left.value - 1)  # no chunk is empty
