@@ -99,6 +99,23 @@ def test_ties(fk, gpu, vocab):
     check(fk, gpu, few, random, min_p=np.exp(rng.uniform(-3, 0, rows)))
 
 
+@pytest.mark.parametrize("vocab", [5, 63, 64, 65, 127, 128, 129, 130, 6000])
+@pytest.mark.parametrize("tied", [False, True])
+def test_short_lists(fk, gpu, vocab, tied):
+    """Lists of up to 64, up to 128 and more tokens, cut by one limit or several, in one place or apart."""
+    rng = np.random.default_rng(vocab)
+    rows = 60
+    logits = (2 * rng.standard_normal((rows, vocab))).astype(np.float32)
+    if tied:
+        logits = np.round(logits * 2) / 2
+    top_k = rng.integers(1, min(vocab, 140) + 1, rows)
+    top_k[::7] = 0
+    top_p = np.where(np.arange(rows) % 3 == 0, 1.0, rng.uniform(0.05, 0.999, rows))
+    min_p = np.where(np.arange(rows) % 4 == 0, np.exp(rng.uniform(-6, 0, rows)), 0.0)
+    check(fk, gpu, logits, rng.random(rows), temperature=np.exp(rng.uniform(-1, 1, rows)), top_k=top_k, top_p=top_p, min_p=min_p)
+    check(fk, gpu, logits, np.linspace(0, 1, rows, endpoint=False), top_k=top_k)
+
+
 def test_zeros_of_both_signs_are_equal(fk, gpu):
     logits = np.full((2, 300), -1.0, np.float32)
     logits[0, 100], logits[0, 200] = -0.0, 0.0
