@@ -516,10 +516,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(Atte
 // Bounded by the matrix cores, with the vector units close behind: of a page and head of 128 a wave has
 // 64 products of 32 cycles and about 1600 cycles of vector work (per score a multiplication by the key's scale, an
 // exponential, the value's scale, the total, the maximum and two f16 pieces), and two waves a SIMD overlap them in part.
-// 8192 tokens of 16 heads of 128 over 4: 511 us, 1076 TFLOP/s in f16 products (two an operand, for the
+// 8192 tokens of 16 heads of 128 over 4: 492 us, 1118 TFLOP/s in f16 products (two an operand, for the
 // pieces), the matrix cores busy 61 % of the time; a large f16 product of the library's reaches 1175. Chunks of 2700
-// tokens, 16 heads of 72 over a window of 1000: 75 us, 336 TFLOP/s: its 350 tiles of 19 pages leave 160 of 256 CUs with
-// one and 96 with two. 32 pairs a wave: with 64, or with four waves a SIMD, the sums do not fit the registers.
+// tokens, 16 heads of 72 over a window of 1000: 75 us, 336 TFLOP/s: its 350 tiles of 19 pages are 1400 waves
+// for 1024 SIMDs, so some have two. 32 pairs a wave: with 64, or with four waves a SIMD, the sums do not fit the registers.
 template <int DP>
 constexpr size_t many_lds() { return size_t(2) * (256 * DP + 2 * kPage * 4); }
 
