@@ -215,7 +215,8 @@ int fg_cache_read(const fg_cache *cache, const fg_batch *batch, float *key, size
  * position p sees its sequence's keys at positions max(0, p - window + 1) .. p, all up to p where
  * `window` is 0. Head h of row r is the head_dim device f32 values at r * stride + h * head_dim of
  * `query` and `out`; `heads` query heads share the cache's heads in consecutive runs. Scores are
- * scale * q.k (|scale| at most 2e38); a row that sees no key gives 0. The work is ordered on `stream`.
+ * scale * q.k (|scale| at most 2e38); a row that sees no key gives 0. `out` may be
+ * `query`, with its stride. The work is ordered on `stream`.
  * `scratch`: device memory of at least fg_cache_attend_scratch's bytes, 16-byte aligned, that nothing else
  * uses until the call's work is done (two graphs that replay at once need one each); NULL: taken from the
  * library's pool as for fg_matmul, under capture too, which costs the call about 8 us of host time. */

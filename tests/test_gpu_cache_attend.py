@@ -258,6 +258,27 @@ def test_sequences_that_share_pages(fk, gpu):
     case.check(case.run())
 
 
+@pytest.mark.parametrize("rows,lengths", [([1, 1], [2500, 40]), ([9], [70]), ([150, 3], [2500, 300]), ([300], [300])])
+def test_outputs_over_the_queries(fk, gpu, rows, lengths):
+    """`out` may be `queries`: a row's are read before its outputs are written."""
+    case = Case(fk, gpu, rows, lengths, 8, 2, 64, padding=2)
+    want = case.run()
+    both = case.query.to(gpu)
+    case.cache.attend(case.step.batch(fk, gpu), both, out=both)
+    import torch
+    n = int(case.step.starts[-1])
+    assert torch.equal(both.cpu()[:n], want[:n]) and torch.equal(both.cpu()[n:], case.query[n:])
+
+
+@pytest.mark.parametrize("rows", [1, 20, 200])
+def test_a_page_named_twice(fk, gpu, rows):
+    """... by one sequence is seen twice."""
+    case = Case(fk, gpu, [rows], [300], 4, 2, 64)
+    case.step.table[0, 0] = case.step.table[0, 2]
+    case.keys[:64], case.values[:64] = case.keys[128:192], case.values[128:192]
+    case.check(case.run())
+
+
 def test_many_sequences(fk, gpu):
     rng = np.random.default_rng(1)
     for high in (2, 9):
