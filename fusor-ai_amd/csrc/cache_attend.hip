@@ -795,7 +795,8 @@ constexpr size_t kUnits = 256;  // CUs
 //
 // attend_few_kernel up to 96 pairs a sequence, few's time and many's: 64 sequences of up to 3200 tokens, 48 pairs
 // (a) 66 and 91, 84 pairs (b) 32 and 43, 96 pairs (a) 92 and 100, (c) 43 and 38; 128 pairs (a) 112 and 114, (c) 50
-// and 40.
+// and 40. Up to 64 for heads past 128: 8 heads of 256 over 2, 48 pairs 89 and 94, 64 pairs 104 and 96, 96 pairs 134
+// and 101; 8 of 192 over 1, 64 pairs 50 and 51, 96 73 and 56.
 //
 // Tiles are split when there are at most as many as CUs, all heads together: 64 sequences of up to 8000 tokens
 // (a) 71 whole and 56 split, (b) 42 and 21; all of 8000, which a CU each serves evenly, (a) 98 and 108; 128 sequences
@@ -809,7 +810,7 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
 {
     Launch l{};
     const size_t group = heads / c->kv_heads, pairs = b->rows * group, sequences = std::min(b->sequences, b->rows);
-    l.few = pairs <= 96 * sequences;
+    l.few = pairs <= (c->padded <= 128 ? 96 : 64) * sequences;
     const size_t tm = l.few ? 16 : 128, units = std::max<size_t>(kUnits / c->kv_heads, 1);
     const size_t tiles = std::max(pairs / tm, sequences);  // about
     l.grid = pairs / tm + sequences;
