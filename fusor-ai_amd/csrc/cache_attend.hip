@@ -805,7 +805,8 @@ constexpr size_t kUnits = 256;  // CUs
 // gives, so the parts aimed at are two a CU, less half of one a tile, whose last part is half a part on average:
 // fewer leave some CUs two parts and others one (eight documents of 30000 to 70000 tokens: 288 parts 105, 350 98,
 // 512 88), more start and end too often (1024: 104). 64 sequences as above (a): 384 parts 61 and of equal lengths
-// 130, 512 56 and 108, 640 64 and 130.
+// 130, 512 56 and 108, 640 64 and 130. Heads past 128 leave one workgroup a CU, and as many parts: 8 heads of 256 over 2,
+// 8 sequences of 8000 tokens, 25 us and for two a CU 38, 64 of up to 2000 28 and 38, a chunk of 512 rows 55 and 72.
 Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
 {
     Launch l{};
@@ -815,7 +816,7 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
     const size_t tiles = std::max(pairs / tm, sequences);  // about
     l.grid = pairs / tm + sequences;
     if (tiles <= units && b->max_pages > 16) {
-        l.target = int(2 * units - tiles / 2);
+        l.target = int((c->padded <= 128 ? 2 : 1) * units - tiles / 2);
         const size_t most = std::min<size_t>((b->max_pages + kMinPages - 1) / kMinPages, kMaxSplit);
         l.grid = std::min(l.grid * most, l.grid + l.target);
         l.note_bytes = (l.grid * sizeof(Note) + 255) / 256 * 256;
