@@ -19,8 +19,9 @@ struct StoreParams {
     size_t stride[2];
 };
 
-// The scale of a head whose largest magnitude is amax, and four of its levels as stored (level + 128).
-__device__ __forceinline__ float head_levels(float amax, const v4f &x, unsigned &packed)
+// The scale of a head whose largest magnitude is amax (`none` where all its levels are 0), and four of its levels as
+// stored (level + 128).
+__device__ __forceinline__ float head_levels(float amax, const v4f &x, float none, unsigned &packed)
 {
     int l0, l1, l2, l3;
     float d;
@@ -28,11 +29,12 @@ __device__ __forceinline__ float head_levels(float amax, const v4f &x, unsigned 
         d = scale_and_levels(amax, x.x, x.y, x.z, x.w, l0, l1, l2, l3);
     } else {
         d = amax / 127.0f;
-        d = d == 0.0f ? 1.0f : d;
-        l0 = quantize_level(x.x, d);
-        l1 = quantize_level(x.y, d);
-        l2 = quantize_level(x.z, d);
-        l3 = quantize_level(x.w, d);
+        const float by = d == 0.0f ? 1.0f : d;
+        l0 = quantize_level(x.x, by);
+        l1 = quantize_level(x.y, by);
+        l2 = quantize_level(x.z, by);
+        l3 = quantize_level(x.w, by);
+        d = d == 0.0f ? none : d;
     }
     packed = unsigned(pack4(l0, l1, l2, l3)) ^ 0x80808080u;
     return d;
@@ -68,11 +70,13 @@ __device__ __forceinline__ v4f levels_to_values(unsigned packed, float d)
     return x;
 }
 
-// Pages of zero levels and scales of 1.
+// Pages of zero levels, with the scales of such.
 __global__ __launch_bounds__(256) void cache_clear_kernel(uint8_t *records, size_t dwords, unsigned levels, unsigned record)
 {
-    for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < dwords; i += size_t(gridDim.x) * 256)
-        reinterpret_cast<unsigned *>(records)[i] = i % record < levels ? 0x80808080u : 0x3F800000u;
+    for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < dwords; i += size_t(gridDim.x) * 256) {
+        const unsigned at = unsigned(i % record);
+        reinterpret_cast<unsigned *>(records)[i] = at < levels ? 0x80808080u : __float_as_uint(at < levels + kPage ? 1.0f : kNoValueScale);
+    }
 }
 
 // A wave per new row and head, for few new tokens a sequence. Four dimensions a lane; heads of up to 128
@@ -106,7 +110,7 @@ __device__ __forceinline__ void store_row(const StoreParams &p, unsigned unit)
             v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
             if (live) x = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + place);
             unsigned packed;
-            const float d = head_levels(team_max(amax4(x), wide), x, packed);
+            const float d = head_levels(team_max(amax4(x), wide), x, value ? kNoValueScale : 1.0f, packed);
             if (live && !value) *reinterpret_cast<unsigned *>(record + key_byte(p.padded, token, dim)) = packed;
             if (live && value) {
 #pragma unroll
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float d = head_levels(team_max(amax4(x[i]), wide), x[i], packed[i]);
+                const float d = head_levels(team_max(amax4(x[i]), wide), x[i], value ? kNoValueScale : 1.0f, packed[i]);
                 if (dim == 0) scales[t + i] = d;
             }
         }

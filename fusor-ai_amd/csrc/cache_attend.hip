@@ -162,7 +162,8 @@ __device__ __forceinline__ Pair pair_of(const AttendParams &p, const Task &t, in
 //            the row's sums are scaled by the power of two between; the total of 2^(t - r) is kept in f32,
 //            and r cancels in the quotient.
 // r rises with the largest of a weight times its value's scale, not with the largest weight alone: a
-// value far larger than the others whose weight is next to nothing does not cost the others their bits.
+// value far larger than the others whose weight is next to nothing does not cost the others their bits. (Nor does a
+// value of zeros: its scale is kNoValueScale.)
 
 // Eight stored levels (level + 128, two dwords) as f16: 0x6400 + u is 1024 + u.
 __device__ __forceinline__ v8h widen8(unsigned a, unsigned b)

@@ -39,6 +39,12 @@ FG_BOTH int value_byte(int padded, int token, int dim)
 FG_BOTH int key_scale_byte(int padded, int token) { return 2 * kPage * padded + token * 4; }
 FG_BOTH int value_scale_byte(int padded, int token) { return 2 * kPage * padded + kPage * 4 + token * 4; }
 
+// The scale kept beside a value all of whose levels are 0 (a key's is 1). It changes no product, but attention sets
+// a row's reference from its largest weight times scale, and what adds nothing may not hide what does: at a scale
+// of 1, zeros beside values of 1e-6 cost these all but 11 bits. Small enough for that, and large enough that a
+// weight is bounded by it: weights reach 2^15 / 2^-80 = 2^95 at most, and 2^30 of them stay in f32's range.
+constexpr float kNoValueScale = 0x1p-80f;
+
 // The new rows of a sequence: rows begin .. begin + rows - 1 of the operands at positions first on
 // (negative ones have no token). The arrays' values are clamped to the operands, so no row outside
 // them is touched whatever the arrays hold.

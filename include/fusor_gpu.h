@@ -171,9 +171,9 @@ int fg_attend(const fg_attention *call, float *out, void *stream);
 /* The keys and values of one layer's attention over many sequences, in pages of FG_CACHE_PAGE tokens
  * that a serving program hands out (no counterpart in the reference, whose caches hold one sequence
  * of fixed capacity). A token's key and value of one head are `head_dim` int8 levels and one f32
- * scale each: scale = a / 127 for the largest magnitude a (NaN ignored; 1 where a / 127 is 0), level
- * rint(x / scale) clamped to +-127, NaN to 0 (the rule of quantize_rows with a head for its group).
- * The handle owns its device memory: pages of zero levels and scales of 1 until written. It belongs
+ * scale each: scale = a / 127 for the largest magnitude a (NaN ignored; where a / 127 is 0 all levels are
+ * 0), level rint(x / scale) clamped to +-127, NaN to 0 (the rule of quantize_rows with a head for its
+ * group). The handle owns its device memory: pages of zero levels until written. It belongs
  * to the device that was current when it was created, and every call on it needs that device
  * current. Calls on one cache may run at once; their order on the device is the caller's, by streams. */
 typedef struct fg_cache fg_cache;
