@@ -158,9 +158,10 @@ __device__ __forceinline__ Pair pair_of(const AttendParams &p, const Task &t, in
 // under f16's normal range):
 //   queries: a row is scaled by a power of two to a largest magnitude in [2^9, 2^10);
 //   weights: 2^(t - r) times the value's scale, for t the score times log2 e and r a reference of the row,
-//            a whole number. r is set when a weight passes 2^15, so that the largest is in (2^9, 2^11], and
-//            the row's sums are scaled by the power of two between; the total of 2^(t - r) is kept in f32,
-//            and r cancels in the quotient.
+//            a whole number. r is set when a weight passes 2^15, so that the largest is in (2^9, 2^11] (or,
+//            where values are so small that none does, when 2^(t - r) passes 2^102), and the row's
+//            sums are scaled by the power of two between; the total of 2^(t - r) is kept in f32, and r
+//            cancels in the quotient.
 // r rises with the largest of a weight times its value's scale, not with the largest weight alone: a
 // value far larger than the others whose weight is next to nothing does not cost the others their bits. (Nor does a
 // value of zeros: its scale is kNoValueScale.)
@@ -223,6 +224,9 @@ __device__ __forceinline__ int query_shift(float amax)
 }
 
 constexpr float kWeightLimit = 32768.0f;
+// Where a value's scale is under kSmallScale 2^(t - r) is looked at too: 2^25 of up to 2^102 stay in f32's range.
+constexpr float kSmallScale = 0x1p-82f, kAloneLimit = 102.0f;
+static_assert(kNoValueScale >= kSmallScale, "zeros are no reason to look");
 
 // Lane n of each row of 16 lanes, to every lane of its row (DPP row_newbcast, which the multiplication that
 // takes it reads by itself). A lane's scores are those of 16 keys that its row of lanes shares, so one register
@@ -253,10 +257,10 @@ struct RowSums {
 
 // 16 scores of one row in this lane, t = s * f, to weights times the values' scales, into x; the row's other
 // scores are in the lanes that `combine` joins. edge: keys outside [low, high] are masked (key(i) is score i's
-// position). rescale(a) scales the row's sums of this lane by a.
+// position). small: a value's scale is under kSmallScale. rescale(a) scales the row's sums of this lane by a.
 template <class Key, class Combine, class Rescale>
-__device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], float vs, float f, bool edge, int low,
-                                      int high, RowSums &sums, Key key, Combine combine, Rescale rescale)
+__device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], float vs, float f, bool small, bool edge,
+                                      int low, int high, RowSums &sums, Key key, Combine combine, Rescale rescale)
 {
     float top = 0.0f, total = 0.0f;
     auto weights = [&]() {
@@ -280,7 +284,7 @@ __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], floa
     };
     if (edge) masked();
     else weights();
-    if (__builtin_expect(__any(top > kWeightLimit), 0)) {
+    if (__builtin_expect(small || __any(top > kWeightLimit), 0)) {
         top = combine(top);
         float u = -INFINITY, m = -INFINITY;
         float logs = vs;
@@ -294,7 +298,7 @@ __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], floa
         });
         u = combine(u);
         m = combine(m);
-        if (top > kWeightLimit) {
+        if (top > kWeightLimit || m - sums.r > kAloneLimit) {
             // (a weight alone stays under 2^100, whatever the values' scales)
             const float r = fmaxf(ceilf(u) - 10.0f, ceilf(m) - 100.0f);
             const float a = __builtin_amdgcn_exp2f(sums.r - r);
@@ -432,7 +436,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(Atte
         const int base = page * kPage + 32 * (g >> 1) + 4 * (g & 1);
         const bool edge = page * kPage + kPage - 1 > first || page * kPage < first_seen(last, p.window);
         const int high = pair.position, low = first_seen(high, p.window);
-        weigh(scores, weights, vs, f, edge, low, high, sums, [&](int n) { return base + 8 * (n / 4) + n % 4; },
+        weigh(scores, weights, vs, f, __any(vs < kSmallScale), edge, low, high, sums, [&](int n) { return base + 8 * (n / 4) + n % 4; },
               [](float a) {
                   float2 w = row_pair(a);
                   w = half_pair(fmaxf(w.x, w.y));
@@ -631,6 +635,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
                 ks[kt] = key_scales[token];
                 vs[kt] = value_scales[token];
             }
+            const bool small = __any(fminf(vs[0], vs[1]) < kSmallScale);
             read_keys(0);
 #pragma unroll
             for (int k = 0; k < K; k++) {
@@ -654,7 +659,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
                 for_scales(ks[kt], [&](int i, float k) { scores[i] = k * s[kt][i]; });
                 if (kt) read_values(0);
                 __builtin_amdgcn_sched_barrier(0);
-                weigh(scores, x, vs[kt], f, edge, low, high, sums,
+                weigh(scores, x, vs[kt], f, small, edge, low, high, sums,
                           [&](int i) { return page * kPage + 32 * kt + 2 * (i & ~3) + 4 * h + i % 4; },
                           [](float v) {
                               const float2 w = half_pair(v);

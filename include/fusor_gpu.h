@@ -217,6 +217,9 @@ int fg_cache_read(const fg_cache *cache, const fg_batch *batch, float *key, size
  * `query` and `out`; `heads` query heads share the cache's heads in consecutive runs. Scores are
  * scale * q.k (|scale| at most 2e38); a row that sees no key gives 0. `out` may be
  * `query`, with its stride. The work is ordered on `stream`.
+ * Magnitudes: keys of up to 1e33 and scores of up to 1e7, past which a row's outputs may be NaN (f32 leaves
+ * such scores no digit after the point). A row's outputs are good to 2e-35 a key at best: of values under
+ * 1e-29 alone bits are lost.
  * `scratch`: device memory of at least fg_cache_attend_scratch's bytes, 16-byte aligned, that nothing else
  * uses until the call's work is done (two graphs that replay at once need one each); NULL: taken from the
  * library's pool as for fg_matmul, under capture too, which costs the call about 8 us of host time. */

@@ -54,3 +54,55 @@ def test_tokens_that_were_never_written(fk, gpu, rows, size):
     step.table, step.pages = case.step.table, case.step.pages
     case.cache.write(step.batch(fk, gpu), keys[20:].to(gpu), values[20:].to(gpu))
     case.check(case.run())
+
+
+@pytest.mark.parametrize("rows,length,every", [(1, 900, 256), (100, 900, 256), (150, 2560, 64)])
+@pytest.mark.parametrize("late", [1.0, 1e-30])
+def test_next_to_nothing_at_rising_scores(fk, gpu, rows, length, every, late):
+    """Values of 1e-36 whose scores rise by 18 (2^26 in weight) every `every` tokens, a page of each wave's: they
+    raise the sum of the weights and leave weight times value small. Values of `late` size come last, at the
+    highest score: the outputs are theirs.
+
+    A weight alone is at most 2^100 and the row's largest over 2^99, so the total is over 2^99; a weight times its
+    value's scale is off by half of f16's smallest step, 2^-25, times the level, 127. So 127 * 2^-25 / 2^99 < 2^-117 a
+    key is added to the bound: of rows that see only values of 1e-36 nothing is left."""
+    import torch
+    print(f"rising {rows} {length} {late}", flush=True)
+    g = torch.Generator().manual_seed(7)
+    keys, values = torch.zeros(length, 1, 32), torch.randn(length, 1, 32, generator=g)
+    keys[:, 0, 0] = 18.0 * (torch.arange(length) // every)
+    values[:-64] *= 1e-36
+    values[-64:] *= late
+    case = Case(fk, gpu, [rows], [length], 2, 1, 32, keys=keys, values=values)
+    case.query = torch.zeros_like(case.query)
+    case.query[:, :, 0] = 1.0
+    got = case.run(scale=1.0).double()
+    want, weighed, largest = serving.attention(case.query, serving.quantized(keys), serving.quantized(values),
+                                               range(length - rows, length), 1.0)
+    most = float(keys.max())  # of |scale q k|
+    bound = weighed * 2.0 ** -24 * (2 * most * (32 + 8) + 2 * length + 16) + length * (2.0 ** -34 * largest[..., None] + 2.0 ** -117)
+    worst = float(((got - want).abs() / bound).max())
+    print(f"  {worst:.3f} of the bound", flush=True)
+    assert worst <= 1
+
+
+@pytest.mark.parametrize("rows,length", [(1, 200), (100, 200)])
+def test_the_largest_keys_and_scores(fk, gpu, rows, length):
+    """Keys of 1e33 against queries of 1e-33, and scores of 1e7: at the ends of what fg_cache_attend documents,
+    every sum is finite. (Where one key has all the weight, an output is that key's value to its weight's two
+    pieces, 2^-22, and four roundings of 2^-24: under 2^-20 of it.)"""
+    import torch
+    g = torch.Generator().manual_seed(8)
+    keys = 1e33 * torch.randn(length, 2, 256, generator=g).clamp(-1, 1)
+    case = Case(fk, gpu, [rows], [length], 4, 2, 256, keys=keys)
+    case.query = case.query * 1e-33
+    case.check(case.run())
+    for size in (1.0, 1e-25, 1e30):  # of the values
+        keys = torch.zeros(length, 1, 64)
+        keys[:, 0, 0] = torch.rand(length, generator=g) - 0.5
+        keys[-rows - 3, 0, 0] = 1.0  # whose weight is all that counts
+        values = size * torch.randn(length, 1, 64, generator=g)
+        case = Case(fk, gpu, [rows], [length], 2, 1, 64, keys=keys, values=values)
+        case.query[:, :, 0] = 1e7
+        got, want = case.run(scale=1.0), serving.quantized(values)[-rows - 3, 0]
+        assert bool(((got.double() - want).abs() <= 2.0 ** -20 * want.abs().max()).all())
