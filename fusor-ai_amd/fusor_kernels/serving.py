@@ -53,7 +53,9 @@ def _on(device, stream):
 
 def _place(device, stream):
     """The tensors' device current, and with `stream` that stream too (what a call allocates is then its
-    own)."""
+    own). A stream of another device is refused: torch would make that device current."""
+    if stream is not None and stream.device != device:
+        raise ShapeError(f"a stream of {stream.device}, the tensors are on {device}")
     if stream is None and device.index == torch._C._cuda_getDevice():
         return _here
     return _on(device, stream)
