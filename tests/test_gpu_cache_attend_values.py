@@ -106,3 +106,37 @@ def test_the_largest_keys_and_scores(fk, gpu, rows, length):
         case.query[:, :, 0] = 1e7
         got, want = case.run(scale=1.0), serving.quantized(values)[-rows - 3, 0]
         assert bool(((got.double() - want).abs() <= 2.0 ** -20 * want.abs().max()).all())
+
+
+@pytest.mark.parametrize("rows,lengths", [([1], [16]), ([2, 1], [16, 9]), ([200], [200])])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_the_pieces_of_weights_and_queries(fk, gpu, rows, lengths, dim):
+    """Scores that f32 holds exactly, over at most 16 keys, so that the bound is close to what the pieces leave.
+
+    Keys are whole numbers k of magnitude up to 127 with one of 127 (scale 1), queries j + i / 2^11 with whole j and i
+    of up to 4 and 2^11 (14 bits: both pieces count), of which a 32nd are not 0: a score's products and sums are
+    multiples of 2^-11 under 2^13, exact in f32. The scale 2^-9 is exact; times log2 e it is rounded (e = 2^-24), so t, at
+    most T = 16 * 1.45 in magnitude, is off by 2 e T, the difference from the reference by 2 e (T + 10) more at most; the
+    exponential adds 4 e. A weight's pieces leave 2^-22 = 4 e, its product with the value's scale e; sums of 16 over and
+    under the division 16 e each, the division e. Together (4 T + 20 + 9 + 33 + 1) e W < 160 e W for the weighed sum
+    W; as elsewhere 2^-34 a key of the largest is added. One f16 piece would leave 2^-12 = 4096 e."""
+    import torch
+    g = torch.Generator().manual_seed(dim)
+    n = sum(lengths)
+    keys = torch.randint(-127, 128, (n, 1, dim), generator=g).float()
+    keys[:, 0, 0] = 127
+    case = Case(fk, gpu, rows, lengths, 2, 1, dim, keys=keys)
+    shape = case.query.shape
+    query = torch.randint(-4, 5, shape, generator=g) + torch.randint(0, 2 ** 11, shape, generator=g) / 2 ** 11
+    case.query = torch.where(torch.rand(shape, generator=g) < 1 / 32, query, torch.zeros(()))
+    assert float((case.query.abs().flatten(0, 1) @ keys[:, 0].abs().T).max()) < 2 ** 13
+    got = case.run(scale=2.0 ** -9, window=16).double()
+    values = serving.quantized(case.values)
+    for s, (r, length) in enumerate(zip(rows, lengths)):
+        a, b = int(case.whole.starts[s]), int(case.step.starts[s])
+        want, weighed, largest = serving.attention(case.query[b:b + r], keys[a:a + length], values[a:a + length],
+                                                   range(length - r, length), 2.0 ** -9, 16)
+        bound = 160 * 2.0 ** -24 * weighed + 16 * 2.0 ** -34 * largest[..., None]
+        worst = float(((got[b:b + r] - want).abs() / bound).max())
+        print(f"  sequence {s}: {worst:.3f} of the bound", flush=True)
+        assert worst <= 1
