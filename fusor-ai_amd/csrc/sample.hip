@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "cache.h"
+#include "sample_bins.h"
 #include "sample_route.h"
 
 namespace fg {
@@ -35,8 +36,6 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 1024;      // of the kernels that walk a row, and of the draw
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 1024;
-constexpr float kPerUnit = 32.0f;   // bins a unit of z
 constexpr int kList = 2560;         // tokens a row's list holds: what 64 KB of LDS hold beside the rest
 constexpr int kRank = 128;          // up to so many listed tokens are compared with each other, all in one step
 constexpr int kFew = 1024;          // up to so many tokens before the cut are all listed: no chunk is walked then
@@ -106,13 +105,6 @@ __device__ __forceinline__ Row row_of(const SampleParams &p, int row)
     r.scale = fmax(double(kPerUnit) / double(t), 1e-290);  // (an infinite temperature: every finite logit weighs 1)
     return r;
 }
-
-// -z in bins of a logit: 32 (largest - logit) / temperature, at least 0. All kernels go by `bins_of` and
-// `weight_of`, so a token's bin and weight are the same in each. (A largest logit of +inf is taken as
-// 1e300: the infinite ones are above it, and all others weigh nothing.)
-__device__ __forceinline__ double bins_of(float x, double top, double scale) { return fmax((top - double(x)) * scale, 0.0); }
-__device__ __forceinline__ int bin_of(double t) { return min(int(t), kBins - 1); }
-__device__ __forceinline__ double top_of(float x) { return x == INFINITY ? 1e300 : double(x); }
 
 // exp(-(b + 1/2) / 32), a bin's middle: -(b + 1/2) / 32 = n ln 2 + r, the Taylor series of exp to r^12
 // (|r| <= 0.347: the next term is under 2^-52 of it), times 2^n.
