@@ -793,22 +793,27 @@ __device__ __forceinline__ void draw_token(const SampleParams &p, int row, const
             __syncthreads();
             return found;
         }
-        if (tid == 0) sh.before[0] = 0;
-        for_listed([&](u64 k, u64 w, int b) {
-            if (take(k, w, b)) sh.chosen = key(k);  // any one
-        });
+        // the bits that some key has, and that some key has not: both are where the keys differ
+        if (tid < 2) sh.before[tid] = 0;
         __syncthreads();
-        const u64 some = sh.chosen;
-        u64 differ = 0;
+        u64 ones = 0, zeros = 0;
         for_listed([&](u64 k, u64 w, int b) {
-            if (take(k, w, b)) differ |= key(k) ^ some;
+            if (take(k, w, b)) {
+                ones |= key(k);
+                zeros |= ~key(k);
+            }
         });
-        differ = wave_or(differ);
-        if (lane == 63) atomicOr(&sh.before[0], differ);
+        ones = wave_or(ones);
+        zeros = wave_or(zeros);
+        if (lane == 63) {
+            atomicOr(&sh.before[0], ones);
+            atomicOr(&sh.before[1], zeros);
+        }
         __syncthreads();
-        differ = sh.before[0];
+        ones = sh.before[0];
+        const u64 differ = ones & sh.before[1];
         const int start = differ ? max(56 - __builtin_clzll(differ), 0) : 0;
-        u64 prefix = start + 8 < 64 ? some >> (start + 8) << (start + 8) : 0, mass_before = 0;
+        u64 prefix = start + 8 < 64 ? ones >> (start + 8) << (start + 8) : 0, mass_before = 0;
         unsigned count_before = 0;
         for (int shift = start, above = start + 8;;) {  // the key's bits from `shift` up to `above`
             const u64 known = above < 64 ? prefix >> above : 0;
