@@ -392,6 +392,7 @@ __device__ __forceinline__ Cut cut_of(const SampleParams &p, const Row &r, float
         sh.mass_low = all_m;
     }
     if (tid < kMaxChunks) sh.whole[tid] = 0;
+    if (tid < 4) sh.edge[tid] = __builtin_nanf("");  // (of none, where nothing is listed)
     __syncthreads();
     // (top_k of all that weigh anything, or more: no cut)
     if (r.has_k && u64(r.top_k) < all_n && before_n < u64(r.top_k) && before_n + n >= u64(r.top_k)) {
