@@ -184,8 +184,11 @@ __global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p
             __syncthreads();
         }
     } else {
-        for (int i = tid; i < pieces; i += kPageThreads)
-            reinterpret_cast<uint4 *>(levels)[i] = page < 0 ? none : reinterpret_cast<const uint4 *>(half)[i];
+        for (int i = tid; i < pieces; i += kPageThreads) {
+            uint4 w = none;  // (a choice between the two would be one of addresses, and `none` in scratch memory)
+            if (page >= 0) w = reinterpret_cast<const uint4 *>(half)[i];
+            reinterpret_cast<uint4 *>(levels)[i] = w;
+        }
         if (tid < kPage) scales[tid] = page < 0 ? 1.0f : record_scales[tid];
         __syncthreads();
     }
