@@ -5,6 +5,7 @@ batch of workgroups takes. The bounds are those of test_gpu_cache_attend.py and 
 import numpy as np
 import pytest
 
+import serving
 import test_gpu_sample as sampling
 from test_gpu_cache_attend import Case
 
@@ -46,3 +47,59 @@ def test_more_rows_than_a_batch(fk, gpu, vocab):
     rows = 4100
     sampling.check(fk, gpu, sampling.logits_of(rng, rows, vocab), rng.random(rows), temperature=rng.uniform(0.3, 1.5, rows),
                    top_k=rng.integers(0, 30, rows), top_p=rng.uniform(0.5, 1.0, rows))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(40, 1), (34, 2), (300, 1)])
+@pytest.mark.parametrize("rows,lengths", [([1], [90]), ([1, 2], [2000, 65]), ([5], [1300])])
+def test_more_heads_of_a_key_head_than_a_tile_has_pairs(fk, gpu, heads, kv_heads, rows, lengths):
+    """One token's heads lie in several tiles, of both kernels, whole and split."""
+    case = Case(fk, gpu, rows, lengths, heads, kv_heads, 32, seed=heads)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("rows,lengths", [([2, 1], [70, 300]), ([20, 0, 150], [100, 9, 400]), ([1, 2], [2000, 1500])])
+def test_rows_before_the_first_sequence(fk, gpu, rows, lengths):
+    """row_starts may begin past 0: the rows before are no sequence's, in writes, reads and attention."""
+    import torch
+    case = Case(fk, gpu, rows, lengths, 4, 2, 64)
+    want = case.run()
+    n, before = int(case.step.starts[-1]), 7
+    keys, values = (torch.randn(before + n, 2, 64, generator=torch.Generator().manual_seed(s)) for s in (1, 2))
+    for s, (r, length) in enumerate(zip(rows, lengths)):  # the same keys and values as are there
+        a, b, end = int(case.step.starts[s]), int(case.step.starts[s + 1]), int(case.whole.starts[s + 1])
+        keys[before + a:before + b], values[before + a:before + b] = case.keys[end - r:end], case.values[end - r:end]
+    case.step.starts = case.step.starts + before
+    batch = case.step.batch(fk, gpu)
+    case.cache.write(batch, keys.to(gpu), values.to(gpu))
+    back_k, back_v = torch.full((before + n, 2, 64), 3.0, device=gpu), torch.full((before + n, 2, 64), 3.0, device=gpu)
+    case.cache.read(batch, back_k, back_v)
+    for x, back in ((keys, back_k), (values, back_v)):
+        assert bool((back[:before] == 3.0).all()) and torch.equal(back[before:].cpu().double(), serving.quantized(x[before:]).float().double())
+    query = torch.cat([torch.full((before, 4, 64), float("nan")), case.query[:n]])
+    out = torch.full_like(query, 5.0, device=gpu)
+    case.cache.attend(batch, query.to(gpu), out=out)
+    assert bool((out[:before] == 5.0).all()) and torch.equal(out[before:].cpu(), want[:n])
+
+
+@pytest.mark.parametrize("rows,lengths,columns", [([1, 2], [700, 200], 3), ([1], [3000], 20), ([150], [400], 3), ([2], [3000], 17)])
+@pytest.mark.parametrize("window", [0, 130])
+def test_tables_shorter_than_the_sequences(fk, gpu, rows, lengths, columns, window):
+    """Positions past the table hold nothing: the last tokens see what it has, or with a window nothing."""
+    case = Case(fk, gpu, rows, lengths, 4, 2, 64, seed=columns)
+    case.step.table = np.ascontiguousarray(case.step.table[:, :columns])
+    got = case.run(window=window)
+    case.check(got, window=window)
+
+
+def test_no_sequences(fk, gpu):
+    """Rows, but no sequence that holds them: nothing is read or written."""
+    import torch
+    cache = fk.PagedCache(2, 2, 64, device=gpu)
+    ints = dict(dtype=torch.int32, device=gpu)
+    batch = fk.Batch(torch.zeros(1, **ints), torch.zeros(0, **ints), torch.zeros(0, 3, **ints))
+    keys, out = torch.full((5, 2, 64), 2.0, device=gpu), torch.full((5, 4, 64), 3.0, device=gpu)
+    cache.write(batch, keys, keys)
+    cache.read(batch, keys, keys.clone())
+    cache.attend(batch, out.clone(), out=out)
+    assert bool((keys == 2.0).all()) and bool((out == 3.0).all())
+    assert not bool(cache.attend(batch, out).any())
