@@ -82,9 +82,9 @@ __global__ __launch_bounds__(256) void cache_clear_kernel(uint8_t *records, size
 // A wave per new row and head, for few new tokens a sequence. Four dimensions a lane; heads of up to 128
 // take half a wave for the key and half for the value. A value's levels go to single bytes, 16 apart, of a kilobyte
 // that 64 tokens share (cache_layout.h): 64 stores of a byte a token, which is what bounds long runs of tokens,
-// and why they take the kernels below. A step's single tokens are bounded by the launch and its three loads one
-// after the other (the row's sequence, its page, its values): 8 tokens of 2 heads of 64 written in 3.4 us, read back
-// in 3.2; 512 of 8 heads of 128 in 7.8 and 5.0.
+// and why they take the kernels below. A step's single tokens are bounded by the launch and three loads one
+// after the other (the row's sequence, its page, then its values, though their address needs neither): 8 tokens of
+// 2 heads of 64 written in 3.3 us, read back in 3.0; 512 of 8 heads of 128 in 7.8 and 5.0.
 template <bool WRITE>
 __device__ __forceinline__ void store_row(const StoreParams &p, unsigned unit)
 {
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
 // at once; the levels meet in LDS in the record's order, and whole 16-byte pieces go to the page or come from it.
 // Pieces that also hold other tokens' values are written in part. Bounded by memory for long runs, and by one load's
 // wait after another for short ones: 3618 tokens of 4 heads of 128 (14.8 MB of f32, 3.8 MB of levels and scales) written
-// in 8.9 us, 2.1 TB/s, and read back in 7.8. Keys and values are each a workgroup's, for twice the loads in flight (both in
+// in 9.2 us, 2.0 TB/s, and read back in 7.5. Keys and values are each a workgroup's, for twice the loads in flight (both in
 // one: 16.8 and 9.8).
 constexpr int kPageThreads = 512;
 

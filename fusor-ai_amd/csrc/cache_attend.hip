@@ -326,9 +326,10 @@ __device__ __forceinline__ float part_factor(float r, float joined) { return r =
 //   values:  16 dimensions by 32 keys: the lane's 16 bytes of dimension l % 16 are those keys', in order.
 // A decode step's pairs are the heads of a key head's group, 4 to 16 in most models: 16 rows leave the
 // matrix cores idle lanes that cost nothing, for memory is what bounds long caches: 8 sequences of 34000 to 70000 tokens,
-// 4 key heads of 128 (442 MB), 87 us, 5.1 TB/s, the rate of a large copy. 64 sequences of 6 to 8001 tokens (87 MB) take
-// 27 us, 3.2 TB/s, for parts of 16 pages or so that each start with a chain of waits (the plan, the
-// table, the first page); one of 511 tokens, 2 key heads of 64, is that chain alone, 7.6 us.
+// 4 key heads of 128 (442 MB), 88 us, 5.0 TB/s, about the rate of a large copy. 64 sequences of 6 to 8001 tokens (87 MB)
+// take 28.7 us, 3.0 TB/s, for parts of 16 pages or so that each start with a chain of waits (the plan, the table, the
+// first page): half of the waves' cycles are waits, over long caches a third. One of 511 tokens, 2 key heads of
+// 64, is that chain alone, 7.7 us.
 // (Two tiles of rows a workgroup, which halves the reading of 17 to 32 pairs, left one workgroup a CU: 64 sequences
 // of up to 3200 tokens, 28 pairs, 25.5 against 24.1 us, 32 pairs over one key head 36.9 against 24.2.)
 template <int DP>
@@ -522,9 +523,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(Atte
 // 64 products of 32 cycles and about 1600 cycles of vector work (per score a multiplication by the key's scale, an
 // exponential, the value's scale, the total, the maximum and two f16 pieces), and two waves a SIMD overlap them in part.
 // 8192 tokens of 16 heads of 128 over 4: 492 us, 1118 TFLOP/s in f16 products (two an operand, for the
-// pieces), the matrix cores busy 61 % of the time; a large f16 product of the library's reaches 1175. Chunks of 2700
-// tokens, 16 heads of 72 over a window of 1000: 75 us, 336 TFLOP/s: its 350 tiles of 19 pages are 1400 waves
-// for 1024 SIMDs, so some have two. 32 pairs a wave: with 64, or with four waves a SIMD, the sums do not fit the registers.
+// pieces), the matrix cores busy 61 % of the time and the vector units 57 %, at the 1.74 GHz that the card keeps under this
+// load (2.35 in the others here); a large f16 product of the library's reaches 1175. Chunks of 2700 tokens, 16 heads of
+// 72 over a window of 1000: 75 us, 336 TFLOP/s: its 350 tiles of 19 pages are 1400 waves for 1024 SIMDs, so some have
+// two, and CUs are busy 69 % of the time. 17 chunks of 1 to 512 tokens, 14 heads of 64 over 2: 52.5 us; CUs are busy
+// 72 % of the time, and then the vector units 51 %, the matrix cores 29, with 1.6 waves a SIMD. 32 pairs a wave: with 64, or with four waves a SIMD, the sums do not fit the registers.
 template <int DP>
 constexpr size_t many_lds() { return size_t(2) * (256 * DP + 2 * kPage * 4); }
 
@@ -813,6 +816,13 @@ constexpr size_t kUnits = 256;  // CUs
 // 512 88), more start and end too often (1024: 104). 64 sequences as above (a): 384 parts 61 and of equal lengths
 // 130, 512 56 and 108, 640 64 and 130. Heads past 128 leave one workgroup a CU, and as many parts: 8 heads of 256 over 2,
 // 8 sequences of 8000 tokens, 25 us and for two a CU 38, 64 of up to 2000 28 and 38, a chunk of 512 rows 55 and 72.
+//
+// Both rules go by a step's means, all that the host knows, and cost uneven steps: 64 sequences of 6 to 8000 tokens, even
+// over their logarithm,
+// (a) 26.5 and 65 of them 59.7; one of 70000 beside 100 of 500 (a) 485, alone 32 (slots without rows are no sequences: with
+// 100 of those 33); 63 tokens after 2000 others each and a chunk of 512 (a) 45, of 2048 97, where the two apart take
+// 30 + 35 and 30 + 64, (b) 25 and 60, apart 15 + 33 and 15 + 43. And every workgroup looks through all sequences for
+// its task, 64 at a time: 256 sequences of 500 tokens (a) 34, 1024 177, 4096 1430, of which memory's share is 417.
 Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
 {
     Launch l{};

@@ -11,16 +11,24 @@
 //   5 draw     the cut among the list; the chunk, or the listed token, on which the random number falls.
 // Few rows take a launch for each, their chunks over the chip; many rows all five in one workgroup a row
 // (sample_route.h).
-// Weights are 64-bit: exp in f64 (one ulp), rounded to a whole number of units of 2^-45 of the first token's
-// (less for more than 2^18 tokens), so that every sum is exact and their order changes nothing. Tokens
-// under half a unit (z < -31.9) weigh 0; the last bin holds only such.
+// Weights are 64-bit: exp in f64 (off by |z| 2^-52 and a few 2^-53 of it, for z is rounded and two series are
+// multiplied), rounded to a whole number of units of 2^-45 of the first token's (less for more than 2^18 tokens), so
+// that every sum is exact and their order changes nothing. Tokens under half a unit (z < -31.9) weigh 0; the last
+// bin holds only such. Equal logits have equal weights; which side of min-p a token within that error of it falls on
+// is not decided.
 //
 // What it costs: a logit is read three times, by top, bins and collect (the draw reads one chunk more), mostly from
 // the Infinity Cache after the first, and takes about 35 vector instructions in f64 and one 64-bit LDS addition in
-// the bins. 64 rows of 151936 (39 MB): top 11 us, 3.5 TB/s; bins 17, the arithmetic; cut 8.3; collect 9, 4.3 TB/s;
-// draw 10. One row: 3.7, 6.0, 7.2, 4.0, 4.2: each launch is a chain of dependent steps on 1 to 16 CUs. In one
-// workgroup a row, 512 rows 200 us: two rounds of 256, of cycles about 48 thousand top, 100 bins, 50 collect and 30 the
-// rest, so a third each is memory's first reading, arithmetic, and the others; 200 rows of 32003 35 us (8, 22, 10, 22).
+// the bins. 64 rows of 151936 (39 MB): top 10.5 us, 3.7 TB/s; bins 17, the arithmetic (the vector units are busy
+// 76 % of the time); cut 8.4; collect 9.4, 4.1 TB/s; draw 9.4. One row: 3.6, 6.0, 7.0, 3.8, 4.5: each launch is a
+// chain of dependent steps on 1 to 16 CUs. In one workgroup a row, 512 rows 200 us: two rounds of 256, of cycles about
+// 48 thousand top (memory's first reading), 100 bins (arithmetic), 50 collect and 30 the rest; 200 rows of 32003 35 us
+// (8, 22, 10, 22). The vector units are busy half the time: one row's waits have no other row's work beside them.
+//
+// Where a cut's bin holds more tokens than a list (kList), the draw walks the row once for each pass over them,
+// about ten a cut, by one workgroup: 151936 logits of spread s at temperature T, top-p 0.9, in microseconds,
+// s / T = 0.7 and 0.5: one row 39 and 273, 64 rows 62 and 472, 512 rows 225 and 1052; with top-k 50000 too, s / T = 2 and 1:
+// 42 and 463, 68 and 811, 233 and 1656. Of 262144 logits top-p alone does so at s / T = 1 (one row 39 and 453 for 2 and 1).
 #include <algorithm>
 #include <type_traits>
 
@@ -404,7 +412,7 @@ __device__ __forceinline__ Cut cut_of(const SampleParams &p, const Row &r, float
     }
     __syncthreads();
     Cut c{kBins, -1, sh.last, sh.before_last, sh.mass_last, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0, r.has_p, 0, r.top_k, r.top_p,
-          top_of(top), r.scale, double(r.min_p) * (1.0 - 0x1p-50) * p.unit};  // (a little less: the rounding of weights)
+          top_of(top), r.scale, double(r.min_p) * (1.0 - 0x1p-50) * p.unit};  // (a little less, for the first's equals at min_p = 1)
     if (r.has_p) {
         // the cut's bin, for a total between the weight under `last` and that up to it
         const double least = double(r.top_p) * double(sh.mass_last) * (1.0 - 0x1p-50);
