@@ -184,8 +184,8 @@ class PagedCache:
         """The attention of the new tokens' `queries` [rows, heads, head_dim] (their keys and values
         written before): each token sees its sequence's tokens up to itself, with `window` the last
         `window` of them. `scale` is 1 / sqrt(head_dim) unless given. A token without a key gives 0;
-        `out` may be
-        `queries`; rows of it that no sequence holds are left as they are (0 in an `out` made here)."""
+        `out` may be `queries`; rows of it that no sequence holds are left as they are (0 in an `out`
+        made here). Keys may reach 1e33 and scores 1e7 in magnitude."""
         if batch.pages.device != self.device:
             raise ShapeError(f"the batch is on {batch.pages.device}, the cache on {self.device}")
         if queries.dim() != 3:
