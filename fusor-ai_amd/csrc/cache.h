@@ -21,7 +21,9 @@ struct BatchParams {
     int sequences, rows, max_pages;
 };
 
-// The arguments that every call over a batch checks.
+// The arguments that every call over a batch checks, the batch's alone (`reads_pages`: its page table is needed), and with a
+// cache's.
+int check_batch_arrays(const fg_batch *batch, bool reads_pages, const char *who);
 int check_batch(const fg_cache *cache, const fg_batch *batch, const char *who);
 
 inline BatchParams batch_params(const fg_batch *b)

@@ -3,12 +3,10 @@
 #include <algorithm>
 #include <new>
 
-#include "cache.h"
+#include "rotary.h"
 
 namespace fg {
 namespace {
-
-typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));  // four floats at any float's address
 
 struct StoreParams {
     BatchParams b;
@@ -17,6 +15,12 @@ struct StoreParams {
     const float *in[2];  // keys, values
     float *out[2];
     size_t stride[2];
+};
+
+// ... and with keys that are turned by their positions before they are kept (and, in the row kernel's launch, queries).
+struct TurnParams : StoreParams {
+    RotaryParams r;
+    RotateParams queries;
 };
 
 // The scale of a head whose largest magnitude is amax (`none` where all its levels are 0), and four of its levels as
@@ -79,14 +83,51 @@ __global__ __launch_bounds__(256) void cache_clear_kernel(uint8_t *records, size
     }
 }
 
+// Four values of a key from dimension dim on, x, turned: `head` is where the head's values lie, `angle(pair)` the pair's
+// factors. Values 2i and 2i + 1 are partners in the lane itself; the partners of halves are read a second time (the
+// lane that has them may be anywhere in the wave, and they come from the cache).
+template <class F>
+__device__ __forceinline__ v4f turned_quad(const RotaryParams &r, const float *head, int dim, const v4f &x, F angle)
+{
+    if (dim >= r.dims) return x;
+    v4f u = x;
+    if (!r.halves) {
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            if (dim + j >= r.dims) continue;
+            const Turn t = angle((dim + j) / 2);
+            u[j] = turned(x[j], x[j + 1], t, true);
+            u[j + 1] = turned(x[j + 1], x[j], t, false);
+        }
+        return u;
+    }
+    const int half = r.dims / 2;
+    v4f partner = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (half % 4 == 0) {
+        partner = *reinterpret_cast<const v4f_any *>(head + (dim < half ? dim + half : dim - half));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = dim + j;
+            if (d < r.dims) partner[j] = head[d < half ? d + half : d - half];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int d = dim + j;
+        if (d < r.dims) u[j] = turned(x[j], partner[j], angle(d < half ? d : d - half), d < half);
+    }
+    return u;
+}
+
 // A wave per new row and head, for few new tokens a sequence. Four dimensions a lane; heads of up to 128
 // take half a wave for the key and half for the value. A value's levels go to single bytes, 16 apart, of a kilobyte
 // that 64 tokens share (cache_layout.h): 64 stores of a byte a token, which is what bounds long runs of tokens,
 // and why they take the kernels below. A step's single tokens are bounded by the launch and three loads one
 // after the other (the row's sequence, its page, then its values, though their address needs neither): 8 tokens of
 // 2 heads of 64 written in 3.3 us, read back in 3.0; 512 of 8 heads of 128 in 7.8 and 5.0.
-template <bool WRITE>
-__device__ __forceinline__ void store_row(const StoreParams &p, unsigned unit)
+template <bool WRITE, bool TURN, class P>
+__device__ __forceinline__ void store_row(const P &p, unsigned unit)
 {
     const int lane = threadIdx.x & 63;
     const int row = int(unit / unsigned(p.kv_heads)), head = int(unit % unsigned(p.kv_heads));
@@ -109,6 +150,10 @@ __device__ __forceinline__ void store_row(const StoreParams &p, unsigned unit)
         if (WRITE) {
             v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
             if (live) x = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + place);
+            if constexpr (TURN) {
+                if (live && !value)
+                    x = turned_quad(p.r, p.in[0] + place - dim, dim, x, [&](int pair) { return turn_at(p.r, pair, position); });
+            }
             unsigned packed;
             const float d = head_levels(team_max(amax4(x), wide), x, value ? kNoValueScale : 1.0f, packed);
             if (live && !value) *reinterpret_cast<unsigned *>(record + key_byte(p.padded, token, dim)) = packed;
@@ -138,7 +183,18 @@ template <bool WRITE>
 __global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
 {
     const unsigned units = unsigned(p.b.rows) * unsigned(p.kv_heads);
-    for (unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += gridDim.x * 4) store_row<WRITE>(p, unit);
+    for (unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += gridDim.x * 4) store_row<WRITE, false>(p, unit);
+}
+
+// The same for keys to be turned, and behind the rows' units those of the queries: one launch for a decode step.
+template <bool QUADS>
+__global__ __launch_bounds__(256) void turn_rows_kernel(TurnParams p)
+{
+    const unsigned units = unsigned(p.b.rows) * unsigned(p.kv_heads), all = units + unsigned(p.b.rows) * unsigned(p.queries.units);
+    for (unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6); unit < all; unit += gridDim.x * 4) {
+        if (unit < units) store_row<true, true>(p, unit);
+        else rotate_unit<QUADS>(p.queries, unit - units);
+    }
 }
 
 // A workgroup per page that new tokens lie in, head, and keys or values. A thread takes four tokens (an
@@ -150,11 +206,9 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
 // one: 16.8 and 9.8).
 constexpr int kPageThreads = 512;
 
-template <bool WRITE>
-__global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p)
+template <bool WRITE, bool TURN, class P>
+__device__ __forceinline__ void store_page(const P &p, uint8_t *levels, float *scales)
 {
-    extern __shared__ __align__(16) uint8_t levels[];
-    __shared__ float scales[kPage];
     const int tid = threadIdx.x, head = int(blockIdx.y), value = int(blockIdx.z);
     int index;
     const int s = find_unit(p.b.sequences, int(blockIdx.x), &index, [&](int q) {
@@ -204,6 +258,16 @@ __global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p
             for (int i = 0; i < 4; i++) {
                 x[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
                 if (live && t + i >= t0 && t + i < t1) x[i] = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + at + i * stride);
+            }
+            if constexpr (TURN) {
+                if (live && !value) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (t + i < t0 || t + i >= t1) continue;
+                        x[i] = turned_quad(p.r, p.in[0] + at - dim + i * stride, dim, x[i],
+                                           [&](int pair) { return turn_at(p.r, pair, place * kPage + t + i); });
+                    }
+                }
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -275,6 +339,31 @@ __global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p
 }
 
 template <bool WRITE>
+__global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p)
+{
+    extern __shared__ __align__(16) uint8_t levels[];
+    __shared__ float scales[kPage];
+    store_page<WRITE, false>(p, levels, scales);
+}
+
+__global__ __launch_bounds__(kPageThreads) void turn_pages_kernel(TurnParams p)
+{
+    extern __shared__ __align__(16) uint8_t levels[];
+    __shared__ float scales[kPage];
+    store_page<true, true>(p, levels, scales);
+}
+
+// A workgroup a page: a run of n rows lies in at most (n + 62) / 64 + 1 pages.
+dim3 page_grid(const StoreParams &p)
+{
+    const size_t runs = size_t(p.b.rows) / kPage + 2 * size_t(std::min(p.b.sequences, p.b.rows));
+    return dim3(unsigned(runs), unsigned(p.kv_heads), 2);
+}
+
+// Whether a write takes the row kernels: up to 16 new tokens a sequence, or 2048 rows times heads (launch_store's figures).
+bool by_rows(const StoreParams &p) { return p.b.rows <= 16 * p.b.sequences || size_t(p.b.rows) * p.kv_heads <= 2048; }
+
+template <bool WRITE>
 int launch_store(const StoreParams &p, hipStream_t s)
 {
     if (p.b.rows == 0 || p.b.sequences == 0) return FG_OK;
@@ -284,27 +373,51 @@ int launch_store(const StoreParams &p, hipStream_t s)
     // Microseconds of a write, rows' and pages': 8 heads of 128, 64 sequences of 1 new token 3.8 and 9.5, 16 11.4 and
     // 11.3, 32 17.6 and 13.2, 128 51 and 23; one of 128 3.8 and 4.8; 8 of 32 4.9 and 5.9, of 128 10.5 and 6.5;
     // 512 (each workgroup of a page looks through all of them) of 1 7.8 and 80, 16 52 and 100, 64 190 and 148.
-    if (p.b.rows <= 16 * p.b.sequences || units <= 2048) {
+    if (by_rows(p)) {
         cache_rows_kernel<WRITE><<<unsigned(std::min((units + 3) / 4, kMaxGrid)), 256, 0, s>>>(p);
     } else {
-        // a run of n rows lies in at most (n + 62) / 64 + 1 pages
-        const size_t runs = size_t(p.b.rows) / kPage + 2 * size_t(std::min(p.b.sequences, p.b.rows));
-        cache_pages_kernel<WRITE><<<dim3(unsigned(runs), unsigned(p.kv_heads), 2), kPageThreads, size_t(kPage * p.padded), s>>>(p);
+        cache_pages_kernel<WRITE><<<page_grid(p), kPageThreads, size_t(kPage * p.padded), s>>>(p);
     }
+    FG_HIP(hipGetLastError());
+    return FG_OK;
+}
+
+int launch_turned(const TurnParams &p, bool quads, hipStream_t s)
+{
+    if (p.b.rows == 0 || p.b.sequences == 0) return FG_OK;
+    const size_t units = size_t(p.b.rows) * p.kv_heads, all = units + size_t(p.b.rows) * p.queries.units;
+    if (all > 0xf0000000) return set_error(FG_ERR_SHAPE, "the paged cache: more rows times heads than a launch takes");
+    if (!by_rows(p)) {
+        turn_pages_kernel<<<page_grid(p), kPageThreads, size_t(kPage * p.padded), s>>>(p);
+        FG_HIP(hipGetLastError());
+        return p.queries.units ? launch_rotate(p.queries, quads, s) : FG_OK;
+    }
+    const unsigned grid = unsigned(std::min((all + 3) / 4, kMaxGrid));
+    if (quads) turn_rows_kernel<true><<<grid, 256, 0, s>>>(p);
+    else turn_rows_kernel<false><<<grid, 256, 0, s>>>(p);
     FG_HIP(hipGetLastError());
     return FG_OK;
 }
 
 }  // namespace
 
+int check_batch_arrays(const fg_batch *b, bool reads_pages, const char *who)
+{
+    const std::string name(who);
+    if (!b) return set_error(FG_ERR_ARG, name + ": a null batch");
+    if (b->sequences > 65536 || b->rows > (size_t(1) << 24) || b->max_pages > (size_t(1) << 24))
+        return set_error(FG_ERR_SHAPE, name + ": at most 65536 sequences, 2^24 rows and 2^24 pages a sequence");
+    if (b->sequences && (!b->row_starts || !b->lengths || (reads_pages && b->max_pages && !b->pages)))
+        return set_error(FG_ERR_ARG, name + ": a null array of the batch");
+    return FG_OK;
+}
+
 int check_batch(const fg_cache *c, const fg_batch *b, const char *who)
 {
     const std::string name(who);
     if (!c || !b) return set_error(FG_ERR_ARG, name + ": a null cache or batch");
-    if (b->sequences > 65536 || b->rows > (size_t(1) << 24) || b->max_pages > (size_t(1) << 24))
-        return set_error(FG_ERR_SHAPE, name + ": at most 65536 sequences, 2^24 rows and 2^24 pages a sequence");
-    if (b->sequences && (!b->row_starts || !b->lengths || (b->max_pages && !b->pages)))
-        return set_error(FG_ERR_ARG, name + ": a null array of the batch");
+    const int rc = check_batch_arrays(b, true, who);
+    if (rc) return rc;
     int device = 0;
     FG_HIP(hipGetDevice(&device));
     if (device != c->device)
@@ -328,9 +441,10 @@ int check_store(const fg_cache *c, const fg_batch *b, const void *key, size_t ke
     return FG_OK;
 }
 
-StoreParams store_params(const fg_cache *c, const fg_batch *b, size_t key_stride, size_t value_stride)
+template <class P>
+P store_params(const fg_cache *c, const fg_batch *b, size_t key_stride, size_t value_stride)
 {
-    StoreParams p{};
+    P p{};
     p.b = batch_params(b);
     p.records = c->records;
     p.pages = c->pages;
@@ -395,17 +509,34 @@ int fg_cache_write(fg_cache *c, const fg_batch *b, const float *key, size_t key_
 {
     const int rc = check_store(c, b, key, key_stride, value, value_stride, false, "fg_cache_write");
     if (rc) return rc;
-    StoreParams p = store_params(c, b, key_stride, value_stride);
+    StoreParams p = store_params<StoreParams>(c, b, key_stride, value_stride);
     p.in[0] = key;
     p.in[1] = value;
     return launch_store<true>(p, as_stream(stream));
+}
+
+int fg_cache_write_rotated(fg_cache *c, const fg_batch *b, const fg_rotary *r, const float *key, size_t key_stride, const float *value,
+                           size_t value_stride, const float *query, size_t query_stride, size_t heads, float *out, size_t out_stride,
+                           void *stream)
+{
+    const char *who = "fg_cache_write_rotated";
+    int rc = check_store(c, b, key, key_stride, value, value_stride, false, who);
+    if (rc) return rc;
+    if ((rc = check_rotary(r, c->device, size_t(c->head_dim), who))) return rc;
+    if ((heads || query || out) && (rc = check_rotated(b, query, query_stride, heads, size_t(c->head_dim), out, out_stride, who))) return rc;
+    TurnParams p = store_params<TurnParams>(c, b, key_stride, value_stride);
+    p.in[0] = key;
+    p.in[1] = value;
+    p.r = rotary_params(r);
+    if (heads) p.queries = rotate_params(r, b, query, query_stride, heads, size_t(c->head_dim), out, out_stride);
+    return launch_turned(p, whole_quads(r), as_stream(stream));
 }
 
 int fg_cache_read(const fg_cache *c, const fg_batch *b, float *key, size_t key_stride, float *value, size_t value_stride, void *stream)
 {
     const int rc = check_store(c, b, key, key_stride, value, value_stride, true, "fg_cache_read");
     if (rc) return rc;
-    StoreParams p = store_params(c, b, key_stride, value_stride);
+    StoreParams p = store_params<StoreParams>(c, b, key_stride, value_stride);
     p.out[0] = key;
     p.out[1] = value;
     return launch_store<false>(p, as_stream(stream));

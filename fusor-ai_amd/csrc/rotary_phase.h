@@ -1,0 +1,63 @@
+// The angles of rotary positions: position times frequency, in turns (plain C++: the kernels and the host share it).
+#pragma once
+
+#include <cmath>
+#include <cstdint>
+
+#include "cache_layout.h"
+
+namespace fg {
+
+// A pair's turn per token is kept as a fraction of 2^64, so that position * step, which drops whole turns as it
+// overflows, is the fraction of the last one: off by position * 2^-65 turns for the step's rounding, at any position. (In
+// f32 such a product has no digit left for far positions: past 2^20 radians its steps are 2^-3.)
+
+struct Angle {
+    double c, s;
+};
+
+// The cosine and sine of a phase: the nearest quarter turn is taken off exactly, and what is left, x in [-pi/4, pi/4], goes
+// through Taylor's series, whose first dropped terms are x^17 / 17! < 5e-17 and x^18 / 18! < 3e-18.
+FG_BOTH Angle angle_of(uint64_t phase)
+{
+    const uint64_t quarter = (phase + (uint64_t(1) << 61)) >> 62;
+    const int64_t rest = int64_t(phase - (quarter << 62));
+    const double x = double(rest) * 0x1.921fb54442d18p-62;  // 2 pi / 2^64
+    const double y = x * x;
+    double s = -1.0 / 1307674368000.0;
+    s = __builtin_fma(s, y, 1.0 / 6227020800.0);
+    s = __builtin_fma(s, y, -1.0 / 39916800.0);
+    s = __builtin_fma(s, y, 1.0 / 362880.0);
+    s = __builtin_fma(s, y, -1.0 / 5040.0);
+    s = __builtin_fma(s, y, 1.0 / 120.0);
+    s = __builtin_fma(s, y, -1.0 / 6.0);
+    s = __builtin_fma(s * y, x, x);
+    double c = 1.0 / 20922789888000.0;
+    c = __builtin_fma(c, y, -1.0 / 87178291200.0);
+    c = __builtin_fma(c, y, 1.0 / 479001600.0);
+    c = __builtin_fma(c, y, -1.0 / 3628800.0);
+    c = __builtin_fma(c, y, 1.0 / 40320.0);
+    c = __builtin_fma(c, y, -1.0 / 720.0);
+    c = __builtin_fma(c, y, 1.0 / 24.0);
+    c = __builtin_fma(c, y, -0.5);
+    c = __builtin_fma(c, y, 1.0);
+    const bool odd = quarter & 1;
+    Angle a;
+    a.c = odd ? s : c;
+    a.s = odd ? c : s;
+    // quarters 1 and 2 have a negative cosine, 2 and 3 a negative sine
+    if (((quarter + 1) & 2) != 0) a.c = -a.c;
+    if ((quarter & 2) != 0) a.s = -a.s;
+    return a;
+}
+
+// `frequency` radians a token as a step: the fraction of a turn, rounded to 2^-64 (80-bit arithmetic).
+inline uint64_t turn_step(double frequency)
+{
+    long double turns = (long double)frequency / 6.28318530717958647692528676655900576L;
+    turns -= floorl(turns);
+    const long double scaled = roundl(turns * 18446744073709551616.0L);
+    return scaled >= 18446744073709551616.0L ? 0 : uint64_t(scaled);
+}
+
+}  // namespace fg

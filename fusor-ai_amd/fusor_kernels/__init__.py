@@ -18,7 +18,7 @@ from .linear import (COLUMN_ALIGN, NARROW_COLUMN_ALIGN, Ctx, Linear, SharedRows,
 from .matmul import (ROWS_PER_CALL, Input, Quantized, QuantizedMatrix, QuantizedRows, matmul, matmul_dots,
                      quantize_rows)
 from .qwen2 import Qwen2, Shape
-from .serving import PAGE, Batch, PagedCache, sample
+from .serving import PAGE, Batch, PagedCache, Pages, Rotary, copy_pages, sample
 from .tensor import BLOCK, QUAD, TERNARY_GROUP, DType, Matrix, QuantFormat, Table, TableUpload, Tensor, Vector, byte_len
 
 __all__ = [
@@ -28,6 +28,6 @@ __all__ = [
     "QuantizedRows", "QuantizedMatrix", "Quantized", "Input", "quantize_rows", "matmul", "matmul_dots",
     "Linear", "Ctx", "SharedRows", "project", "project_input", "project_residual", "project_residual_input",
     "Patches", "project_rows", "Qwen2", "Shape", "Call", "Operand", "Exponentials", "attend",
-    "PAGE", "Batch", "PagedCache", "sample",
+    "PAGE", "Batch", "PagedCache", "Pages", "Rotary", "copy_pages", "sample",
     "Error", "FormatError", "ShapeError", "GpuError", "lib",
 ]

@@ -84,6 +84,11 @@ SIGNATURES = {
     "fg_cache_write": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
     "fg_cache_read": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
     "fg_cache_attend": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _S, _F, _S, _P, _S, _P, _S, _P]),
+    "fg_rotary_create": (_I, [ctypes.POINTER(ctypes.c_double), _S, _I, ctypes.c_double, _P, ctypes.POINTER(_P)]),
+    "fg_rotary_free": (_I, [_P]),
+    "fg_rotary_rotate": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _S, _S, _P, _S, _P]),
+    "fg_cache_write_rotated": (_I, [_P, ctypes.POINTER(FgBatch), _P, _P, _S, _P, _S, _P, _S, _S, _P, _S, _P]),
+    "fg_cache_copy": (_I, [ctypes.POINTER(_P), _S, _P, _P, _S, _P]),
     "fg_cache_attend_scratch": (_S, [_P, ctypes.POINTER(FgBatch), _S]),
     "fg_sample": (_I, [_P, _S, _S, _S, ctypes.POINTER(FgSampling), _P, _P, _P, _S, _P]),
     "fg_sample_scratch": (_S, [_S, _S]),

@@ -11,7 +11,7 @@ import ctypes
 import math
 
 from . import _lib
-from ._lib import FgBatch, FgSampling, ShapeError, check, lib, stream_handle
+from ._lib import Error, FgBatch, FgSampling, ShapeError, check, lib, stream_handle
 
 PAGE = 64  # tokens of a page: FG_CACHE_PAGE
 
@@ -132,6 +132,93 @@ class Batch:
         return FgBatch(sequences, rows, max_pages, self.row_starts.data_ptr(), self.lengths.data_ptr(), p.data_ptr())
 
 
+def _rotated_out(x, head_dim, out):
+    """`out` for the rows `x` [rows, heads, head_dim] turned (made here where None: rows that no sequence holds
+    are then 0), both checked."""
+    if x.dim() != 3:
+        raise ShapeError("rows of shape [rows, heads, head_dim]")
+    _check_heads("rows to turn", x, x.shape[1], head_dim, x.device, False)
+    if not x.is_cuda:
+        raise ShapeError("rows to turn: a device tensor")
+    if out is None:
+        return torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+    _check_heads("out", out, x.shape[1], head_dim, x.device, True)
+    if out.shape[0] != x.shape[0]:
+        raise ShapeError(f"{x.shape[0]} rows to turn and {out.shape[0]} of out")
+    return out
+
+
+class Rotary:
+    """Rotary positions (fg_rotary): the first `dims` values of a head in pairs, pair i turned at position p by
+    p * f_i radians, f_i = base ** (-2 i / dims); with `layout` "halves" value i's partner is i + dims / 2, with
+    "pairs" 2 i's is 2 i + 1. Cosines and sines are computed in 64 bits at any position.
+
+    For contexts longer than a model was trained on, `stretch` divides the frequencies; with `trained`, the
+    tokens it was trained on, only those that turn fewer than `slow` times over them are divided whole, those
+    that turn more than `fast` times not at all, and between the two the share of the undivided frequency
+    rises evenly with the turns. `magnitude` multiplies the turned values. `frequencies` (dims / 2 numbers,
+    radians a token) takes the place of all of these but the magnitude."""
+
+    LAYOUTS = {"halves": 0, "pairs": 1}
+
+    def __init__(self, dims, base=10000.0, layout="halves", stretch=1.0, trained=None, slow=1.0, fast=32.0, magnitude=1.0,
+                 frequencies=None, device=None, stream=None):
+        _load()
+        if layout not in self.LAYOUTS:
+            raise ValueError(f'layout {layout!r}: "halves" or "pairs"')
+        if dims < 2 or dims % 2:
+            raise ShapeError(f"{dims} values to turn: an even number expected")
+        if frequencies is None:
+            frequencies = self._frequencies(dims, base, stretch, trained, slow, fast)
+        self.frequencies = [float(f) for f in frequencies]
+        if len(self.frequencies) != dims // 2:
+            raise ShapeError(f"{len(self.frequencies)} frequencies for {dims} values")
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ShapeError("rotary positions are on a GPU")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.dims, self.layout, self.magnitude, self.device = dims, layout, float(magnitude), device
+        handle = ctypes.c_void_p()
+        with _place(device, stream):
+            check(lib().fg_rotary_create((ctypes.c_double * (dims // 2))(*self.frequencies), dims, self.LAYOUTS[layout], self.magnitude,
+                                         stream_handle(), ctypes.byref(handle)))
+        self.handle = handle
+
+    @staticmethod
+    def _frequencies(dims, base, stretch, trained, slow, fast):
+        if not base > 0 or not stretch > 0:
+            raise ValueError("a base and a stretch above 0")
+        if trained is not None and (not trained > 0 or not fast > slow):
+            raise ValueError("trained tokens above 0, and more turns for `fast` than for `slow`")
+        out = []
+        for i in range(dims // 2):
+            f = float(base) ** (-2.0 * i / dims)
+            share = 0.0
+            if trained is not None:
+                share = min(max((trained * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0)
+            out.append(f * (share + (1.0 - share) / stretch))
+        return out
+
+    def __del__(self):
+        h = getattr(self, "handle", None)
+        if h is not None and _lib is not None and _lib._lib is not None:  # (None as the interpreter ends)
+            _lib._lib.fg_rotary_free(h)
+            self.handle = None
+
+    def rotate(self, batch, x, out=None, stream=None):
+        """The batch's new rows of `x` [rows, heads, head_dim] turned by their positions, into `out`, which may be
+        `x`. Rows of `out` that no sequence holds are left as they are (0 in an `out` made here)."""
+        if x.dim() != 3 or x.device != self.device or batch.pages.device != self.device:
+            raise ShapeError(f"rows [rows, heads, head_dim] and a batch on {self.device}")
+        head_dim = x.shape[2]
+        with _place(self.device, stream):
+            out = _rotated_out(x, head_dim, out)
+            check(lib().fg_rotary_rotate(self.handle, ctypes.byref(batch._ffi(x.shape[0])), x.data_ptr(), x.stride(0), x.shape[1], head_dim,
+                                         out.data_ptr(), out.stride(0), _stream(self.device)))
+        return out
+
+
 class PagedCache:
     """The keys and values of one layer's attention over many sequences (fg_cache): `pages` pages of
     PAGE tokens for `kv_heads` heads of `head_dim` values (whole quads, at most 256), each token's
@@ -165,13 +252,37 @@ class PagedCache:
             raise ShapeError(f"{keys.shape[0]} rows of keys and {values.shape[0]} of values")
         return batch._ffi(keys.shape[0])
 
-    def write(self, batch, keys, values, stream=None):
+    def write(self, batch, keys, values, stream=None, rotary=None, queries=None, out=None):
         """The new tokens' `keys` and `values` [rows, kv_heads, head_dim] quantized into their pages
-        (a page that is written to belongs to one sequence)."""
+        (a page that is written to belongs to one sequence). With `rotary` (Rotary) the keys are turned by
+        their positions on the way, and `queries` [rows, heads, head_dim], if given, by the same call into
+        `out`, which is returned (`out` as for Rotary.rotate)."""
         fg = self._rows(batch, keys, values, False)
+        if rotary is not None:
+            return self._write_rotated(fg, keys, values, stream, rotary, queries, out)
+        if queries is not None or out is not None:
+            raise ShapeError("queries are turned by `rotary`: none given")
         with _place(self.device, stream):
             check(lib().fg_cache_write(self.handle, ctypes.byref(fg), keys.data_ptr(), keys.stride(0), values.data_ptr(),
                                        values.stride(0), _stream(self.device)))
+
+    def _write_rotated(self, fg, keys, values, stream, rotary, queries, out):
+        if rotary.device != self.device:
+            raise ShapeError(f"the rotary positions are on {rotary.device}, the cache on {self.device}")
+        if queries is None and out is not None:
+            raise ShapeError("an `out` without queries")
+        heads = query = query_stride = place = stride = 0
+        with _place(self.device, stream):
+            if queries is not None:
+                out = _rotated_out(queries, self.head_dim, out)
+                if queries.device != self.device or queries.shape[0] != keys.shape[0]:
+                    raise ShapeError(f"queries of {queries.shape[0]} rows on {queries.device}, keys of {keys.shape[0]} on {self.device}")
+                heads, query, query_stride = queries.shape[1], queries.data_ptr(), queries.stride(0)
+                place, stride = out.data_ptr(), out.stride(0)
+            check(lib().fg_cache_write_rotated(self.handle, ctypes.byref(fg), rotary.handle, keys.data_ptr(), keys.stride(0),
+                                               values.data_ptr(), values.stride(0), query, query_stride, heads, place, stride,
+                                               _stream(self.device)))
+        return out
 
     def read(self, batch, keys, values, stream=None):
         """The same tokens read back into `keys` and `values`: level * scale."""
@@ -207,6 +318,114 @@ class PagedCache:
                                           1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, out.data_ptr(),
                                           out.stride(0), _at(scratch), size, _stream(self.device)))
         return out
+
+
+def copy_pages(caches, sources, targets, stream=None):
+    """Pages copied in every one of `caches` (fg_cache_copy): sources[i] to targets[i], whole. The ids are int32 device
+    tensors [pages], which a captured graph's replay reads as they are then, or lists, which are checked here: no
+    target twice, and none that is a source too (a page with itself apart)."""
+    _load()
+    caches = list(caches)
+    if not caches:
+        return
+    device = caches[0].device
+    if any(c.device != device for c in caches):
+        raise ShapeError("the caches are on one device")
+    if not isinstance(sources, torch.Tensor) and not isinstance(targets, torch.Tensor):
+        sources, targets = list(sources), list(targets)
+        moved = [(s, t) for s, t in zip(sources, targets) if s != t]
+        kept = {t for s, t in zip(sources, targets) if s == t}
+        ends = {t for _, t in moved}
+        if len(ends) != len(moved) or ends & {s for s, _ in moved} or ends & kept:
+            raise ShapeError("a page is copied to that is named twice")
+        limit = min(c.pages for c in caches)
+        if any(not 0 <= p < limit for p in sources + targets):
+            raise ShapeError(f"pages 0 to {limit - 1}")
+        with _place(device, stream):
+            sources, targets = (torch.tensor(p, dtype=torch.int32, device=device) for p in (sources, targets))
+            return _copy_pages(caches, sources, targets, device)
+    for name, t in (("sources", sources), ("targets", targets)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 1:
+            raise ShapeError(f"{name}: int32 device tensors [pages] both, or lists both")
+        _check_ints(name, t, None)
+        if t.device != device:
+            raise ShapeError(f"{name} are on {t.device}, the caches on {device}")
+    with _place(device, stream):
+        _copy_pages(caches, sources, targets, device)
+
+
+def _copy_pages(caches, sources, targets, device):
+    if sources.shape != targets.shape:
+        raise ShapeError(f"{sources.shape[0]} sources and {targets.shape[0]} targets")
+    handles = (ctypes.c_void_p * len(caches))(*[c.handle.value for c in caches])
+    check(lib().fg_cache_copy(handles, len(caches), sources.data_ptr(), targets.data_ptr(), sources.shape[0], _stream(device)))
+
+
+class Pages:
+    """Which of a cache's `count` pages are in use, and by how many sequences: the host's side of forks and compactions
+    (one for all layers' caches, which hold a token under the same page id)."""
+
+    def __init__(self, count):
+        self.count = count
+        self._free = list(range(count - 1, -1, -1))  # the last is handed out next: the lowest ids first
+        self._users = [0] * count
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def users(self, page):
+        """How many sequences hold `page`."""
+        return self._users[page]
+
+    def take(self, count):
+        """`count` pages that no sequence holds."""
+        if count < 0 or count > len(self._free):
+            raise Error(f"{count} pages asked for, {len(self._free)} of {self.count} are free")
+        pages = [self._free.pop() for _ in range(count)]
+        for p in pages:
+            self._users[p] = 1
+        return pages
+
+    def fork(self, pages, length):
+        """A second sequence with the `length` tokens that lie in `pages`: its pages, and the copies to make, (sources,
+        targets) for copy_pages. Whole pages are shared; one that is partly full, which both go on writing to, is copied."""
+        held = -(-length // PAGE)
+        if length < 0 or held > len(pages):
+            raise ShapeError(f"{length} tokens in {len(pages)} pages")
+        whole = length // PAGE
+        self._held(pages[:held])
+        if whole < held and not self._free:
+            raise Error("a page asked for, none is free")
+        for p in pages[:whole]:
+            self._users[p] += 1
+        copies = self.take(held - whole)
+        return pages[:whole] + copies, (list(pages[whole:held]), list(copies))
+
+    def free(self, pages):
+        """A sequence lets go of its pages."""
+        self._held(pages)
+        for p in pages:
+            self._users[p] -= 1
+            if self._users[p] == 0:
+                self._free.append(p)
+
+    def compact(self):
+        """The pages in use moved to the lowest ids: {old id: new id} of those that move. Its keys and values are
+        copy_pages' sources and targets; every sequence's table takes the new ids. The pages from the number in use on
+        are free then, so that a smaller cache could hold the rest."""
+        used = self.count - len(self._free)
+        low = sorted(p for p in self._free if p < used)
+        high = [p for p in range(used, self.count) if self._users[p]]
+        moves = dict(zip(high, low))
+        for old, new in moves.items():
+            self._users[new], self._users[old] = self._users[old], 0
+        self._free = list(range(self.count - 1, used - 1, -1))
+        return moves
+
+    def _held(self, pages):
+        if len(set(pages)) != len(pages) or any(not 0 <= p < self.count or not self._users[p] for p in pages):
+            raise ShapeError("pages that no sequence holds, or one of them twice")
 
 
 def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, chances=None, stream=None):

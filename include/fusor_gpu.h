@@ -228,6 +228,35 @@ int fg_cache_attend(const fg_cache *cache, const fg_batch *batch, const float *q
                     float scale, size_t window, float *out, size_t out_stride, void *scratch, size_t scratch_bytes,
                     void *stream);
 
+/* Rotary positions: value pairs (a, b) of a head's first `dims` values, pair i turned at position p by the angle
+ * p * frequencies[i]:  (a c - b s, b c + a s), c and s the angle's cosine and sine times `magnitude`. Angles are
+ * computed in 64 bits, at any position; c and s are rounded to f32 once, and products and sums are f32, rounded one by
+ * one. The values behind `dims` stay. (The decoder above turns its own heads by tables as the reference computes them,
+ * transformer.rs:185-219.) The handle owns its device memory, on the device that was current when it was created. */
+typedef struct fg_rotary fg_rotary;
+#define FG_ROTARY_HALVES 0 /* pair i is values i and i + dims / 2 */
+#define FG_ROTARY_PAIRS 1  /* pair i is values 2 i and 2 i + 1 */
+/* `frequencies` [dims / 2], radians a token, host memory, of at most 1024 in magnitude; dims even, at most 256.
+ * Waits for `stream`. */
+int fg_rotary_create(const double *frequencies, size_t dims, int layout, double magnitude, void *stream, fg_rotary **out);
+int fg_rotary_free(fg_rotary *rotary);
+/* The batch's new rows (its page table is not read) turned by their positions: head h of row r is the head_dim device f32
+ * values at r * stride + h * head_dim; heads of whole quads, at most 256, of at least `dims`. Rows at a negative
+ * position give 0. `out` may be `x`, with its stride; otherwise the two do not overlap. */
+int fg_rotary_rotate(const fg_rotary *rotary, const fg_batch *batch, const float *x, size_t x_stride, size_t heads, size_t head_dim,
+                     float *out, size_t out_stride, void *stream);
+/* fg_cache_write of keys that are turned first, and fg_rotary_rotate of the same rows' queries, `heads` of them, into `out` (none
+ * where heads is 0 and both are NULL). Turned keys are quantized from the f32 values that fg_rotary_rotate gives. */
+int fg_cache_write_rotated(fg_cache *cache, const fg_batch *batch, const fg_rotary *rotary, const float *key, size_t key_stride,
+                           const float *value, size_t value_stride, const float *query, size_t query_stride, size_t heads,
+                           float *out, size_t out_stride, void *stream);
+
+/* Pages copied in up to 65536 caches at once (a model's layers): page sources[i] of each to its page targets[i], whole, for the
+ * `pages` device int32 ids. A pair with an id outside a cache's pages, or of one page with itself, changes nothing there.
+ * No page is named twice among the targets, nor among sources and targets both (what such pages hold then is unspecified; the
+ * others are as they should be). What a fork of a sequence, or a compaction, moves. */
+int fg_cache_copy(fg_cache *const *caches, size_t count, const int32_t *sources, const int32_t *targets, size_t pages, void *stream);
+
 /* Next tokens drawn from logits (Prediction::predict, lm.rs:147-166, takes the largest). Row r of the
  * device f32 `logits`, at r * stride, orders its tokens by logit, the largest first, equal ones by
  * index; NaN counts as -inf. A token's weight is exp((logit - largest) / temperature); -inf weighs 0.

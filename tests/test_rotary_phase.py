@@ -1,0 +1,116 @@
+"""CPU checks of rotary positions: angles against 80-bit arithmetic at near and far positions, the frequencies of a
+stretched context, and the calls that are refused before any device work."""
+
+import ctypes
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fusor-ai_amd", "csrc")
+SOURCE = """
+#include "rotary_phase.h"
+using namespace fg;
+extern "C" {
+void angles(double frequency, const long long *positions, int count, double *c, double *s)
+{
+    const uint64_t step = turn_step(frequency);
+    for (int i = 0; i < count; i++) { const Angle a = angle_of(uint64_t(positions[i]) * step); c[i] = a.c; s[i] = a.s; }
+}
+unsigned long long step(double frequency) { return turn_step(frequency); }
+void phase(unsigned long long p, double *out) { const Angle a = angle_of(p); out[0] = a.c; out[1] = a.s; }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def phase(tmp_path_factory):
+    where = tmp_path_factory.mktemp("phase")
+    source, lib = where / "phase.cpp", where / "phase.so"
+    source.write_text(SOURCE)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", CSRC,
+                    str(source), "-o", str(lib)], check=True)
+    handle = ctypes.CDLL(str(lib))
+    handle.step.restype = ctypes.c_ulonglong
+    handle.step.argtypes = [ctypes.c_double]
+    return handle
+
+
+TWO_PI = np.longdouble("6.28318530717958647692528676655900577")
+
+
+@pytest.mark.parametrize("frequency", [1.0, 0.5, 1e6 ** (-30 / 32), 1e4 ** -0.25, 5e5 ** -0.99, 0.0, -0.3, 3.0, 1024.0])
+def test_angles(phase, frequency):
+    """Off by position * 2^-65 turns (the step's rounding), for frequencies past a turn 2^-64 of them more, and what 64
+    bits round; the 80-bit product that this is held against by position * frequency * 2^-64."""
+    rng = np.random.default_rng(0)
+    positions = np.concatenate([np.arange(200), rng.integers(0, 2 ** 31, 200), [2 ** 20, 2 ** 24, 2 ** 31 - 1]]).astype(np.int64)
+    c, s = np.zeros(len(positions)), np.zeros(len(positions))
+    d = ctypes.POINTER(ctypes.c_double)
+    phase.angles(ctypes.c_double(frequency), positions.ctypes.data_as(ctypes.c_void_p), len(positions), c.ctypes.data_as(d), s.ctypes.data_as(d))
+    f = np.longdouble(frequency)
+    angle = np.fmod(positions.astype(np.longdouble) * f, TWO_PI)
+    far = positions.astype(np.float64)
+    bound = far * (2.0 ** -65 * 6.3 * (2 + abs(frequency))) + far * abs(frequency) * 2.0 ** -62 + 2.0 ** -51
+    assert (np.abs(c - np.cos(angle).astype(np.float64)) <= bound).all()
+    assert (np.abs(s - np.sin(angle).astype(np.float64)) <= bound).all()
+
+
+def test_quarters_and_their_borders(phase):
+    out = (ctypes.c_double * 2)()
+    for eighth in range(8):
+        for off in (-1, 0, 1):
+            p = (eighth * 2 ** 61 + off) % 2 ** 64
+            phase.phase(ctypes.c_ulonglong(p), out)
+            turn = math.pi * eighth / 4
+            assert abs(out[0] - math.cos(turn)) < 1e-15 and abs(out[1] - math.sin(turn)) < 1e-15, (eighth, off)
+    phase.phase(ctypes.c_ulonglong(2 ** 62), out)
+    assert tuple(out) == (0.0, 1.0)
+    step = phase.step(2 * math.pi)  # a whole turn, to the double's rounding of 2^-51 radians
+    assert min(step, 2 ** 64 - step) < 2 ** 64 * 2.0 ** -51 / 6
+
+
+def test_frequencies():
+    from fusor_kernels import Rotary
+    plain = Rotary._frequencies(8, 1e4, 1.0, None, 1.0, 32.0)
+    assert plain == pytest.approx([1.0, 0.1, 0.01, 0.001], rel=1e-15)
+    assert Rotary._frequencies(8, 1e4, 4.0, None, 1.0, 32.0) == pytest.approx([f / 4 for f in plain], rel=1e-15)
+    # over 1000 tokens the four turn 159, 15.9, 1.59 and 0.159 times
+    by_parts = Rotary._frequencies(8, 1e4, 4.0, 1000, 1.0, 32.0)
+    share = [(1000 * f / (2 * math.pi) - 1) / 31 for f in plain]
+    assert by_parts[0] == plain[0] and by_parts[3] == plain[3] / 4
+    assert by_parts[1:3] == pytest.approx([f * s + f / 4 * (1 - s) for f, s in zip(plain[1:3], share[1:3])], rel=1e-14)
+    for arguments in ((8, 0.0, 1.0, None, 1.0, 32.0), (8, 1e4, 0.0, None, 1.0, 32.0), (8, 1e4, 2.0, 0, 1.0, 32.0),
+                      (8, 1e4, 2.0, 100, 2.0, 2.0), (8, float("nan"), 1.0, None, 1.0, 32.0)):
+        with pytest.raises(ValueError):
+            Rotary._frequencies(*arguments)
+
+
+def test_refusals_before_any_device_work():
+    import fusor_kernels as fk
+    from fusor_kernels import _lib
+    lib = _lib.lib()
+    handle = ctypes.c_void_p()
+
+    def create(frequencies, dims, layout=0, magnitude=1.0, out=ctypes.byref(handle)):
+        array = None if frequencies is None else (ctypes.c_double * max(len(frequencies), 1))(*frequencies)
+        return lib.fg_rotary_create(array, dims, layout, magnitude, None, out)
+
+    ones = [1.0] * 200
+    assert create(ones, 8, out=None) == _lib.FG_ERR_ARG
+    for dims in (0, 7, 258):
+        assert create(ones, dims) == _lib.FG_ERR_SHAPE and "fg_rotary_create" in lib.fg_last_error().decode()
+    assert create(None, 8) == create(ones, 8, layout=2) == create(ones, 8, magnitude=float("nan")) == _lib.FG_ERR_ARG
+    for bad in (float("nan"), float("inf"), 1025.0, -1025.0):
+        assert create([1.0, bad], 4) == _lib.FG_ERR_ARG
+    assert not handle
+    assert lib.fg_rotary_free(None) == _lib.FG_OK
+    batch = _lib.FgBatch(1, 1, 1, None, None, None)
+    assert lib.fg_rotary_rotate(None, ctypes.byref(batch), None, 0, 1, 64, None, 0, None) == _lib.FG_ERR_ARG
+    assert lib.fg_cache_write_rotated(None, ctypes.byref(batch), None, None, 0, None, 0, None, 0, 0, None, 0, None) == _lib.FG_ERR_ARG
+    for arguments, error in (({"layout": "other"}, ValueError), ({"dims": 7}, fk.ShapeError), ({"dims": 0}, fk.ShapeError),
+                             ({"frequencies": [1.0]}, fk.ShapeError), ({"device": "cpu"}, fk.ShapeError)):
+        with pytest.raises(error):
+            fk.Rotary(**{"dims": 8, **arguments})
