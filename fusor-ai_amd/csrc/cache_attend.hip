@@ -936,3 +936,31 @@ extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float
     }
     return rc;
 }
+
+namespace fg {
+namespace {
+
+int check_prefixes(const fg_prefixes *f, const char *who)
+{
+    if (!f) return set_error(FG_ERR_ARG, std::string(who) + ": null prefixes");
+    if (f->groups > 65536) return set_error(FG_ERR_SHAPE, std::string(who) + ": at most 65536 groups");
+    if (f->groups && (!f->starts || !f->pages)) return set_error(FG_ERR_ARG, std::string(who) + ": a null array of the prefixes");
+    return FG_OK;
+}
+
+}  // namespace
+}  // namespace fg
+
+extern "C" size_t fg_cache_attend_shared_scratch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads)
+{
+    return f ? fg_cache_attend_scratch(c, b, heads) : 0;
+}
+
+extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, const float *query, size_t query_stride,
+                                      size_t heads, float scale, size_t window, float *out, size_t out_stride, void *scratch,
+                                      size_t scratch_bytes, void *stream)
+{
+    const int rc = check_prefixes(f, "fg_cache_attend_shared");
+    if (rc) return rc;
+    return fg_cache_attend(c, b, query, query_stride, heads, scale, window, out, out_stride, scratch, scratch_bytes, stream);
+}

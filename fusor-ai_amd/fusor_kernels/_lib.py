@@ -52,6 +52,10 @@ class FgBatch(ctypes.Structure):
     _fields_ = [("sequences", _S), ("rows", _S), ("max_pages", _S), ("row_starts", _P), ("lengths", _P), ("pages", _P)]
 
 
+class FgPrefixes(ctypes.Structure):
+    _fields_ = [("groups", _S), ("starts", _P), ("pages", _P)]
+
+
 class FgSampling(ctypes.Structure):
     _fields_ = [("random", _P), ("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P)]
 
@@ -84,6 +88,8 @@ SIGNATURES = {
     "fg_cache_write": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
     "fg_cache_read": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _P, _S, _P]),
     "fg_cache_attend": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _S, _F, _S, _P, _S, _P, _S, _P]),
+    "fg_cache_attend_shared": (_I, [_P, ctypes.POINTER(FgBatch), ctypes.POINTER(FgPrefixes), _P, _S, _S, _F, _S, _P, _S, _P, _S, _P]),
+    "fg_cache_attend_shared_scratch": (_S, [_P, ctypes.POINTER(FgBatch), ctypes.POINTER(FgPrefixes), _S]),
     "fg_rotary_create": (_I, [ctypes.POINTER(ctypes.c_double), _S, _I, ctypes.c_double, _P, ctypes.POINTER(_P)]),
     "fg_rotary_free": (_I, [_P]),
     "fg_rotary_rotate": (_I, [_P, ctypes.POINTER(FgBatch), _P, _S, _S, _S, _P, _S, _P]),

@@ -11,7 +11,7 @@ import ctypes
 import math
 
 from . import _lib
-from ._lib import Error, FgBatch, FgSampling, ShapeError, check, lib, stream_handle
+from ._lib import Error, FgBatch, FgPrefixes, FgSampling, ShapeError, check, lib, stream_handle
 
 PAGE = 64  # tokens of a page: FG_CACHE_PAGE
 
@@ -130,6 +130,29 @@ class Batch:
         p = self.pages
         sequences, max_pages = p.shape
         return FgBatch(sequences, rows, max_pages, self.row_starts.data_ptr(), self.lengths.data_ptr(), p.data_ptr())
+
+
+class Prefixes:
+    """Runs of a batch's sequences that begin with the same pages (fg_prefixes), as int32 device tensors that the
+    kernels read: `starts` [groups + 1], group g is the sequences starts[g] .. starts[g + 1] - 1, and `pages` [groups],
+    how many pages the tables of all of them begin with. Sequences that no group holds share nothing."""
+
+    def __init__(self, starts, pages):
+        _load()
+        if pages.dim() != 1:
+            raise ShapeError("pages: [groups]")
+        _check_ints("starts", starts, [pages.shape[0] + 1])
+        _check_ints("pages", pages, None)
+        if starts.device != pages.device:
+            raise ShapeError("the prefixes' tensors are on one device")
+        self.starts, self.pages = starts, pages
+
+    @property
+    def groups(self):
+        return self.pages.shape[0]
+
+    def _ffi(self):
+        return FgPrefixes(self.pages.shape[0], self.starts.data_ptr(), self.pages.data_ptr())
 
 
 def _rotated_out(x, head_dim, out):
@@ -291,12 +314,13 @@ class PagedCache:
             check(lib().fg_cache_read(self.handle, ctypes.byref(fg), keys.data_ptr(), keys.stride(0), values.data_ptr(),
                                       values.stride(0), _stream(self.device)))
 
-    def attend(self, batch, queries, out=None, scale=None, window=0, stream=None):
+    def attend(self, batch, queries, out=None, scale=None, window=0, stream=None, prefixes=None):
         """The attention of the new tokens' `queries` [rows, heads, head_dim] (their keys and values
         written before): each token sees its sequence's tokens up to itself, with `window` the last
         `window` of them. `scale` is 1 / sqrt(head_dim) unless given. A token without a key gives 0;
         `out` may be `queries`; rows of it that no sequence holds are left as they are (0 in an `out`
-        made here). Keys may reach 1e33 and scores 1e7 in magnitude."""
+        made here). Keys may reach 1e33 and scores 1e7 in magnitude. With `prefixes` (Prefixes) the pages that a group
+        of sequences begins with are worked through once for all of them."""
         if batch.pages.device != self.device:
             raise ShapeError(f"the batch is on {batch.pages.device}, the cache on {self.device}")
         if queries.dim() != 3:
@@ -312,6 +336,16 @@ class PagedCache:
             if out.shape[0] != queries.shape[0]:
                 raise ShapeError(f"{queries.shape[0]} rows of queries and {out.shape[0]} of out")
             fg, library = ctypes.byref(batch._ffi(queries.shape[0])), lib()
+            if prefixes is not None:
+                if prefixes.pages.device != self.device:
+                    raise ShapeError(f"the prefixes are on {prefixes.pages.device}, the cache on {self.device}")
+                shared = ctypes.byref(prefixes._ffi())
+                size = library.fg_cache_attend_shared_scratch(self.handle, fg, shared, heads)
+                scratch = _scratch(size, self.device)
+                check(library.fg_cache_attend_shared(self.handle, fg, shared, queries.data_ptr(), queries.stride(0), heads,
+                                                     1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, out.data_ptr(),
+                                                     out.stride(0), _at(scratch), size, _stream(self.device)))
+                return out
             size = library.fg_cache_attend_scratch(self.handle, fg, heads)
             scratch = _scratch(size, self.device)
             check(library.fg_cache_attend(self.handle, fg, queries.data_ptr(), queries.stride(0), heads,

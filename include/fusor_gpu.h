@@ -228,6 +228,23 @@ int fg_cache_attend(const fg_cache *cache, const fg_batch *batch, const float *q
                     float scale, size_t window, float *out, size_t out_stride, void *scratch, size_t scratch_bytes,
                     void *stream);
 
+/* Runs of a batch's sequences that begin with the same pages, as device int32 arrays like the batch's:
+ *   starts [groups + 1], not falling: group g is the sequences starts[g] .. starts[g + 1] - 1; sequences that no group
+ *          holds share nothing;
+ *   pages  [groups]: the first pages[g] ids of the tables of all of its sequences are the same.
+ * (Which sequence's table a shared page's id is taken from is unspecified.) */
+typedef struct {
+    size_t groups; /* at most 65536 */
+    const int32_t *starts, *pages;
+} fg_prefixes;
+
+/* fg_cache_attend, with each group's shared pages worked through once for all of its rows where that is faster: what it
+ * gives is the same, but for the order of additions. */
+size_t fg_cache_attend_shared_scratch(const fg_cache *cache, const fg_batch *batch, const fg_prefixes *prefixes, size_t heads);
+int fg_cache_attend_shared(const fg_cache *cache, const fg_batch *batch, const fg_prefixes *prefixes, const float *query,
+                           size_t query_stride, size_t heads, float scale, size_t window, float *out, size_t out_stride,
+                           void *scratch, size_t scratch_bytes, void *stream);
+
 /* Rotary positions: value pairs (a, b) of a head's first `dims` values, pair i turned at position p by the angle
  * p * frequencies[i]:  (a c - b s, b c + a s), c and s the angle's cosine and sine times `magnitude`. Angles are
  * computed in 64 bits, at any position; c and s are rounded to f32 once, and products and sums are f32, rounded one by
