@@ -9,8 +9,12 @@
 #include "cache.h"
 
 namespace fg {
-namespace {
 
+// The arguments that calls of attention check.
+int check_attend(const fg_cache *c, const fg_batch *b, const float *query, size_t heads, float scale, const float *out, size_t out_stride,
+                 const char *who);
+
+namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -35,6 +39,28 @@ struct AttendParams {
     Note *notes;   // [grid]
 };
 
+template <class P>
+P attend_params(const fg_cache *c, const fg_batch *b, const float *query, size_t query_stride, size_t heads, float scale, size_t window,
+                float *out, size_t out_stride)
+{
+    P p{};
+    p.b = batch_params(b);
+    p.records = c->records;
+    p.pages = c->pages;
+    p.kv_heads = c->kv_heads;
+    p.heads = int(heads);
+    p.group = int(heads) / c->kv_heads;
+    p.head_dim = c->head_dim;
+    p.query = query;
+    p.query_stride = query_stride;
+    p.out = out;
+    p.out_stride = out_stride;
+    p.scale2 = scale * 1.44269504088896340736f;
+    p.window = int(window < size_t(INT_MAX) ? window : size_t(INT_MAX));
+    return p;
+}
+
+constexpr size_t kUnits = 256;  // CUs
 constexpr int kMaxSplit = 64;   // parts of one row tile
 constexpr int kMinPages = 4;    // pages of a part, a wave each
 
@@ -53,18 +79,21 @@ __device__ __forceinline__ Task uniform(Task t)
     return t;
 }
 
-// Where the rows of a task's span are, and the positions that a tile's rows lie between: those of one sequence follow each
-// other.
-struct InSequence {
-    int first, low, high;
-    __device__ __forceinline__ int of(int at) const { return first + at; }
-};
-
 // One pair of a tile: its operand row, query head and position.
 struct Pair {
     int row, head, position;
     bool live;
 };
+
+// Where the rows of a task's span are, and the positions that a tile's rows lie between: those of one sequence follow each
+// other.
+struct InSequence {
+    int first, low, high;
+    __device__ __forceinline__ int of(int at) const { return first + at; }
+    // the position of a lane's pair, once more
+    __device__ __forceinline__ int again(const Pair &pair, int) const { return pair.position; }
+};
+
 template <class Places>
 __device__ __forceinline__ Pair pair_of(const AttendParams &p, const Task &t, int kv, int m, const Places &places)
 {
@@ -202,9 +231,12 @@ __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], floa
     };
     auto masked = [&]() {
         top = total = 0.0f;
+        // (an f of its own: else the compiler may take the exponentials out of both branches, 16 registers more than there are)
+        float g = f;
+        asm volatile("" : "+v"(g));
         for_scales(vs, [&](int i, float v) {
             const bool seen = key(i) >= low && key(i) <= high;
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], f, -sums.r));
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], g, -sums.r));
             x[i] = seen ? v * e : 0.0f;
             total = total + (seen ? e : 0.0f);
             top = fmaxf(top, x[i]);
@@ -217,6 +249,7 @@ __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], floa
         float u = -INFINITY, m = -INFINITY;
         float logs = vs;
         asm volatile("" : "+v"(logs));  // (keeps the logarithm in this branch)
+        asm volatile("" : "+v"(low), "+v"(high));  // (the masks once more: all of them kept do not fit the scalar registers)
         logs = __builtin_amdgcn_logf(logs);
         for_scales(logs, [&](int i, float v) {
             const float t = s[i] * f;
@@ -480,9 +513,11 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
     auto load = [&](int id) {  // a page's record into registers
         if (id < 0) return;
         const uint8_t *record = p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP);
+        unsigned thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));  // (a 32-bit offset beside a scalar address, no 64-bit one kept in registers)
 #pragma unroll
-        for (int c = 0; c < L; c++) staged[c] = *reinterpret_cast<const uint4 *>(record + (c * 256 + tid) * 16);
-        if (tid < 2 * kPage) staged_scale = *reinterpret_cast<const float *>(record + key_scale_byte(DP, tid));
+        for (int c = 0; c < L; c++) staged[c] = *reinterpret_cast<const uint4 *>(record + c * 4096 + thread * 16u);
+        if (tid < 2 * kPage) staged_scale = *reinterpret_cast<const float *>(record + key_scale_byte(DP, 0) + thread * 4u);
     };
     auto store = [&](uint8_t *to) {  // ... widened into a buffer: each kilobyte of 64 lanes as two
 #pragma unroll
@@ -552,13 +587,20 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
             v16f s[2] = {};
             v8h a[2][2];
             float ks[2], vs[2];
+            // (places computed from the lane once more in every page, not kept: the registers are full)
+            int here_lane = int(threadIdx.x);
+            asm volatile("" : "+v"(here_lane));
+            int high = places.again(pair, (here_lane >> 6) * 32 + (here_lane & 31));
+            asm volatile("" : "+v"(high));
+            here_lane &= 63;
+            const int low = first_seen(high, p.window), keys_at = page * kPage + 4 * (here_lane >> 5);
             auto read_keys = [&](int k) {
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++) a[k & 1][kt] = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + lane * 16);
+                for (int kt = 0; kt < 2; kt++) a[k & 1][kt] = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + here_lane * 16);
             };
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {
-                const int token = 32 * kt + 8 * ((lane >> 2) & 3) + 4 * h + (lane & 3);
+                const int token = 32 * kt + 8 * ((here_lane >> 2) & 3) + 4 * (here_lane >> 5) + (here_lane & 3);
                 ks[kt] = key_scales[token];
                 vs[kt] = value_scales[token];
             }
@@ -574,11 +616,10 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
                 for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k & 1][kt], qh[k], s[kt], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const int high = pair.position, low = first_seen(high, p.window);
             v8h wh[4], wl[4], b[2][T];
             auto read_values = [&](int c) {
 #pragma unroll
-                for (int d = 0; d < T; d++) b[c & 1][d] = *reinterpret_cast<const v8h *>(values + ((d * 2 + c / 2) * 2 + c % 2) * 1024 + lane * 16);
+                for (int d = 0; d < T; d++) b[c & 1][d] = *reinterpret_cast<const v8h *>(values + ((d * 2 + c / 2) * 2 + c % 2) * 1024 + here_lane * 16);
             };
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {  // 32 keys at a time: half the registers
@@ -587,7 +628,7 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
                 if (kt) read_values(0);
                 __builtin_amdgcn_sched_barrier(0);
                 weigh(scores, x, vs[kt], f, small, edge, low, high, sums,
-                          [&](int i) { return page * kPage + 32 * kt + 2 * (i & ~3) + 4 * h + i % 4; },
+                          [&](int i) { return keys_at + 32 * kt + 2 * (i & ~3) + i % 4; },
                           [](float v) {
                               const float2 w = half_pair(v);
                               return fmaxf(w.x, w.y);
@@ -627,7 +668,9 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
     }
     const float2 w = half_pair(sums.total);
     sums.total = w.x + w.y;
-    if (!pair.live) return;
+    int thread = int(threadIdx.x);
+    asm volatile("" : "+v"(thread));
+    if (task.tile * TM + (thread >> 6) * 32 + (thread & 31) >= task.span.rows * p.group) return;  // (a pair that is not live)
     if (parts) {
         float *part = parts + wave * many_floats(DP);
         part[lane] = sums.r;

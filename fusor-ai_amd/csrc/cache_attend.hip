@@ -190,8 +190,6 @@ struct Launch {
     size_t note_bytes, partial_bytes;
 };
 
-constexpr size_t kUnits = 256;  // CUs
-
 // Which kernel a step takes, and whether its tiles are split, from what the host knows of it: microseconds of
 // decode steps and chunks over caches of random or equal lengths, 16 query heads of 128 over 4 key heads (a), 14 of
 // 64 over 2 (b), 8 of 128 over 1 (c).
@@ -264,6 +262,26 @@ int launch_attend(const AttendParams &p, const Launch &l, hipStream_t s)
 }
 
 }  // namespace
+
+int check_attend(const fg_cache *c, const fg_batch *b, const float *query, size_t heads, float scale, const float *out, size_t out_stride,
+                 const char *who)
+{
+    const std::string name(who);
+    const int rc = check_batch(c, b, who);
+    if (rc) return rc;
+    if (!heads || heads % c->kv_heads || heads > 65536)
+        return set_error(FG_ERR_SHAPE, name + ": the heads must be a positive multiple of the cache's, at most 65536");
+    if (!(std::fabs(scale) <= 2e38f))  // (times log2 e it is in f32's range)
+        return set_error(FG_ERR_ARG, name + ": the scale must be a number of at most 2e38");
+    if (!b->rows || !b->sequences) return FG_OK;
+    if (!query || !out) return set_error(FG_ERR_ARG, name + ": a null query or output");
+    const size_t width = heads * c->head_dim;
+    if (b->rows > 1 && out_stride < width) return set_error(FG_ERR_SHAPE, name + ": a row's heads run past the row stride");
+    if (b->rows * (heads / c->kv_heads) > (size_t(1) << 30))
+        return set_error(FG_ERR_SHAPE, name + ": at most 2^30 rows times heads of a key head");
+    return FG_OK;
+}
+
 }  // namespace fg
 
 using namespace fg;
@@ -279,35 +297,13 @@ extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float
                                float scale, size_t window, float *out, size_t out_stride, void *scratch, size_t scratch_bytes,
                                void *stream)
 {
-    int rc = check_batch(c, b, "fg_cache_attend");
+    int rc = check_attend(c, b, query, heads, scale, out, out_stride, "fg_cache_attend");
     if (rc) return rc;
-    if (!heads || heads % c->kv_heads || heads > 65536)
-        return set_error(FG_ERR_SHAPE, "fg_cache_attend: the heads must be a positive multiple of the cache's, at most 65536");
-    if (!(std::fabs(scale) <= 2e38f))  // (times log2 e it is in f32's range)
-        return set_error(FG_ERR_ARG, "fg_cache_attend: the scale must be a number of at most 2e38");
     if (!b->rows || !b->sequences) return FG_OK;
-    if (!query || !out) return set_error(FG_ERR_ARG, "fg_cache_attend: a null query or output");
-    const size_t width = heads * c->head_dim;
-    if (b->rows > 1 && out_stride < width) return set_error(FG_ERR_SHAPE, "fg_cache_attend: a row's heads run past the row stride");
-    if (b->rows * (heads / c->kv_heads) > (size_t(1) << 30))
-        return set_error(FG_ERR_SHAPE, "fg_cache_attend: at most 2^30 rows times heads of a key head");
     const hipStream_t s = as_stream(stream);
     const Launch l = plan_launch(c, b, heads);
     if (l.grid * c->kv_heads > kMaxGrid) return set_error(FG_ERR_SHAPE, "fg_cache_attend: more sequences times heads than a launch takes");
-    AttendParams p{};
-    p.b = batch_params(b);
-    p.records = c->records;
-    p.pages = c->pages;
-    p.kv_heads = c->kv_heads;
-    p.heads = int(heads);
-    p.group = int(heads) / c->kv_heads;
-    p.head_dim = c->head_dim;
-    p.query = query;
-    p.query_stride = query_stride;
-    p.out = out;
-    p.out_stride = out_stride;
-    p.scale2 = scale * 1.44269504088896340736f;
-    p.window = int(std::min<size_t>(window, INT_MAX));
+    AttendParams p = attend_params<AttendParams>(c, b, query, query_stride, heads, scale, window, out, out_stride);
     p.grid = int(l.grid);
     p.target = l.target;
     void *ws = nullptr;
@@ -329,32 +325,4 @@ extern "C" int fg_cache_attend(const fg_cache *c, const fg_batch *b, const float
         if (rc == FG_OK && e != hipSuccess) rc = check_hip(e, "hipFreeAsync");
     }
     return rc;
-}
-
-namespace fg {
-namespace {
-
-int check_prefixes(const fg_prefixes *f, const char *who)
-{
-    if (!f) return set_error(FG_ERR_ARG, std::string(who) + ": null prefixes");
-    if (f->groups > 65536) return set_error(FG_ERR_SHAPE, std::string(who) + ": at most 65536 groups");
-    if (f->groups && (!f->starts || !f->pages)) return set_error(FG_ERR_ARG, std::string(who) + ": a null array of the prefixes");
-    return FG_OK;
-}
-
-}  // namespace
-}  // namespace fg
-
-extern "C" size_t fg_cache_attend_shared_scratch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads)
-{
-    return f ? fg_cache_attend_scratch(c, b, heads) : 0;
-}
-
-extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, const float *query, size_t query_stride,
-                                      size_t heads, float scale, size_t window, float *out, size_t out_stride, void *scratch,
-                                      size_t scratch_bytes, void *stream)
-{
-    const int rc = check_prefixes(f, "fg_cache_attend_shared");
-    if (rc) return rc;
-    return fg_cache_attend(c, b, query, query_stride, heads, scale, window, out, out_stride, scratch, scratch_bytes, stream);
 }
