@@ -293,20 +293,20 @@ __device__ __forceinline__ float part_factor(float r, float joined) { return r =
 // 64, is that chain alone, 7.7 us.
 // (Two tiles of rows a workgroup, which halves the reading of 17 to 32 pairs, left one workgroup a CU: 64 sequences
 // of up to 3200 tokens, 28 pairs, 25.5 against 24.1 us, 32 pairs over one key head 36.9 against 24.2.)
-// The tile's sums over the pages `range` of `table`, to `part`, or where that is null divided to the output.
+// The tile's sums over the pages `range` of `table`, to `part`, or where that is null divided to the output: by WAVES waves
+// together, 4, or by one for itself, which needs no `join`.
 constexpr int few_floats(int DP) { return 16 * DP + 128; }  // of a part
 template <int DP>
 struct FewJoin {  // the waves' sums on their way to each other
     float sums[2][DP / 16 * 4 + 2][64];
 };
-template <int DP, class Places>
+template <int DP, int WAVES, class Places>
 __device__ __forceinline__ void attend_few(const AttendParams &p, const Task &task, const PageRange range, const int32_t *table, int kv,
-                                           const Places &places, FewJoin<DP> &join, float *part)
+                                           const Places &places, FewJoin<DP> *join, float *part)
 {
     constexpr int TM = 16, J = (DP + 63) / 64, T = DP / 16, R = DP / 32;
-    float(*joined)[T * 4 + 2][64] = join.sums;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     const Pair pair = pair_of(p, task, kv, task.tile * TM + i, places);
     v8h qh[J][2], ql[J][2];
     float f;
@@ -367,14 +367,14 @@ __device__ __forceinline__ void attend_few(const AttendParams &p, const Task &ta
         for (int d = 0; d < T; d++)
             v[d] = *reinterpret_cast<const uint4 *>(record + kPage * DP + ((d >> 1) * 2 + (g >> 1)) * 1024 + ((g & 1) * 32 + (d & 1) * 16 + i) * 16);
     };
-    int id = id_of(entry_of(range.lo + wave)), next = entry_of(range.lo + wave + 4), loaded = max(id, 0);
+    int id = id_of(entry_of(range.lo + wave)), next = entry_of(range.lo + wave + WAVES), loaded = max(id, 0);
     load_keys(loaded);
     load_values(loaded);
-    for (int page = range.lo + wave; page < range.hi; page += 4) {
+    for (int page = range.lo + wave; page < range.hi; page += WAVES) {
         const bool held = id >= 0;
         id = id_of(next);
         loaded = id >= 0 ? id : loaded;  // (what is loaded already, again, where there is no next one)
-        next = entry_of(page + 8);
+        next = entry_of(page + 2 * WAVES);
         if (!held) {
             load_keys(loaded);
             load_values(loaded);
@@ -431,7 +431,8 @@ __device__ __forceinline__ void attend_few(const AttendParams &p, const Task &ta
     }
     // the waves' sums joined, lane by lane: waves 2 and 3 into 0 and 1, then 1 into 0
 #pragma unroll
-    for (int step = 2; step >= 1; step >>= 1) {
+    for (int step = WAVES / 2; step >= 1; step >>= 1) {
+        float(*joined)[T * 4 + 2][64] = join->sums;
         float(*to)[64] = joined[wave & 1];
         if (wave >= step && wave < 2 * step) {
             to[0][lane] = sums.r;

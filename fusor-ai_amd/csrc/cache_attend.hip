@@ -101,8 +101,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(Atte
     const int low = task.span.first + task.tile * TM / p.group;
     const int high = task.span.first + min((task.tile * TM + TM - 1) / p.group, task.span.rows - 1);
     float *part = task.nsplit > 1 ? p.partial + (size_t(task.slot) * p.kv_heads + kv) * few_floats(DP) : nullptr;
-    attend_few<DP>(p, task, task_pages(p, task, TM), p.b.pages + size_t(task.seq) * p.b.max_pages, kv,
-                   InSequence{task.span.first, low, high}, join, part);
+    attend_few<DP, 4>(p, task, task_pages(p, task, TM), p.b.pages + size_t(task.seq) * p.b.max_pages, kv,
+                      InSequence{task.span.first, low, high}, &join, part);
 }
 
 template <int DP>

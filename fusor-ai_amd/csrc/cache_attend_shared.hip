@@ -1,6 +1,6 @@
 // Attention of a step's new tokens over the paged 8-bit cache where groups of sequences begin with the same pages
 // (fg_cache_attend_shared): a group's pages once for all rows of its sequences, each sequence's own pages, and the join of
-// both. cache_attend.h has what a workgroup does with a task.
+// both. cache_attend.h has what a workgroup, or a wave, does with a task.
 #include <algorithm>
 #include <atomic>
 
@@ -12,38 +12,71 @@ namespace {
 // ---------------------------------------------------------------------------- the plan
 //
 // Spans of rows to work through: the groups' (the rows of all of a group's sequences, over the shared pages), then the
-// sequences' (over the pages behind them). A span's (row, query head) pairs lie in tiles as in cache_attend.hip, of 128 or, in
-// spans of few pairs, of 16, and a tile's pages are split into parts of about the same work; a part is a task, a
-// workgroup's for each key head. Every workgroup finds its task from the arrays, all 256 threads together.
+// sequences' (over the pages behind them). A span's (row, query head) pairs lie in tiles as in cache_attend.hip: large ones of
+// 128, a workgroup's, or, in spans of few pairs, small ones of 16, a wave's. A tile's pages are split into parts of about the
+// same time; a part of a tile is a task, for each key head. One workgroup lists the tasks from the batch's arrays, and what
+// the join then does: nothing about the lengths is known on the host. (Each task's workgroup looking for itself, as in
+// cache_attend.hip, took 2.7 us of each one's time, and 6.7 from 257 spans on.)
 
-// Where the sums of a row's pairs are, in the order in which the tasks lie: tile t's part s at slot base + (tiles - 1 - t)
-// parts + s of the large tiles' or the small ones'.
-struct RowNote {
-    int base, begin;  // begin: the span's first row
-    int tiles;
-    int parts;        // of a tile; 0: its outputs are written already
+struct TaskRecord {
+    int table;          // the sequence whose table has the pages
+    int tile, split, nsplit;
+    int begin, rows;    // the span's
+    int first;          // the position of a sequence's first row
+    int lo, hi;         // pages [lo, hi) at most
+    int shared, whole;  // a group's; a small tile whose task is its only one and writes its outputs
+    int fill[5];
 };
-constexpr int kLargeTiles = 1 << 16, kAfterShared = 1 << 17;  // flags in `parts`
+
+// A tile's, or a large tile's quarter's, parts to be joined.
+struct JoinRecord {
+    int begin, rows;     // the span's
+    int pair;            // the first one
+    int slot, parts;     // its first part's task, and how many
+    int wave;            // the quarter of a large tile; -1: a small one
+    int shared;          // each row's own parts are joined too
+    int fill;
+};
+
+// Where a sequence's parts are: tile t's part s is task base + (tiles - 1 - t) parts + s of the large or the small ones.
+struct SequenceNote {
+    int base, begin, tiles, parts;
+};
+constexpr int kLarge = 1 << 16;  // a flag in `parts`
+
+struct RowNote {
+    int sequence, position;
+};
+
+struct PlanHeader {
+    int large, small, joins;
+};
 
 struct SharedParams : AttendParams {
     const int32_t *starts, *counts;
     int groups;
-    int limit;        // pairs of a span that small tiles take
-    int large_slots, small_slots;
+    int limit;  // pairs of a span that small tiles take
+    int large_slots, small_slots, join_slots;
+    PlanHeader *header;
+    TaskRecord *large_tasks, *small_tasks;
+    JoinRecord *joins;
+    SequenceNote *notes_of;  // [sequences]
+    RowNote *rows_of;        // [rows]
     float *small_partial;
-    RowNote *own, *shared;  // [rows]
 };
+
+// What a part takes: at least so many pages, and of the whole work, in units of a small tile's page, a share of the target.
+constexpr int kLargePages = 4, kSmallPages = 2, kLargeCost = 2;
+constexpr int kSharedSplit = 256;  // parts of a tile, at most
 
 struct Entity {
     Span span;
-    int tiles, pages;  // pages: that a tile sees at most
-    int first_page;    // of the span's
-    bool large, joined;
+    int tiles, lo, hi, pages;  // pages [lo, hi) at most, and how many of them a tile sees at most
+    int table;
+    bool large, shared, joined;  // joined: a sequence's whose rows see shared pages too
 };
 
-// How many of a group's sequences' first pages are shared, within what any table holds.
 __device__ __forceinline__ int shared_pages(const SharedParams &p, int count) { return max(0, min(count, p.b.max_pages)); }
-
 __device__ __forceinline__ int sequence_index(const SharedParams &p, int start) { return max(0, min(start, p.b.sequences)); }
 
 // Span e, the groups' first. Every lane of the wave takes part.
@@ -51,6 +84,7 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, int e)
 {
     Entity n{};
     const int lane = threadIdx.x & 63, s = e - p.groups;
+    if (s >= 0 && s < p.b.sequences) n.span = sequence_span(p.b, s);
     // the shared pages of sequence s: those of the last group that starts at or before it
     int before = 0;
     for (int g0 = 0; g0 <= p.groups; g0 += 64) {
@@ -62,319 +96,347 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, int e)
             before = s >= at ? pages : before;
         }
     }
-    if (e < p.groups) {
+    n.table = s;
+    if (s < 0) {
         const int a = sequence_index(p, p.starts[e]), b = sequence_index(p, p.starts[e + 1]);
         if (b <= a) return n;
         n.span = span_of(p.b.row_starts[a], p.b.row_starts[b], 0, p.b.rows);
-        n.pages = shared_pages(p, p.counts[e]);
+        n.table = a;
+        n.shared = true;
+        n.pages = n.hi = shared_pages(p, p.counts[e]);
         // (each row sees less than a window of the pages before its sequence's own)
         if (p.window > 0) n.pages = min(n.pages, p.window / kPage + 2);
-        if (n.pages == 0) return n;
-    } else if (s < p.b.sequences) {
-        n.span = sequence_span(p.b, s);
-        n.first_page = shared_pages(p, before);
-        n.joined = n.first_page > 0;
+        if (n.hi == 0) return n;
+    } else {
+        n.lo = shared_pages(p, before);
+        n.joined = n.lo > 0;
     }
     if (n.span.rows == 0) return n;
     const int pairs = n.span.rows * p.group;
     n.large = pairs > p.limit;
     const int tm = n.large ? 128 : 16;
     n.tiles = (pairs + tm - 1) / tm;
-    if (e >= p.groups) {
+    if (!n.shared) {
         const PageRange r = pages_seen(n.span, 0, n.span.rows - 1, p.window, p.b.max_pages);
-        n.pages = max(0, r.hi - max(r.lo, n.first_page));
+        n.hi = r.hi;
+        n.pages = max(0, r.hi - max(r.lo, n.lo));
         if (p.window > 0) n.pages = min(n.pages, p.window / kPage + tm / p.group / kPage + 3);
     }
     return n;
 }
 
-__device__ __forceinline__ float wave_total(float v) { return wave_allsum(v); }
-__device__ __forceinline__ int wave_total(int v)
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+
+// A thread a span, 1024 at a time; then a thread a task or join of theirs.
+__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p)
 {
-    int total;
-    (void)wave_scan(v, &total);
-    return total;
-}
-
-// A sum over the workgroup's threads, in an order that is always the same.
-template <class T>
-__device__ __forceinline__ T block_sum(T v, T *wave_totals)
-{
-    v = wave_total(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) wave_totals[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return wave_totals[0] + wave_totals[1] + wave_totals[2] + wave_totals[3];
-}
-
-struct Found {
-    Task task;
-    int entity, first_page, joined, large;
-};
-
-__device__ __forceinline__ int splits_of(int pages, int part) { return pages <= part ? 1 : min((pages + part - 1) / part, kMaxSplit); }
-
-// The task of index x into *found (its entity -1 where there is none).
-__device__ __forceinline__ void find_task(const SharedParams &p, int x, Found *found)
-{
-    __shared__ float works[4];
-    __shared__ int counts[4];
-    const int tid = threadIdx.x, all = p.groups + p.b.sequences;
-    Entity n = entity_of(p, tid);
+    __shared__ float works[kPlanWaves];
+    __shared__ int totals[3][kPlanWaves];
+    __shared__ int upto[3][kPlanThreads];  // large tasks, small ones, joins, up to a span's last
+    __shared__ Entity spans[kPlanThreads];
+    __shared__ int splits[kPlanThreads];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, all = p.groups + p.b.sequences;
+    Entity n{};
     float work = 0.0f;
-    for (int e0 = 0;;) {
-        work = work + float(n.tiles) * float(n.pages);
-        e0 += 256;
-        if (e0 >= all) break;
+    for (int e0 = 0; e0 < all; e0 += kPlanThreads) {
         n = entity_of(p, e0 + tid);
-    }
-    // (a little more than a share: the sum is in f32)
-    const float share = block_sum(work, works) * 1.00001f / float(p.target) + 1.0f;
-    const int part = share < float(kMinPages) ? kMinPages : share > 1e9f ? 1000000000 : int(share);
-    auto units = [&]() { return n.tiles ? n.tiles * splits_of(n.pages, part) : 0; };
-    // the tasks of large tiles come first
-    int large = 0;
-    for (int e0 = 0; e0 < all; e0 += 256) {
-        if (all > 256) n = entity_of(p, e0 + tid);
-        large += n.large ? units() : 0;
-    }
-    large = block_sum(large, counts);
-    const bool is_large = x < large;
-    const int index = is_large ? x : x - large;
-    if (tid == 0) found->entity = -1;
-    int before = 0;
-    for (int e0 = 0; e0 < all; e0 += 256) {
-        if (all > 256) n = entity_of(p, e0 + tid);
-        const int mine = n.large == is_large ? units() : 0;
-        int total;
-        const int upto = wave_scan(mine, &total);
-        __syncthreads();
-        if ((tid & 63) == 0) counts[tid >> 6] = total;
-        __syncthreads();
-        int start = before + upto - mine;
-        for (int w = 0; w < (tid >> 6); w++) start += counts[w];
-        before += counts[0] + counts[1] + counts[2] + counts[3];
-        const int within = index - start;
-        if (within >= 0 && within < mine) {
-            const int nsplit = splits_of(n.pages, part);
-            Task t{};
-            t.seq = e0 + tid < p.groups ? sequence_index(p, p.starts[e0 + tid]) : e0 + tid - p.groups;
-            t.tile = n.tiles - 1 - within / nsplit;
-            t.split = within % nsplit;
-            t.nsplit = nsplit;
-            t.slot = index;
-            t.span = n.span;
-            *found = Found{t, e0 + tid, n.first_page, n.joined, n.large};
+        work = work + float(n.tiles) * float(n.pages) * (n.large ? float(kLargeCost) : 1.0f);
+        // the rows' sequences and positions: a lane its own few, the wave those of one with many after the other
+        const int s = e0 + tid - p.groups, rows = s >= 0 ? n.span.rows : 0;
+        for (int r = 0; r < min(rows, 4); r++) p.rows_of[n.span.begin + r] = RowNote{s, n.span.first + r};
+        unsigned long long many = __ballot(rows > 4);
+        while (many) {
+            const int l = __builtin_ctzll(many);
+            many &= many - 1;
+            const int count = __builtin_amdgcn_readlane(rows, l), begin = __builtin_amdgcn_readlane(n.span.begin, l);
+            const int first = __builtin_amdgcn_readlane(n.span.first, l), sequence = __builtin_amdgcn_readlane(s, l);
+            for (int r = 4 + lane; r < count; r += 64) p.rows_of[begin + r] = RowNote{sequence, first + r};
         }
-        if (before > index) break;
     }
+    work = wave_allsum(work);
+    if (lane == 0) works[wave] = work;
     __syncthreads();
+    work = 0.0f;
+    for (int w = 0; w < kPlanWaves; w++) work = work + works[w];
+    // (a little more than a share: the sum is in f32)
+    const float share = work * 1.00001f / float(p.target);
+    auto pages_of = [&](float share, int least) { return share + 1.0f < float(least) ? least : share > 1e9f ? 1000000000 : int(share + 1.0f); };
+    const int large_part = pages_of(share / float(kLargeCost), kLargePages), small_part = pages_of(share / 4.0f, kSmallPages);
+    int done[3] = {0, 0, 0};
+    for (int e0 = 0; e0 < all; e0 += kPlanThreads) {
+        if (all > kPlanThreads) n = entity_of(p, e0 + tid);
+        const int part = n.large ? large_part : small_part;
+        const int nsplit = n.pages <= part ? 1 : min((n.pages + part - 1) / part, kSharedSplit);
+        const int units = n.tiles * nsplit;
+        const bool whole = !n.shared && !n.joined && !n.large && nsplit == 1;
+        const int pairs = n.span.rows * p.group;
+        const int joins = n.tiles == 0 || (!n.shared && n.joined) || whole ? 0 : n.large ? (pairs + 31) / 32 : n.tiles;
+        int mine[3] = {n.large ? units : 0, n.large ? 0 : units, joins}, sums[3];
+        __syncthreads();  // (what the last round read is read)
+        for (int k = 0; k < 3; k++) {
+            sums[k] = wave_scan(mine[k], &totals[k][wave]);
+        }
+        __syncthreads();
+        int ends[3];
+        for (int k = 0; k < 3; k++) {
+            int before = 0, total = 0;
+            for (int w = 0; w < kPlanWaves; w++) {
+                before += w < wave ? totals[k][w] : 0;
+                total += totals[k][w];
+            }
+            sums[k] += before;
+            upto[k][tid] = sums[k];
+            ends[k] = total;
+        }
+        spans[tid] = n;
+        splits[tid] = nsplit;
+        const int s = e0 + tid - p.groups;
+        if (s >= 0 && s < p.b.sequences) {
+            const int k = n.large ? 0 : 1;
+            p.notes_of[s] = SequenceNote{done[k] + sums[k] - mine[k], n.span.begin, n.tiles, nsplit | (n.large ? kLarge : 0)};
+        }
+        __syncthreads();
+        // the span that has unit u, and the unit within it
+        auto find = [&](const int (&upto)[kPlanThreads], int u, int *within) {
+            int lo = 0;  // the first whose upto is past u
+            for (int step = kPlanThreads / 2; step; step >>= 1)
+                if (upto[lo + step - 1] <= u) lo += step;
+            *within = u - (lo ? upto[lo - 1] : 0);
+            return lo;
+        };
+        for (int k = 0; k < 2; k++) {
+            TaskRecord *tasks = k == 0 ? p.large_tasks : p.small_tasks;
+            const int room = (k == 0 ? p.large_slots : p.small_slots) - done[k];
+            for (int u = tid; u < min(ends[k], room); u += kPlanThreads) {
+                int within;
+                const int i = find(upto[k], u, &within);
+                const Entity &e = spans[i];
+                TaskRecord t{};
+                t.table = e.table;
+                t.nsplit = splits[i];
+                t.tile = e.tiles - 1 - within / t.nsplit;  // the last tiles see the most keys: they come first
+                t.split = within % t.nsplit;
+                t.begin = e.span.begin;
+                t.rows = e.span.rows;
+                t.first = e.span.first;
+                t.lo = e.lo;
+                t.hi = e.hi;
+                t.shared = e.shared;
+                t.whole = !e.shared && !e.joined && !e.large && t.nsplit == 1;
+                tasks[done[k] + u] = t;
+            }
+        }
+        for (int u = tid; u < min(ends[2], p.join_slots - done[2]); u += kPlanThreads) {
+            int within;
+            const int i = find(upto[2], u, &within);
+            const Entity &e = spans[i];
+            const int k = e.large ? 0 : 1, tile = e.large ? within / 4 : within;
+            JoinRecord j{};
+            j.begin = e.span.begin;
+            j.rows = e.span.rows;
+            j.pair = within * (e.large ? 32 : 16);
+            j.parts = splits[i];
+            j.slot = done[k] + (i ? upto[k][i - 1] : 0) + (e.tiles - 1 - tile) * j.parts;
+            j.wave = e.large ? within % 4 : -1;
+            j.shared = e.shared;
+            p.joins[done[2] + u] = j;
+        }
+        for (int k = 0; k < 3; k++) done[k] += ends[k];
+    }
+    // (more tasks than there is room for are those of a batch whose starts fall)
+    if (tid == 0) *p.header = PlanHeader{min(done[0], p.large_slots), min(done[1], p.small_slots), min(done[2], p.join_slots)};
 }
 
 // ------------------------------------------------------------------------------ the tasks
 
-// The positions of a tile's rows, by the row within the span (those of a group's are its sequences'), and of its pairs.
+// The positions of a tile's rows: one after the other in a sequence, in a group's span its sequences'. A lane's
+// pair has its position in LDS too, from where it is read in every page rather than kept.
 struct InTile {
-    const int *positions, *pairs;
-    int row0, low, high;
-    __device__ __forceinline__ int of(int at) const { return positions[at - row0]; }
+    const RowNote *rows;  // null: a sequence's
+    int first, low, high;
+    const int *pairs;
+    __device__ __forceinline__ int of(int at) const { return rows ? rows[at].position : first + at; }
     __device__ __forceinline__ int again(const Pair &, int pair) const { return pairs[pair]; }
 };
 
-constexpr int kTileRows = 129;  // that 128 pairs lie in, at most
+// The least and the largest of the wave's values.
+__device__ __forceinline__ void wave_ends(int v, int &low, int &high)
+{
+    low = high = v;
+#pragma unroll
+    for (int step = 32; step; step >>= 1) {
+        low = min(low, __shfl_xor(low, step));
+        high = max(high, __shfl_xor(high, step));
+    }
+    low = __builtin_amdgcn_readfirstlane(low), high = __builtin_amdgcn_readfirstlane(high);
+}
 
-template <int DP>
-constexpr size_t shared_lds() { return many_lds<DP>() > sizeof(FewJoin<DP>) ? many_lds<DP>() : sizeof(FewJoin<DP>); }
+// The pages of a task: of those from lo to hi that rows at positions low to high see, its part.
+__device__ __forceinline__ PageRange part_of(const TaskRecord &t, int low, int high, int window)
+{
+    PageRange r;
+    r.hi = min(t.hi, high < 0 ? 0 : high / kPage + 1);
+    r.lo = min(max(first_seen(low, window) / kPage, t.lo), r.hi);
+    const int n = (r.hi - r.lo + t.nsplit - 1) / t.nsplit;
+    r.lo = min(r.lo + t.split * n, r.hi);
+    r.hi = min(r.lo + n, r.hi);
+    r.lo = __builtin_amdgcn_readfirstlane(r.lo), r.hi = __builtin_amdgcn_readfirstlane(r.hi);
+    return r;
+}
 
-// A workgroup a task and key head.
+// A workgroup a large task and key head, or a wave a small one and key head.
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(SharedParams p)
 {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ Found found;
-    __shared__ int positions[kTileRows + 3], pair_positions[128];
-    const int tid = threadIdx.x, lane = tid & 63, kv = int(blockIdx.x % unsigned(p.kv_heads));
-    find_task(p, int(blockIdx.x / unsigned(p.kv_heads)), &found);
-    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const int entity = same(found.entity);
-    if (entity < 0) return;  // the whole workgroup
-    const Task task = uniform(found.task);
-    const bool large = same(found.large), own = entity >= p.groups, joined = same(found.joined);
-    const int first_page = same(found.first_page), tm = large ? 128 : 16;
-    if (task.slot >= (large ? p.large_slots : p.small_slots)) return;  // (starts that fall: more tiles than the rows have)
-    // the tile's rows, within the span
-    const int row0 = task.tile * tm / p.group, row1 = min((task.tile * tm + tm - 1) / p.group, task.span.rows - 1);
-    // (a large tile always leaves parts: what its lanes would need to find their outputs does not fit their registers)
-    const bool direct = own && !joined && task.nsplit == 1 && !large;
-    if (kv == 0 && task.split == 0) {
-        // rows whose first pair lies in the tile
-        const int parts = direct ? 0 : task.nsplit | (large ? kLargeTiles : 0) | (joined ? kAfterShared : 0);
-        const int tiles = (task.span.rows * p.group + tm - 1) / tm, base = task.slot - (tiles - 1 - task.tile) * task.nsplit;
-        for (int r = row0 + tid; r <= row1; r += 256)
-            if (r * p.group >= task.tile * tm) (own ? p.own : p.shared)[task.span.begin + r] = RowNote{base, task.span.begin, tiles, parts};
-    }
+    __shared__ int pair_positions[128];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const PlanHeader header = *p.header;
+    const unsigned large_blocks = unsigned(header.large) * unsigned(p.kv_heads);
+    const bool large = blockIdx.x < large_blocks;
+    const unsigned unit = large ? blockIdx.x : (blockIdx.x - large_blocks) * 4 + unsigned(wave);
+    const int index = int(unit / unsigned(p.kv_heads)), kv = int(unit % unsigned(p.kv_heads));
+    if (!large && index >= header.small) return;  // the wave
+    const TaskRecord t = (large ? p.large_tasks : p.small_tasks)[index];
+    Task task{};
+    task.seq = t.table;
+    task.tile = t.tile;
+    task.nsplit = t.nsplit;
+    task.span = Span{t.begin, t.rows, t.first, 0};
+    task = uniform(task);
     const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
-    if (own) {
-        for (int i = tid; i <= row1 - row0; i += 256) positions[i] = task.span.first + row0 + i;
-    } else {
-        for (int i = tid; i <= row1 - row0; i += 256) positions[i] = -1;
-        __syncthreads();
-        const int begin = sequence_index(p, p.starts[entity]), end = sequence_index(p, p.starts[entity + 1]);
-        for (int s = begin + tid; s < end; s += 256) {
-            const Span span = sequence_span(p.b, s);
-            const int from = max(span.begin, task.span.begin + row0), to = min(span.begin + span.rows - 1, task.span.begin + row1);
-            for (int r = from; r <= to; r++) positions[r - task.span.begin - row0] = span.first + (r - span.begin);
-        }
-    }
-    __syncthreads();
-    // (past the pairs the last again)
-    const int pairs = task.span.rows * p.group;
-    if (tid < tm) pair_positions[tid] = positions[min(task.tile * tm + tid, pairs - 1) / p.group - row0];
-    __syncthreads();
-    // the first and last position of the tile, and of a wave's pairs
-    auto ends = [&](int first, int last, int &low, int &high) {
-        low = INT_MAX, high = INT_MIN;
-        for (int i = first + lane; i < last; i += 64) {
-            low = min(low, pair_positions[i]);
-            high = max(high, pair_positions[i]);
-        }
-#pragma unroll
-        for (int step = 32; step; step >>= 1) {
-            low = min(low, __shfl_xor(low, step));
-            high = max(high, __shfl_xor(high, step));
-        }
-        low = same(low), high = same(high);
-    };
-    InTile places{positions, pair_positions, row0, 0, 0};
-    ends(0, tm, places.low, places.high);
-    PageRange range;
-    range.lo = own ? first_page : 0;
-    range.hi = own ? p.b.max_pages : shared_pages(p, p.counts[entity]);
-    range.hi = min(range.hi, places.high < 0 ? 0 : places.high / kPage + 1);
-    range.lo = min(max(first_seen(places.low, p.window) / kPage, range.lo), range.hi);
-    const int n = (range.hi - range.lo + task.nsplit - 1) / task.nsplit;
-    range.lo = min(range.lo + task.split * n, range.hi);
-    range.hi = same(min(range.lo + n, range.hi)), range.lo = same(range.lo);
+    InTile places{t.shared ? p.rows_of + t.begin : nullptr, t.first, 0, 0, pair_positions};
+    const int pairs = t.rows * p.group, tm = large ? 128 : 16;
+    auto position = [&](int pair) { return places.of(min(t.tile * tm + pair, pairs - 1) / p.group); };
     if (large) {
-        ends(same(tid >> 6) * 32, same(tid >> 6) * 32 + 32, places.low, places.high);
-        float *parts = p.partial + (size_t(task.slot) * p.kv_heads + kv) * 4 * many_floats(DP);
+        const int mine = position(wave * 32 + (lane & 31));
+        if (lane < 32) pair_positions[wave * 32 + lane] = mine;
+        __syncthreads();
+        int low, high;
+        wave_ends(min(pair_positions[lane], pair_positions[64 + lane]), low, high);
+        int other;
+        wave_ends(max(pair_positions[lane], pair_positions[64 + lane]), other, high);
+        const PageRange range = part_of(t, low, high, p.window);
+        wave_ends(mine, places.low, places.high);
+        float *parts = p.partial + size_t(blockIdx.x) * 4 * many_floats(DP);
         __builtin_assume(parts != nullptr);
         attend_many<DP>(p, task, range, table, kv, places, lds, parts);
     } else {
-        float *part = direct ? nullptr : p.small_partial + (size_t(task.slot) * p.kv_heads + kv) * few_floats(DP);
-        attend_few<DP>(p, task, range, table, kv, places, *reinterpret_cast<FewJoin<DP> *>(lds), part);
+        wave_ends(position(lane & 15), places.low, places.high);
+        const PageRange range = part_of(t, places.low, places.high, p.window);
+        attend_few<DP, 1>(p, task, range, table, kv, places, static_cast<FewJoin<DP> *>(nullptr),
+                          t.whole ? nullptr : p.small_partial + size_t(unit) * few_floats(DP));
     }
 }
 
 // ------------------------------------------------------------------------------- the join
 
-// A row and head's parts, one after the other: those over the shared pages, then its own.
-struct Parts {
-    const float *at;  // the first one's
-    size_t step;
-    int count;
-    int sums, values;  // where in a part this lane's reference and four values are (the totals 64 behind the references)
+struct Sums {
+    float r, total;
+    v4f o;
 };
 
-template <int DP>
-__device__ __forceinline__ Parts parts_of(const SharedParams &p, const RowNote &note, int row, int kv, int in_group, int quad)
+__device__ __forceinline__ void add_sums(Sums &to, const Sums &from)
 {
-    const bool large = note.parts & kLargeTiles;
-    Parts r{};
-    r.count = note.parts & (kLargeTiles - 1);
-    // (64 bits and every check, for the notes of a batch whose starts fall may hold anything)
-    const int64_t m = (int64_t(row) - note.begin) * p.group + in_group, tm = large ? 128 : 16, tile = m / tm;
-    int64_t slot = note.base + (note.tiles - 1 - tile) * r.count;
-    if (r.count > kMaxSplit || m < 0 || tile >= note.tiles || slot < 0 || slot + r.count > (large ? p.large_slots : p.small_slots))
-        r.count = 0, slot = 0;
-    const int pair = int(m & (tm - 1));
-    if (large) {
-        r.at = p.partial + ((size_t(slot) * p.kv_heads + kv) * 4 + pair / 32) * many_floats(DP);
-        r.step = size_t(p.kv_heads) * 4 * many_floats(DP);
-        r.sums = pair % 32;
-        r.values = 128 + (quad / 2) * 256 + (pair % 32 + 32 * (quad & 1)) * 4;
-    } else {
-        r.at = p.small_partial + (size_t(slot) * p.kv_heads + kv) * few_floats(DP);
-        r.step = size_t(p.kv_heads) * few_floats(DP);
-        r.sums = pair;
-        r.values = 128 + (quad / 4) * 256 + (pair + 16 * (quad & 3)) * 4;
-    }
-    return r;
+    const float r = fmaxf(to.r, from.r);
+    const float a = part_factor(to.r, r), b = part_factor(from.r, r);
+    to.r = r;
+    to.total = to.total * a + from.total * b;
+#pragma unroll
+    for (int e = 0; e < 4; e++) to.o[e] = to.o[e] * a + from.o[e] * b;
 }
 
-struct Joined {
-    float r = -INFINITY, total = 0.0f;
-    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-};
-
-__device__ __forceinline__ void join_parts(Joined &j, const Parts &parts)
+// `count` parts, from the one at `part` on, `step` floats apart: the row's sums are at `row` in each, the four values at `values`.
+__device__ __forceinline__ void add_parts(Sums &to, const float *part, size_t step, int count, int row, int values)
 {
     constexpr int kAhead = 8;
-    for (int s0 = 0; s0 < parts.count; s0 += kAhead) {
-        float rs[kAhead], totals[kAhead];
-        v4f os[kAhead];
+    for (int s0 = 0; s0 < count; s0 += kAhead) {
+        Sums from[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const float *from = parts.at + size_t(min(s0 + i, parts.count - 1)) * parts.step;
-            rs[i] = from[parts.sums];
-            totals[i] = from[64 + parts.sums];
-            os[i] = *reinterpret_cast<const v4f *>(from + parts.values);
+            const float *at = part + size_t(min(s0 + i, count - 1)) * step;
+            from[i] = Sums{at[row], at[64 + row], *reinterpret_cast<const v4f *>(at + values)};
         }
-        float top = j.r;
+        float top = to.r;
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) top = s0 + i < parts.count ? fmaxf(top, rs[i]) : top;
-        const float a = part_factor(j.r, top);
-        j.r = top;
-        j.total = j.total * a;
+        for (int i = 0; i < kAhead; i++) top = s0 + i < count ? fmaxf(top, from[i].r) : top;
+        const float a = part_factor(to.r, top);
+        to.r = top;
+        to.total = to.total * a;
 #pragma unroll
-        for (int e = 0; e < 4; e++) j.o[e] = j.o[e] * a;
+        for (int e = 0; e < 4; e++) to.o[e] = to.o[e] * a;
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            if (s0 + i >= parts.count) continue;
-            const float b = part_factor(rs[i], top);
-            j.total = j.total + totals[i] * b;
+            if (s0 + i >= count) continue;
+            const float b = part_factor(from[i].r, top);
+            to.total = to.total + from[i].total * b;
 #pragma unroll
-            for (int e = 0; e < 4; e++) j.o[e] = j.o[e] + os[i][e] * b;
+            for (int e = 0; e < 4; e++) to.o[e] = to.o[e] + from[i].o[e] * b;
         }
     }
 }
 
-// A team of lanes a row and query head, four dimensions a lane.
+// A workgroup a join, key head and kilobyte of a part: lane l has a pair and four dimensions, as the tasks left them, so that
+// parts are read whole lines at a time. Its waves take the parts in turn, but one the rows' own where these are apart.
 template <int DP>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedParams p)
 {
-    constexpr int kTeam = DP == 32 ? 8 : DP == 64 ? 16 : DP <= 128 ? 32 : 64;
-    const int quad = threadIdx.x & (kTeam - 1);
-    const int first = p.b.row_starts[0], last = min(p.b.row_starts[p.b.sequences], p.b.rows);
-    const unsigned units = unsigned(p.b.rows) * unsigned(p.heads);
-    for (unsigned unit = blockIdx.x * (256 / kTeam) + threadIdx.x / kTeam; unit < units; unit += gridDim.x * (256 / kTeam)) {
-        const int row = int(unit / unsigned(p.heads)), head = int(unit % unsigned(p.heads));
-        if (row < first || row >= last || 4 * quad >= p.head_dim) continue;
-        const RowNote own = p.own[row];
-        if ((own.parts & (kLargeTiles - 1)) == 0) continue;
-        const int kv = head / p.group, in_group = head - kv * p.group;
-        Joined j;
-        if (own.parts & kAfterShared) join_parts(j, parts_of<DP>(p, p.shared[row], row, kv, in_group, quad));
-        join_parts(j, parts_of<DP>(p, own, row, kv, in_group, quad));
-        v4f x;
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = j.total == 0.0f ? 0.0f : j.o[e] / j.total;
-        *reinterpret_cast<v4f_any *>(p.out + size_t(row) * p.out_stride + size_t(head) * p.head_dim + 4 * quad) = x;
+    __shared__ Sums sums[4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int index = int(blockIdx.x / unsigned(p.kv_heads)), kv = int(blockIdx.x % unsigned(p.kv_heads)), piece = int(blockIdx.y);
+    if (index >= p.header->joins) return;  // the workgroup
+    const JoinRecord j = p.joins[index];
+    const bool large = j.wave >= 0;
+    const int rows = large ? 32 : 16;
+    if (piece >= rows * DP / 256) return;
+    const int pair = j.pair + (lane & (rows - 1)), dim = piece * (256 / rows) + 4 * (lane / rows);
+    const bool live = pair < j.rows * p.group && dim < p.head_dim;
+    const int at = min(pair, j.rows * p.group - 1) / p.group, row = j.begin + at, in_group = min(pair, j.rows * p.group - 1) - at * p.group;
+    Sums mine{-INFINITY, 0.0f, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+    const int others = j.shared ? 3 : 4;
+    if (wave < others) {
+        const size_t floats = large ? many_floats(DP) : few_floats(DP), task = large ? 4 * floats : floats;
+        const float *part = (large ? p.partial : p.small_partial) + (size_t(j.slot + wave) * p.kv_heads + kv) * task + (large ? j.wave * floats : 0);
+        const int count = (j.parts - wave + others - 1) / others;
+        if (wave < j.parts) add_parts(mine, part, size_t(others) * p.kv_heads * task, count, lane, 128 + piece * 256 + lane * 4);
+    } else {
+        // (64 bits and every check: a row that no sequence holds, of a batch whose starts fall, may have any note)
+        const int s = p.rows_of[row].sequence;
+        const SequenceNote note = p.notes_of[s >= 0 && s < p.b.sequences ? s : 0];
+        const bool own_large = note.parts & kLarge;
+        const int tm = own_large ? 128 : 16, parts = note.parts & (kLarge - 1);
+        const int64_t m = (int64_t(row) - note.begin) * p.group + in_group, tile = m / tm;
+        const int64_t slot = note.base + (note.tiles - 1 - tile) * parts;
+        const bool there = live && m >= 0 && tile < note.tiles && parts <= kSharedSplit && slot >= 0 &&
+                           slot + parts <= (own_large ? p.large_slots : p.small_slots);
+        const int q = dim / 4, own = int(m & (tm - 1));
+        const size_t floats = own_large ? many_floats(DP) : few_floats(DP), task = own_large ? 4 * floats : floats;
+        const float *part = (own_large ? p.partial : p.small_partial);
+        if (there) {
+            part += (size_t(slot) * p.kv_heads + kv) * task + (own_large ? own / 32 * floats : 0);
+            if (own_large) add_parts(mine, part, p.kv_heads * task, parts, own % 32, 128 + (q / 2) * 256 + (own % 32 + 32 * (q & 1)) * 4);
+            else add_parts(mine, part, p.kv_heads * task, parts, own, 128 + (q / 4) * 256 + (own + 16 * (q & 3)) * 4);
+        }
     }
+    sums[wave][lane] = mine;
+    __syncthreads();
+    if (wave != 0 || !live) return;
+#pragma unroll
+    for (int w = 1; w < 4; w++) add_sums(mine, sums[w][lane]);
+    v4f x;
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = mine.total == 0.0f ? 0.0f : mine.o[e] / mine.total;
+    *reinterpret_cast<v4f_any *>(p.out + size_t(row) * p.out_stride + size_t(kv * p.group + in_group) * p.head_dim + dim) = x;
 }
 
 // ------------------------------------------------------------------------------- the host
 
 struct Launch {
     bool shared;  // or each sequence by itself
-    int limit;
-    size_t large_slots, small_slots, grid;  // a key head's
-    int target;
-    size_t note_bytes, large_bytes, small_bytes;
-    size_t bytes() const { return 2 * note_bytes + large_bytes + small_bytes; }
+    int limit, target;
+    size_t large_slots, small_slots, join_slots, blocks;  // of a key head but the blocks
+    size_t at[8];  // where in the scratch the arrays are, and its size
 };
-
-size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads)
 {
@@ -386,40 +448,46 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, s
     if (!l.shared) return l;
     const size_t units = std::max<size_t>(kUnits / c->kv_heads, 1);
     l.target = int((c->padded <= 128 ? 2 : 1) * units);
-    // spans of n pairs have at most n / 128 + 1 large tiles, n / 16 + 1 small ones; the parts beyond a tile's first are the target
+    // spans of n pairs have at most n / 128 + 1 large tiles, or n / 16 + 1 small ones; what a share of the target
+    // leaves of the work are its tiles' further parts, of small tiles four times as many
     size_t large = 0, small = 0;
     for (size_t spans : {groups, sequences}) {
         large += pairs > size_t(l.limit) ? pairs / 128 + std::min(spans, pairs / (l.limit + 1)) : 0;
         small += std::min(pairs / 16 + spans, size_t(l.limit / 16) * spans);
     }
     l.large_slots = large ? large + l.target : 0;
-    l.small_slots = small + l.target;
-    l.grid = large + small + l.target;
-    l.note_bytes = up(b->rows * sizeof(RowNote));
-    l.large_bytes = up(l.large_slots * c->kv_heads * 4 * many_floats(c->padded) * 4);
-    l.small_bytes = up(l.small_slots * c->kv_heads * few_floats(c->padded) * 4);
+    l.small_slots = small + 4 * l.target;
+    l.join_slots = 4 * large + small;
+    l.blocks = l.large_slots * c->kv_heads + (l.small_slots * c->kv_heads + 3) / 4;
+    const size_t floats = 4 * size_t(many_floats(c->padded));
+    const size_t bytes[7] = {sizeof(PlanHeader), l.large_slots * sizeof(TaskRecord), l.small_slots * sizeof(TaskRecord),
+                             l.join_slots * sizeof(JoinRecord), b->sequences * sizeof(SequenceNote), b->rows * sizeof(RowNote),
+                             l.large_slots * c->kv_heads * floats * 4};
+    for (int i = 0; i < 7; i++) l.at[i + 1] = l.at[i] + (bytes[i] + 255) / 256 * 256;
     return l;
 }
+
+size_t scratch_of(const fg_cache *c, const Launch &l) { return l.at[7] + l.small_slots * c->kv_heads * few_floats(c->padded) * 4; }
 
 template <int DP>
 int launch_shared(const SharedParams &p, const Launch &l, hipStream_t s)
 {
-    if (shared_lds<DP>() > 60 * 1024) {  // more than the default limit, with what the plan takes: raised once a device
+    if (many_lds<DP>() > 60 * 1024) {  // more than the default limit, with the positions: raised once a device
         static std::atomic<unsigned long long> raised{0};
         int device = 0;
         FG_HIP(hipGetDevice(&device));
         const unsigned long long bit = 1ull << (device & 63);
         if (device > 63 || !(raised.load() & bit)) {
             FG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(shared_tasks_kernel<DP>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       int(shared_lds<DP>())));
+                                       int(many_lds<DP>())));
             raised.fetch_or(bit);
         }
     }
-    shared_tasks_kernel<DP><<<unsigned(p.kv_heads * l.grid), 256, shared_lds<DP>(), s>>>(p);
+    shared_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
     FG_HIP(hipGetLastError());
-    constexpr int kTeam = DP == 32 ? 8 : DP == 64 ? 16 : DP <= 128 ? 32 : 64;
-    const size_t units = size_t(p.b.rows) * p.heads, grid = (units + 256 / kTeam - 1) / (256 / kTeam);
-    shared_join_kernel<DP><<<unsigned(std::min(grid, size_t(1) << 20)), 256, 0, s>>>(p);
+    shared_tasks_kernel<DP><<<unsigned(l.blocks), 256, many_lds<DP>(), s>>>(p);
+    FG_HIP(hipGetLastError());
+    shared_join_kernel<DP><<<dim3(unsigned(l.join_slots * p.kv_heads), DP / 8), 256, 0, s>>>(p);
     FG_HIP(hipGetLastError());
     return FG_OK;
 }
@@ -441,7 +509,7 @@ extern "C" size_t fg_cache_attend_shared_scratch(const fg_cache *c, const fg_bat
 {
     if (!c || !b || !f || !heads || heads % c->kv_heads) return 0;
     const Launch l = plan_launch(c, b, f, heads);
-    return l.shared ? l.bytes() : fg_cache_attend_scratch(c, b, heads);
+    return l.shared ? scratch_of(c, l) : fg_cache_attend_scratch(c, b, heads);
 }
 
 extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, const float *query, size_t query_stride,
@@ -457,12 +525,12 @@ extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, cons
     const Launch l = plan_launch(c, b, f, heads);
     if (!l.shared)
         return fg_cache_attend(c, b, query, query_stride, heads, scale, window, out, out_stride, scratch, scratch_bytes, stream);
-    if (l.grid * c->kv_heads > kMaxGrid || b->rows * heads > 0xf0000000)
+    if (l.blocks > kMaxGrid || l.join_slots * c->kv_heads > kMaxGrid)
         return set_error(FG_ERR_SHAPE, std::string(who) + ": more sequences times heads than a launch takes");
     const hipStream_t s = as_stream(stream);
     void *ws = nullptr;
     bool owned = false;
-    rc = stream_scratch(scratch, scratch_bytes, l.bytes(), who, s, &ws, &owned);
+    rc = stream_scratch(scratch, scratch_bytes, scratch_of(c, l), who, s, &ws, &owned);
     if (rc) return rc;
     SharedParams p = attend_params<SharedParams>(c, b, query, query_stride, heads, scale, window, out, out_stride);
     p.starts = f->starts;
@@ -472,11 +540,16 @@ extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, cons
     p.target = l.target;
     p.large_slots = int(l.large_slots);
     p.small_slots = int(l.small_slots);
+    p.join_slots = int(l.join_slots);
     char *at = static_cast<char *>(ws);
-    p.own = reinterpret_cast<RowNote *>(at);
-    p.shared = reinterpret_cast<RowNote *>(at + l.note_bytes);
-    p.partial = reinterpret_cast<float *>(at + 2 * l.note_bytes);
-    p.small_partial = reinterpret_cast<float *>(at + 2 * l.note_bytes + l.large_bytes);
+    p.header = reinterpret_cast<PlanHeader *>(at);
+    p.large_tasks = reinterpret_cast<TaskRecord *>(at + l.at[1]);
+    p.small_tasks = reinterpret_cast<TaskRecord *>(at + l.at[2]);
+    p.joins = reinterpret_cast<JoinRecord *>(at + l.at[3]);
+    p.notes_of = reinterpret_cast<SequenceNote *>(at + l.at[4]);
+    p.rows_of = reinterpret_cast<RowNote *>(at + l.at[5]);
+    p.partial = reinterpret_cast<float *>(at + l.at[6]);
+    p.small_partial = reinterpret_cast<float *>(at + l.at[7]);
     switch (c->padded) {
     case 32: rc = launch_shared<32>(p, l, s); break;
     case 64: rc = launch_shared<64>(p, l, s); break;
