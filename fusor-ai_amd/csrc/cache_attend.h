@@ -180,6 +180,64 @@ __device__ __forceinline__ int query_shift(float amax)
     return amax > 0.0f ? min(10 - __builtin_amdgcn_frexp_expf(amax), 126) : 0;
 }
 
+// The operand rows' queries, each split into its two pieces by the lanes that multiply them: `pair` is the pair's place among a
+// key head's of all rows.
+struct RawQueries {
+    template <int DP>
+    __device__ __forceinline__ void few(const AttendParams &p, const Pair &pair, int, int, int g, v8h (&qh)[(DP + 63) / 64][2],
+                                        v8h (&ql)[(DP + 63) / 64][2], float &f) const
+    {
+        constexpr int J = (DP + 63) / 64;
+        const float *row = p.query + size_t(pair.row) * p.query_stride + size_t(pair.head) * p.head_dim;
+        float q[J][2][8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                load8(row, 64 * j + 16 * g + 8 * e, p.head_dim, q[j][e]);
+#pragma unroll
+                for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(q[j][e][k]));
+            }
+        float2 w = row_pair(amax);
+        w = half_pair(fmaxf(w.x, w.y));
+        const int shift = query_shift(fmaxf(w.x, w.y));
+        f = ldexpf(p.scale2, -shift);
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) q[j][e][k] = ldexpf(q[j][e][k], shift);
+                split8(q[j][e], qh[j][e], ql[j][e]);
+            }
+    }
+    template <int DP>
+    __device__ __forceinline__ void many(const AttendParams &p, const Pair &pair, int, int, int h, v8h (&qh)[DP / 16], v8h (&ql)[DP / 16],
+                                         float &f) const
+    {
+        constexpr int K = DP / 16;
+        const float *row = p.query + size_t(pair.row) * p.query_stride + size_t(pair.head) * p.head_dim;
+        float x[K][8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            load8(row, 32 * (k >> 1) + 16 * h + 8 * (k & 1), p.head_dim, x[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[k][e]));
+        }
+        const float2 w = half_pair(amax);
+        const int shift = query_shift(fmaxf(w.x, w.y));
+        f = ldexpf(p.scale2, -shift);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[k][e] = ldexpf(x[k][e], shift);
+            split8(x[k], qh[k], ql[k]);
+        }
+    }
+};
+
 constexpr float kWeightLimit = 32768.0f;
 // Where a value's scale is under kSmallScale 2^(t - r) is looked at too: 2^25 of up to 2^102 stay in f32's range.
 constexpr float kSmallScale = 0x1p-82f, kAloneLimit = 102.0f;
@@ -300,9 +358,9 @@ template <int DP>
 struct FewJoin {  // the waves' sums on their way to each other
     float sums[2][DP / 16 * 4 + 2][64];
 };
-template <int DP, int WAVES, class Places>
+template <int DP, int WAVES, class Places, class Queries>
 __device__ __forceinline__ void attend_few(const AttendParams &p, const Task &task, const PageRange range, const int32_t *table, int kv,
-                                           const Places &places, FewJoin<DP> *join, float *part)
+                                           const Places &places, const Queries &queries, FewJoin<DP> *join, float *part)
 {
     constexpr int TM = 16, J = (DP + 63) / 64, T = DP / 16, R = DP / 32;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -310,31 +368,7 @@ __device__ __forceinline__ void attend_few(const AttendParams &p, const Task &ta
     const Pair pair = pair_of(p, task, kv, task.tile * TM + i, places);
     v8h qh[J][2], ql[J][2];
     float f;
-    {
-        const float *row = p.query + size_t(pair.row) * p.query_stride + size_t(pair.head) * p.head_dim;
-        float q[J][2][8];
-        float amax = 0.0f;
-#pragma unroll
-        for (int j = 0; j < J; j++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                load8(row, 64 * j + 16 * g + 8 * e, p.head_dim, q[j][e]);
-#pragma unroll
-                for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(q[j][e][k]));
-            }
-        float2 w = row_pair(amax);
-        w = half_pair(fmaxf(w.x, w.y));
-        const int shift = query_shift(fmaxf(w.x, w.y));
-        f = ldexpf(p.scale2, -shift);
-#pragma unroll
-        for (int j = 0; j < J; j++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) q[j][e][k] = ldexpf(q[j][e][k], shift);
-                split8(q[j][e], qh[j][e], ql[j][e]);
-            }
-    }
+    queries.template few<DP>(p, pair, kv, task.span.begin * p.group + min(task.tile * TM + i, task.span.rows * p.group - 1), g, qh, ql, f);
     RowSums sums{-INFINITY, 0.0f};
     v4f o[T];
 #pragma unroll
@@ -496,9 +530,9 @@ constexpr size_t many_lds() { return size_t(2) * (256 * DP + 2 * kPage * 4); }
 // The tile's sums over the pages `range` of `table`, to `parts`, four of them, or where that is null divided to the output.
 // `places` are those of the wave's pairs.
 constexpr int many_floats(int DP) { return 32 * DP + 128; }  // of a wave's part
-template <int DP, class Places>
+template <int DP, class Places, class Queries>
 __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &task, const PageRange range, const int32_t *table, int kv,
-                                            const Places &places, uint8_t *lds, float *parts)
+                                            const Places &places, const Queries &queries, uint8_t *lds, float *parts)
 {
     constexpr int TM = 128, K = DP / 16, T = DP / 32, L = DP / 32;  // steps, tiles of 32 dimensions, 16-byte loads a thread
     constexpr int kBuffer = 256 * DP + 2 * kPage * 4;
@@ -539,26 +573,8 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
     const Pair pair = pair_of(p, task, kv, task.tile * TM + wave * 32 + l31, places);
     v8h qh[K], ql[K];
     float f;
-    {
-        const float *row = p.query + size_t(pair.row) * p.query_stride + size_t(pair.head) * p.head_dim;
-        float x[K][8];
-        float amax = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            load8(row, 32 * (k >> 1) + 16 * h + 8 * (k & 1), p.head_dim, x[k]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[k][e]));
-        }
-        const float2 w = half_pair(amax);
-        const int shift = query_shift(fmaxf(w.x, w.y));
-        f = ldexpf(p.scale2, -shift);
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[k][e] = ldexpf(x[k][e], shift);
-            split8(x[k], qh[k], ql[k]);
-        }
-    }
+    queries.template many<DP>(p, pair, kv, task.span.begin * p.group + min(task.tile * TM + wave * 32 + l31, task.span.rows * p.group - 1), h, qh,
+                              ql, f);
     RowSums sums{-INFINITY, 0.0f};
     v16f o[T];
 #pragma unroll

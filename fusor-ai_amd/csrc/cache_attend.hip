@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_few_kernel(Atte
     const int high = task.span.first + min((task.tile * TM + TM - 1) / p.group, task.span.rows - 1);
     float *part = task.nsplit > 1 ? p.partial + (size_t(task.slot) * p.kv_heads + kv) * few_floats(DP) : nullptr;
     attend_few<DP, 4>(p, task, task_pages(p, task, TM), p.b.pages + size_t(task.seq) * p.b.max_pages, kv,
-                      InSequence{task.span.first, low, high}, &join, part);
+                      InSequence{task.span.first, low, high}, RawQueries{}, &join, part);
 }
 
 template <int DP>
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     const int low = task.span.first + min(m0, pairs - 1) / p.group, high = task.span.first + min(m0 + 31, pairs - 1) / p.group;
     float *parts = task.nsplit > 1 ? p.partial + (size_t(task.slot) * p.kv_heads + kv) * 4 * many_floats(DP) : nullptr;
     attend_many<DP>(p, task, task_pages(p, task, TM), p.b.pages + size_t(task.seq) * p.b.max_pages, kv,
-                    InSequence{task.span.first, low, high}, lds, parts);
+                    InSequence{task.span.first, low, high}, RawQueries{}, lds, parts);
 }
 
 // The parts of split tiles joined: per slot where a tile's parts start and head, a wave for each tile of

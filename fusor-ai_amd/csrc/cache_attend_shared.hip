@@ -63,6 +63,8 @@ struct SharedParams : AttendParams {
     SequenceNote *notes_of;  // [sequences]
     RowNote *rows_of;        // [rows]
     float *small_partial;
+    uint4 *pieces;           // [key head][row, query head of it][block of 8 dimensions][2]: the queries' two f16 pieces
+    float *factors;          // [key head][row, query head of it]: of its scores
 };
 
 // What a part takes: at least so many pages, and of the whole work, in units of a small tile's page, a share of the target.
@@ -127,9 +129,86 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, int e)
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
-// A thread a span, 1024 at a time; then a thread a task or join of theirs.
-__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p)
+// The queries split into their two pieces, once for all tasks that multiply them: a team of lanes a row and head, eight
+// dimensions a lane.
+__device__ __forceinline__ void split_queries(const SharedParams &p, int padded)
 {
+    const int blocks = padded / 8;
+    int team = 4;
+    while (team < blocks) team *= 2;
+    const int first = max(0, p.b.row_starts[0]), rows = min(p.b.row_starts[p.b.sequences], p.b.rows) - first;
+    if (rows <= 0) return;
+    const unsigned units = unsigned(rows) * unsigned(p.heads), step = (gridDim.x - 1) * unsigned(kPlanThreads / team);
+    const int block = threadIdx.x & (team - 1);
+    for (unsigned unit = (blockIdx.x - 1) * unsigned(kPlanThreads / team) + threadIdx.x / team; unit < units; unit += step) {  // whole teams
+        const int row = first + int(unit / unsigned(p.heads)), head = int(unit % unsigned(p.heads));
+        float x[8];
+        load8(p.query + size_t(row) * p.query_stride + size_t(head) * p.head_dim, 8 * block, p.head_dim, x);
+        float amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(x[k]));
+        for (int m = 1; m < team; m *= 2) amax = fmaxf(amax, __shfl_xor(amax, m));
+        const int shift = query_shift(amax);
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = ldexpf(x[k], shift);
+        v8h hi, lo;
+        split8(x, hi, lo);
+        const int kv = head / p.group;
+        const size_t pair = (size_t(kv) * p.b.rows + row) * p.group + (head - kv * p.group);
+        if (block < blocks) {
+            p.pieces[(pair * blocks + block) * 2] = __builtin_bit_cast(uint4, hi);
+            p.pieces[(pair * blocks + block) * 2 + 1] = __builtin_bit_cast(uint4, lo);
+        }
+        if (block == 0) p.factors[pair] = ldexpf(p.scale2, -shift);
+    }
+}
+
+struct SplitQueries {
+    const uint4 *pieces;
+    const float *factors;
+    template <int DP>
+    __device__ __forceinline__ void few(const AttendParams &p, const Pair &, int kv, int pair, int g, v8h (&qh)[(DP + 63) / 64][2],
+                                        v8h (&ql)[(DP + 63) / 64][2], float &f) const
+    {
+        const size_t at = size_t(kv) * p.b.rows * p.group + pair;
+        f = factors[at];
+#pragma unroll
+        for (int j = 0; j < (DP + 63) / 64; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int block = 8 * j + 2 * g + e;
+                uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                if (DP % 64 == 0 || block < DP / 8) {
+                    hi = pieces[(at * (DP / 8) + block) * 2];
+                    lo = pieces[(at * (DP / 8) + block) * 2 + 1];
+                }
+                qh[j][e] = __builtin_bit_cast(v8h, hi);
+                ql[j][e] = __builtin_bit_cast(v8h, lo);
+            }
+    }
+    template <int DP>
+    __device__ __forceinline__ void many(const AttendParams &p, const Pair &, int kv, int pair, int h, v8h (&qh)[DP / 16], v8h (&ql)[DP / 16],
+                                         float &f) const
+    {
+        const size_t at = size_t(kv) * p.b.rows * p.group + pair;
+        f = factors[at];
+#pragma unroll
+        for (int k = 0; k < DP / 16; k++) {
+            const size_t block = at * (DP / 8) + 4 * (k >> 1) + 2 * h + (k & 1);
+            qh[k] = __builtin_bit_cast(v8h, pieces[block * 2]);
+            ql[k] = __builtin_bit_cast(v8h, pieces[block * 2 + 1]);
+        }
+    }
+};
+
+// The first workgroup lists the tasks, a thread a span, 1024 at a time, then a thread a task or join of theirs; the others
+// split the queries.
+__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p, int padded)
+{
+    if (blockIdx.x > 0) {
+        split_queries(p, padded);
+        return;
+    }
     __shared__ float works[kPlanWaves];
     __shared__ int totals[3][kPlanWaves];
     __shared__ int upto[3][kPlanThreads];  // large tasks, small ones, joins, up to a span's last
@@ -320,22 +399,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(Sh
         wave_ends(mine, places.low, places.high);
         float *parts = p.partial + size_t(blockIdx.x) * 4 * many_floats(DP);
         __builtin_assume(parts != nullptr);
-        attend_many<DP>(p, task, range, table, kv, places, lds, parts);
+        attend_many<DP>(p, task, range, table, kv, places, SplitQueries{p.pieces, p.factors}, lds, parts);
     } else {
         wave_ends(position(lane & 15), places.low, places.high);
         const PageRange range = part_of(t, places.low, places.high, p.window);
-        attend_few<DP, 1>(p, task, range, table, kv, places, static_cast<FewJoin<DP> *>(nullptr),
+        attend_few<DP, 1>(p, task, range, table, kv, places, SplitQueries{p.pieces, p.factors}, static_cast<FewJoin<DP> *>(nullptr),
                           t.whole ? nullptr : p.small_partial + size_t(unit) * few_floats(DP));
     }
 }
 
 // ------------------------------------------------------------------------------- the join
 
+constexpr int kPieces = 2;  // of a part, a kilobyte each, that a wave has at once
+constexpr int kJoinWaves = 8;
+
 struct Sums {
     float r, total;
-    v4f o;
+    v4f o[kPieces];
 };
 
+// The sums of both in `to`.
 __device__ __forceinline__ void add_sums(Sums &to, const Sums &from)
 {
     const float r = fmaxf(to.r, from.r);
@@ -343,19 +426,25 @@ __device__ __forceinline__ void add_sums(Sums &to, const Sums &from)
     to.r = r;
     to.total = to.total * a + from.total * b;
 #pragma unroll
-    for (int e = 0; e < 4; e++) to.o[e] = to.o[e] * a + from.o[e] * b;
+    for (int i = 0; i < kPieces; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) to.o[i][e] = to.o[i][e] * a + from.o[i][e] * b;
 }
 
-// `count` parts, from the one at `part` on, `step` floats apart: the row's sums are at `row` in each, the four values at `values`.
-__device__ __forceinline__ void add_parts(Sums &to, const float *part, size_t step, int count, int row, int values)
+// `count` parts, from the one at `part` on, `step` floats apart: the row's sums are at `row` in each, the pieces' values at
+// `values` and `next`.
+__device__ __forceinline__ void add_parts(Sums &to, const float *part, size_t step, int count, int row, int values, int next)
 {
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 6;
     for (int s0 = 0; s0 < count; s0 += kAhead) {
         Sums from[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             const float *at = part + size_t(min(s0 + i, count - 1)) * step;
-            from[i] = Sums{at[row], at[64 + row], *reinterpret_cast<const v4f *>(at + values)};
+            from[i].r = at[row];
+            from[i].total = at[64 + row];
+            from[i].o[0] = *reinterpret_cast<const v4f *>(at + values);
+            from[i].o[1] = *reinterpret_cast<const v4f *>(at + next);
         }
         float top = to.r;
 #pragma unroll
@@ -364,69 +453,88 @@ __device__ __forceinline__ void add_parts(Sums &to, const float *part, size_t st
         to.r = top;
         to.total = to.total * a;
 #pragma unroll
-        for (int e = 0; e < 4; e++) to.o[e] = to.o[e] * a;
+        for (int k = 0; k < kPieces; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) to.o[k][e] = to.o[k][e] * a;
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             if (s0 + i >= count) continue;
             const float b = part_factor(from[i].r, top);
             to.total = to.total + from[i].total * b;
 #pragma unroll
-            for (int e = 0; e < 4; e++) to.o[e] = to.o[e] + from[i].o[e] * b;
+            for (int k = 0; k < kPieces; k++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) to.o[k][e] = to.o[k][e] + from[i].o[k][e] * b;
         }
     }
 }
 
-// A workgroup a join, key head and kilobyte of a part: lane l has a pair and four dimensions, as the tasks left them, so that
-// parts are read whole lines at a time. Its waves take the parts in turn, but one the rows' own where these are apart.
+// A workgroup a join, key head and two kilobytes of a part: lane l has a pair and four dimensions of each, as the tasks left
+// them, so that parts are read whole lines at a time. The waves take the parts in turn, but the last one the rows' own where
+// these are apart.
 template <int DP>
-__global__ __launch_bounds__(256) void shared_join_kernel(SharedParams p)
+__global__ __launch_bounds__(kJoinWaves * 64) void shared_join_kernel(SharedParams p)
 {
-    __shared__ Sums sums[4][64];
+    constexpr unsigned kSteps = DP / 16;  // of a large tile's quarter; a small tile has half
+    __shared__ Sums sums[kJoinWaves][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int index = int(blockIdx.x / unsigned(p.kv_heads)), kv = int(blockIdx.x % unsigned(p.kv_heads)), piece = int(blockIdx.y);
-    if (index >= p.header->joins) return;  // the workgroup
-    const JoinRecord j = p.joins[index];
-    const bool large = j.wave >= 0;
-    const int rows = large ? 32 : 16;
-    if (piece >= rows * DP / 256) return;
-    const int pair = j.pair + (lane & (rows - 1)), dim = piece * (256 / rows) + 4 * (lane / rows);
-    const bool live = pair < j.rows * p.group && dim < p.head_dim;
-    const int at = min(pair, j.rows * p.group - 1) / p.group, row = j.begin + at, in_group = min(pair, j.rows * p.group - 1) - at * p.group;
-    Sums mine{-INFINITY, 0.0f, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
-    const int others = j.shared ? 3 : 4;
-    if (wave < others) {
-        const size_t floats = large ? many_floats(DP) : few_floats(DP), task = large ? 4 * floats : floats;
-        const float *part = (large ? p.partial : p.small_partial) + (size_t(j.slot + wave) * p.kv_heads + kv) * task + (large ? j.wave * floats : 0);
-        const int count = (j.parts - wave + others - 1) / others;
-        if (wave < j.parts) add_parts(mine, part, size_t(others) * p.kv_heads * task, count, lane, 128 + piece * 256 + lane * 4);
-    } else {
-        // (64 bits and every check: a row that no sequence holds, of a batch whose starts fall, may have any note)
-        const int s = p.rows_of[row].sequence;
-        const SequenceNote note = p.notes_of[s >= 0 && s < p.b.sequences ? s : 0];
-        const bool own_large = note.parts & kLarge;
-        const int tm = own_large ? 128 : 16, parts = note.parts & (kLarge - 1);
-        const int64_t m = (int64_t(row) - note.begin) * p.group + in_group, tile = m / tm;
-        const int64_t slot = note.base + (note.tiles - 1 - tile) * parts;
-        const bool there = live && m >= 0 && tile < note.tiles && parts <= kSharedSplit && slot >= 0 &&
-                           slot + parts <= (own_large ? p.large_slots : p.small_slots);
-        const int q = dim / 4, own = int(m & (tm - 1));
-        const size_t floats = own_large ? many_floats(DP) : few_floats(DP), task = own_large ? 4 * floats : floats;
-        const float *part = (own_large ? p.partial : p.small_partial);
-        if (there) {
-            part += (size_t(slot) * p.kv_heads + kv) * task + (own_large ? own / 32 * floats : 0);
-            if (own_large) add_parts(mine, part, p.kv_heads * task, parts, own % 32, 128 + (q / 2) * 256 + (own % 32 + 32 * (q & 1)) * 4);
-            else add_parts(mine, part, p.kv_heads * task, parts, own, 128 + (q / 4) * 256 + (own + 16 * (q & 3)) * 4);
+    const unsigned units = unsigned(p.header->joins) * unsigned(p.kv_heads) * kSteps;
+    for (unsigned unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const int piece = int(unit % kSteps) * kPieces, kv = int(unit / kSteps % unsigned(p.kv_heads));
+        const JoinRecord j = p.joins[unit / kSteps / unsigned(p.kv_heads)];
+        const bool large = j.wave >= 0;
+        const int rows = large ? 32 : 16, width = 256 / rows;
+        if (piece >= rows * DP / 256) continue;  // the workgroup
+        const int pair = j.pair + (lane & (rows - 1)), dim = piece * width + 4 * (lane / rows);
+        const bool live = pair < j.rows * p.group;
+        const int at = min(pair, j.rows * p.group - 1) / p.group, row = j.begin + at, in_group = min(pair, j.rows * p.group - 1) - at * p.group;
+        Sums mine{-INFINITY, 0.0f, {}};
+        const int others = j.shared ? kJoinWaves - 1 : kJoinWaves;
+        if (wave < others) {
+            const size_t floats = large ? many_floats(DP) : few_floats(DP), task = large ? 4 * floats : floats;
+            const float *part = (large ? p.partial : p.small_partial) + (size_t(j.slot + wave) * p.kv_heads + kv) * task + (large ? j.wave * floats : 0);
+            const int values = 128 + piece * 256 + lane * 4;
+            if (wave < j.parts)
+                add_parts(mine, part, size_t(others) * p.kv_heads * task, (j.parts - wave + others - 1) / others, lane, values, values + 256);
+        } else {
+            // (64 bits and every check: a row that no sequence holds, of a batch whose starts fall, may have any note)
+            const int s = p.rows_of[row].sequence;
+            const SequenceNote note = p.notes_of[s >= 0 && s < p.b.sequences ? s : 0];
+            const bool own_large = note.parts & kLarge;
+            const int tm = own_large ? 128 : 16, parts = note.parts & (kLarge - 1);
+            const int64_t m = (int64_t(row) - note.begin) * p.group + in_group, tile = m / tm;
+            const int64_t slot = note.base + (note.tiles - 1 - tile) * parts;
+            const bool there = live && m >= 0 && tile < note.tiles && parts <= kSharedSplit && slot >= 0 &&
+                               slot + parts <= (own_large ? p.large_slots : p.small_slots);
+            const int own = int(m & (tm - 1));
+            // where in a part the four values from dimension d on are
+            auto values = [&](int d) {
+                const int q = d / 4;
+                return own_large ? 128 + (q / 2) * 256 + (own % 32 + 32 * (q & 1)) * 4 : 128 + (q / 4) * 256 + (own + 16 * (q & 3)) * 4;
+            };
+            const size_t floats = own_large ? many_floats(DP) : few_floats(DP), task = own_large ? 4 * floats : floats;
+            if (there) {
+                const float *part = (own_large ? p.partial : p.small_partial) + (size_t(slot) * p.kv_heads + kv) * task +
+                                    (own_large ? own / 32 * floats : 0);
+                add_parts(mine, part, p.kv_heads * task, parts, own_large ? own % 32 : own, values(dim), values(dim + width));
+            }
         }
+        sums[wave][lane] = mine;
+        __syncthreads();
+        if (wave == 0 && live) {
+#pragma unroll
+            for (int w = 1; w < kJoinWaves; w++) add_sums(mine, sums[w][lane]);
+            float *to = p.out + size_t(row) * p.out_stride + size_t(kv * p.group + in_group) * p.head_dim + dim;
+#pragma unroll
+            for (int i = 0; i < kPieces; i++) {
+                v4f x;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = mine.total == 0.0f ? 0.0f : mine.o[i][e] / mine.total;
+                if (dim + i * width < p.head_dim) *reinterpret_cast<v4f_any *>(to + i * width) = x;
+            }
+        }
+        __syncthreads();
     }
-    sums[wave][lane] = mine;
-    __syncthreads();
-    if (wave != 0 || !live) return;
-#pragma unroll
-    for (int w = 1; w < 4; w++) add_sums(mine, sums[w][lane]);
-    v4f x;
-#pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = mine.total == 0.0f ? 0.0f : mine.o[e] / mine.total;
-    *reinterpret_cast<v4f_any *>(p.out + size_t(row) * p.out_stride + size_t(kv * p.group + in_group) * p.head_dim + dim) = x;
 }
 
 // ------------------------------------------------------------------------------- the host
@@ -435,7 +543,7 @@ struct Launch {
     bool shared;  // or each sequence by itself
     int limit, target;
     size_t large_slots, small_slots, join_slots, blocks;  // of a key head but the blocks
-    size_t at[8];  // where in the scratch the arrays are, and its size
+    size_t at[11];  // where in the scratch the arrays are, and its size
 };
 
 Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads)
@@ -460,14 +568,13 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, s
     l.join_slots = 4 * large + small;
     l.blocks = l.large_slots * c->kv_heads + (l.small_slots * c->kv_heads + 3) / 4;
     const size_t floats = 4 * size_t(many_floats(c->padded));
-    const size_t bytes[7] = {sizeof(PlanHeader), l.large_slots * sizeof(TaskRecord), l.small_slots * sizeof(TaskRecord),
+    const size_t bytes[10] = {sizeof(PlanHeader), l.large_slots * sizeof(TaskRecord), l.small_slots * sizeof(TaskRecord),
                              l.join_slots * sizeof(JoinRecord), b->sequences * sizeof(SequenceNote), b->rows * sizeof(RowNote),
-                             l.large_slots * c->kv_heads * floats * 4};
-    for (int i = 0; i < 7; i++) l.at[i + 1] = l.at[i] + (bytes[i] + 255) / 256 * 256;
+                             l.large_slots * c->kv_heads * floats * 4, l.small_slots * c->kv_heads * size_t(few_floats(c->padded)) * 4,
+                             b->rows * heads * size_t(c->padded) * 4, b->rows * heads * 4};
+    for (int i = 0; i < 10; i++) l.at[i + 1] = l.at[i] + (bytes[i] + 255) / 256 * 256;
     return l;
 }
-
-size_t scratch_of(const fg_cache *c, const Launch &l) { return l.at[7] + l.small_slots * c->kv_heads * few_floats(c->padded) * 4; }
 
 template <int DP>
 int launch_shared(const SharedParams &p, const Launch &l, hipStream_t s)
@@ -483,11 +590,12 @@ int launch_shared(const SharedParams &p, const Launch &l, hipStream_t s)
             raised.fetch_or(bit);
         }
     }
-    shared_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
+    const size_t per = size_t(kPlanThreads / (DP <= 32 ? 4 : DP == 64 ? 8 : DP <= 128 ? 16 : 32));  // rows and heads of a workgroup
+    shared_plan_kernel<<<unsigned(1 + std::min<size_t>((size_t(p.b.rows) * p.heads + per - 1) / per, 2 * kUnits)), kPlanThreads, 0, s>>>(p, DP);
     FG_HIP(hipGetLastError());
     shared_tasks_kernel<DP><<<unsigned(l.blocks), 256, many_lds<DP>(), s>>>(p);
     FG_HIP(hipGetLastError());
-    shared_join_kernel<DP><<<dim3(unsigned(l.join_slots * p.kv_heads), DP / 8), 256, 0, s>>>(p);
+    shared_join_kernel<DP><<<unsigned(std::min(l.join_slots * p.kv_heads * (DP / 16), 4 * kUnits)), kJoinWaves * 64, 0, s>>>(p);
     FG_HIP(hipGetLastError());
     return FG_OK;
 }
@@ -509,7 +617,7 @@ extern "C" size_t fg_cache_attend_shared_scratch(const fg_cache *c, const fg_bat
 {
     if (!c || !b || !f || !heads || heads % c->kv_heads) return 0;
     const Launch l = plan_launch(c, b, f, heads);
-    return l.shared ? scratch_of(c, l) : fg_cache_attend_scratch(c, b, heads);
+    return l.shared ? l.at[10] : fg_cache_attend_scratch(c, b, heads);
 }
 
 extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, const float *query, size_t query_stride,
@@ -525,12 +633,12 @@ extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, cons
     const Launch l = plan_launch(c, b, f, heads);
     if (!l.shared)
         return fg_cache_attend(c, b, query, query_stride, heads, scale, window, out, out_stride, scratch, scratch_bytes, stream);
-    if (l.blocks > kMaxGrid || l.join_slots * c->kv_heads > kMaxGrid)
+    if (l.blocks > kMaxGrid || l.join_slots * c->kv_heads * (c->padded / 16) > 0xf0000000)
         return set_error(FG_ERR_SHAPE, std::string(who) + ": more sequences times heads than a launch takes");
     const hipStream_t s = as_stream(stream);
     void *ws = nullptr;
     bool owned = false;
-    rc = stream_scratch(scratch, scratch_bytes, scratch_of(c, l), who, s, &ws, &owned);
+    rc = stream_scratch(scratch, scratch_bytes, l.at[10], who, s, &ws, &owned);
     if (rc) return rc;
     SharedParams p = attend_params<SharedParams>(c, b, query, query_stride, heads, scale, window, out, out_stride);
     p.starts = f->starts;
@@ -550,6 +658,8 @@ extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, cons
     p.rows_of = reinterpret_cast<RowNote *>(at + l.at[5]);
     p.partial = reinterpret_cast<float *>(at + l.at[6]);
     p.small_partial = reinterpret_cast<float *>(at + l.at[7]);
+    p.pieces = reinterpret_cast<uint4 *>(at + l.at[8]);
+    p.factors = reinterpret_cast<float *>(at + l.at[9]);
     switch (c->padded) {
     case 32: rc = launch_shared<32>(p, l, s); break;
     case 64: rc = launch_shared<64>(p, l, s); break;
