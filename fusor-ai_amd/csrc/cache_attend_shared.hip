@@ -18,34 +18,23 @@ namespace {
 // the join then does: nothing about the lengths is known on the host. (Each task's workgroup looking for itself, as in
 // cache_attend.hip, took 2.7 us of each one's time, and 6.7 from 257 spans on.)
 
-struct TaskRecord {
-    int table;          // the sequence whose table has the pages
-    int tile, split, nsplit;
-    int begin, rows;    // the span's
-    int first;          // the position of a sequence's first row
-    int lo, hi;         // pages [lo, hi) at most
-    int shared, whole;  // a group's; a small tile whose task is its only one and writes its outputs
-    int fill[5];
+struct SpanRecord {
+    int table;         // the sequence whose table has the pages
+    int begin, rows;
+    int first;         // the position of a sequence's first row
+    int lo, hi;        // pages [lo, hi) at most
+    int tiles, nsplit;
+    int base;          // the first of its tasks: tile t's part s is base + (tiles - 1 - t) nsplit + s (the last tiles see the most keys)
+    int flags;
+    int fill[6];
 };
+// large tiles; a group's; a sequence's whose rows see shared pages too; a sequence's of small tiles whose tasks are single and
+// write its outputs
+constexpr int kLarge = 1, kShared = 2, kJoined = 4, kWhole = 8;
 
-// A tile's, or a large tile's quarter's, parts to be joined.
-struct JoinRecord {
-    int begin, rows;     // the span's
-    int pair;            // the first one
-    int slot, parts;     // its first part's task, and how many
-    int wave;            // the quarter of a large tile; -1: a small one
-    int shared;          // each row's own parts are joined too
-    int fill;
-};
-
-// Where a sequence's parts are: tile t's part s is task base + (tiles - 1 - t) parts + s of the large or the small ones.
-struct SequenceNote {
-    int base, begin, tiles, parts;
-};
-constexpr int kLarge = 1 << 16;  // a flag in `parts`
-
-struct RowNote {
-    int sequence, position;
+// A span's task or join `at` (of a large tile four joins, of 32 pairs each).
+struct Place {
+    int span, at;
 };
 
 struct PlanHeader {
@@ -58,10 +47,9 @@ struct SharedParams : AttendParams {
     int limit;  // pairs of a span that small tiles take
     int large_slots, small_slots, join_slots;
     PlanHeader *header;
-    TaskRecord *large_tasks, *small_tasks;
-    JoinRecord *joins;
-    SequenceNote *notes_of;  // [sequences]
-    RowNote *rows_of;        // [rows]
+    SpanRecord *spans;  // the groups', the sequences'
+    Place *large_tasks, *small_tasks, *joins;
+    int *span_of_row;   // [rows]: the sequences'
     float *small_partial;
     uint4 *pieces;           // [key head][row, query head of it][block of 8 dimensions][2]: the queries' two f16 pieces
     float *factors;          // [key head][row, query head of it]: of its scores
@@ -209,34 +197,43 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         split_queries(p, padded);
         return;
     }
-    __shared__ float works[kPlanWaves];
+    __shared__ float works[2][kPlanWaves];
     __shared__ int totals[3][kPlanWaves];
-    __shared__ int upto[3][kPlanThreads];  // large tasks, small ones, joins, up to a span's last
-    __shared__ Entity spans[kPlanThreads];
-    __shared__ int splits[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, all = p.groups + p.b.sequences;
-    Entity n{};
-    float work = 0.0f;
-    for (int e0 = 0; e0 < all; e0 += kPlanThreads) {
-        n = entity_of(p, e0 + tid);
-        work = work + float(n.tiles) * float(n.pages) * (n.large ? float(kLargeCost) : 1.0f);
-        // the rows' sequences and positions: a lane its own few, the wave those of one with many after the other
-        const int s = e0 + tid - p.groups, rows = s >= 0 ? n.span.rows : 0;
-        for (int r = 0; r < min(rows, 4); r++) p.rows_of[n.span.begin + r] = RowNote{s, n.span.first + r};
-        unsigned long long many = __ballot(rows > 4);
+    // span e's places 0 .. count - 1 (or so many 4 bytes of e) at list[base] on, up to `room`: a lane writes its own few, and the
+    // wave those of one that has many after the other
+    auto list_places = [&](int e, int count, int base, int room, auto write) {
+        constexpr int kOwn = 3;
+        for (int i = 0; i < min(count, kOwn); i++)
+            if (base + i < room) write(base + i, e, i);
+        unsigned long long many = __ballot(count > kOwn);
         while (many) {
             const int l = __builtin_ctzll(many);
             many &= many - 1;
-            const int count = __builtin_amdgcn_readlane(rows, l), begin = __builtin_amdgcn_readlane(n.span.begin, l);
-            const int first = __builtin_amdgcn_readlane(n.span.first, l), sequence = __builtin_amdgcn_readlane(s, l);
-            for (int r = 4 + lane; r < count; r += 64) p.rows_of[begin + r] = RowNote{sequence, first + r};
+            const int span = __builtin_amdgcn_readlane(e, l), from = __builtin_amdgcn_readlane(base, l);
+            const int end = min(__builtin_amdgcn_readlane(count, l), room - from);
+            for (int i = kOwn + lane; i < end; i += 64) write(from + i, span, i);
         }
+    };
+    Entity n{};
+    float work = 0.0f, rows = 0.0f;
+    for (int e0 = 0; e0 < all; e0 += kPlanThreads) {
+        n = entity_of(p, e0 + tid);
+        work = work + float(n.tiles) * float(n.pages) * (n.large ? float(kLargeCost) : 1.0f);
+        rows = rows + float(n.span.rows);
     }
     work = wave_allsum(work);
-    if (lane == 0) works[wave] = work;
+    rows = wave_allsum(rows);
+    if (lane == 0) works[0][wave] = work, works[1][wave] = rows;
     __syncthreads();
-    work = 0.0f;
-    for (int w = 0; w < kPlanWaves; w++) work = work + works[w];
+    work = rows = 0.0f;
+    for (int w = 0; w < kPlanWaves; w++) work = work + works[0][w], rows = rows + works[1][w];
+    // Spans apart have each row twice at most, a sequence's and a group's. A batch whose starts fall may have it thousands of
+    // times: no room holds, nor any int counts, what that would be to do, and nothing is done.
+    if (rows > 2.01f * float(p.b.rows) + 1.0f) {
+        if (tid == 0) *p.header = PlanHeader{0, 0, 0};
+        return;
+    }
     // (a little more than a share: the sum is in f32)
     const float share = work * 1.00001f / float(p.target);
     auto pages_of = [&](float share, int least) { return share + 1.0f < float(least) ? least : share > 1e9f ? 1000000000 : int(share + 1.0f); };
@@ -250,79 +247,32 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         const bool whole = !n.shared && !n.joined && !n.large && nsplit == 1;
         const int pairs = n.span.rows * p.group;
         const int joins = n.tiles == 0 || (!n.shared && n.joined) || whole ? 0 : n.large ? (pairs + 31) / 32 : n.tiles;
-        int mine[3] = {n.large ? units : 0, n.large ? 0 : units, joins}, sums[3];
+        const int mine[3] = {n.large ? units : 0, n.large ? 0 : units, joins};
+        int at[3];  // the span's first
         __syncthreads();  // (what the last round read is read)
         for (int k = 0; k < 3; k++) {
-            sums[k] = wave_scan(mine[k], &totals[k][wave]);
+            int total;
+            at[k] = done[k] + wave_scan(mine[k], &total) - mine[k];
+            if (lane == 0) totals[k][wave] = total;
         }
         __syncthreads();
-        int ends[3];
         for (int k = 0; k < 3; k++) {
-            int before = 0, total = 0;
             for (int w = 0; w < kPlanWaves; w++) {
-                before += w < wave ? totals[k][w] : 0;
-                total += totals[k][w];
-            }
-            sums[k] += before;
-            upto[k][tid] = sums[k];
-            ends[k] = total;
-        }
-        spans[tid] = n;
-        splits[tid] = nsplit;
-        const int s = e0 + tid - p.groups;
-        if (s >= 0 && s < p.b.sequences) {
-            const int k = n.large ? 0 : 1;
-            p.notes_of[s] = SequenceNote{done[k] + sums[k] - mine[k], n.span.begin, n.tiles, nsplit | (n.large ? kLarge : 0)};
-        }
-        __syncthreads();
-        // the span that has unit u, and the unit within it
-        auto find = [&](const int (&upto)[kPlanThreads], int u, int *within) {
-            int lo = 0;  // the first whose upto is past u
-            for (int step = kPlanThreads / 2; step; step >>= 1)
-                if (upto[lo + step - 1] <= u) lo += step;
-            *within = u - (lo ? upto[lo - 1] : 0);
-            return lo;
-        };
-        for (int k = 0; k < 2; k++) {
-            TaskRecord *tasks = k == 0 ? p.large_tasks : p.small_tasks;
-            const int room = (k == 0 ? p.large_slots : p.small_slots) - done[k];
-            for (int u = tid; u < min(ends[k], room); u += kPlanThreads) {
-                int within;
-                const int i = find(upto[k], u, &within);
-                const Entity &e = spans[i];
-                TaskRecord t{};
-                t.table = e.table;
-                t.nsplit = splits[i];
-                t.tile = e.tiles - 1 - within / t.nsplit;  // the last tiles see the most keys: they come first
-                t.split = within % t.nsplit;
-                t.begin = e.span.begin;
-                t.rows = e.span.rows;
-                t.first = e.span.first;
-                t.lo = e.lo;
-                t.hi = e.hi;
-                t.shared = e.shared;
-                t.whole = !e.shared && !e.joined && !e.large && t.nsplit == 1;
-                tasks[done[k] + u] = t;
+                at[k] += w < wave ? totals[k][w] : 0;
+                done[k] += totals[k][w];
             }
         }
-        for (int u = tid; u < min(ends[2], p.join_slots - done[2]); u += kPlanThreads) {
-            int within;
-            const int i = find(upto[2], u, &within);
-            const Entity &e = spans[i];
-            const int k = e.large ? 0 : 1, tile = e.large ? within / 4 : within;
-            JoinRecord j{};
-            j.begin = e.span.begin;
-            j.rows = e.span.rows;
-            j.pair = within * (e.large ? 32 : 16);
-            j.parts = splits[i];
-            j.slot = done[k] + (i ? upto[k][i - 1] : 0) + (e.tiles - 1 - tile) * j.parts;
-            j.wave = e.large ? within % 4 : -1;
-            j.shared = e.shared;
-            p.joins[done[2] + u] = j;
+        const int e = e0 + tid;
+        if (e < all) {
+            const int flags = (n.large ? kLarge : 0) | (n.shared ? kShared : 0) | (n.joined ? kJoined : 0) | (whole ? kWhole : 0);
+            p.spans[e] = SpanRecord{n.table, n.span.begin, n.span.rows, n.span.first, n.lo, n.hi, n.tiles, nsplit, n.large ? at[0] : at[1], flags, {}};
         }
-        for (int k = 0; k < 3; k++) done[k] += ends[k];
+        // (more tasks than there is room for are those of a batch whose starts fall)
+        list_places(e, mine[0], at[0], p.large_slots, [&](int to, int e, int i) { p.large_tasks[to] = Place{e, i}; });
+        list_places(e, mine[1], at[1], p.small_slots, [&](int to, int e, int i) { p.small_tasks[to] = Place{e, i}; });
+        list_places(e, mine[2], at[2], p.join_slots, [&](int to, int e, int i) { p.joins[to] = Place{e, i}; });
+        list_places(e, n.shared ? 0 : n.span.rows, n.span.begin, p.b.rows, [&](int to, int e, int) { p.span_of_row[to] = e; });
     }
-    // (more tasks than there is room for are those of a batch whose starts fall)
     if (tid == 0) *p.header = PlanHeader{min(done[0], p.large_slots), min(done[1], p.small_slots), min(done[2], p.join_slots)};
 }
 
@@ -330,11 +280,22 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
 
 // The positions of a tile's rows: one after the other in a sequence, in a group's span its sequences'. A lane's
 // pair has its position in LDS too, from where it is read in every page rather than kept.
+__device__ __forceinline__ int sequence_span_of(int span, int groups, int sequences)
+{
+    return max(groups, min(span, groups + sequences - 1));  // (no sequence's row, of a batch whose starts fall, may have any)
+}
 struct InTile {
-    const RowNote *rows;  // null: a sequence's
-    int first, low, high;
+    const int *span_of_row;  // of the span's rows; null: a sequence's
+    const SpanRecord *spans;  // the sequences', `sequences` of them behind the `groups`
+    int groups, sequences;
+    int begin, first, low, high;
     const int *pairs;
-    __device__ __forceinline__ int of(int at) const { return rows ? rows[at].position : first + at; }
+    __device__ __forceinline__ int of(int at) const
+    {
+        if (!span_of_row) return first + at;
+        const SpanRecord &s = spans[sequence_span_of(span_of_row[at], groups, sequences)];
+        return s.first + (begin + at - s.begin);
+    }
     __device__ __forceinline__ int again(const Pair &, int pair) const { return pairs[pair]; }
 };
 
@@ -351,13 +312,13 @@ __device__ __forceinline__ void wave_ends(int v, int &low, int &high)
 }
 
 // The pages of a task: of those from lo to hi that rows at positions low to high see, its part.
-__device__ __forceinline__ PageRange part_of(const TaskRecord &t, int low, int high, int window)
+__device__ __forceinline__ PageRange part_of(const SpanRecord &t, int split, int low, int high, int window)
 {
     PageRange r;
-    r.hi = min(t.hi, high < 0 ? 0 : high / kPage + 1);
+    r.hi = min(t.hi, high < 0 ? 0 : high / kPage + 1);  // (the largest int: all)
     r.lo = min(max(first_seen(low, window) / kPage, t.lo), r.hi);
     const int n = (r.hi - r.lo + t.nsplit - 1) / t.nsplit;
-    r.lo = min(r.lo + t.split * n, r.hi);
+    r.lo = min(r.lo + split * n, r.hi);
     r.hi = min(r.lo + n, r.hi);
     r.lo = __builtin_amdgcn_readfirstlane(r.lo), r.hi = __builtin_amdgcn_readfirstlane(r.hi);
     return r;
@@ -376,35 +337,42 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(Sh
     const unsigned unit = large ? blockIdx.x : (blockIdx.x - large_blocks) * 4 + unsigned(wave);
     const int index = int(unit / unsigned(p.kv_heads)), kv = int(unit % unsigned(p.kv_heads));
     if (!large && index >= header.small) return;  // the wave
-    const TaskRecord t = (large ? p.large_tasks : p.small_tasks)[index];
+    const Place place = (large ? p.large_tasks : p.small_tasks)[index];
+    const SpanRecord t = p.spans[__builtin_amdgcn_readfirstlane(place.span)];
+    const int split = place.at % t.nsplit, tile = t.tiles - 1 - place.at / t.nsplit;
+    const bool shared = t.flags & kShared;
     Task task{};
     task.seq = t.table;
-    task.tile = t.tile;
+    task.tile = tile;
     task.nsplit = t.nsplit;
     task.span = Span{t.begin, t.rows, t.first, 0};
     task = uniform(task);
     const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
-    InTile places{t.shared ? p.rows_of + t.begin : nullptr, t.first, 0, 0, pair_positions};
+    InTile places{shared ? p.span_of_row + t.begin : nullptr, p.spans, p.groups, p.b.sequences, t.begin, t.first, 0, 0, pair_positions};
     const int pairs = t.rows * p.group, tm = large ? 128 : 16;
-    auto position = [&](int pair) { return places.of(min(t.tile * tm + pair, pairs - 1) / p.group); };
+    auto row_of = [&](int pair) { return min(tile * tm + pair, pairs - 1) / p.group; };
+    // the positions of the tile's first and last row, of a group's only where a window asks for them: with none its rows see
+    // all shared pages (or the mask hides what they do not)
+    int low = 0, high = INT_MAX;
+    if (!shared) low = t.first + row_of(0), high = t.first + row_of(tm - 1);
     if (large) {
-        const int mine = position(wave * 32 + (lane & 31));
+        const int mine = places.of(row_of(wave * 32 + (lane & 31)));
         if (lane < 32) pair_positions[wave * 32 + lane] = mine;
-        __syncthreads();
-        int low, high;
-        wave_ends(min(pair_positions[lane], pair_positions[64 + lane]), low, high);
-        int other;
-        wave_ends(max(pair_positions[lane], pair_positions[64 + lane]), other, high);
-        const PageRange range = part_of(t, low, high, p.window);
+        if (shared && p.window > 0) {
+            __syncthreads();
+            int other;
+            wave_ends(min(pair_positions[lane], pair_positions[64 + lane]), low, other);
+        }
+        const PageRange range = part_of(t, split, low, high, p.window);
         wave_ends(mine, places.low, places.high);
         float *parts = p.partial + size_t(blockIdx.x) * 4 * many_floats(DP);
         __builtin_assume(parts != nullptr);
         attend_many<DP>(p, task, range, table, kv, places, SplitQueries{p.pieces, p.factors}, lds, parts);
     } else {
-        wave_ends(position(lane & 15), places.low, places.high);
-        const PageRange range = part_of(t, places.low, places.high, p.window);
+        wave_ends(places.of(row_of(lane & 15)), places.low, places.high);
+        const PageRange range = part_of(t, split, shared ? places.low : low, high, p.window);
         attend_few<DP, 1>(p, task, range, table, kv, places, SplitQueries{p.pieces, p.factors}, static_cast<FewJoin<DP> *>(nullptr),
-                          t.whole ? nullptr : p.small_partial + size_t(unit) * few_floats(DP));
+                          t.flags & kWhole ? nullptr : p.small_partial + size_t(unit) * few_floats(DP));
     }
 }
 
@@ -469,43 +437,49 @@ __device__ __forceinline__ void add_parts(Sums &to, const float *part, size_t st
     }
 }
 
-// A workgroup a join, key head and two kilobytes of a part: lane l has a pair and four dimensions of each, as the tasks left
-// them, so that parts are read whole lines at a time. The waves take the parts in turn, but the last one the rows' own where
-// these are apart.
+// Eight waves, or where there are many of them four, a join, key head and two kilobytes of a part: lane l has a pair and four
+// dimensions of each, as the tasks left them, so that parts are read whole lines at a time. The waves take the parts in
+// turn, but the last one the rows' own where these are apart.
 template <int DP>
 __global__ __launch_bounds__(kJoinWaves * 64) void shared_join_kernel(SharedParams p)
 {
     constexpr unsigned kSteps = DP / 16;  // of a large tile's quarter; a small tile has half
     __shared__ Sums sums[kJoinWaves][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned units = unsigned(p.header->joins) * unsigned(p.kv_heads) * kSteps;
-    for (unsigned unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int waves = units <= 2 * kUnits ? kJoinWaves : kJoinWaves / 2;
+    const int wave = all_waves % waves;
+    const unsigned at_once = unsigned(kJoinWaves / waves);
+    for (unsigned unit0 = blockIdx.x * at_once; unit0 < units; unit0 += gridDim.x * at_once) {
+        const unsigned unit = unit0 + unsigned(all_waves / waves);
         const int piece = int(unit % kSteps) * kPieces, kv = int(unit / kSteps % unsigned(p.kv_heads));
-        const JoinRecord j = p.joins[unit / kSteps / unsigned(p.kv_heads)];
-        const bool large = j.wave >= 0;
-        const int rows = large ? 32 : 16, width = 256 / rows;
-        if (piece >= rows * DP / 256) continue;  // the workgroup
-        const int pair = j.pair + (lane & (rows - 1)), dim = piece * width + 4 * (lane / rows);
-        const bool live = pair < j.rows * p.group;
-        const int at = min(pair, j.rows * p.group - 1) / p.group, row = j.begin + at, in_group = min(pair, j.rows * p.group - 1) - at * p.group;
+        Place place{0, 0};
+        SpanRecord t{};
+        if (unit < units) {
+            place = p.joins[unit / kSteps / unsigned(p.kv_heads)];
+            t = p.spans[__builtin_amdgcn_readfirstlane(place.span)];
+        }
+        const bool large = t.flags & kLarge, shared = t.flags & kShared;
+        const int rows = large ? 32 : 16, width = 256 / rows, pairs = t.rows * p.group;
+        const int tile = large ? place.at / 4 : place.at, slot = t.base + (t.tiles - 1 - tile) * t.nsplit;
+        const int pair = place.at * rows + (lane & (rows - 1)), dim = piece * width + 4 * (lane / rows);
+        const bool live = pair < pairs && piece < rows * DP / 256;
+        const int at = min(pair, pairs - 1) / p.group, row = t.begin + at, in_group = min(pair, pairs - 1) - at * p.group;
         Sums mine{-INFINITY, 0.0f, {}};
-        const int others = j.shared ? kJoinWaves - 1 : kJoinWaves;
+        const int others = shared ? waves - 1 : waves;
         if (wave < others) {
             const size_t floats = large ? many_floats(DP) : few_floats(DP), task = large ? 4 * floats : floats;
-            const float *part = (large ? p.partial : p.small_partial) + (size_t(j.slot + wave) * p.kv_heads + kv) * task + (large ? j.wave * floats : 0);
+            const float *part = (large ? p.partial : p.small_partial) + (size_t(slot + wave) * p.kv_heads + kv) * task + (large ? place.at % 4 * floats : 0);
             const int values = 128 + piece * 256 + lane * 4;
-            if (wave < j.parts)
-                add_parts(mine, part, size_t(others) * p.kv_heads * task, (j.parts - wave + others - 1) / others, lane, values, values + 256);
-        } else {
-            // (64 bits and every check: a row that no sequence holds, of a batch whose starts fall, may have any note)
-            const int s = p.rows_of[row].sequence;
-            const SequenceNote note = p.notes_of[s >= 0 && s < p.b.sequences ? s : 0];
-            const bool own_large = note.parts & kLarge;
-            const int tm = own_large ? 128 : 16, parts = note.parts & (kLarge - 1);
-            const int64_t m = (int64_t(row) - note.begin) * p.group + in_group, tile = m / tm;
-            const int64_t slot = note.base + (note.tiles - 1 - tile) * parts;
-            const bool there = live && m >= 0 && tile < note.tiles && parts <= kSharedSplit && slot >= 0 &&
-                               slot + parts <= (own_large ? p.large_slots : p.small_slots);
+            if (wave < t.nsplit && unit < units && piece < rows * DP / 256)
+                add_parts(mine, part, size_t(others) * p.kv_heads * task, (t.nsplit - wave + others - 1) / others, lane, values, values + 256);
+        } else if (live) {
+            // (64 bits and every check, for the same reason)
+            const SpanRecord o = p.spans[sequence_span_of(p.span_of_row[row], p.groups, p.b.sequences)];
+            const bool own_large = o.flags & kLarge;
+            const int tm = own_large ? 128 : 16, parts = o.nsplit;
+            const int64_t m = (int64_t(row) - o.begin) * p.group + in_group, tile = m / tm;
+            const int64_t slot = o.base + (o.tiles - 1 - tile) * parts;
             const int own = int(m & (tm - 1));
             // where in a part the four values from dimension d on are
             auto values = [&](int d) {
@@ -513,17 +487,17 @@ __global__ __launch_bounds__(kJoinWaves * 64) void shared_join_kernel(SharedPara
                 return own_large ? 128 + (q / 2) * 256 + (own % 32 + 32 * (q & 1)) * 4 : 128 + (q / 4) * 256 + (own + 16 * (q & 3)) * 4;
             };
             const size_t floats = own_large ? many_floats(DP) : few_floats(DP), task = own_large ? 4 * floats : floats;
-            if (there) {
+            if (m >= 0 && tile < o.tiles && slot >= 0 &&
+                slot + parts <= (own_large ? p.large_slots : p.small_slots)) {
                 const float *part = (own_large ? p.partial : p.small_partial) + (size_t(slot) * p.kv_heads + kv) * task +
                                     (own_large ? own / 32 * floats : 0);
                 add_parts(mine, part, p.kv_heads * task, parts, own_large ? own % 32 : own, values(dim), values(dim + width));
             }
         }
-        sums[wave][lane] = mine;
+        sums[all_waves][lane] = mine;
         __syncthreads();
         if (wave == 0 && live) {
-#pragma unroll
-            for (int w = 1; w < kJoinWaves; w++) add_sums(mine, sums[w][lane]);
+            for (int w = 1; w < waves; w++) add_sums(mine, sums[all_waves + w][lane]);
             float *to = p.out + size_t(row) * p.out_stride + size_t(kv * p.group + in_group) * p.head_dim + dim;
 #pragma unroll
             for (int i = 0; i < kPieces; i++) {
@@ -568,8 +542,8 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, s
     l.join_slots = 4 * large + small;
     l.blocks = l.large_slots * c->kv_heads + (l.small_slots * c->kv_heads + 3) / 4;
     const size_t floats = 4 * size_t(many_floats(c->padded));
-    const size_t bytes[10] = {sizeof(PlanHeader), l.large_slots * sizeof(TaskRecord), l.small_slots * sizeof(TaskRecord),
-                             l.join_slots * sizeof(JoinRecord), b->sequences * sizeof(SequenceNote), b->rows * sizeof(RowNote),
+    const size_t bytes[10] = {sizeof(PlanHeader), l.large_slots * sizeof(Place), l.small_slots * sizeof(Place),
+                             l.join_slots * sizeof(Place), b->rows * sizeof(int), (f->groups + b->sequences) * sizeof(SpanRecord),
                              l.large_slots * c->kv_heads * floats * 4, l.small_slots * c->kv_heads * size_t(few_floats(c->padded)) * 4,
                              b->rows * heads * size_t(c->padded) * 4, b->rows * heads * 4};
     for (int i = 0; i < 10; i++) l.at[i + 1] = l.at[i] + (bytes[i] + 255) / 256 * 256;
@@ -651,11 +625,11 @@ extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, cons
     p.join_slots = int(l.join_slots);
     char *at = static_cast<char *>(ws);
     p.header = reinterpret_cast<PlanHeader *>(at);
-    p.large_tasks = reinterpret_cast<TaskRecord *>(at + l.at[1]);
-    p.small_tasks = reinterpret_cast<TaskRecord *>(at + l.at[2]);
-    p.joins = reinterpret_cast<JoinRecord *>(at + l.at[3]);
-    p.notes_of = reinterpret_cast<SequenceNote *>(at + l.at[4]);
-    p.rows_of = reinterpret_cast<RowNote *>(at + l.at[5]);
+    p.large_tasks = reinterpret_cast<Place *>(at + l.at[1]);
+    p.small_tasks = reinterpret_cast<Place *>(at + l.at[2]);
+    p.joins = reinterpret_cast<Place *>(at + l.at[3]);
+    p.span_of_row = reinterpret_cast<int *>(at + l.at[4]);
+    p.spans = reinterpret_cast<SpanRecord *>(at + l.at[5]);
     p.partial = reinterpret_cast<float *>(at + l.at[6]);
     p.small_partial = reinterpret_cast<float *>(at + l.at[7]);
     p.pieces = reinterpret_cast<uint4 *>(at + l.at[8]);
