@@ -32,10 +32,25 @@ struct SpanRecord {
 // write its outputs
 constexpr int kLarge = 1, kShared = 2, kJoined = 4, kWhole = 8;
 
-// A span's task or join `at` (of a large tile four joins, of 32 pairs each).
+// A span's task `at`.
 struct Place {
     int span, at;
 };
+
+// A small tile, or a quarter of a large one, whose parts are to be joined.
+struct JoinRecord {
+    int begin, rows;  // the span's
+    int at;           // its pairs are 16 at, or 32 at, on
+    int slot, parts;  // its first part's task, and how many
+    int flags;
+    int fill[2];
+};
+
+// Where a row's own parts are: a sequence's `base`, first row, tiles and nsplit.
+struct OwnRecord {
+    int base, begin, tiles, parts;  // parts with kOwnLarge: of large tiles
+};
+constexpr int kOwnLarge = 1 << 16;
 
 struct PlanHeader {
     int large, small, joins;
@@ -48,8 +63,10 @@ struct SharedParams : AttendParams {
     int large_slots, small_slots, join_slots;
     PlanHeader *header;
     SpanRecord *spans;  // the groups', the sequences'
-    Place *large_tasks, *small_tasks, *joins;
-    int *span_of_row;   // [rows]: the sequences'
+    Place *large_tasks, *small_tasks;
+    JoinRecord *joins;
+    int *positions;     // [rows]
+    OwnRecord *own;     // [rows]
     float *small_partial;
     uint4 *pieces;           // [key head][row, query head of it][block of 8 dimensions][2]: the queries' two f16 pieces
     float *factors;          // [key head][row, query head of it]: of its scores
@@ -69,31 +86,35 @@ struct Entity {
 __device__ __forceinline__ int shared_pages(const SharedParams &p, int count) { return max(0, min(count, p.b.max_pages)); }
 __device__ __forceinline__ int sequence_index(const SharedParams &p, int start) { return max(0, min(start, p.b.sequences)); }
 
-// Span e, the groups' first. Every lane of the wave takes part.
-__device__ __forceinline__ Entity entity_of(const SharedParams &p, int e)
+// The groups' arrays, in LDS where they fit.
+constexpr int kGroupsHeld = 1024;
+struct Groups {
+    const int *starts, *counts;
+};
+
+// Span e, the groups' first.
+__device__ __forceinline__ Entity entity_of(const SharedParams &p, const Groups &groups, int e)
 {
     Entity n{};
-    const int lane = threadIdx.x & 63, s = e - p.groups;
-    if (s >= 0 && s < p.b.sequences) n.span = sequence_span(p.b, s);
-    // the shared pages of sequence s: those of the last group that starts at or before it
+    const int s = e - p.groups;
     int before = 0;
-    for (int g0 = 0; g0 <= p.groups; g0 += 64) {
-        const int start = g0 + lane <= p.groups ? p.starts[g0 + lane] : INT_MAX;
-        const int count = g0 + lane < p.groups ? p.counts[g0 + lane] : 0;
-        const int here = min(64, p.groups + 1 - g0);
-        for (int i = 0; i < here; i++) {
-            const int at = __builtin_amdgcn_readlane(start, i), pages = __builtin_amdgcn_readlane(count, i);
-            before = s >= at ? pages : before;
-        }
+    if (s >= 0) {
+        if (s >= p.b.sequences) return n;
+        n.span = sequence_span(p.b, s);
+        // the shared pages of sequence s: those of the last group that starts at or before it
+        int upto = 0;  // so many starts are
+        for (int step = 1 << (31 - __builtin_clz(p.groups + 1)); step; step >>= 1)
+            if (upto + step <= p.groups + 1 && groups.starts[upto + step - 1] <= s) upto += step;
+        if (upto > 0 && upto <= p.groups) before = groups.counts[upto - 1];
     }
     n.table = s;
     if (s < 0) {
-        const int a = sequence_index(p, p.starts[e]), b = sequence_index(p, p.starts[e + 1]);
+        const int a = sequence_index(p, groups.starts[e]), b = sequence_index(p, groups.starts[e + 1]);
         if (b <= a) return n;
         n.span = span_of(p.b.row_starts[a], p.b.row_starts[b], 0, p.b.rows);
         n.table = a;
         n.shared = true;
-        n.pages = n.hi = shared_pages(p, p.counts[e]);
+        n.pages = n.hi = shared_pages(p, groups.counts[e]);
         // (each row sees less than a window of the pages before its sequence's own)
         if (p.window > 0) n.pages = min(n.pages, p.window / kPage + 2);
         if (n.hi == 0) return n;
@@ -115,7 +136,7 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, int e)
     return n;
 }
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanThreads = 1024, kFewSpans = 512;  // half as many threads up to so many spans: fewer waves to wait for
 
 // The queries split into their two pieces, once for all tasks that multiply them: a team of lanes a row and head, eight
 // dimensions a lane.
@@ -126,9 +147,9 @@ __device__ __forceinline__ void split_queries(const SharedParams &p, int padded)
     while (team < blocks) team *= 2;
     const int first = max(0, p.b.row_starts[0]), rows = min(p.b.row_starts[p.b.sequences], p.b.rows) - first;
     if (rows <= 0) return;
-    const unsigned units = unsigned(rows) * unsigned(p.heads), step = (gridDim.x - 1) * unsigned(kPlanThreads / team);
+    const unsigned units = unsigned(rows) * unsigned(p.heads), step = (gridDim.x - 1) * (blockDim.x / team);
     const int block = threadIdx.x & (team - 1);
-    for (unsigned unit = (blockIdx.x - 1) * unsigned(kPlanThreads / team) + threadIdx.x / team; unit < units; unit += step) {  // whole teams
+    for (unsigned unit = (blockIdx.x - 1) * (blockDim.x / team) + threadIdx.x / team; unit < units; unit += step) {  // whole teams
         const int row = first + int(unit / unsigned(p.heads)), head = int(unit % unsigned(p.heads));
         float x[8];
         load8(p.query + size_t(row) * p.query_stride + size_t(head) * p.head_dim, 8 * block, p.head_dim, x);
@@ -189,7 +210,7 @@ struct SplitQueries {
     }
 };
 
-// The first workgroup lists the tasks, a thread a span, 1024 at a time, then a thread a task or join of theirs; the others
+// The first workgroup lists the tasks, a thread a span; the others
 // split the queries.
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p, int padded)
 {
@@ -197,28 +218,41 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         split_queries(p, padded);
         return;
     }
-    __shared__ float works[2][kPlanWaves];
-    __shared__ int totals[3][kPlanWaves];
+    __shared__ float works[2][kPlanThreads / 64];
+    __shared__ int totals[3][kPlanThreads / 64], held[2][kGroupsHeld + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, all = p.groups + p.b.sequences;
-    // span e's places 0 .. count - 1 (or so many 4 bytes of e) at list[base] on, up to `room`: a lane writes its own few, and the
-    // wave those of one that has many after the other
-    auto list_places = [&](int e, int count, int base, int room, auto write) {
-        constexpr int kOwn = 3;
-        for (int i = 0; i < min(count, kOwn); i++)
-            if (base + i < room) write(base + i, e, i);
+    const int threads = int(blockDim.x), waves = threads / 64;
+    Groups groups{p.starts, p.counts};
+    if (p.groups <= kGroupsHeld) {
+        for (int g = tid; g <= p.groups; g += threads) {
+            held[0][g] = p.starts[g];
+            held[1][g] = g < p.groups ? p.counts[g] : 0;
+        }
+        groups = Groups{held[0], held[1]};
+        __syncthreads();
+    }
+    // write(item, i) for each lane's `item` and i from 0 to its `count`: a lane does its own few, and the wave those of one
+    // that has many after the other
+    auto each = [&](int count, const auto &item, auto write) {
+        constexpr int kOwn = 8, kInts = sizeof(item) / 4;
+        for (int i = 0; i < min(count, kOwn); i++) write(item, i);
         unsigned long long many = __ballot(count > kOwn);
         while (many) {
             const int l = __builtin_ctzll(many);
             many &= many - 1;
-            const int span = __builtin_amdgcn_readlane(e, l), from = __builtin_amdgcn_readlane(base, l);
-            const int end = min(__builtin_amdgcn_readlane(count, l), room - from);
-            for (int i = kOwn + lane; i < end; i += 64) write(from + i, span, i);
+            const int end = __builtin_amdgcn_readlane(count, l);
+            auto of_lane = item;
+            int ints[kInts];
+            __builtin_memcpy(ints, &item, sizeof(item));
+            for (int k = 0; k < kInts; k++) ints[k] = __builtin_amdgcn_readlane(ints[k], l);
+            __builtin_memcpy(&of_lane, ints, sizeof(item));
+            for (int i = kOwn + lane; i < end; i += 64) write(of_lane, i);
         }
     };
     Entity n{};
     float work = 0.0f, rows = 0.0f;
-    for (int e0 = 0; e0 < all; e0 += kPlanThreads) {
-        n = entity_of(p, e0 + tid);
+    for (int e0 = 0; e0 < all; e0 += threads) {
+        n = entity_of(p, groups, e0 + tid);
         work = work + float(n.tiles) * float(n.pages) * (n.large ? float(kLargeCost) : 1.0f);
         rows = rows + float(n.span.rows);
     }
@@ -227,7 +261,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
     if (lane == 0) works[0][wave] = work, works[1][wave] = rows;
     __syncthreads();
     work = rows = 0.0f;
-    for (int w = 0; w < kPlanWaves; w++) work = work + works[0][w], rows = rows + works[1][w];
+    for (int w = 0; w < waves; w++) work = work + works[0][w], rows = rows + works[1][w];
     // Spans apart have each row twice at most, a sequence's and a group's. A batch whose starts fall may have it thousands of
     // times: no room holds, nor any int counts, what that would be to do, and nothing is done.
     if (rows > 2.01f * float(p.b.rows) + 1.0f) {
@@ -239,8 +273,8 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
     auto pages_of = [&](float share, int least) { return share + 1.0f < float(least) ? least : share > 1e9f ? 1000000000 : int(share + 1.0f); };
     const int large_part = pages_of(share / float(kLargeCost), kLargePages), small_part = pages_of(share / 4.0f, kSmallPages);
     int done[3] = {0, 0, 0};
-    for (int e0 = 0; e0 < all; e0 += kPlanThreads) {
-        if (all > kPlanThreads) n = entity_of(p, e0 + tid);
+    for (int e0 = 0; e0 < all; e0 += threads) {
+        if (all > threads) n = entity_of(p, groups, e0 + tid);
         const int part = n.large ? large_part : small_part;
         const int nsplit = n.pages <= part ? 1 : min((n.pages + part - 1) / part, kSharedSplit);
         const int units = n.tiles * nsplit;
@@ -257,21 +291,37 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         }
         __syncthreads();
         for (int k = 0; k < 3; k++) {
-            for (int w = 0; w < kPlanWaves; w++) {
+            for (int w = 0; w < waves; w++) {
                 at[k] += w < wave ? totals[k][w] : 0;
                 done[k] += totals[k][w];
             }
         }
-        const int e = e0 + tid;
-        if (e < all) {
-            const int flags = (n.large ? kLarge : 0) | (n.shared ? kShared : 0) | (n.joined ? kJoined : 0) | (whole ? kWhole : 0);
-            p.spans[e] = SpanRecord{n.table, n.span.begin, n.span.rows, n.span.first, n.lo, n.hi, n.tiles, nsplit, n.large ? at[0] : at[1], flags, {}};
-        }
+        const int e = e0 + tid, base = n.large ? at[0] : at[1];
+        const int flags = (n.large ? kLarge : 0) | (n.shared ? kShared : 0) | (n.joined ? kJoined : 0) | (whole ? kWhole : 0);
+        if (e < all) p.spans[e] = SpanRecord{n.table, n.span.begin, n.span.rows, n.span.first, n.lo, n.hi, n.tiles, nsplit, base, flags, {}};
         // (more tasks than there is room for are those of a batch whose starts fall)
-        list_places(e, mine[0], at[0], p.large_slots, [&](int to, int e, int i) { p.large_tasks[to] = Place{e, i}; });
-        list_places(e, mine[1], at[1], p.small_slots, [&](int to, int e, int i) { p.small_tasks[to] = Place{e, i}; });
-        list_places(e, mine[2], at[2], p.join_slots, [&](int to, int e, int i) { p.joins[to] = Place{e, i}; });
-        list_places(e, n.shared ? 0 : n.span.rows, n.span.begin, p.b.rows, [&](int to, int e, int) { p.span_of_row[to] = e; });
+        struct Tasks {
+            int span, base, large;
+        };
+        each(units, Tasks{e, base, n.large}, [&](const Tasks &u, int i) {
+            if (u.base + i < (u.large ? p.large_slots : p.small_slots)) (u.large ? p.large_tasks : p.small_tasks)[u.base + i] = Place{u.span, i};
+        });
+        struct Joins {
+            int to, begin, rows, base, tiles, parts, flags;
+        };
+        each(joins, Joins{at[2], n.span.begin, n.span.rows, base, n.tiles, nsplit, flags}, [&](const Joins &u, int i) {
+            const int tile = u.flags & kLarge ? i / 4 : i;
+            if (u.to + i < p.join_slots) p.joins[u.to + i] = JoinRecord{u.begin, u.rows, i, u.base + (u.tiles - 1 - tile) * u.parts, u.parts, u.flags, {}};
+        });
+        struct Rows {
+            OwnRecord own;
+            int first;
+        };
+        each(n.shared ? 0 : n.span.rows, Rows{OwnRecord{base, n.span.begin, n.tiles, nsplit | (n.large ? kOwnLarge : 0)}, n.span.first},
+             [&](const Rows &u, int i) {
+                 p.positions[u.own.begin + i] = u.first + i;
+                 p.own[u.own.begin + i] = u.own;
+             });
     }
     if (tid == 0) *p.header = PlanHeader{min(done[0], p.large_slots), min(done[1], p.small_slots), min(done[2], p.join_slots)};
 }
@@ -280,22 +330,11 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
 
 // The positions of a tile's rows: one after the other in a sequence, in a group's span its sequences'. A lane's
 // pair has its position in LDS too, from where it is read in every page rather than kept.
-__device__ __forceinline__ int sequence_span_of(int span, int groups, int sequences)
-{
-    return max(groups, min(span, groups + sequences - 1));  // (no sequence's row, of a batch whose starts fall, may have any)
-}
 struct InTile {
-    const int *span_of_row;  // of the span's rows; null: a sequence's
-    const SpanRecord *spans;  // the sequences', `sequences` of them behind the `groups`
-    int groups, sequences;
-    int begin, first, low, high;
+    const int *positions;  // the span's rows'; null: a sequence's
+    int first, low, high;
     const int *pairs;
-    __device__ __forceinline__ int of(int at) const
-    {
-        if (!span_of_row) return first + at;
-        const SpanRecord &s = spans[sequence_span_of(span_of_row[at], groups, sequences)];
-        return s.first + (begin + at - s.begin);
-    }
+    __device__ __forceinline__ int of(int at) const { return positions ? positions[at] : first + at; }
     __device__ __forceinline__ int again(const Pair &, int pair) const { return pairs[pair]; }
 };
 
@@ -348,7 +387,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(Sh
     task.span = Span{t.begin, t.rows, t.first, 0};
     task = uniform(task);
     const int32_t *table = p.b.pages + size_t(task.seq) * p.b.max_pages;
-    InTile places{shared ? p.span_of_row + t.begin : nullptr, p.spans, p.groups, p.b.sequences, t.begin, t.first, 0, 0, pair_positions};
+    InTile places{shared ? p.positions + t.begin : nullptr, t.first, 0, 0, pair_positions};
     const int pairs = t.rows * p.group, tm = large ? 128 : 16;
     auto row_of = [&](int pair) { return min(tile * tm + pair, pairs - 1) / p.group; };
     // the positions of the tile's first and last row, of a group's only where a window asks for them: with none its rows see
@@ -403,7 +442,7 @@ __device__ __forceinline__ void add_sums(Sums &to, const Sums &from)
 // `values` and `next`.
 __device__ __forceinline__ void add_parts(Sums &to, const float *part, size_t step, int count, int row, int values, int next)
 {
-    constexpr int kAhead = 6;
+    constexpr int kAhead = 4;
     for (int s0 = 0; s0 < count; s0 += kAhead) {
         Sums from[kAhead];
 #pragma unroll
@@ -453,33 +492,27 @@ __global__ __launch_bounds__(kJoinWaves * 64) void shared_join_kernel(SharedPara
     for (unsigned unit0 = blockIdx.x * at_once; unit0 < units; unit0 += gridDim.x * at_once) {
         const unsigned unit = unit0 + unsigned(all_waves / waves);
         const int piece = int(unit % kSteps) * kPieces, kv = int(unit / kSteps % unsigned(p.kv_heads));
-        Place place{0, 0};
-        SpanRecord t{};
-        if (unit < units) {
-            place = p.joins[unit / kSteps / unsigned(p.kv_heads)];
-            t = p.spans[__builtin_amdgcn_readfirstlane(place.span)];
-        }
-        const bool large = t.flags & kLarge, shared = t.flags & kShared;
-        const int rows = large ? 32 : 16, width = 256 / rows, pairs = t.rows * p.group;
-        const int tile = large ? place.at / 4 : place.at, slot = t.base + (t.tiles - 1 - tile) * t.nsplit;
-        const int pair = place.at * rows + (lane & (rows - 1)), dim = piece * width + 4 * (lane / rows);
-        const bool live = pair < pairs && piece < rows * DP / 256;
+        JoinRecord t = p.joins[min(unit / kSteps / unsigned(p.kv_heads), unsigned(p.join_slots - 1))];  // (asked for beside their number)
+        const bool there = unit < units, large = t.flags & kLarge, shared = t.flags & kShared;
+        const int rows = large ? 32 : 16, width = 256 / rows, pairs = there ? t.rows * p.group : 0;
+        const int pair = t.at * rows + (lane & (rows - 1)), dim = piece * width + 4 * (lane / rows);
+        const bool live = there && pair < pairs && piece < rows * DP / 256;
         const int at = min(pair, pairs - 1) / p.group, row = t.begin + at, in_group = min(pair, pairs - 1) - at * p.group;
         Sums mine{-INFINITY, 0.0f, {}};
         const int others = shared ? waves - 1 : waves;
         if (wave < others) {
             const size_t floats = large ? many_floats(DP) : few_floats(DP), task = large ? 4 * floats : floats;
-            const float *part = (large ? p.partial : p.small_partial) + (size_t(slot + wave) * p.kv_heads + kv) * task + (large ? place.at % 4 * floats : 0);
+            const float *part = (large ? p.partial : p.small_partial) + (size_t(t.slot + wave) * p.kv_heads + kv) * task + (large ? t.at % 4 * floats : 0);
             const int values = 128 + piece * 256 + lane * 4;
-            if (wave < t.nsplit && unit < units && piece < rows * DP / 256)
-                add_parts(mine, part, size_t(others) * p.kv_heads * task, (t.nsplit - wave + others - 1) / others, lane, values, values + 256);
+            if (there && wave < t.parts && piece < rows * DP / 256)
+                add_parts(mine, part, size_t(others) * p.kv_heads * task, (t.parts - wave + others - 1) / others, lane, values, values + 256);
         } else if (live) {
-            // (64 bits and every check, for the same reason)
-            const SpanRecord o = p.spans[sequence_span_of(p.span_of_row[row], p.groups, p.b.sequences)];
-            const bool own_large = o.flags & kLarge;
-            const int tm = own_large ? 128 : 16, parts = o.nsplit;
+            // (64 bits and every check: a row that no sequence holds, of a batch whose starts fall, may have any record)
+            const OwnRecord o = p.own[row];
+            const bool own_large = o.parts & kOwnLarge;
+            const int tm = own_large ? 128 : 16, parts = o.parts & (kOwnLarge - 1);
             const int64_t m = (int64_t(row) - o.begin) * p.group + in_group, tile = m / tm;
-            const int64_t slot = o.base + (o.tiles - 1 - tile) * parts;
+            const int64_t slot = o.base + (int64_t(o.tiles) - 1 - tile) * parts;
             const int own = int(m & (tm - 1));
             // where in a part the four values from dimension d on are
             auto values = [&](int d) {
@@ -487,7 +520,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void shared_join_kernel(SharedPara
                 return own_large ? 128 + (q / 2) * 256 + (own % 32 + 32 * (q & 1)) * 4 : 128 + (q / 4) * 256 + (own + 16 * (q & 3)) * 4;
             };
             const size_t floats = own_large ? many_floats(DP) : few_floats(DP), task = own_large ? 4 * floats : floats;
-            if (m >= 0 && tile < o.tiles && slot >= 0 &&
+            if (m >= 0 && tile < o.tiles && parts <= kSharedSplit && slot >= 0 &&
                 slot + parts <= (own_large ? p.large_slots : p.small_slots)) {
                 const float *part = (own_large ? p.partial : p.small_partial) + (size_t(slot) * p.kv_heads + kv) * task +
                                     (own_large ? own / 32 * floats : 0);
@@ -543,7 +576,7 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, s
     l.blocks = l.large_slots * c->kv_heads + (l.small_slots * c->kv_heads + 3) / 4;
     const size_t floats = 4 * size_t(many_floats(c->padded));
     const size_t bytes[10] = {sizeof(PlanHeader), l.large_slots * sizeof(Place), l.small_slots * sizeof(Place),
-                             l.join_slots * sizeof(Place), b->rows * sizeof(int), (f->groups + b->sequences) * sizeof(SpanRecord),
+                             l.join_slots * sizeof(JoinRecord), b->rows * (sizeof(int) + sizeof(OwnRecord)), (f->groups + b->sequences) * sizeof(SpanRecord),
                              l.large_slots * c->kv_heads * floats * 4, l.small_slots * c->kv_heads * size_t(few_floats(c->padded)) * 4,
                              b->rows * heads * size_t(c->padded) * 4, b->rows * heads * 4};
     for (int i = 0; i < 10; i++) l.at[i + 1] = l.at[i] + (bytes[i] + 255) / 256 * 256;
@@ -564,8 +597,9 @@ int launch_shared(const SharedParams &p, const Launch &l, hipStream_t s)
             raised.fetch_or(bit);
         }
     }
-    const size_t per = size_t(kPlanThreads / (DP <= 32 ? 4 : DP == 64 ? 8 : DP <= 128 ? 16 : 32));  // rows and heads of a workgroup
-    shared_plan_kernel<<<unsigned(1 + std::min<size_t>((size_t(p.b.rows) * p.heads + per - 1) / per, 2 * kUnits)), kPlanThreads, 0, s>>>(p, DP);
+    const unsigned threads = size_t(p.groups) + p.b.sequences <= kFewSpans ? kPlanThreads / 2 : kPlanThreads;
+    const size_t per = size_t(threads / (DP <= 32 ? 4 : DP == 64 ? 8 : DP <= 128 ? 16 : 32));  // rows and heads of a workgroup
+    shared_plan_kernel<<<unsigned(1 + std::min<size_t>((size_t(p.b.rows) * p.heads + per - 1) / per, 2 * kUnits)), threads, 0, s>>>(p, DP);
     FG_HIP(hipGetLastError());
     shared_tasks_kernel<DP><<<unsigned(l.blocks), 256, many_lds<DP>(), s>>>(p);
     FG_HIP(hipGetLastError());
@@ -627,8 +661,9 @@ extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, cons
     p.header = reinterpret_cast<PlanHeader *>(at);
     p.large_tasks = reinterpret_cast<Place *>(at + l.at[1]);
     p.small_tasks = reinterpret_cast<Place *>(at + l.at[2]);
-    p.joins = reinterpret_cast<Place *>(at + l.at[3]);
-    p.span_of_row = reinterpret_cast<int *>(at + l.at[4]);
+    p.joins = reinterpret_cast<JoinRecord *>(at + l.at[3]);
+    p.own = reinterpret_cast<OwnRecord *>(at + l.at[4]);
+    p.positions = reinterpret_cast<int *>(at + l.at[4] + b->rows * sizeof(OwnRecord));
     p.spans = reinterpret_cast<SpanRecord *>(at + l.at[5]);
     p.partial = reinterpret_cast<float *>(at + l.at[6]);
     p.small_partial = reinterpret_cast<float *>(at + l.at[7]);
