@@ -1,5 +1,8 @@
 """Attention of sequences that share prefixes against 64 bits, with the bound of test_gpu_cache_attend.py: the
-order of additions differs, their number does not."""
+order of additions differs, their number does not.
+
+Shared pages are worked through apart where the sequences' tables together have room for 256 MiB; the tables here are
+widened with columns of no page for that."""
 
 import numpy as np
 import pytest
@@ -20,8 +23,14 @@ class Shared(Case):
     """A step of groups of sequences: group g's first starts[g + 1] - starts[g] sequences begin with pages[g] pages of the
     group's first sequence."""
 
-    def __init__(self, fk, gpu, rows, lengths, starts, pages, heads, kv_heads, dim, **options):
+    def __init__(self, fk, gpu, rows, lengths, starts, pages, heads, kv_heads, dim, wide=True, **options):
         super().__init__(fk, gpu, rows, lengths, heads, kv_heads, dim, **options)
+        if wide:
+            page = kv_heads * (128 * (-(-dim // 32) * 32) + 512)  # bytes, at least
+            columns = -(-2 ** 28 // (page * min(len(rows), sum(rows))))
+            more = np.full((len(rows), max(0, columns - self.step.table.shape[1])), -1, np.int32)
+            self.step.table = np.concatenate([self.step.table, more], 1)
+            self.whole.table = self.step.table
         self.groups = (list(starts), list(pages))
         for g, n in enumerate(pages):
             for s in range(starts[g] + 1, starts[g + 1]):
@@ -57,6 +66,13 @@ def test_against_64_bits(fk, gpu, step, heads, kv_heads, dim):
     case.check(got)
     import torch
     assert torch.equal(got, case.run())  # nothing in the result depends on timing
+
+
+@pytest.mark.parametrize("step", range(len(STEPS)))
+def test_narrow_tables(fk, gpu, step):
+    """... where each sequence reads its table by itself."""
+    case = Shared(fk, gpu, *STEPS[step], 4, 2, 64, wide=False, seed=step, padding=1)
+    case.check(case.run())
 
 
 @pytest.mark.parametrize("window", [1, 63, 64, 100, 1250, 1400, 5000, 2 ** 31 - 1])
