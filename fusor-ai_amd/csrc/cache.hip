@@ -83,8 +83,8 @@ __global__ __launch_bounds__(256) void cache_clear_kernel(uint8_t *records, size
     }
 }
 
-// Four values of a key from dimension dim on, x, turned: `head` is where the head's values lie, `angle(pair)` the pair's
-// factors. Values 2i and 2i + 1 are partners in the lane itself; the partners of halves are read a second time (the
+// Four values of a key from dimension dim on, x, turned: `head` is where the head's values lie, `angle(pair, j)` the pair's
+// factors (its j-th of this lane's). Values 2i and 2i + 1 are partners in the lane itself; the partners of halves are read a second time (the
 // lane that has them may be anywhere in the wave, and they come from the cache).
 template <class F>
 __device__ __forceinline__ v4f turned_quad(const RotaryParams &r, const float *head, int dim, const v4f &x, F angle)
@@ -95,7 +95,7 @@ __device__ __forceinline__ v4f turned_quad(const RotaryParams &r, const float *h
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {
             if (dim + j >= r.dims) continue;
-            const Turn t = angle((dim + j) / 2);
+            const Turn t = angle((dim + j) / 2, j / 2);
             u[j] = turned(x[j], x[j + 1], t, true);
             u[j + 1] = turned(x[j + 1], x[j], t, false);
         }
@@ -115,7 +115,7 @@ __device__ __forceinline__ v4f turned_quad(const RotaryParams &r, const float *h
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int d = dim + j;
-        if (d < r.dims) u[j] = turned(x[j], partner[j], angle(d < half ? d : d - half), d < half);
+        if (d < r.dims) u[j] = turned(x[j], partner[j], angle(d < half ? d : d - half, j), d < half);
     }
     return u;
 }
@@ -152,7 +152,7 @@ __device__ __forceinline__ void store_row(const P &p, unsigned unit)
             if (live) x = *reinterpret_cast<const v4f_any *>((value ? p.in[1] : p.in[0]) + place);
             if constexpr (TURN) {
                 if (live && !value)
-                    x = turned_quad(p.r, p.in[0] + place - dim, dim, x, [&](int pair) { return turn_at(p.r, pair, position); });
+                    x = turned_quad(p.r, p.in[0] + place - dim, dim, x, [&](int pair, int) { return turn_at(p.r, pair, position); });
             }
             unsigned packed;
             const float d = head_levels(team_max(amax4(x), wide), x, value ? kNoValueScale : 1.0f, packed);
@@ -190,10 +190,12 @@ __global__ __launch_bounds__(256) void cache_rows_kernel(StoreParams p)
 template <bool QUADS>
 __global__ __launch_bounds__(256) void turn_rows_kernel(TurnParams p)
 {
+    RotateParams queries = p.queries;
+    queries.b = p.b, queries.r = p.r;  // (the same scalar registers)
     const unsigned units = unsigned(p.b.rows) * unsigned(p.kv_heads), all = units + unsigned(p.b.rows) * unsigned(p.queries.units);
     for (unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6); unit < all; unit += gridDim.x * 4) {
         if (unit < units) store_row<true, true>(p, unit);
-        else rotate_unit<QUADS>(p.queries, unit - units);
+        else rotate_unit<QUADS>(queries, unit - units);
     }
 }
 
@@ -261,11 +263,16 @@ __device__ __forceinline__ void store_page(const P &p, uint8_t *levels, float *s
             }
             if constexpr (TURN) {
                 if (live && !value) {
+                    Angle four[4];  // of t, a whole four
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        if (t + i < t0 || t + i >= t1) continue;
-                        x[i] = turned_quad(p.r, p.in[0] + at - dim + i * stride, dim, x[i],
-                                           [&](int pair) { return turn_at(p.r, pair, place * kPage + t + i); });
+                        // (tokens that are not new have the first new one's partners, and their levels go nowhere)
+                        const float *row = p.in[0] + (row0 + min(max(t + i, t0), t1 - 1)) * stride + size_t(head) * p.head_dim;
+                        x[i] = turned_quad(p.r, row, dim, x[i], [&](int pair, int j) {
+                            const RotaryPair &r = p.r.pairs[pair];
+                            if (i == 0) four[j] = whole_four(r, place * kPage + t);
+                            return turn_of(both(four[j], r.more[i]), p.r.magnitude);
+                        });
                     }
                 }
             }
@@ -346,7 +353,9 @@ __global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p
     store_page<WRITE, false>(p, levels, scales);
 }
 
-__global__ __launch_bounds__(kPageThreads) void turn_pages_kernel(TurnParams p)
+// (Bounded to two workgroups a CU: the angles' 64-bit arithmetic took 129 registers, and one fewer of them is two workgroups
+// instead of one. 3618 tokens of 4 heads of 128, 64 values turned: 11.7 us, with one 15.9, with three, which spill, 21.5.)
+__global__ __launch_bounds__(kPageThreads, 4) void turn_pages_kernel(TurnParams p)
 {
     extern __shared__ __align__(16) uint8_t levels[];
     __shared__ float scales[kPage];

@@ -8,13 +8,13 @@ struct fg_rotary {
     int device;
     int dims, halves;  // the values of a head that are turned, and whether value i's partner is i + dims / 2
     double magnitude;
-    uint64_t *steps;  // [dims / 2]
+    fg::RotaryPair *pairs;  // [dims / 2]
 };
 
 namespace fg {
 
 struct RotaryParams {
-    const uint64_t *steps;
+    const RotaryPair *pairs;
     int dims, halves;
     double magnitude;
 };
@@ -28,7 +28,7 @@ struct Turn {
 __device__ __forceinline__ Turn turn_of(const Angle &a, double magnitude) { return Turn{float(a.c * magnitude), float(a.s * magnitude)}; }
 __device__ __forceinline__ Turn turn_at(const RotaryParams &r, int pair, int position)
 {
-    return turn_of(angle_of(uint64_t(unsigned(position)) * r.steps[pair]), r.magnitude);
+    return turn_of(angle_at(r.pairs[pair], position), r.magnitude);
 }
 
 // Rows to turn out of place or in place: rows * units of `unit_heads` heads, a wave each.
@@ -141,7 +141,7 @@ __device__ __forceinline__ void rotate_unit(const RotateParams &p, unsigned unit
 // Whether a head's pairs come in whole quads.
 inline bool whole_quads(const fg_rotary *r) { return r->dims % (r->halves ? 8 : 4) == 0; }
 
-inline RotaryParams rotary_params(const fg_rotary *r) { return RotaryParams{r->steps, r->dims, r->halves, r->magnitude}; }
+inline RotaryParams rotary_params(const fg_rotary *r) { return RotaryParams{r->pairs, r->dims, r->halves, r->magnitude}; }
 
 // A batch's rows of `heads` heads for rotate_unit.
 RotateParams rotate_params(const fg_rotary *r, const fg_batch *b, const float *x, size_t x_stride, size_t heads, size_t head_dim,

@@ -91,19 +91,19 @@ int fg_rotary_create(const double *frequencies, size_t dims, int layout, double 
         return set_error(FG_ERR_ARG, "fg_rotary_create: the layout must be FG_ROTARY_HALVES or FG_ROTARY_PAIRS");
     if (!frequencies) return set_error(FG_ERR_ARG, "fg_rotary_create: null frequencies");
     if (!(std::fabs(magnitude) <= 1e30)) return set_error(FG_ERR_ARG, "fg_rotary_create: the magnitude must be a number of at most 1e30");
-    uint64_t steps[128];
+    RotaryPair pairs[128];
     for (size_t i = 0; i < dims / 2; i++) {
         if (!(std::fabs(frequencies[i]) <= 1024.0))
             return set_error(FG_ERR_ARG, "fg_rotary_create: frequencies must be numbers of at most 1024 radians a token");
-        steps[i] = turn_step(frequencies[i]);
+        pairs[i] = rotary_pair(frequencies[i]);
     }
     int device = 0;
     FG_HIP(hipGetDevice(&device));
-    uint64_t *memory = nullptr;
-    hipError_t e = hipMalloc(reinterpret_cast<void **>(&memory), dims / 2 * sizeof(uint64_t));
+    RotaryPair *memory = nullptr;
+    hipError_t e = hipMalloc(reinterpret_cast<void **>(&memory), dims / 2 * sizeof(RotaryPair));
     if (e != hipSuccess) return check_hip(e, "fg_rotary_create: hipMalloc");
     const hipStream_t s = as_stream(stream);
-    e = hipMemcpyAsync(memory, steps, dims / 2 * sizeof(uint64_t), hipMemcpyHostToDevice, s);
+    e = hipMemcpyAsync(memory, pairs, dims / 2 * sizeof(RotaryPair), hipMemcpyHostToDevice, s);
     const hipError_t waited = hipStreamSynchronize(s);
     if (e == hipSuccess) e = waited;
     if (e != hipSuccess) {
@@ -122,7 +122,7 @@ int fg_rotary_create(const double *frequencies, size_t dims, int layout, double 
 int fg_rotary_free(fg_rotary *r)
 {
     if (!r) return FG_OK;
-    (void)hipFree(r->steps);
+    (void)hipFree(r->pairs);
     delete r;
     return FG_OK;
 }

@@ -11,9 +11,15 @@ namespace fg {
 // A pair's turn per token is kept as a fraction of 2^64, so that position * step, which drops whole turns as it
 // overflows, is the fraction of the last one: off by position * 2^-65 turns for the step's rounding, at any position. (In
 // f32 such a product has no digit left for far positions: past 2^20 radians its steps are 2^-3.)
-
+//
+// The angle of position p is that of the whole four positions before it and of p % 4 more tokens, together: four tokens in a row
+// share the series, and a position's angle is the same to the bit wherever it is computed.
 struct Angle {
     double c, s;
+};
+struct RotaryPair {
+    uint64_t step;
+    Angle more[4];  // by 0 to 3 tokens
 };
 
 // The cosine and sine of a phase: the nearest quarter turn is taken off exactly, and what is left, x in [-pi/4, pi/4], goes
@@ -51,6 +57,10 @@ FG_BOTH Angle angle_of(uint64_t phase)
     return a;
 }
 
+FG_BOTH Angle both(const Angle &a, const Angle &b) { return Angle{__builtin_fma(a.c, b.c, -(a.s * b.s)), __builtin_fma(a.s, b.c, a.c * b.s)}; }
+FG_BOTH Angle whole_four(const RotaryPair &r, int position) { return angle_of(uint64_t(unsigned(position) & ~3u) * r.step); }
+FG_BOTH Angle angle_at(const RotaryPair &r, int position) { return both(whole_four(r, position), r.more[position & 3]); }
+
 // `frequency` radians a token as a step: the fraction of a turn, rounded to 2^-64 (80-bit arithmetic).
 inline uint64_t turn_step(double frequency)
 {
@@ -58,6 +68,14 @@ inline uint64_t turn_step(double frequency)
     turns -= floorl(turns);
     const long double scaled = roundl(turns * 18446744073709551616.0L);
     return scaled >= 18446744073709551616.0L ? 0 : uint64_t(scaled);
+}
+
+inline RotaryPair rotary_pair(double frequency)
+{
+    RotaryPair r;
+    r.step = turn_step(frequency);
+    for (uint64_t k = 0; k < 4; k++) r.more[k] = angle_of(k * r.step);
+    return r;
 }
 
 }  // namespace fg

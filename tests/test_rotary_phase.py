@@ -16,8 +16,8 @@ using namespace fg;
 extern "C" {
 void angles(double frequency, const long long *positions, int count, double *c, double *s)
 {
-    const uint64_t step = turn_step(frequency);
-    for (int i = 0; i < count; i++) { const Angle a = angle_of(uint64_t(positions[i]) * step); c[i] = a.c; s[i] = a.s; }
+    const RotaryPair r = rotary_pair(frequency);
+    for (int i = 0; i < count; i++) { const Angle a = angle_at(r, int(positions[i])); c[i] = a.c; s[i] = a.s; }
 }
 unsigned long long step(double frequency) { return turn_step(frequency); }
 void phase(unsigned long long p, double *out) { const Angle a = angle_of(p); out[0] = a.c; out[1] = a.s; }
