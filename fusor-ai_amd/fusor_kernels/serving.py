@@ -155,19 +155,20 @@ class Prefixes:
         return FgPrefixes(self.pages.shape[0], self.starts.data_ptr(), self.pages.data_ptr())
 
 
-def _rotated_out(x, head_dim, out):
-    """`out` for the rows `x` [rows, heads, head_dim] turned (made here where None: rows that no sequence holds
-    are then 0), both checked."""
-    if x.dim() != 3:
-        raise ShapeError("rows of shape [rows, heads, head_dim]")
-    _check_heads("rows to turn", x, x.shape[1], head_dim, x.device, False)
-    if not x.is_cuda:
-        raise ShapeError("rows to turn: a device tensor")
+def _rotated_out(x, rows, head_dim, device, out):
+    """`out` for `rows` rows `x` [rows, heads, head_dim] turned (made here where None: rows that no sequence holds are
+    then 0), both checked."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != rows:
+        raise ShapeError(f"rows to turn of shape {list(shape)}, [{rows}, heads, {head_dim}] expected")
+    heads = shape[1]
+    _check_heads("rows to turn", x, heads, head_dim, device, out is x)
     if out is None:
-        return torch.zeros(x.shape, dtype=torch.float32, device=x.device)
-    _check_heads("out", out, x.shape[1], head_dim, x.device, True)
-    if out.shape[0] != x.shape[0]:
-        raise ShapeError(f"{x.shape[0]} rows to turn and {out.shape[0]} of out")
+        return torch.zeros(shape, dtype=torch.float32, device=device)
+    if out is not x:
+        _check_heads("out", out, heads, head_dim, device, True)
+        if out.shape[0] != rows:
+            raise ShapeError(f"{rows} rows to turn and {out.shape[0]} of out")
     return out
 
 
@@ -232,12 +233,12 @@ class Rotary:
     def rotate(self, batch, x, out=None, stream=None):
         """The batch's new rows of `x` [rows, heads, head_dim] turned by their positions, into `out`, which may be
         `x`. Rows of `out` that no sequence holds are left as they are (0 in an `out` made here)."""
-        if x.dim() != 3 or x.device != self.device or batch.pages.device != self.device:
+        if x.dim() != 3 or batch.pages.device != self.device:
             raise ShapeError(f"rows [rows, heads, head_dim] and a batch on {self.device}")
-        head_dim = x.shape[2]
+        rows, heads, head_dim = x.shape
         with _place(self.device, stream):
-            out = _rotated_out(x, head_dim, out)
-            check(lib().fg_rotary_rotate(self.handle, ctypes.byref(batch._ffi(x.shape[0])), x.data_ptr(), x.stride(0), x.shape[1], head_dim,
+            out = _rotated_out(x, rows, head_dim, self.device, out)
+            check(lib().fg_rotary_rotate(self.handle, ctypes.byref(batch._ffi(rows)), x.data_ptr(), x.stride(0), heads, head_dim,
                                          out.data_ptr(), out.stride(0), _stream(self.device)))
         return out
 
@@ -294,16 +295,14 @@ class PagedCache:
             raise ShapeError(f"the rotary positions are on {rotary.device}, the cache on {self.device}")
         if queries is None and out is not None:
             raise ShapeError("an `out` without queries")
-        heads = query = query_stride = place = stride = 0
+        heads = query = query_stride = to = to_stride = 0
         with _place(self.device, stream):
             if queries is not None:
-                out = _rotated_out(queries, self.head_dim, out)
-                if queries.device != self.device or queries.shape[0] != keys.shape[0]:
-                    raise ShapeError(f"queries of {queries.shape[0]} rows on {queries.device}, keys of {keys.shape[0]} on {self.device}")
+                out = _rotated_out(queries, keys.shape[0], self.head_dim, self.device, out)
                 heads, query, query_stride = queries.shape[1], queries.data_ptr(), queries.stride(0)
-                place, stride = out.data_ptr(), out.stride(0)
+                to, to_stride = out.data_ptr(), out.stride(0)
             check(lib().fg_cache_write_rotated(self.handle, ctypes.byref(fg), rotary.handle, keys.data_ptr(), keys.stride(0),
-                                               values.data_ptr(), values.stride(0), query, query_stride, heads, place, stride,
+                                               values.data_ptr(), values.stride(0), query, query_stride, heads, to, to_stride,
                                                _stream(self.device)))
         return out
 
