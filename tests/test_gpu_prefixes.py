@@ -90,11 +90,27 @@ def test_many_pairs_of_a_group(fk, gpu, heads, kv_heads, dim):
         case.check(case.run(), skip=set(range(2, count - 2)))
 
 
-def test_prefixes_longer_than_a_sequence(fk, gpu):
+@pytest.mark.parametrize("rows", [[3, 70, 1, 200], [3, 70, 1, 100], [1, 5, 1, 2]])
+def test_prefixes_longer_than_a_sequence(fk, gpu, rows):
     """Tokens inside the shared pages see what lies up to them, whether the step wrote them or not."""
-    case = Shared(fk, gpu, [3, 70, 1, 200], [1300, 1250, 640, 1290], [0, 4], [20], 4, 2, 64)
+    for heads, kv_heads in ((4, 2), (2, 2)):
+        case = Shared(fk, gpu, rows, [1300, 1250, 640, 1290], [0, 4], [20], heads, kv_heads, 64)
+        case.check(case.run())
+        case.check(case.run(window=500), window=500)
+
+
+def test_sequences_of_no_tokens_and_one(fk, gpu):
+    """... in groups and between them, beside long ones."""
+    import torch
+    case = Shared(fk, gpu, [1, 0, 1, 1, 0, 1, 1], [1300, 0, 1, 1310, 0, 1, 1290], [0, 2, 5], [20, 0], 4, 2, 64)
     case.check(case.run())
-    case.check(case.run(window=500), window=500)
+    case.step.lengths[3] = 0  # a new row of a sequence without tokens has no position
+    got = case.run()
+    assert not bool(got[2].any())
+    case.check(got, skip={3})
+    empty = case.cache.attend(fk.Batch(*(torch.zeros(s, dtype=torch.int32, device=gpu) for s in (1, 0, (0, 30)))), case.query.to(gpu)[:0],
+                              prefixes=fk.Prefixes(*(torch.zeros(s, dtype=torch.int32, device=gpu) for s in (1, 0))))
+    assert empty.shape == (0, 4, 64)
 
 
 def test_arrays_of_any_values(fk, gpu):
@@ -131,6 +147,19 @@ def test_pages_that_are_not_there(fk, gpu):
     got = case.run()
     case.check(got)
     assert not bool(got[2:7].any())
+
+
+def test_few_rows_past_their_sequence_length(fk, gpu):
+    import torch
+    case = Shared(fk, gpu, [1, 1, 1], [1300, 1300, 80], [0, 2], [20], 2, 2, 64)
+    step = case.step
+    step.rows, step.starts = [1, 1, 90], np.array([0, 1, 2, 92], np.int32)  # the last: 90 rows, 80 tokens
+    case.query = torch.randn(92, 2, 64, generator=torch.Generator().manual_seed(1))
+    got = case.run()
+    assert not bool(got[2:12].any())
+    step.rows, step.starts = [1, 1, 80], np.array([0, 1, 2, 82], np.int32)
+    case.query = torch.cat([case.query[:2], case.query[12:]])
+    case.check(torch.cat([got[:2], got[12:]]))
 
 
 def test_rows_past_their_sequence_length(fk, gpu):
