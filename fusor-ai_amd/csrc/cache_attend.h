@@ -273,7 +273,8 @@ struct RowSums {
 // 16 scores of one row in this lane, t = s * f, to weights times the values' scales, into x; the row's other
 // scores are in the lanes that `combine` joins. edge: keys outside [low, high] are masked (key(i) is score i's
 // position). small: a value's scale is under kSmallScale. rescale(a) scales the row's sums of this lane by a.
-template <class Key, class Combine, class Rescale>
+// LEAN: in a kernel whose registers are full.
+template <bool LEAN, class Key, class Combine, class Rescale>
 __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], float vs, float f, bool small, bool edge,
                                       int low, int high, RowSums &sums, Key key, Combine combine, Rescale rescale)
 {
@@ -291,7 +292,7 @@ __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], floa
         top = total = 0.0f;
         // (an f of its own: else the compiler may take the exponentials out of both branches, 16 registers more than there are)
         float g = f;
-        asm volatile("" : "+v"(g));
+        if constexpr (LEAN) asm volatile("" : "+v"(g));
         for_scales(vs, [&](int i, float v) {
             const bool seen = key(i) >= low && key(i) <= high;
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], g, -sums.r));
@@ -307,7 +308,7 @@ __device__ __forceinline__ void weigh(const float (&s)[16], float (&x)[16], floa
         float u = -INFINITY, m = -INFINITY;
         float logs = vs;
         asm volatile("" : "+v"(logs));  // (keeps the logarithm in this branch)
-        asm volatile("" : "+v"(low), "+v"(high));  // (the masks once more: all of them kept do not fit the scalar registers)
+        if constexpr (LEAN) asm volatile("" : "+v"(low), "+v"(high));  // (the masks once more: all of them kept do not fit the scalar registers)
         logs = __builtin_amdgcn_logf(logs);
         for_scales(logs, [&](int i, float v) {
             const float t = s[i] * f;
@@ -433,7 +434,7 @@ __device__ __forceinline__ void attend_few(const AttendParams &p, const Task &ta
         const int base = page * kPage + 32 * (g >> 1) + 4 * (g & 1);
         const bool edge = page * kPage + kPage - 1 > first || page * kPage < first_seen(last, p.window);
         const int high = pair.position, low = first_seen(high, p.window);
-        weigh(scores, weights, vs, f, __any(vs < kSmallScale), edge, low, high, sums, [&](int n) { return base + 8 * (n / 4) + n % 4; },
+        weigh<true>(scores, weights, vs, f, __any(vs < kSmallScale), edge, low, high, sums, [&](int n) { return base + 8 * (n / 4) + n % 4; },
               [](float a) {
                   float2 w = row_pair(a);
                   w = half_pair(fmaxf(w.x, w.y));
@@ -528,9 +529,11 @@ template <int DP>
 constexpr size_t many_lds() { return size_t(2) * (256 * DP + 2 * kPage * 4); }
 
 // The tile's sums over the pages `range` of `table`, to `parts`, four of them, or where that is null divided to the output.
-// `places` are those of the wave's pairs.
+// `places` are those of the wave's pairs. LEAN: what a lane knows of its place is computed in every page from its index, not
+// kept, for a kernel that has other things in registers too (heads of 128 leave it five); kept it is 4 % faster: a prompt of 8192
+// tokens, 16 heads of 128 over 4, 496 and 519 us.
 constexpr int many_floats(int DP) { return 32 * DP + 128; }  // of a wave's part
-template <int DP, class Places, class Queries>
+template <int DP, bool LEAN, class Places, class Queries>
 __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &task, const PageRange range, const int32_t *table, int kv,
                                             const Places &places, const Queries &queries, uint8_t *lds, float *parts)
 {
@@ -548,11 +551,17 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
     auto load = [&](int id) {  // a page's record into registers
         if (id < 0) return;
         const uint8_t *record = p.records + (size_t(id) * p.kv_heads + kv) * record_bytes(DP);
-        unsigned thread = threadIdx.x;
-        asm volatile("" : "+v"(thread));  // (a 32-bit offset beside a scalar address, no 64-bit one kept in registers)
+        if constexpr (LEAN) {
+            unsigned thread = threadIdx.x;
+            asm volatile("" : "+v"(thread));  // (a 32-bit offset beside a scalar address, no 64-bit one kept in registers)
 #pragma unroll
-        for (int c = 0; c < L; c++) staged[c] = *reinterpret_cast<const uint4 *>(record + c * 4096 + thread * 16u);
-        if (tid < 2 * kPage) staged_scale = *reinterpret_cast<const float *>(record + key_scale_byte(DP, 0) + thread * 4u);
+            for (int c = 0; c < L; c++) staged[c] = *reinterpret_cast<const uint4 *>(record + c * 4096 + thread * 16u);
+            if (tid < 2 * kPage) staged_scale = *reinterpret_cast<const float *>(record + key_scale_byte(DP, 0) + thread * 4u);
+        } else {
+#pragma unroll
+            for (int c = 0; c < L; c++) staged[c] = *reinterpret_cast<const uint4 *>(record + (c * 256 + tid) * 16);
+            if (tid < 2 * kPage) staged_scale = *reinterpret_cast<const float *>(record + key_scale_byte(DP, tid));
+        }
     };
     auto store = [&](uint8_t *to) {  // ... widened into a buffer: each kilobyte of 64 lanes as two
 #pragma unroll
@@ -604,20 +613,22 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
             v16f s[2] = {};
             v8h a[2][2];
             float ks[2], vs[2];
-            // (places computed from the lane once more in every page, not kept: the registers are full)
-            int here_lane = int(threadIdx.x);
-            asm volatile("" : "+v"(here_lane));
-            int high = places.again(pair, (here_lane >> 6) * 32 + (here_lane & 31));
-            asm volatile("" : "+v"(high));
-            here_lane &= 63;
-            const int low = first_seen(high, p.window), keys_at = page * kPage + 4 * (here_lane >> 5);
+            int here_lane = lane, high = pair.position;
+            if constexpr (LEAN) {
+                here_lane = int(threadIdx.x);
+                asm volatile("" : "+v"(here_lane));
+                high = places.again(pair, (here_lane >> 6) * 32 + (here_lane & 31));
+                asm volatile("" : "+v"(high));
+                here_lane &= 63;
+            }
+            const int low = first_seen(high, p.window), here_half = here_lane >> 5;
             auto read_keys = [&](int k) {
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++) a[k & 1][kt] = *reinterpret_cast<const v8h *>(buffer + (kt * K + k) * 1024 + here_lane * 16);
             };
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {
-                const int token = 32 * kt + 8 * ((here_lane >> 2) & 3) + 4 * (here_lane >> 5) + (here_lane & 3);
+                const int token = 32 * kt + 8 * ((here_lane >> 2) & 3) + 4 * here_half + (here_lane & 3);
                 ks[kt] = key_scales[token];
                 vs[kt] = value_scales[token];
             }
@@ -644,8 +655,8 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
                 for_scales(ks[kt], [&](int i, float k) { scores[i] = k * s[kt][i]; });
                 if (kt) read_values(0);
                 __builtin_amdgcn_sched_barrier(0);
-                weigh(scores, x, vs[kt], f, small, edge, low, high, sums,
-                          [&](int i) { return keys_at + 32 * kt + 2 * (i & ~3) + i % 4; },
+                weigh<LEAN>(scores, x, vs[kt], f, small, edge, low, high, sums,
+                          [&](int i) { return page * kPage + 32 * kt + 2 * (i & ~3) + 4 * here_half + i % 4; },
                           [](float v) {
                               const float2 w = half_pair(v);
                               return fmaxf(w.x, w.y);
@@ -685,9 +696,13 @@ __device__ __forceinline__ void attend_many(const AttendParams &p, const Task &t
     }
     const float2 w = half_pair(sums.total);
     sums.total = w.x + w.y;
-    int thread = int(threadIdx.x);
-    asm volatile("" : "+v"(thread));
-    if (task.tile * TM + (thread >> 6) * 32 + (thread & 31) >= task.span.rows * p.group) return;  // (a pair that is not live)
+    if constexpr (LEAN) {
+        int thread = int(threadIdx.x);
+        asm volatile("" : "+v"(thread));
+        if (task.tile * TM + (thread >> 6) * 32 + (thread & 31) >= task.span.rows * p.group) return;  // (a pair that is not live)
+    } else if (!pair.live) {
+        return;
+    }
     if (parts) {
         float *part = parts + wave * many_floats(DP);
         part[lane] = sums.r;

@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_many_kernel(Att
     const int pairs = task.span.rows * p.group, m0 = task.tile * TM + int(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 32;
     const int low = task.span.first + min(m0, pairs - 1) / p.group, high = task.span.first + min(m0 + 31, pairs - 1) / p.group;
     float *parts = task.nsplit > 1 ? p.partial + (size_t(task.slot) * p.kv_heads + kv) * 4 * many_floats(DP) : nullptr;
-    attend_many<DP>(p, task, task_pages(p, task, TM), p.b.pages + size_t(task.seq) * p.b.max_pages, kv,
+    attend_many<DP, false>(p, task, task_pages(p, task, TM), p.b.pages + size_t(task.seq) * p.b.max_pages, kv,
                     InSequence{task.span.first, low, high}, RawQueries{}, lds, parts);
 }
 

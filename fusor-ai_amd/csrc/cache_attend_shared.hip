@@ -406,7 +406,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(Sh
         wave_ends(mine, places.low, places.high);
         float *parts = p.partial + size_t(blockIdx.x) * 4 * many_floats(DP);
         __builtin_assume(parts != nullptr);
-        attend_many<DP>(p, task, range, table, kv, places, SplitQueries{p.pieces, p.factors}, lds, parts);
+        attend_many<DP, true>(p, task, range, table, kv, places, SplitQueries{p.pieces, p.factors}, lds, parts);
     } else {
         wave_ends(places.of(row_of(lane & 15)), places.low, places.high);
         const PageRange range = part_of(t, split, shared ? places.low : low, high, p.window);
