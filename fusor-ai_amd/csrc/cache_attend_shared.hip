@@ -16,7 +16,7 @@ namespace {
 // 128, a workgroup's, or, in spans of few pairs, small ones of 16, a wave's. A tile's pages are split into parts of about the
 // same time; a part of a tile is a task, for each key head. One workgroup lists the tasks from the batch's arrays, and what
 // the join then does: nothing about the lengths is known on the host. (Each task's workgroup looking for itself, as in
-// cache_attend.hip, took 2.7 us of each one's time, and 6.7 from 257 spans on.)
+// cache_attend.hip, took 2.7 us of each one's time, and 6.7 from 257 spans on: 256 sequences in five groups 98 us, listed 76.)
 
 struct SpanRecord {
     int table;         // the sequence whose table has the pages
@@ -72,7 +72,11 @@ struct SharedParams : AttendParams {
     float *factors;          // [key head][row, query head of it]: of its scores
 };
 
-// What a part takes: at least so many pages, and of the whole work, in units of a small tile's page, a share of the target.
+// What a part takes: at least so many pages, and of the whole work, in units of a small tile's page, a share of the target, two
+// workgroups a CU. Microseconds of 64 conversations behind 128 pages / 32 questions behind 940 / 256 in five groups, 16 heads
+// of 128 over 4: 36 / 58 / 72; at least 2, 8 pages of a large tile 40 / 63 / 79 and 42 / 58 / 73; 4, 8 of a small one 39 / 64 / 77
+// and 44 / 63 / 78; a large tile's page for one, three small ones' 37 / 64 / 88 and 37 / 64 / 83; three or four workgroups a CU 37 /
+// 73 / 81 and 37 / 77 / 82 (the second and later ones taken when these read 36.7 / 63.6 / 77.8).
 constexpr int kLargePages = 4, kSmallPages = 2, kLargeCost = 2;
 constexpr int kSharedSplit = 256;  // parts of a tile, at most
 
@@ -210,8 +214,8 @@ struct SplitQueries {
     }
 };
 
-// The first workgroup lists the tasks, a thread a span; the others
-// split the queries.
+// The first workgroup lists the tasks, a thread a span; the others split the queries. Bounded by its launch and a chain of waits:
+// the groups, their rows, two sums over the workgroup. 65 spans 5.5 us, 261 6.3, 1040 13.4.
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p, int padded)
 {
     if (blockIdx.x > 0) {
@@ -363,7 +367,16 @@ __device__ __forceinline__ PageRange part_of(const SpanRecord &t, int split, int
     return r;
 }
 
-// A workgroup a large task and key head, or a wave a small one and key head.
+// A workgroup a large task and key head, or a wave a small one and key head: both kinds in one launch, the large ones first,
+// so that the sequences' own pages are read while the shared ones multiply.
+// Bounded by the matrix cores and vector units in turns, like attend_many_kernel: a large tile's page takes 5000 cycles with one
+// workgroup a CU and 6100 to 7100 with two, after 10000 to 13000 for the record, the queries and the first page, 3000 more in the
+// first page, whose code is not in the instruction cache yet, and 2000 for the part. 32 questions behind 60160 tokens (16 heads of
+// 128 over 4): 45 us, 31.6 GF of two-piece products, 702 TFLOP/s; the matrix cores are busy 40 % of the cycles, the vector
+// units 44, waits are 22. 64 conversations behind 8192, whose four pages a part are mostly the first: 22 us, 395 TFLOP/s, 23 %.
+// 256 sequences in five groups, 73 MB of their own pages beside them: 59 us.
+// (Eight waves a workgroup, four every second page, which halves the parts: 37 / 55 / 72 us for these against 36 / 57 / 72, and
+// where parts are few 10 % slower; waves of the same SIMD at different priorities, or started apart: no difference.)
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(SharedParams p)
 {
@@ -479,6 +492,9 @@ __device__ __forceinline__ void add_parts(Sums &to, const float *part, size_t st
 // Eight waves, or where there are many of them four, a join, key head and two kilobytes of a part: lane l has a pair and four
 // dimensions of each, as the tasks left them, so that parts are read whole lines at a time. The waves take the parts in
 // turn, but the last one the rows' own where these are apart.
+// Bounded by waits: its record, a row's own, the parts, the exchange, one after the other, 80 % of the waves' cycles. 1024 pairs
+// of 32 parts, 17 MB, 7.9 us; 512 of 118, 31 MB, 9.9; 3920 of up to 23 9.6. (A team of lanes a row and head, whose parts
+// lie in lines that others read too: 12.5, 18.1 and 13.0.)
 template <int DP>
 __global__ __launch_bounds__(kJoinWaves * 64) void shared_join_kernel(SharedParams p)
 {

@@ -51,9 +51,9 @@ __device__ __forceinline__ float turned(float a, float b, Turn t, bool first)
     return first ? own - other : own + other;
 }
 
-// The unit's heads of one row. A team of lanes, a power of two, has a head's items: a pair of quads (halves), a quad of two
+// The unit's heads of one row, a wave. A team of lanes, a power of two, has a head's items: a pair of quads (halves), a quad of two
 // pairs, or, where pairs do not come in quads (QUADS false), one pair; then the head's values that are not turned. A lane's
-// angles serve all heads of the unit.
+// angles, some 60 f64 operations each, serve all heads of the unit.
 constexpr int kAhead = 4;  // heads of a lane whose loads are on their way at once
 
 template <bool QUADS>
