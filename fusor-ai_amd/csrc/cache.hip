@@ -210,11 +210,11 @@ __global__ __launch_bounds__(256) void turn_rows_kernel(TurnParams p)
 constexpr int kPageThreads = 512;
 
 template <bool WRITE, bool TURN, class P>
-__device__ __forceinline__ void store_page(const P &p, uint8_t *levels, float *scales)
+__device__ __forceinline__ void store_page(const P &p, int run, int head, int value, uint8_t *levels, float *scales)
 {
-    const int tid = threadIdx.x, head = int(blockIdx.y), value = int(blockIdx.z);
+    const int tid = threadIdx.x;
     int index;
-    const int s = find_unit(p.b.sequences, int(blockIdx.x), &index, [&](int q) {
+    const int s = find_unit(p.b.sequences, run, &index, [&](int q) {
         const PageRange r = pages_of_new(sequence_span(p.b, q));
         return r.hi - r.lo;
     });
@@ -351,16 +351,29 @@ __global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p
 {
     extern __shared__ __align__(16) uint8_t levels[];
     __shared__ float scales[kPage];
-    store_page<WRITE, false>(p, levels, scales);
+    store_page<WRITE, false>(p, int(blockIdx.x), int(blockIdx.y), int(blockIdx.z), levels, scales);
 }
 
-// (Bounded to two workgroups a CU: the angles' 64-bit arithmetic took 129 registers, and one fewer of them is two workgroups
-// instead of one. 3618 tokens of 4 heads of 128, 64 values turned: 11.7 us, with one 15.9, with three, which spill, 21.5.)
-__global__ __launch_bounds__(kPageThreads, 4) void turn_pages_kernel(TurnParams p)
+// The same for keys to be turned, and behind the pages' workgroups those of the queries' rows, which memory bounds while the
+// pages wait for one load after another. (Bounded to two workgroups a CU: the angles' 64-bit arithmetic took 129 registers, and
+// one fewer of them is two workgroups instead of one. 3618 tokens of 4 heads of 128, 64 values turned: 11.7 us, with one
+// 15.9, with three, which spill, 21.5.)
+template <bool QUADS>
+__global__ __launch_bounds__(kPageThreads, 4) void turn_pages_kernel(TurnParams p, unsigned runs)
 {
     extern __shared__ __align__(16) uint8_t levels[];
     __shared__ float scales[kPage];
-    store_page<true, true>(p, levels, scales);
+    const unsigned pages = runs * unsigned(p.kv_heads) * 2;
+    if (blockIdx.x < pages) {
+        const unsigned run = blockIdx.x / 2 / unsigned(p.kv_heads);
+        store_page<true, true>(p, int(run), int(blockIdx.x / 2 - run * unsigned(p.kv_heads)), int(blockIdx.x & 1), levels, scales);
+        return;
+    }
+    RotateParams queries = p.queries;
+    queries.b = p.b, queries.r = p.r;
+    const unsigned units = unsigned(p.b.rows) * unsigned(p.queries.units), step = (gridDim.x - pages) * (kPageThreads / 64);
+    for (unsigned unit = (blockIdx.x - pages) * (kPageThreads / 64) + (threadIdx.x >> 6); unit < units; unit += step)
+        rotate_unit<QUADS>(queries, unit);
 }
 
 // A workgroup a page: a run of n rows lies in at most (n + 62) / 64 + 1 pages.
@@ -398,9 +411,14 @@ int launch_turned(const TurnParams &p, bool quads, hipStream_t s)
     const size_t units = size_t(p.b.rows) * p.kv_heads, all = units + size_t(p.b.rows) * p.queries.units;
     if (all > 0xf0000000) return set_error(FG_ERR_SHAPE, "the paged cache: more rows times heads than a launch takes");
     if (!by_rows(p)) {
-        turn_pages_kernel<<<page_grid(p), kPageThreads, size_t(kPage * p.padded), s>>>(p);
+        const size_t runs = page_grid(p).x, pages = runs * size_t(p.kv_heads) * 2, waves = kPageThreads / 64;
+        if (pages > kMaxGrid / 4) return set_error(FG_ERR_SHAPE, "the paged cache: more rows times heads than a launch takes");
+        const size_t rows = std::min((size_t(p.b.rows) * p.queries.units + waves - 1) / waves, kMaxGrid / 4);
+        const unsigned grid = unsigned(pages + rows);
+        if (quads) turn_pages_kernel<true><<<grid, kPageThreads, size_t(kPage * p.padded), s>>>(p, unsigned(runs));
+        else turn_pages_kernel<false><<<grid, kPageThreads, size_t(kPage * p.padded), s>>>(p, unsigned(runs));
         FG_HIP(hipGetLastError());
-        return p.queries.units ? launch_rotate(p.queries, quads, s) : FG_OK;
+        return FG_OK;
     }
     const unsigned grid = unsigned(std::min((all + 3) / 4, kMaxGrid));
     if (quads) turn_rows_kernel<true><<<grid, 256, 0, s>>>(p);

@@ -8,7 +8,7 @@ import pytest
 from test_serving_resources import READELF, kernels  # noqa: F401 (a fixture)
 
 KERNELS = {"shared_plan_kernel": 1, "shared_tasks_kernel": 6, "shared_join_kernel": 6, "rotate_kernel": 2, "turn_rows_kernel": 2,
-           "turn_pages_kernel": 1, "copy_pages_kernel": 1}
+           "turn_pages_kernel": 2, "copy_pages_kernel": 1}
 
 
 @pytest.mark.skipif(not os.path.exists(READELF), reason="no llvm-readelf")
