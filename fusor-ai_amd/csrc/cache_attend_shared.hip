@@ -68,8 +68,8 @@ struct SharedParams : AttendParams {
     int *positions;     // [rows]
     OwnRecord *own;     // [rows]
     float *small_partial;
-    uint4 *pieces;           // [key head][row, query head of it][block of 8 dimensions][2]: the queries' two f16 pieces
-    float *factors;          // [key head][row, query head of it]: of its scores
+    uint4 *pieces;           // the queries' two f16 pieces (piece_at)
+    float *factors;          // [key head][pair]: of its scores
 };
 
 // What a part takes: at least so many pages, and of the whole work, in units of a small tile's page, a share of the target, two
@@ -142,6 +142,17 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, const Groups 
 
 constexpr int kPlanThreads = 1024, kFewSpans = 512;  // half as many threads up to so many spans: fewer waves to wait for
 
+// Where the high piece of eight dimensions, block `block` of them, of a pair is, in 16 bytes (the low one 64 further on). `pair` is its
+// place among all rows' of the key head; 32 in a row lie as a large tile's step takes them, a kilobyte of 64 lanes (pair, half of
+// the step's 32 dimensions), whatever the tile's first pair is: at most two runs. (One pair after the other, each lane of a load
+// asked for a line of its own, and a tile's queries took 6000 cycles.)
+__host__ __device__ __forceinline__ size_t pair_blocks(size_t rows, int group) { return (rows * size_t(group) + 31) / 32; }
+__device__ __forceinline__ size_t piece_at(int DP, size_t blocks32, int kv, int pair, int block)
+{
+    const int step = 2 * (block >> 2) + (block & 1), half = (block >> 1) & 1;
+    return (((size_t(kv) * blocks32 + (pair >> 5)) * (DP / 16) + step) * 4 + half) * 32 + (pair & 31);
+}
+
 // The queries split into their two pieces, once for all tasks that multiply them: a team of lanes a row and head, eight
 // dimensions a lane.
 __device__ __forceinline__ void split_queries(const SharedParams &p, int padded)
@@ -166,13 +177,14 @@ __device__ __forceinline__ void split_queries(const SharedParams &p, int padded)
         for (int k = 0; k < 8; k++) x[k] = ldexpf(x[k], shift);
         v8h hi, lo;
         split8(x, hi, lo);
-        const int kv = head / p.group;
-        const size_t pair = (size_t(kv) * p.b.rows + row) * p.group + (head - kv * p.group);
+        const int kv = head / p.group, pair = row * p.group + (head - kv * p.group);
+        const size_t blocks32 = pair_blocks(p.b.rows, p.group);
         if (block < blocks) {
-            p.pieces[(pair * blocks + block) * 2] = __builtin_bit_cast(uint4, hi);
-            p.pieces[(pair * blocks + block) * 2 + 1] = __builtin_bit_cast(uint4, lo);
+            const size_t at = piece_at(padded, blocks32, kv, pair, block);
+            p.pieces[at] = __builtin_bit_cast(uint4, hi);
+            p.pieces[at + 64] = __builtin_bit_cast(uint4, lo);
         }
-        if (block == 0) p.factors[pair] = ldexpf(p.scale2, -shift);
+        if (block == 0) p.factors[size_t(kv) * blocks32 * 32 + pair] = ldexpf(p.scale2, -shift);
     }
 }
 
@@ -183,8 +195,8 @@ struct SplitQueries {
     __device__ __forceinline__ void few(const AttendParams &p, const Pair &, int kv, int pair, int g, v8h (&qh)[(DP + 63) / 64][2],
                                         v8h (&ql)[(DP + 63) / 64][2], float &f) const
     {
-        const size_t at = size_t(kv) * p.b.rows * p.group + pair;
-        f = factors[at];
+        const size_t blocks32 = pair_blocks(p.b.rows, p.group);
+        f = factors[size_t(kv) * blocks32 * 32 + pair];
 #pragma unroll
         for (int j = 0; j < (DP + 63) / 64; j++)
 #pragma unroll
@@ -192,8 +204,9 @@ struct SplitQueries {
                 const int block = 8 * j + 2 * g + e;
                 uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
                 if (DP % 64 == 0 || block < DP / 8) {
-                    hi = pieces[(at * (DP / 8) + block) * 2];
-                    lo = pieces[(at * (DP / 8) + block) * 2 + 1];
+                    const size_t at = piece_at(DP, blocks32, kv, pair, block);
+                    hi = pieces[at];
+                    lo = pieces[at + 64];
                 }
                 qh[j][e] = __builtin_bit_cast(v8h, hi);
                 ql[j][e] = __builtin_bit_cast(v8h, lo);
@@ -203,13 +216,13 @@ struct SplitQueries {
     __device__ __forceinline__ void many(const AttendParams &p, const Pair &, int kv, int pair, int h, v8h (&qh)[DP / 16], v8h (&ql)[DP / 16],
                                          float &f) const
     {
-        const size_t at = size_t(kv) * p.b.rows * p.group + pair;
-        f = factors[at];
+        const size_t blocks32 = pair_blocks(p.b.rows, p.group);
+        f = factors[size_t(kv) * blocks32 * 32 + pair];
+        const uint4 *from = pieces + piece_at(DP, blocks32, kv, pair, 2 * h);
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) {
-            const size_t block = at * (DP / 8) + 4 * (k >> 1) + 2 * h + (k & 1);
-            qh[k] = __builtin_bit_cast(v8h, pieces[block * 2]);
-            ql[k] = __builtin_bit_cast(v8h, pieces[block * 2 + 1]);
+            qh[k] = __builtin_bit_cast(v8h, from[k * 128]);
+            ql[k] = __builtin_bit_cast(v8h, from[k * 128 + 64]);
         }
     }
 };
@@ -606,7 +619,8 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, s
     const size_t bytes[10] = {sizeof(PlanHeader), l.large_slots * sizeof(Place), l.small_slots * sizeof(Place),
                              l.join_slots * sizeof(JoinRecord), b->rows * (sizeof(int) + sizeof(OwnRecord)), (f->groups + b->sequences) * sizeof(SpanRecord),
                              l.large_slots * c->kv_heads * floats * 4, l.small_slots * c->kv_heads * size_t(few_floats(c->padded)) * 4,
-                             b->rows * heads * size_t(c->padded) * 4, b->rows * heads * 4};
+                             pair_blocks(b->rows, int(group)) * 32 * c->kv_heads * size_t(c->padded) * 4,
+                             pair_blocks(b->rows, int(group)) * 32 * c->kv_heads * 4};
     for (int i = 0; i < 10; i++) l.at[i + 1] = l.at[i] + (bytes[i] + 255) / 256 * 256;
     return l;
 }
