@@ -357,7 +357,7 @@ __global__ __launch_bounds__(kPageThreads) void cache_pages_kernel(StoreParams p
 // The same for keys to be turned, and behind the pages' workgroups those of the queries' rows, which memory bounds while the
 // pages wait for one load after another. (Bounded to two workgroups a CU: the angles' 64-bit arithmetic took 129 registers, and
 // one fewer of them is two workgroups instead of one. 3618 tokens of 4 heads of 128, 64 values turned: 11.7 us, with one
-// 15.9, with three, which spill, 21.5.)
+// 15.9, with three, which spill, 21.5; with the queries' 16 heads in the same launch 20.9, where the two apart take 11.9 + 11.7.)
 template <bool QUADS>
 __global__ __launch_bounds__(kPageThreads, 4) void turn_pages_kernel(TurnParams p, unsigned runs)
 {

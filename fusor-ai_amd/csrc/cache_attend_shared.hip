@@ -228,7 +228,7 @@ struct SplitQueries {
 };
 
 // The first workgroup lists the tasks, a thread a span; the others split the queries. Bounded by its launch and a chain of waits:
-// the groups, their rows, two sums over the workgroup. 65 spans 5.5 us, 261 6.3, 1040 13.4.
+// the groups, their rows, two sums over the workgroup. 65 spans 5.8 us, 261 6.6, 1040 13.7.
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p, int padded)
 {
     if (blockIdx.x > 0) {
@@ -382,14 +382,15 @@ __device__ __forceinline__ PageRange part_of(const SpanRecord &t, int split, int
 
 // A workgroup a large task and key head, or a wave a small one and key head: both kinds in one launch, the large ones first,
 // so that the sequences' own pages are read while the shared ones multiply.
-// Bounded by the matrix cores and vector units in turns, like attend_many_kernel: a large tile's page takes 5000 cycles with one
-// workgroup a CU and 6100 to 7100 with two, after 10000 to 13000 for the record, the queries and the first page, 3000 more in the
-// first page, whose code is not in the instruction cache yet, and 2000 for the part. 32 questions behind 60160 tokens (16 heads of
-// 128 over 4): 45 us, 31.6 GF of two-piece products, 702 TFLOP/s; the matrix cores are busy 40 % of the cycles, the vector
-// units 44, waits are 22. 64 conversations behind 8192, whose four pages a part are mostly the first: 22 us, 395 TFLOP/s, 23 %.
-// 256 sequences in five groups, 73 MB of their own pages beside them: 59 us.
+// Bounded by the matrix cores and vector units in turns, like attend_many_kernel: a large tile's page takes 4900 cycles with one
+// workgroup a CU and 5800 to 7000 with two, after 8500 to 10500 for the record, the queries and the first page, 3000 to 4000 more in
+// the first page, whose code is not in the instruction cache yet, and 2200 for the part. 32 questions behind 60160 tokens (16 heads of
+// 128 over 4): 42 us, 31.6 GF of two-piece products, 745 TFLOP/s; the matrix cores are busy 42 % of the cycles, the vector
+// units 46, waits are 23. 64 conversations behind 8192, whose four pages a part are mostly the first: 21 us, 417 TFLOP/s, 24 %.
+// 256 sequences in five groups, 73 MB of their own pages beside them: 57 us.
 // (Eight waves a workgroup, four every second page, which halves the parts: 37 / 55 / 72 us for these against 36 / 57 / 72, and
-// where parts are few 10 % slower; waves of the same SIMD at different priorities, or started apart: no difference.)
+// where parts are few 10 % slower; waves of the same SIMD at different priorities, or started apart, the queries asked for before the page table's entries, the
+// next page stored after the products instead of before: no difference.)
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(SharedParams p)
 {
