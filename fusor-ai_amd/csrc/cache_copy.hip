@@ -90,7 +90,7 @@ extern "C" int fg_cache_copy(fg_cache *const *caches, size_t count, const int32_
         p.targets = targets;
         p.pages = unsigned(pages);
         p.pieces = pieces_of(p.page_bytes);
-        p.piece_bytes = unsigned((p.page_bytes / p.pieces + 255) / 256 * 256);
+        p.piece_bytes = unsigned((p.page_bytes + p.pieces * 256 - 1) / (p.pieces * size_t(256)) * 256);
         copy_pages_kernel<<<dim3(unsigned(std::min<size_t>(pages * p.pieces, 65536)), unsigned(n)), 256, 0, as_stream(stream)>>>(p);
         FG_HIP(hipGetLastError());
         first += n;

@@ -61,6 +61,19 @@ def test_copies(fk, gpu, shapes, count):
                 assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("heads,dim", [(1849, 32), (977, 64), (513, 128), (257, 256)])
+def test_many_heads(fk, gpu, heads, dim):
+    """Pages of so many pieces that what is left after dividing a page among them is more than none."""
+    import torch
+    print(f"copy {heads} heads of {dim}", flush=True)
+    cache, batch = filled(fk, gpu, 3, heads, dim, 0)
+    old = contents(cache, batch)
+    fk.copy_pages([cache], [0], [2])
+    for got, want in zip(contents(cache, batch), old):
+        want[2] = want[0]
+        assert torch.equal(got, want)
+
+
 def test_ids_outside_and_pages_onto_themselves(fk, gpu):
     """Pairs that name no page change nothing, in the cache whose page it is not; one source for several targets."""
     import torch
