@@ -410,9 +410,9 @@ int launch_turned(const TurnParams &p, bool quads, hipStream_t s)
     if (p.b.rows == 0 || p.b.sequences == 0) return FG_OK;
     const size_t units = size_t(p.b.rows) * p.kv_heads, all = units + size_t(p.b.rows) * p.queries.units;
     if (all > 0xf0000000) return set_error(FG_ERR_SHAPE, "the paged cache: more rows times heads than a launch takes");
-    if (!by_rows(p)) {
-        const size_t runs = page_grid(p).x, pages = runs * size_t(p.kv_heads) * 2, waves = kPageThreads / 64;
-        if (pages > kMaxGrid / 4) return set_error(FG_ERR_SHAPE, "the paged cache: more rows times heads than a launch takes");
+    const size_t runs = page_grid(p).x, pages = runs * size_t(p.kv_heads) * 2, waves = kPageThreads / 64;
+    // (a launch has fewer than 2^32 threads in one direction: batches whose pages times heads are more than 2^22 go by rows)
+    if (!by_rows(p) && pages <= kMaxGrid / 4) {
         const size_t rows = std::min((size_t(p.b.rows) * p.queries.units + waves - 1) / waves, kMaxGrid / 4);
         const unsigned grid = unsigned(pages + rows);
         if (quads) turn_pages_kernel<true><<<grid, kPageThreads, size_t(kPage * p.padded), s>>>(p, unsigned(runs));
