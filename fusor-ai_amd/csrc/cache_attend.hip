@@ -201,8 +201,12 @@ struct Launch {
 //
 // Tiles are split when there are at most as many as CUs, all heads together: 64 sequences of up to 8000 tokens
 // (a) 71 whole and 56 split, (b) 42 and 21; all of 8000, which a CU each serves evenly, (a) 98 and 108; 128 sequences
-// (a), two a CU, 132 and 135. Not over tables of up to 16 pages: joining costs about 4 us, as much as ten pages, and
-// as much again on the host (500 tokens: 10.3 whole, 11.2 split). Two workgroups a CU read at once what memory
+// (a), two a CU, 132 and 135. Of small tiles not over tables of up to 16 pages: joining costs about 4 us, as
+// much as ten pages, and as much again on the host (500 tokens: 10.3 whole, 11.2 split). A large tile's page costs 1.5 to 3.5 us,
+// and what joining costs grows with the tiles: they are split over more than 4 pages, or more than 32 pages times the share of the
+// CUs that they fill (to 16). A chunk of 102 rows over 5 / 7 / 11 pages, whole and split: (b) 15.4 14.5 / 18.4 15.8 / 24.5 16.3,
+// (a) 19.8 17.7 / 24.3 19.9 / 32.4 19.9, 8 of 256 over 2 32 26 / 39 29 / 54 30; four of 120 over 7 / 9 / 13 (a) 25 25 / 29 24 / 37 32;
+// 13 of 78, half of the CUs, over 7 / 16 (a) 25 35 / 44 40, (b) 19 24 / 33 38. Two workgroups a CU read at once what memory
 // gives, so the parts aimed at are two a CU, less half of one a tile, whose last part is half a part on average:
 // fewer leave some CUs two parts and others one (eight documents of 30000 to 70000 tokens: 288 parts 105, 350 98,
 // 512 88), more start and end too often (1024: 104). 64 sequences as above (a): 384 parts 61 and of equal lengths
@@ -223,7 +227,7 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, size_t heads)
     const size_t tm = l.few ? 16 : 128, units = std::max<size_t>(kUnits / c->kv_heads, 1);
     const size_t tiles = std::max(pairs / tm, sequences);  // about
     l.grid = pairs / tm + sequences;
-    if (tiles <= units && b->max_pages > 16) {
+    if (tiles <= units && b->max_pages > (l.few ? 16 : std::min<size_t>(std::max<size_t>(32 * tiles / units, 4), 16))) {
         l.target = int((c->padded <= 128 ? 2 : 1) * units - tiles / 2);
         const size_t most = std::min<size_t>((b->max_pages + kMinPages - 1) / kMinPages, kMaxSplit);
         l.grid = std::min(l.grid * most, l.grid + l.target);

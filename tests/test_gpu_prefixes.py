@@ -75,6 +75,17 @@ def test_narrow_tables(fk, gpu, step):
     case.check(case.run())
 
 
+@pytest.mark.parametrize("rows,pages", [([102], 4), ([102], 5), ([250, 250], 7), ([250, 3], 9), ([120] * 4, 8), ([120] * 4, 9), ([78] * 13, 16)])
+@pytest.mark.parametrize("window", [0, 200])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(14, 2, 64), (16, 4, 128), (8, 2, 256), (5, 5, 36)])
+def test_chunks_over_short_tables(fk, gpu, rows, pages, window, heads, kv_heads, dim):
+    """Tables of 4 to 16 pages, to both sides of where a chunk's tiles are split."""
+    print(f"chunks {rows} {pages} pages {heads}/{kv_heads}x{dim} window {window}", flush=True)
+    lengths = [64 * pages - 17 * s for s in range(len(rows))]
+    case = Shared(fk, gpu, rows, lengths, [0, len(rows)], [1], heads, kv_heads, dim, wide=False, seed=pages)
+    case.check(case.run(window=window), window=window)
+
+
 @pytest.mark.parametrize("window", [1, 63, 64, 100, 1250, 1400, 5000, 2 ** 31 - 1])
 @pytest.mark.parametrize("step", [0, 1, 2, 3])
 def test_windows(fk, gpu, step, window):
