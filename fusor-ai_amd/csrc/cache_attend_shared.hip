@@ -584,23 +584,25 @@ struct Launch {
 };
 
 // Whether a step's shared pages are worked through apart: three launches, of which the plan and the join cost 10 to 15 us, pay
-// where all sequences' tables together hold 256 MiB (the host knows no more of the lengths). Microseconds, each
-// sequence by itself and shared, of S sequences of one new token behind P shared pages and up to 5 of their own: 16 heads of 128
-// over 4 (a page is 66 KiB), S = 8: P = 115 19 and 24, 400 32 and 32, 1000 56 and 46; S = 32: 45 23 and 28, 115 34 and 30, 400 78
+// where what all sequences may see of their tables together, all of them or a window, holds 256 MiB (the host knows no more of the
+// lengths). Microseconds, each sequence by itself and shared, of S sequences of one new token behind P shared pages and up to 5 of
+// their own: 16 heads of 128 over 4 (a page is 66 KiB), S = 8: P = 115 19 and 24, 400 32 and 32, 1000 56 and 46; S = 32: 45 23 and 28, 115 34 and 30, 400 78
 // and 42, 1000 171 and 60; S = 256: 8 31 and 31, 20 45 and 33, 200 260 and 81; 14 of 64 over 2 (17 KiB), S = 32: 400 32
-// and 36, 1000 61 and 46; S = 128: 45 22 and 26, 115 36 and 36, 400 91 and 55.
+// and 36, 1000 61 and 46; S = 128: 45 22 and 26, 115 36 and 36, 400 91 and 55. With windows over 400 pages of 66 KiB: S = 64, 800
+// tokens 18 and 30, 3000 28 and 31, 8000 53 and 36; S = 256: 100 21 and 28, 800 36 and 35, 3000 77 and 46.
 // Nor where the sequences have more than 96 pairs of a new token and a head of a key head on average (64 of heads past 128): a
 // prompt's chunks fill tiles of their own, and the parts cost what is left to gain: 17 chunks of 1 to 512 tokens behind 94
 // pages, 14 heads of 64 over 2, 95 and 124; 16 of 60 tokens behind 100, 16 of 128 over 4, 123 and 156.
 constexpr double kSharedBytes = 0x1p28;
 
-Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads)
+Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads, size_t window)
 {
     Launch l{};
     const size_t group = heads / c->kv_heads, pairs = b->rows * group, sequences = std::min(b->sequences, b->rows);
     const size_t groups = std::min(f->groups, sequences);
     l.limit = c->padded <= 128 ? 96 : 64;
-    const double bytes_held = double(sequences) * double(b->max_pages) * double(c->kv_heads) * double(record_bytes(c->padded));
+    const size_t pages = window ? std::min(b->max_pages, window / kPage + 2) : b->max_pages;
+    const double bytes_held = double(sequences) * double(pages) * double(c->kv_heads) * double(record_bytes(c->padded));
     l.shared = groups && sequences > groups && bytes_held >= kSharedBytes && pairs <= size_t(l.limit) * sequences;
     if (!l.shared) return l;
     const size_t units = std::max<size_t>(kUnits / c->kv_heads, 1);
@@ -667,8 +669,9 @@ using namespace fg;
 extern "C" size_t fg_cache_attend_shared_scratch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads)
 {
     if (!c || !b || !f || !heads || heads % c->kv_heads) return 0;
-    const Launch l = plan_launch(c, b, f, heads);
-    return l.shared ? l.at[10] : fg_cache_attend_scratch(c, b, heads);
+    // (either way: with a window the call may take the other one)
+    const Launch l = plan_launch(c, b, f, heads, 0);
+    return std::max(l.at[10], fg_cache_attend_scratch(c, b, heads));
 }
 
 extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, const float *query, size_t query_stride,
@@ -681,7 +684,7 @@ extern "C" int fg_cache_attend_shared(const fg_cache *c, const fg_batch *b, cons
     rc = check_attend(c, b, query, heads, scale, out, out_stride, who);
     if (rc) return rc;
     if (!b->rows || !b->sequences) return FG_OK;
-    const Launch l = plan_launch(c, b, f, heads);
+    const Launch l = plan_launch(c, b, f, heads, window);
     if (!l.shared)
         return fg_cache_attend(c, b, query, query_stride, heads, scale, window, out, out_stride, scratch, scratch_bytes, stream);
     if (l.blocks > kMaxGrid || l.join_slots * c->kv_heads * (c->padded / 16) > 0xf0000000)

@@ -1,8 +1,8 @@
 """Attention of sequences that share prefixes against 64 bits, with the bound of test_gpu_cache_attend.py: the
 order of additions differs, their number does not.
 
-Shared pages are worked through apart where the sequences' tables together have room for 256 MiB; the tables here are
-widened with columns of no page for that."""
+Shared pages are worked through apart where what the sequences may see of their tables together, all of them or a window,
+has room for 256 MiB; the tables here are widened with columns of no page for that, or with sequences of no tokens."""
 
 import numpy as np
 import pytest
@@ -23,8 +23,9 @@ class Shared(Case):
     """A step of groups of sequences: group g's first starts[g + 1] - starts[g] sequences begin with pages[g] pages of the
     group's first sequence."""
 
-    def __init__(self, fk, gpu, rows, lengths, starts, pages, heads, kv_heads, dim, wide=True, **options):
-        super().__init__(fk, gpu, rows, lengths, heads, kv_heads, dim, **options)
+    def __init__(self, fk, gpu, rows, lengths, starts, pages, heads, kv_heads, dim, wide=True, empty=0, padding=0, **options):
+        rows, lengths = list(rows) + [0] * empty, list(lengths) + [0] * empty
+        super().__init__(fk, gpu, rows, lengths, heads, kv_heads, dim, padding=max(padding, empty), **options)
         if wide:
             page = kv_heads * (128 * (-(-dim // 32) * 32) + 512)  # bytes, at least
             columns = -(-2 ** 28 // (page * min(len(rows), sum(rows))))
@@ -88,8 +89,9 @@ def test_chunks_over_short_tables(fk, gpu, rows, pages, window, heads, kv_heads,
 
 @pytest.mark.parametrize("window", [1, 63, 64, 100, 1250, 1400, 5000, 2 ** 31 - 1])
 @pytest.mark.parametrize("step", [0, 1, 2, 3])
-def test_windows(fk, gpu, step, window):
-    case = Shared(fk, gpu, *STEPS[step], 4, 2, 64, seed=window % 1000, padding=1)
+@pytest.mark.parametrize("empty", [0, 8000])  # (as many windows of two pages of 17 KiB are 256 MiB)
+def test_windows(fk, gpu, step, window, empty):
+    case = Shared(fk, gpu, *STEPS[step], 4, 2, 64, seed=window % 1000, padding=1, empty=empty)
     case.check(case.run(window=window), window=window)
 
 
@@ -105,9 +107,10 @@ def test_many_pairs_of_a_group(fk, gpu, heads, kv_heads, dim):
 def test_prefixes_longer_than_a_sequence(fk, gpu, rows):
     """Tokens inside the shared pages see what lies up to them, whether the step wrote them or not."""
     for heads, kv_heads in ((4, 2), (2, 2)):
-        case = Shared(fk, gpu, rows, [1300, 1250, 640, 1290], [0, 4], [20], heads, kv_heads, 64)
-        case.check(case.run())
-        case.check(case.run(window=500), window=500)
+        for empty in (0, 2000):
+            case = Shared(fk, gpu, rows, [1300, 1250, 640, 1290], [0, 4], [20], heads, kv_heads, 64, empty=empty)
+            case.check(case.run())
+            case.check(case.run(window=500), window=500)
 
 
 def test_sequences_of_no_tokens_and_one(fk, gpu):
