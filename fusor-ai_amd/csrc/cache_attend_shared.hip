@@ -59,7 +59,7 @@ struct PlanHeader {
 struct SharedParams : AttendParams {
     const int32_t *starts, *counts;
     int groups;
-    int limit;  // pairs of a span that small tiles take
+    int limit;  // pairs of a sequence that small tiles take
     int large_slots, small_slots, join_slots;
     PlanHeader *header;
     SpanRecord *spans;  // the groups', the sequences'
@@ -77,7 +77,12 @@ struct SharedParams : AttendParams {
 // of 128 over 4: 36 / 58 / 72; at least 2, 8 pages of a large tile 40 / 63 / 79 and 42 / 58 / 73; 4, 8 of a small one 39 / 64 / 77
 // and 44 / 63 / 78; a large tile's page for one, three small ones' 37 / 64 / 88 and 37 / 64 / 83; three or four workgroups a CU 37 /
 // 73 / 81 and 37 / 77 / 82 (the second and later ones taken when these read 36.7 / 63.6 / 77.8).
-constexpr int kLargePages = 4, kSmallPages = 2, kLargeCost = 2;
+// A group's small tiles, whose pages are many, lie in fewer parts, and a group of more than 48 pairs, three small tiles, takes large
+// ones: in 38 cases of 9 to 128 sequences in groups of 20 to 96 pairs behind 60 to 1500 pages at least 5 pages are 1.5 % faster than 2 on
+// average (12 sequences behind 400 pages, 16 heads of 128 over 4, 34 and 28), 8 are 20 % slower in some; and with large tiles from 32 /
+// 48 / 64 / 80 pairs on 1.5 / 2.6 / 0.6 / 0.7 % faster than from 96 on (24 sequences behind 900 pages 70 and 50).
+constexpr int kLargePages = 4, kSmallPages = 2, kGroupPages = 5, kLargeCost = 2;
+constexpr int kGroupLimit = 48;  // pairs of a group that small tiles take
 constexpr int kSharedSplit = 256;  // parts of a tile, at most
 
 struct Entity {
@@ -128,7 +133,7 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, const Groups 
     }
     if (n.span.rows == 0) return n;
     const int pairs = n.span.rows * p.group;
-    n.large = pairs > p.limit;
+    n.large = pairs > (n.shared ? kGroupLimit : p.limit);
     const int tm = n.large ? 128 : 16;
     n.tiles = (pairs + tm - 1) / tm;
     if (!n.shared) {
@@ -292,7 +297,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
     int done[3] = {0, 0, 0};
     for (int e0 = 0; e0 < all; e0 += threads) {
         if (all > threads) n = entity_of(p, groups, e0 + tid);
-        const int part = n.large ? large_part : small_part;
+        const int part = n.large ? large_part : n.shared ? max(small_part, kGroupPages) : small_part;
         const int nsplit = n.pages <= part ? 1 : min((n.pages + part - 1) / part, kSharedSplit);
         const int units = n.tiles * nsplit;
         const bool whole = !n.shared && !n.joined && !n.large && nsplit == 1;
@@ -610,10 +615,12 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, s
     // spans of n pairs have at most n / 128 + 1 large tiles, or n / 16 + 1 small ones; what a share of the target
     // leaves of the work are its tiles' further parts, of small tiles four times as many
     size_t large = 0, small = 0;
-    for (size_t spans : {groups, sequences}) {
-        large += pairs > size_t(l.limit) ? pairs / 128 + std::min(spans, pairs / (l.limit + 1)) : 0;
-        small += std::min(pairs / 16 + spans, size_t(l.limit / 16) * spans);
-    }
+    auto add = [&](size_t spans, size_t limit) {
+        large += pairs > limit ? pairs / 128 + std::min(spans, pairs / (limit + 1)) : 0;
+        small += std::min(pairs / 16 + spans, limit / 16 * spans);
+    };
+    add(groups, kGroupLimit);
+    add(sequences, size_t(l.limit));
     l.large_slots = large ? large + l.target : 0;
     l.small_slots = small + 4 * l.target;
     l.join_slots = 4 * large + small;

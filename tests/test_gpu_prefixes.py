@@ -98,7 +98,7 @@ def test_windows(fk, gpu, step, window, empty):
 @pytest.mark.parametrize("heads,kv_heads,dim", [(16, 4, 128), (14, 2, 64), (1, 1, 32), (34, 1, 32), (300, 1, 32)])
 def test_many_pairs_of_a_group(fk, gpu, heads, kv_heads, dim):
     """Tiles whose pairs begin in the middle of a token's heads, groups around the sizes where the kernels change."""
-    for count in (2, 6, 7, 13, 14, 24, 25, 33):
+    for count in (2, 6, 7, 12, 13, 14, 24, 25, 33):
         case = Shared(fk, gpu, [1] * count, [1200 + 3 * s for s in range(count)], [0, count], [18], heads, kv_heads, dim, seed=count)
         case.check(case.run(), skip=set(range(2, count - 2)))
 
