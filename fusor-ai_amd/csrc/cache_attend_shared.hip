@@ -589,16 +589,18 @@ struct Launch {
 };
 
 // Whether a step's shared pages are worked through apart: three launches, of which the plan and the join cost 10 to 15 us, pay
-// where what all sequences may see of their tables together, all of them or a window, holds 256 MiB (the host knows no more of the
+// where what all sequences may see of their tables together, all of them or a window, holds 224 MiB (the host knows no more of the
 // lengths). Microseconds, each sequence by itself and shared, of S sequences of one new token behind P shared pages and up to 5 of
 // their own: 16 heads of 128 over 4 (a page is 66 KiB), S = 8: P = 115 19 and 24, 400 32 and 32, 1000 56 and 46; S = 32: 45 23 and 28, 115 34 and 30, 400 78
 // and 42, 1000 171 and 60; S = 256: 8 31 and 31, 20 45 and 33, 200 260 and 81; 14 of 64 over 2 (17 KiB), S = 32: 400 32
 // and 36, 1000 61 and 46; S = 128: 45 22 and 26, 115 36 and 36, 400 91 and 55. With windows over 400 pages of 66 KiB: S = 64, 800
 // tokens 18 and 30, 3000 28 and 31, 8000 53 and 36; S = 256: 100 21 and 28, 800 36 and 35, 3000 77 and 46.
+// Of 220 steps of 4 to 256 sequences in 1 to 5 groups behind 10 to 900 pages, 1 to 10 rows each, heads of 36 to 256, the way chosen so
+// takes 1.9 % longer than the faster one on average (from 160 or 256 MiB on 2.5 and 3.0; always the one way or the other 17 and 16).
 // Nor where the sequences have more than 96 pairs of a new token and a head of a key head on average (64 of heads past 128): a
 // prompt's chunks fill tiles of their own, and the parts cost what is left to gain: 17 chunks of 1 to 512 tokens behind 94
 // pages, 14 heads of 64 over 2, 95 and 124; 16 of 60 tokens behind 100, 16 of 128 over 4, 123 and 156.
-constexpr double kSharedBytes = 0x1p28;
+constexpr double kSharedBytes = 7 * 0x1p25;
 
 Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, size_t heads, size_t window)
 {

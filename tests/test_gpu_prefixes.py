@@ -2,7 +2,7 @@
 order of additions differs, their number does not.
 
 Shared pages are worked through apart where what the sequences may see of their tables together, all of them or a window,
-has room for 256 MiB; the tables here are widened with columns of no page for that, or with sequences of no tokens."""
+has room for 224 MiB; the tables here are widened with columns of no page for that, or with sequences of no tokens."""
 
 import numpy as np
 import pytest
@@ -89,7 +89,7 @@ def test_chunks_over_short_tables(fk, gpu, rows, pages, window, heads, kv_heads,
 
 @pytest.mark.parametrize("window", [1, 63, 64, 100, 1250, 1400, 5000, 2 ** 31 - 1])
 @pytest.mark.parametrize("step", [0, 1, 2, 3])
-@pytest.mark.parametrize("empty", [0, 8000])  # (as many windows of two pages of 17 KiB are 256 MiB)
+@pytest.mark.parametrize("empty", [0, 8000])  # (as many windows of two pages of 17 KiB are more than that)
 def test_windows(fk, gpu, step, window, empty):
     case = Shared(fk, gpu, *STEPS[step], 4, 2, 64, seed=window % 1000, padding=1, empty=empty)
     case.check(case.run(window=window), window=window)
