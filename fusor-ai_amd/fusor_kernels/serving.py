@@ -84,21 +84,23 @@ def _check_ints(name, t, shape):
 
 
 def _check_heads(name, t, heads, head_dim, device, written):
-    """[rows, heads, head_dim] float32 whose rows are runs of heads * head_dim values."""
+    """[rows, heads, head_dim] float32 whose rows are runs of heads * head_dim values. Returns how far apart rows are (asking
+    a tensor for it costs twice what its contiguity does)."""
     if t.dtype is not torch.float32 or t.device != device:
         raise ShapeError(f"{name}: a float32 tensor on {device}")
     shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
         raise ShapeError(f"{name} of shape {list(shape)}, [rows, {heads}, {head_dim}] expected")
     if t.is_contiguous():
-        return
+        return heads * head_dim
     row, head, value = t.stride()
     if shape[0] == 0:
-        return
+        return row
     if value != 1 or (heads > 1 and head != head_dim):
         raise ShapeError(f"{name}: a row's heads lie one after the other")
     if written and shape[0] > 1 and row < heads * head_dim:
         raise ShapeError(f"{name}: its rows overlap")
+    return row
 
 
 class Batch:
@@ -157,19 +159,20 @@ class Prefixes:
 
 def _rotated_out(x, rows, head_dim, device, out):
     """`out` for `rows` rows `x` [rows, heads, head_dim] turned (made here where None: rows that no sequence holds are
-    then 0), both checked."""
+    then 0), both checked; the heads, and how far apart the rows of both are."""
     shape = x.shape
     if len(shape) != 3 or shape[0] != rows:
         raise ShapeError(f"rows to turn of shape {list(shape)}, [{rows}, heads, {head_dim}] expected")
     heads = shape[1]
-    _check_heads("rows to turn", x, heads, head_dim, device, out is x)
+    stride = out_stride = _check_heads("rows to turn", x, heads, head_dim, device, out is x)
     if out is None:
-        return torch.zeros(shape, dtype=torch.float32, device=device)
-    if out is not x:
-        _check_heads("out", out, heads, head_dim, device, True)
+        out = torch.zeros(shape, dtype=torch.float32, device=device)
+        out_stride = heads * head_dim
+    elif out is not x:
+        out_stride = _check_heads("out", out, heads, head_dim, device, True)
         if out.shape[0] != rows:
             raise ShapeError(f"{rows} rows to turn and {out.shape[0]} of out")
-    return out
+    return out, heads, stride, out_stride
 
 
 class Rotary:
@@ -235,11 +238,11 @@ class Rotary:
         `x`. Rows of `out` that no sequence holds are left as they are (0 in an `out` made here)."""
         if x.dim() != 3 or batch.pages.device != self.device:
             raise ShapeError(f"rows [rows, heads, head_dim] and a batch on {self.device}")
-        rows, heads, head_dim = x.shape
+        rows, _, head_dim = x.shape
         with _place(self.device, stream):
-            out = _rotated_out(x, rows, head_dim, self.device, out)
-            check(lib().fg_rotary_rotate(self.handle, ctypes.byref(batch._ffi(rows)), x.data_ptr(), x.stride(0), heads, head_dim,
-                                         out.data_ptr(), out.stride(0), _stream(self.device)))
+            out, heads, stride, out_stride = _rotated_out(x, rows, head_dim, self.device, out)
+            check(lib().fg_rotary_rotate(self.handle, ctypes.byref(batch._ffi(rows)), x.data_ptr(), stride, heads, head_dim,
+                                         out.data_ptr(), out_stride, _stream(self.device)))
         return out
 
 
@@ -270,27 +273,28 @@ class PagedCache:
     def _rows(self, batch, keys, values, written):
         if batch.pages.device != self.device:
             raise ShapeError(f"the batch is on {batch.pages.device}, the cache on {self.device}")
-        _check_heads("keys", keys, self.kv_heads, self.head_dim, self.device, written)
-        _check_heads("values", values, self.kv_heads, self.head_dim, self.device, written)
-        if keys.shape[0] != values.shape[0]:
-            raise ShapeError(f"{keys.shape[0]} rows of keys and {values.shape[0]} of values")
-        return batch._ffi(keys.shape[0])
+        key_stride = _check_heads("keys", keys, self.kv_heads, self.head_dim, self.device, written)
+        value_stride = _check_heads("values", values, self.kv_heads, self.head_dim, self.device, written)
+        rows = keys.shape[0]
+        if rows != values.shape[0]:
+            raise ShapeError(f"{rows} rows of keys and {values.shape[0]} of values")
+        return ctypes.byref(batch._ffi(rows)), key_stride, value_stride
 
     def write(self, batch, keys, values, stream=None, rotary=None, queries=None, out=None):
         """The new tokens' `keys` and `values` [rows, kv_heads, head_dim] quantized into their pages
         (a page that is written to belongs to one sequence). With `rotary` (Rotary) the keys are turned by
         their positions on the way, and `queries` [rows, heads, head_dim], if given, by the same call into
         `out`, which is returned (`out` as for Rotary.rotate)."""
-        fg = self._rows(batch, keys, values, False)
+        fg, key_stride, value_stride = self._rows(batch, keys, values, False)
         if rotary is not None:
-            return self._write_rotated(fg, keys, values, stream, rotary, queries, out)
+            return self._write_rotated(fg, keys, key_stride, values, value_stride, stream, rotary, queries, out)
         if queries is not None or out is not None:
             raise ShapeError("queries are turned by `rotary`: none given")
         with _place(self.device, stream):
-            check(lib().fg_cache_write(self.handle, ctypes.byref(fg), keys.data_ptr(), keys.stride(0), values.data_ptr(),
-                                       values.stride(0), _stream(self.device)))
+            check(lib().fg_cache_write(self.handle, fg, keys.data_ptr(), key_stride, values.data_ptr(), value_stride,
+                                       _stream(self.device)))
 
-    def _write_rotated(self, fg, keys, values, stream, rotary, queries, out):
+    def _write_rotated(self, fg, keys, key_stride, values, value_stride, stream, rotary, queries, out):
         if rotary.device != self.device:
             raise ShapeError(f"the rotary positions are on {rotary.device}, the cache on {self.device}")
         if queries is None and out is not None:
@@ -298,20 +302,18 @@ class PagedCache:
         heads = query = query_stride = to = to_stride = 0
         with _place(self.device, stream):
             if queries is not None:
-                out = _rotated_out(queries, keys.shape[0], self.head_dim, self.device, out)
-                heads, query, query_stride = queries.shape[1], queries.data_ptr(), queries.stride(0)
-                to, to_stride = out.data_ptr(), out.stride(0)
-            check(lib().fg_cache_write_rotated(self.handle, ctypes.byref(fg), rotary.handle, keys.data_ptr(), keys.stride(0),
-                                               values.data_ptr(), values.stride(0), query, query_stride, heads, to, to_stride,
-                                               _stream(self.device)))
+                out, heads, query_stride, to_stride = _rotated_out(queries, keys.shape[0], self.head_dim, self.device, out)
+                query, to = queries.data_ptr(), out.data_ptr()
+            check(lib().fg_cache_write_rotated(self.handle, fg, rotary.handle, keys.data_ptr(), key_stride, values.data_ptr(),
+                                               value_stride, query, query_stride, heads, to, to_stride, _stream(self.device)))
         return out
 
     def read(self, batch, keys, values, stream=None):
         """The same tokens read back into `keys` and `values`: level * scale."""
-        fg = self._rows(batch, keys, values, True)
+        fg, key_stride, value_stride = self._rows(batch, keys, values, True)
         with _place(self.device, stream):
-            check(lib().fg_cache_read(self.handle, ctypes.byref(fg), keys.data_ptr(), keys.stride(0), values.data_ptr(),
-                                      values.stride(0), _stream(self.device)))
+            check(lib().fg_cache_read(self.handle, fg, keys.data_ptr(), key_stride, values.data_ptr(), value_stride,
+                                      _stream(self.device)))
 
     def attend(self, batch, queries, out=None, scale=None, window=0, stream=None, prefixes=None):
         """The attention of the new tokens' `queries` [rows, heads, head_dim] (their keys and values
@@ -325,13 +327,13 @@ class PagedCache:
         if queries.dim() != 3:
             raise ShapeError("queries: [rows, heads, head_dim]")
         heads = queries.shape[1]
-        _check_heads("queries", queries, heads, self.head_dim, self.device, False)
+        stride = _check_heads("queries", queries, heads, self.head_dim, self.device, False)
         if window < 0:
             raise ShapeError("a window of at least one token, or 0 for all")
         with _place(self.device, stream):
             if out is None:
                 out = torch.zeros(queries.shape, dtype=torch.float32, device=self.device)
-            _check_heads("out", out, heads, self.head_dim, self.device, True)
+            out_stride = _check_heads("out", out, heads, self.head_dim, self.device, True)
             if out.shape[0] != queries.shape[0]:
                 raise ShapeError(f"{queries.shape[0]} rows of queries and {out.shape[0]} of out")
             fg, library = ctypes.byref(batch._ffi(queries.shape[0])), lib()
@@ -341,15 +343,15 @@ class PagedCache:
                 shared = ctypes.byref(prefixes._ffi())
                 size = library.fg_cache_attend_shared_scratch(self.handle, fg, shared, heads)
                 scratch = _scratch(size, self.device)
-                check(library.fg_cache_attend_shared(self.handle, fg, shared, queries.data_ptr(), queries.stride(0), heads,
+                check(library.fg_cache_attend_shared(self.handle, fg, shared, queries.data_ptr(), stride, heads,
                                                      1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, out.data_ptr(),
-                                                     out.stride(0), _at(scratch), size, _stream(self.device)))
+                                                     out_stride, _at(scratch), size, _stream(self.device)))
                 return out
             size = library.fg_cache_attend_scratch(self.handle, fg, heads)
             scratch = _scratch(size, self.device)
-            check(library.fg_cache_attend(self.handle, fg, queries.data_ptr(), queries.stride(0), heads,
+            check(library.fg_cache_attend(self.handle, fg, queries.data_ptr(), stride, heads,
                                           1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, out.data_ptr(),
-                                          out.stride(0), _at(scratch), size, _stream(self.device)))
+                                          out_stride, _at(scratch), size, _stream(self.device)))
         return out
 
 
