@@ -95,10 +95,11 @@ struct Entity {
 __device__ __forceinline__ int shared_pages(const SharedParams &p, int count) { return max(0, min(count, p.b.max_pages)); }
 __device__ __forceinline__ int sequence_index(const SharedParams &p, int start) { return max(0, min(start, p.b.sequences)); }
 
-// The groups' arrays, in LDS where they fit.
-constexpr int kGroupsHeld = 1024;
+// The groups' arrays and the sequences', in LDS where they fit: a group's rows are found by its starts, and one load after the other
+// is most of the plan's time.
+constexpr int kHeld = 1024;
 struct Groups {
-    const int *starts, *counts;
+    const int *starts, *counts, *rows, *lengths;
 };
 
 // Span e, the groups' first.
@@ -109,7 +110,7 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, const Groups 
     int before = 0;
     if (s >= 0) {
         if (s >= p.b.sequences) return n;
-        n.span = sequence_span(p.b, s);
+        n.span = span_of(groups.rows[s], groups.rows[s + 1], groups.lengths[s], p.b.rows);
         // the shared pages of sequence s: those of the last group that starts at or before it
         int upto = 0;  // so many starts are
         for (int step = 1 << (31 - __builtin_clz(p.groups + 1)); step; step >>= 1)
@@ -120,7 +121,7 @@ __device__ __forceinline__ Entity entity_of(const SharedParams &p, const Groups 
     if (s < 0) {
         const int a = sequence_index(p, groups.starts[e]), b = sequence_index(p, groups.starts[e + 1]);
         if (b <= a) return n;
-        n.span = span_of(p.b.row_starts[a], p.b.row_starts[b], 0, p.b.rows);
+        n.span = span_of(groups.rows[a], groups.rows[b], 0, p.b.rows);
         n.table = a;
         n.shared = true;
         n.pages = n.hi = shared_pages(p, groups.counts[e]);
@@ -233,7 +234,8 @@ struct SplitQueries {
 };
 
 // The first workgroup lists the tasks, a thread a span; the others split the queries. Bounded by its launch and a chain of waits:
-// the groups, their rows, two sums over the workgroup. 65 spans 5.8 us, 261 6.6, 1040 13.7.
+// the groups, their rows, two sums over the workgroup. 65 spans 5.3 us, 261 6.2, 1040 12.0; with the
+// sequences' rows looked up in memory behind the groups, and sums over the waves one after the other, 5.8, 6.6 and 13.7.
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p, int padded)
 {
     if (blockIdx.x > 0) {
@@ -241,16 +243,20 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         return;
     }
     __shared__ float works[2][kPlanThreads / 64];
-    __shared__ int totals[3][kPlanThreads / 64], held[2][kGroupsHeld + 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, all = p.groups + p.b.sequences;
+    __shared__ int totals[3][kPlanThreads / 64], held[4][kHeld + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), all = p.groups + p.b.sequences;
     const int threads = int(blockDim.x), waves = threads / 64;
-    Groups groups{p.starts, p.counts};
-    if (p.groups <= kGroupsHeld) {
-        for (int g = tid; g <= p.groups; g += threads) {
-            held[0][g] = p.starts[g];
-            held[1][g] = g < p.groups ? p.counts[g] : 0;
+    Groups groups{p.starts, p.counts, p.b.row_starts, p.b.lengths};
+    if (p.groups <= kHeld && p.b.sequences <= kHeld) {
+        for (int i = tid; i <= max(p.groups, p.b.sequences); i += threads) {
+            int x[4] = {};
+            if (i <= p.groups) x[0] = p.starts[i];
+            if (i < p.groups) x[1] = p.counts[i];
+            if (i <= p.b.sequences) x[2] = p.b.row_starts[i];
+            if (i < p.b.sequences) x[3] = p.b.lengths[i];
+            for (int k = 0; k < 4; k++) held[k][i] = x[k];
         }
-        groups = Groups{held[0], held[1]};
+        groups = Groups{held[0], held[1], held[2], held[3]};
         __syncthreads();
     }
     // write(item, i) for each lane's `item` and i from 0 to its `count`: a lane does its own few, and the wave those of one
@@ -282,8 +288,8 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
     rows = wave_allsum(rows);
     if (lane == 0) works[0][wave] = work, works[1][wave] = rows;
     __syncthreads();
-    work = rows = 0.0f;
-    for (int w = 0; w < waves; w++) work = work + works[0][w], rows = rows + works[1][w];
+    work = wave_allsum(lane < waves ? works[0][lane] : 0.0f);
+    rows = wave_allsum(lane < waves ? works[1][lane] : 0.0f);
     // Spans apart have each row twice at most, a sequence's and a group's. A batch whose starts fall may have it thousands of
     // times: no room holds, nor any int counts, what that would be to do, and nothing is done.
     if (rows > 2.01f * float(p.b.rows) + 1.0f) {
@@ -305,18 +311,19 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         const int joins = n.tiles == 0 || (!n.shared && n.joined) || whole ? 0 : n.large ? (pairs + 31) / 32 : n.tiles;
         const int mine[3] = {n.large ? units : 0, n.large ? 0 : units, joins};
         int at[3];  // the span's first
-        __syncthreads();  // (what the last round read is read)
+        if (e0) __syncthreads();  // (what the last round read is read)
         for (int k = 0; k < 3; k++) {
             int total;
-            at[k] = done[k] + wave_scan(mine[k], &total) - mine[k];
+            at[k] = wave_scan(mine[k], &total) - mine[k];
             if (lane == 0) totals[k][wave] = total;
         }
         __syncthreads();
         for (int k = 0; k < 3; k++) {
-            for (int w = 0; w < waves; w++) {
-                at[k] += w < wave ? totals[k][w] : 0;
-                done[k] += totals[k][w];
-            }
+            const int of_wave = lane < waves ? totals[k][lane] : 0;
+            int total;
+            const int upto = wave_scan(of_wave, &total);
+            at[k] += done[k] + __builtin_amdgcn_readlane(upto - of_wave, wave);
+            done[k] += total;
         }
         const int e = e0 + tid, base = n.large ? at[0] : at[1];
         const int flags = (n.large ? kLarge : 0) | (n.shared ? kShared : 0) | (n.joined ? kJoined : 0) | (whole ? kWhole : 0);
