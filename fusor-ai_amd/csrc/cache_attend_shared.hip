@@ -401,9 +401,9 @@ __device__ __forceinline__ PageRange part_of(const SpanRecord &t, int split, int
 // units 46, waits are 23. 64 conversations behind 8192, whose four pages a part are mostly the first: 21 us, 417 TFLOP/s, 24 %.
 // 256 sequences in five groups, 73 MB of their own pages beside them: 57 us.
 // (Eight waves a workgroup, four every second page, which halves the parts: 37 / 55 / 72 us for these against 36 / 57 / 72, and
-// where parts are few 10 % slower; waves of the same SIMD at different priorities, or started apart, the queries asked for before the page table's entries, the
-// next page stored after the products instead of before: no difference. A large task a CU, small ones beside them, then the other
-// large ones: 256 sequences 70, the last large ones starting late.)
+// where parts are few 10 % slower; waves of the same SIMD at different priorities, or started apart, the queries asked for before
+// the page table's entries, the next page stored after the products instead of before: no difference. A large task a CU, small
+// ones beside them, then the other large ones: 256 sequences 70, the last large ones starting late.)
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_tasks_kernel(SharedParams p)
 {
