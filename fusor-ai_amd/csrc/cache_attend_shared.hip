@@ -339,8 +339,10 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
             int to, begin, rows, base, tiles, parts, flags;
         };
         each(joins, Joins{at[2], n.span.begin, n.span.rows, base, n.tiles, nsplit, flags}, [&](const Joins &u, int i) {
-            const int tile = u.flags & kLarge ? i / 4 : i;
-            if (u.to + i < p.join_slots) p.joins[u.to + i] = JoinRecord{u.begin, u.rows, i, u.base + (u.tiles - 1 - tile) * u.parts, u.parts, u.flags, {}};
+            const int tile = u.flags & kLarge ? i / 4 : i, slot = u.base + (u.tiles - 1 - tile) * u.parts;
+            // (nor has a tile parts past that room)
+            const int parts = slot + u.parts <= (u.flags & kLarge ? p.large_slots : p.small_slots) ? u.parts : 0;
+            if (u.to + i < p.join_slots) p.joins[u.to + i] = JoinRecord{u.begin, u.rows, i, slot, parts, u.flags, {}};
         });
         struct Rows {
             OwnRecord own;
