@@ -9,6 +9,7 @@ float32 device tensors, the arrays that describe a step int32 ones.
 import contextlib
 import ctypes
 import math
+import operator
 
 from . import _lib
 from ._lib import Error, FgBatch, FgPrefixes, FgSampling, ShapeError, check, lib, stream_handle
@@ -426,21 +427,21 @@ class Pages:
         """A second sequence with the `length` tokens that lie in `pages`: its pages, and the copies to make, (sources,
         targets) for copy_pages. Whole pages are shared; one that is partly full, which both go on writing to, is copied."""
         held = -(-length // PAGE)
+        pages = list(pages)
         if length < 0 or held > len(pages):
             raise ShapeError(f"{length} tokens in {len(pages)} pages")
         whole = length // PAGE
-        self._held(pages[:held])
+        pages = self._held(pages[:held])
         if whole < held and not self._free:
             raise Error("a page asked for, none is free")
         for p in pages[:whole]:
             self._users[p] += 1
         copies = self.take(held - whole)
-        return pages[:whole] + copies, (list(pages[whole:held]), list(copies))
+        return pages[:whole] + copies, (pages[whole:], list(copies))
 
     def free(self, pages):
         """A sequence lets go of its pages."""
-        self._held(pages)
-        for p in pages:
+        for p in self._held(pages):
             self._users[p] -= 1
             if self._users[p] == 0:
                 self._free.append(p)
@@ -459,8 +460,11 @@ class Pages:
         return moves
 
     def _held(self, pages):
+        """The ids as a list of whole numbers (a table's row adds, and holds numbers that compare but do not hash alike)."""
+        pages = [operator.index(p) for p in pages]
         if len(set(pages)) != len(pages) or any(not 0 <= p < self.count or not self._users[p] for p in pages):
             raise ShapeError("pages that no sequence holds, or one of them twice")
+        return pages
 
 
 def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, chances=None, stream=None):

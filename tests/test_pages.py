@@ -85,6 +85,27 @@ def test_compaction(seed):
     assert pages.compact() == {} and sorted(pages.take(count - used)) == list(range(used, count))
 
 
+@pytest.mark.parametrize("kind", ["tuple", "array", "tensor", "iterator"])
+def test_pages_of_any_kind_of_sequence(kind):
+    """A row of a step's page table, for one: its ids, no sums with them, and none freed twice."""
+    import torch
+    of = {"tuple": tuple, "array": lambda p: np.array(p, np.int32), "tensor": lambda p: torch.tensor(p, dtype=torch.int32), "iterator": iter}[kind]
+    pages = fk.Pages(10)
+    a = pages.take(3)
+    b, copies = pages.fork(of(a + [-1, -1]), 2 * 64 + 5)  # (a table's columns behind the sequence's)
+    assert b == [0, 1, 3] and copies == ([2], [3]) and all(type(p) is int for p in b + copies[0])
+    assert [pages.users(p) for p in range(5)] == [2, 2, 1, 1, 0] and pages.free_pages == 6
+    with pytest.raises(fk.ShapeError):
+        pages.free(of([1, 1]))
+    pages.free(of(b))
+    assert [pages.users(p) for p in range(5)] == [1, 1, 1, 0, 0]
+    for bad in ([0.5], [None]):
+        with pytest.raises(TypeError):
+            pages.free(bad)
+    pages.free(of(a))
+    assert pages.free_pages == 10 and not any(pages.users(p) for p in range(10)) and sorted(pages.take(10)) == list(range(10))
+
+
 class Cache:
     """What copy_pages looks at of a cache before any device work."""
 
