@@ -368,7 +368,7 @@ def copy_pages(caches, sources, targets, stream=None):
     if any(c.device != device for c in caches):
         raise ShapeError("the caches are on one device")
     if not isinstance(sources, torch.Tensor) and not isinstance(targets, torch.Tensor):
-        sources, targets = list(sources), list(targets)
+        sources, targets = ([operator.index(p) for p in ids] for ids in (sources, targets))
         moved = [(s, t) for s, t in zip(sources, targets) if s != t]
         kept = {t for s, t in zip(sources, targets) if s == t}
         ends = {t for _, t in moved}

@@ -120,6 +120,16 @@ def test_lists_that_are_refused(sources, targets):
         fk.copy_pages([Cache(8), Cache(9)], sources, targets)
 
 
+def test_ids_of_lists_are_whole_numbers():
+    """... also where they come as tensors, which compare but do not hash alike."""
+    import torch
+    two = [torch.tensor(3), torch.tensor(3)]
+    with pytest.raises(fk.ShapeError, match="named twice"):
+        fk.copy_pages([Cache(8)], [1, 2], two)
+    with pytest.raises(TypeError):
+        fk.copy_pages([Cache(8)], [1, 2], [3.2, 3.7])
+
+
 def test_copies_that_are_refused():
     import torch
     assert fk.copy_pages([], [1], [2]) is None
