@@ -61,13 +61,19 @@ FG_BOTH Angle both(const Angle &a, const Angle &b) { return Angle{__builtin_fma(
 FG_BOTH Angle whole_four(const RotaryPair &r, int position) { return angle_of(uint64_t(unsigned(position) & ~3u) * r.step); }
 FG_BOTH Angle angle_at(const RotaryPair &r, int position) { return both(whole_four(r, position), r.more[position & 3]); }
 
-// `frequency` radians a token as a step: the fraction of a turn, rounded to 2^-64 (80-bit arithmetic).
+// `frequency` radians a token, of at most 1024 in magnitude, as a step: its turns' fraction, rounded to 2^-64, in whole numbers. The
+// frequency's 53 bits times the first 126 of 1 / (2 pi) are off by less than 2^-53 of a step.
 inline uint64_t turn_step(double frequency)
 {
-    long double turns = (long double)frequency / 6.28318530717958647692528676655900576L;
-    turns -= floorl(turns);
-    const long double scaled = roundl(turns * 18446744073709551616.0L);
-    return scaled >= 18446744073709551616.0L ? 0 : uint64_t(scaled);
+    constexpr uint64_t kHigh = 0x28be60db9391054a, kLow = 0x7f09d5f47d4d3770;  // 2^128 / (2 pi)
+    int exponent;
+    const uint64_t digits = uint64_t(std::ldexp(std::frexp(std::fabs(frequency), &exponent), 53));
+    // digits 2^(exponent - 53) 2^64 / (2 pi), without the product's lowest 64 bits
+    const unsigned __int128 product = (unsigned __int128)digits * kHigh + uint64_t(((unsigned __int128)digits * kLow) >> 64);
+    const int drop = 53 - exponent;  // of its bits, at least 42
+    uint64_t step = 0;
+    if (drop <= 128) step = uint64_t(product >> (drop - 1) >> 1) + uint64_t(product >> (drop - 1) & 1);
+    return frequency < 0 ? -step : step;
 }
 
 inline RotaryPair rotary_pair(double frequency)

@@ -58,6 +58,27 @@ def test_angles(phase, frequency):
     assert (np.abs(s - np.sin(angle).astype(np.float64)) <= bound).all()
 
 
+# 2^256 / (2 pi), rounded down
+TURN_BITS = 0x28be60db9391054a7f09d5f47d4d377036d8a5664f10e4107f9458eaf7aef158
+
+
+@pytest.mark.parametrize("frequency", [777.7, 1023.9, 1024.0, 1023.9999999999999, 100.0, 6.3, 2 * math.pi, math.pi, 3.0, 1.0, 1e6 ** -0.9, 1e-7,
+                                       1e-18, 1e-19, 1e-20, 5e-324, 0.0, -0.3, -1023.9, -1e-20])
+def test_steps_to_half_their_last_bit(phase, frequency):
+    """... for every frequency that is taken, whole turns a token among them. (A frequency times 2^256 / (2 pi), whole numbers and
+    powers of two, is exact to 2^-246 turns.)"""
+    numerator, denominator = frequency.as_integer_ratio()
+    turns = numerator * TURN_BITS * 2 ** 64 // denominator  # times 2^320
+    off = (phase.step(frequency) * 2 ** 256 - turns + 2 ** 319) % 2 ** 320 - 2 ** 319
+    assert abs(off) <= 2 ** 255 + 2 ** 200, off / 2 ** 256
+
+
+def test_steps_of_random_frequencies(phase):
+    rng = np.random.default_rng(0)
+    for frequency in np.concatenate([rng.uniform(-1024, 1024, 2000), np.exp(rng.uniform(-50, math.log(1024), 2000))]):
+        test_steps_to_half_their_last_bit(phase, float(frequency))
+
+
 def test_quarters_and_their_borders(phase):
     out = (ctypes.c_double * 2)()
     for eighth in range(8):
