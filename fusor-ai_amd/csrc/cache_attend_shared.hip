@@ -607,6 +607,10 @@ struct Launch {
 // tokens 18 and 30, 3000 28 and 31, 8000 53 and 36; S = 256: 100 21 and 28, 800 36 and 35, 3000 77 and 46.
 // Of 220 steps of 4 to 256 sequences in 1 to 5 groups behind 10 to 900 pages, 1 to 10 rows each, heads of 36 to 256, the way chosen so
 // takes 1.9 % longer than the faster one on average (from 160 or 256 MiB on 2.5 and 3.0; always the one way or the other 17 and 16).
+// (How many groups are named says nothing: arrays with room for a group a sequence may hold one group of all. Such arrays and arrays of
+// one group take the same time, 16 of 128 over 4, S = 8: P = 1301 49 and 49, 64 by itself; S = 128: 79 37 and 37, 58. Where
+// nothing is shared the two launches and the single waves cost, groups of one sequence each: S = 8: P = 478 60, 52 by itself, 1304 145 and
+// 137; S = 128: 30 68 and 46, 82 153 and 130; S = 256: 41 166 and 128.)
 // Nor where the sequences have more than 96 pairs of a new token and a head of a key head on average (64 of heads past 128): a
 // prompt's chunks fill tiles of their own, and the parts cost what is left to gain: 17 chunks of 1 to 512 tokens behind 94
 // pages, 14 heads of 64 over 2, 95 and 124; 16 of 60 tokens behind 100, 16 of 128 over 4, 123 and 156.
@@ -620,7 +624,7 @@ Launch plan_launch(const fg_cache *c, const fg_batch *b, const fg_prefixes *f, s
     l.limit = c->padded <= 128 ? 96 : 64;
     const size_t pages = window ? std::min(b->max_pages, window / kPage + 2) : b->max_pages;
     const double bytes_held = double(sequences) * double(pages) * double(c->kv_heads) * double(record_bytes(c->padded));
-    l.shared = groups && sequences > groups && bytes_held >= kSharedBytes && pairs <= size_t(l.limit) * sequences;
+    l.shared = groups && sequences > 1 && bytes_held >= kSharedBytes && pairs <= size_t(l.limit) * sequences;
     if (!l.shared) return l;
     const size_t units = std::max<size_t>(kUnits / c->kv_heads, 1);
     l.target = int((c->padded <= 128 ? 2 : 1) * units);

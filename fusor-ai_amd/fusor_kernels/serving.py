@@ -322,7 +322,8 @@ class PagedCache:
         `window` of them. `scale` is 1 / sqrt(head_dim) unless given. A token without a key gives 0;
         `out` may be `queries`; rows of it that no sequence holds are left as they are (0 in an `out`
         made here). Keys may reach 1e33 and scores 1e7 in magnitude. With `prefixes` (Prefixes) the pages that a group
-        of sequences begins with are worked through once for all of them."""
+        of sequences begins with are worked through once for all of them, if the batch's tables have room for 224 MiB together and
+        its sequences few new tokens on average (fg_cache_attend_shared has the rule); if not, each sequence reads its own."""
         if batch.pages.device != self.device:
             raise ShapeError(f"the batch is on {batch.pages.device}, the cache on {self.device}")
         if queries.dim() != 3:

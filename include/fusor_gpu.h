@@ -238,8 +238,12 @@ typedef struct {
     const int32_t *starts, *pages;
 } fg_prefixes;
 
-/* fg_cache_attend, with each group's shared pages worked through once for all of its rows where that is faster: what it
- * gives is the same, but for the order of additions. */
+/* fg_cache_attend, with each group's shared pages worked through once for all of its rows: what it gives is the same, but for the
+ * order of additions. The host knows no lengths, so one rule for the whole call says whether that is done: at least two sequences,
+ * tables that together have room for 224 MiB (max_pages, or what a window sees), and on average at most 96 pairs of a row and
+ * one of a key head's query heads a sequence (64 for heads past 128). Otherwise each sequence reads its table by itself: one long
+ * chunk beside single tokens does that to all of them. Short sequences in wide tables, and groups that share nothing,
+ * pay some 10 us and up. */
 size_t fg_cache_attend_shared_scratch(const fg_cache *cache, const fg_batch *batch, const fg_prefixes *prefixes, size_t heads);
 int fg_cache_attend_shared(const fg_cache *cache, const fg_batch *batch, const fg_prefixes *prefixes, const float *query,
                            size_t query_stride, size_t heads, float scale, size_t window, float *out, size_t out_stride,

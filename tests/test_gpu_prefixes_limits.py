@@ -4,6 +4,8 @@ import ctypes
 
 import pytest
 
+from test_gpu_prefixes import Shared
+
 pytestmark = pytest.mark.gpu
 
 
@@ -37,3 +39,28 @@ def test_starts_that_fall_read_no_memory_behind_the_scratch(fk, gpu):
     torch.cuda.synchronize()
     assert not bool(torch.isnan(out).any()) and not bool(out[5:].any())
     assert bool(torch.isnan(memory[size // 4:]).all())
+
+
+def sizes_of_scratch(case):
+    """... of a case's call, and of the one over each sequence's own table."""
+    import torch
+    from fusor_kernels import _lib
+    fg = case.step.batch(case.fk, case.gpu)._ffi(case.step.total())
+    prefixes = case.fk.Prefixes(*(torch.tensor(x, dtype=torch.int32, device=case.gpu) for x in case.groups))
+    lib, ffi = _lib.lib(), prefixes._ffi()
+    return (lib.fg_cache_attend_shared_scratch(case.cache.handle, ctypes.byref(fg), ctypes.byref(ffi), case.heads),
+            lib.fg_cache_attend_scratch(case.cache.handle, ctypes.byref(fg), case.heads))
+
+
+def test_arrays_with_room_for_more_groups(fk, gpu):
+    """... than the batch has sequences, all but one of them empty, work a prefix through once as arrays of one group do."""
+    import torch
+    case = Shared(fk, gpu, [1] * 9, [1300 + 9 * s for s in range(9)], [0, 9], [20], 8, 2, 64)
+    shared, by_itself = sizes_of_scratch(case)
+    assert shared > by_itself
+    want = case.run()
+    case.check(want)
+    for room in (8, 9, 40):
+        case.groups = ([0] + [9] * room, [20] + [0] * (room - 1))
+        assert sizes_of_scratch(case)[0] > by_itself
+        assert torch.equal(case.run(), want)
