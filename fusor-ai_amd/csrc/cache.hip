@@ -552,6 +552,9 @@ int fg_cache_write_rotated(fg_cache *c, const fg_batch *b, const fg_rotary *r, c
     if (rc) return rc;
     if ((rc = check_rotary(r, c->device, size_t(c->head_dim), who))) return rc;
     if ((heads || query || out) && (rc = check_rotated(b, query, query_stride, heads, size_t(c->head_dim), out, out_stride, who))) return rc;
+    const size_t width = size_t(c->kv_heads) * c->head_dim, turned = heads * c->head_dim;
+    if (rows_meet(out, out_stride, turned, key, key_stride, width, b->rows) || rows_meet(out, out_stride, turned, value, value_stride, width, b->rows))
+        return set_error(FG_ERR_SHAPE, std::string(who) + ": turned queries lie over the keys or values, which the same launch reads");
     TurnParams p = store_params<TurnParams>(c, b, key_stride, value_stride);
     p.in[0] = key;
     p.in[1] = value;

@@ -148,6 +148,9 @@ RotateParams rotate_params(const fg_rotary *r, const fg_batch *b, const float *x
                            float *out, size_t out_stride);
 int launch_rotate(const RotateParams &p, bool quads, hipStream_t s);
 
+// Whether `rows` rows of a and of b share memory (rows of different strides among each other: not told).
+bool rows_meet(const float *a, size_t a_stride, size_t a_width, const float *b, size_t b_stride, size_t b_width, size_t rows);
+
 // The arguments that rotating calls check; `device` is the current one.
 int check_rotary(const fg_rotary *r, int device, size_t head_dim, const std::string &who);
 int check_rotated(const fg_batch *b, const float *x, size_t x_stride, size_t heads, size_t head_dim, const float *out, size_t out_stride,

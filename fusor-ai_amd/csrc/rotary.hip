@@ -1,6 +1,7 @@
 // Rotary positions (fg_rotary): a step's rows turned by their positions. cache.hip turns keys on their way into the cache.
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <new>
 #include <vector>
 
@@ -67,6 +68,18 @@ int check_rotary(const fg_rotary *r, int device, size_t head_dim, const std::str
     return FG_OK;
 }
 
+bool rows_meet(const float *a, size_t a_stride, size_t a_width, const float *b, size_t b_stride, size_t b_width, size_t rows)
+{
+    if (!rows || !a || !b) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    if (y >= x + ((rows - 1) * a_stride + a_width) * sizeof(float) || x >= y + ((rows - 1) * b_stride + b_width) * sizeof(float)) return false;
+    if (rows == 1) return true;
+    if (a_stride != b_stride || !a_stride) return false;
+    // b's rows begin so far behind a's (as each begins before the other's end, the rows that meet are there)
+    const size_t stride = a_stride * sizeof(float), behind = y >= x ? (y - x) % stride : (stride - (x - y) % stride) % stride;
+    return behind < a_width * sizeof(float) || stride - behind < b_width * sizeof(float);
+}
+
 int check_rotated(const fg_batch *b, const float *x, size_t x_stride, size_t heads, size_t head_dim, const float *out, size_t out_stride,
                   const std::string &who)
 {
@@ -75,6 +88,8 @@ int check_rotated(const fg_batch *b, const float *x, size_t x_stride, size_t hea
     if (b->rows > 1 && out_stride < heads * head_dim) return set_error(FG_ERR_SHAPE, who + ": a row's heads run past the row stride");
     if (out == x && out_stride != x_stride && b->rows > 1)
         return set_error(FG_ERR_SHAPE, who + ": outputs over the rows have the rows' stride");
+    if (out != x && rows_meet(out, out_stride, heads * head_dim, x, x_stride, heads * head_dim, b->rows))
+        return set_error(FG_ERR_SHAPE, who + ": outputs lie over a part of the rows");
     return FG_OK;
 }
 

@@ -236,7 +236,7 @@ class Rotary:
 
     def rotate(self, batch, x, out=None, stream=None):
         """The batch's new rows of `x` [rows, heads, head_dim] turned by their positions, into `out`, which may be
-        `x`. Rows of `out` that no sequence holds are left as they are (0 in an `out` made here)."""
+        `x` and otherwise does not overlap it. Rows of `out` that no sequence holds are left as they are (0 in an `out` made here)."""
         if x.dim() != 3 or batch.pages.device != self.device:
             raise ShapeError(f"rows [rows, heads, head_dim] and a batch on {self.device}")
         rows, _, head_dim = x.shape
@@ -285,7 +285,7 @@ class PagedCache:
         """The new tokens' `keys` and `values` [rows, kv_heads, head_dim] quantized into their pages
         (a page that is written to belongs to one sequence). With `rotary` (Rotary) the keys are turned by
         their positions on the way, and `queries` [rows, heads, head_dim], if given, by the same call into
-        `out`, which is returned (`out` as for Rotary.rotate)."""
+        `out`, which is returned (`out` as for Rotary.rotate; it overlaps neither `keys` nor `values`)."""
         fg, key_stride, value_stride = self._rows(batch, keys, values, False)
         if rotary is not None:
             return self._write_rotated(fg, keys, key_stride, values, value_stride, stream, rotary, queries, out)
