@@ -521,7 +521,7 @@ __device__ __forceinline__ void attend_few(const AttendParams &p, const Task &ta
 // exponential, the value's scale, the total, the maximum and two f16 pieces), and two waves a SIMD overlap them in part.
 // 8192 tokens of 16 heads of 128 over 4: 492 us, 1118 TFLOP/s in f16 products (two an operand, for the
 // pieces), the matrix cores busy 61 % of the time and the vector units 57 %, at the 1.74 GHz that the card keeps under this
-// load (2.35 in the others here); a large f16 product of the library's reaches 1175. Chunks of 2700 tokens, 16 heads of
+// load (2.35 in the others here); a large f16 product of the library's reaches 1339. Chunks of 2700 tokens, 16 heads of
 // 72 over a window of 1000: 75 us, 336 TFLOP/s: its 350 tiles of 19 pages are 1400 waves for 1024 SIMDs, so some have
 // two, and CUs are busy 69 % of the time. 17 chunks of 1 to 512 tokens, 14 heads of 64 over 2: 52.5 us; CUs are busy
 // 72 % of the time, and then the vector units 51 %, the matrix cores 29, with 1.6 waves a SIMD. 32 pairs a wave: with 64, or with four waves a SIMD, the sums do not fit the registers.

@@ -205,7 +205,8 @@ struct Launch {
 // much as ten pages, and as much again on the host (500 tokens: 10.3 whole, 11.2 split). A large tile's page costs 1.5 to 3.5 us,
 // and what joining costs grows with the tiles: they are split over more than 4 pages, or more than 32 pages times the share of the
 // CUs that they fill (to 16). A chunk of 102 rows over 5 / 7 / 11 pages, whole and split: (b) 15.4 14.5 / 18.4 15.8 / 24.5 16.3,
-// (a) 19.8 17.7 / 24.3 19.9 / 32.4 19.9, 8 of 256 over 2 32 26 / 39 29 / 54 30; four of 120 over 7 / 9 / 13 (a) 25 25 / 29 24 / 37 32;
+// (a) 19.8 17.7 / 24.3 19.9 / 32.4 19.9, 8 of 256 over 2 32 26 / 39 29 / 54 30 (the host knows the table, not the
+// length: the same rows with nothing before them, two pages, pay for the join, 13.0 and 10.8, (a) 16.1 and 13.7); four of 120 over 7 / 9 / 13 (a) 25 25 / 29 24 / 37 32;
 // 13 of 78, half of the CUs, over 7 / 16 (a) 25 35 / 44 40, (b) 19 24 / 33 38. Two workgroups a CU read at once what memory
 // gives, so the parts aimed at are two a CU, less half of one a tile, whose last part is half a part on average:
 // fewer leave some CUs two parts and others one (eight documents of 30000 to 70000 tokens: 288 parts 105, 350 98,
