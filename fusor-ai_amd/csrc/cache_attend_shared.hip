@@ -605,8 +605,8 @@ struct Launch {
 // and 42, 1000 171 and 60; S = 256: 8 31 and 31, 20 45 and 33, 200 260 and 81; 14 of 64 over 2 (17 KiB), S = 32: 400 32
 // and 36, 1000 61 and 46; S = 128: 45 22 and 26, 115 36 and 36, 400 91 and 55. With windows over 400 pages of 66 KiB: S = 64, 800
 // tokens 18 and 30, 3000 28 and 31, 8000 53 and 36; S = 256: 100 21 and 28, 800 36 and 35, 3000 77 and 46.
-// Of 220 steps of 4 to 256 sequences in 1 to 5 groups behind 10 to 900 pages, 1 to 10 rows each (as many in all sequences of a step), heads of 36 to 256, the way chosen so
-// takes 1.9 % longer than the faster one on average (from 160 or 256 MiB on 2.5 and 3.0; always the one way or the other 17 and 16).
+// Of 220 steps of 4 to 256 sequences in 1 to 5 groups behind 10 to 900 pages, 1 to 10 rows each (as many in all sequences of a
+// step), heads of 36 to 256, the way chosen so takes 1.9 % longer than the faster one on average (from 160 or 256 MiB on 2.5 and 3.0; always the one way or the other 17 and 16).
 // (How many groups are named says nothing: arrays with room for a group a sequence may hold one group of all. Such arrays and arrays of
 // one group take the same time, 16 of 128 over 4, S = 8: P = 1301 49 and 49, 64 by itself; S = 128: 79 37 and 37, 58. Where
 // nothing is shared the two launches and the single waves cost, groups of one sequence each: S = 8: P = 478 60, 52 by itself, 1304 145 and

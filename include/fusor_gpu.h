@@ -267,7 +267,8 @@ int fg_rotary_free(fg_rotary *rotary);
 int fg_rotary_rotate(const fg_rotary *rotary, const fg_batch *batch, const float *x, size_t x_stride, size_t heads, size_t head_dim,
                      float *out, size_t out_stride, void *stream);
 /* fg_cache_write of keys that are turned first, and fg_rotary_rotate of the same rows' queries, `heads` of them, into `out` (none
- * where heads is 0 and both are NULL), which overlaps neither `key` nor `value`: one launch has both. Turned keys are quantized from the f32 values that fg_rotary_rotate gives. */
+ * where heads is 0 and both are NULL), which overlaps neither `key` nor `value`: one launch has both. Turned keys are quantized
+ * from the f32 values that fg_rotary_rotate gives. */
 int fg_cache_write_rotated(fg_cache *cache, const fg_batch *batch, const fg_rotary *rotary, const float *key, size_t key_stride,
                            const float *value, size_t value_stride, const float *query, size_t query_stride, size_t heads,
                            float *out, size_t out_stride, void *stream);
